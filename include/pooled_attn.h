@@ -327,6 +327,103 @@ int pa_set_weight_cache(pa_ctx* ctx, size_t max_bytes);
 int pa_attn_layer_prefill(pa_ctx* ctx, uint32_t layer, const pa_weight* w_qkv, const pa_weight* w_o, const float* d_attn_norm_w,
                           const float* d_qw, const float* d_kw, float* d_x, uint32_t x_stride, uint32_t base_pos, uint32_t n_cols);
 
+/* ---- the gated delta rule: the token mixer of the layers of a hybrid model that have no attention (three of four in the
+ *      MoE and 27B shapes; the reference's DeltaNet kernels, engine/wgsl/qwen35.js:1-368, :417-826).  Where attention keeps
+ *      cache rows, such a layer keeps per v head h a matrix S [head_v][head_k], and the last conv_width - 1 inputs of a short
+ *      convolution.  With k head h / (n_v_heads / n_k_heads), a token t is
+ *        S' = exp(g) S;  u = beta (v - S' k);  S = S' + u k^T;  o = scale S q
+ *      and, with PA_DELTA_L2NORM, q and k are first divided by sqrt(sum of their squares + eps).  All in f32.
+ *      g and beta may be any numbers: g = -inf empties a head's state in front of the token, beta = 0 leaves a token out. ---- */
+#define PA_DELTA_L2NORM 1u
+typedef struct pa_delta_config {
+  uint32_t n_k_heads;    /* q and k heads */
+  uint32_t n_v_heads;    /* a multiple of n_k_heads */
+  uint32_t head_k;       /* 64 or 128 */
+  uint32_t head_v;       /* a multiple of 16, at most 512 */
+  uint32_t conv_width;   /* taps of pa_delta_glue's convolution, 1 to 4; 0: no pre-step (pa_delta_glue refuses) */
+  uint32_t n_layers;     /* states; a layer index counts these layers alone */
+  float scale;           /* of q; 0: 1 / sqrt(head_k) */
+  float eps;             /* of PA_DELTA_L2NORM */
+  uint32_t flags;        /* PA_DELTA_* */
+} pa_delta_config;
+typedef struct pa_delta pa_delta;
+/* The states of all layers, zeroed, and the workspace of pa_delta_prefill (allocated here, so that no later call allocates and
+ * every call can be captured).  A handle belongs to the context that made it, as a weight does: destroy it first.  Its calls are
+ * ordered like all of the context's: one at a time, in the order of the stream; graphs captured from one handle share its
+ * states and workspace, so replays of them must not overlap either. */
+int pa_delta_create(pa_ctx* ctx, const pa_delta_config* cfg, pa_delta** out);
+int pa_delta_destroy(pa_ctx* ctx, pa_delta* dn);
+/* a layer's states to zero, queued on the context's stream: a new session */
+int pa_delta_reset(pa_ctx* ctx, pa_delta* dn, uint32_t layer);
+/* which: 0 = S, f32 [n_v_heads][head_v][head_k]; 1 = the convolution's inputs, f32 [conv_width - 1][channels], oldest first, a
+ * channel row being [q heads | k heads | v heads].  Host copies block; the device address is for pa_copy_d2d, which makes
+ * checkpoints on the device as pa_slot_save does for cache rows.  pa_delta_state_bytes: of one layer, 0 for a state the handle does not have. */
+int pa_delta_read(pa_ctx* ctx, const pa_delta* dn, uint32_t layer, int which, void* h_dst);
+int pa_delta_write(pa_ctx* ctx, pa_delta* dn, uint32_t layer, int which, const void* h_src);
+size_t pa_delta_state_bytes(const pa_delta* dn, int which);
+void* pa_delta_state_ptr(pa_delta* dn, uint32_t layer, int which);
+/* pa_delta_glue: the pre-step of n_cols columns,
+ *   d_out[c] = silu(bias + sum_j conv_w[.][j] x[c - (conv_width - 1) + j]) over the channels of d_qkv, inputs in front of the call from the state;
+ *   d_g = -exp(a_log) softplus(a + dt_bias),  d_beta = sigmoid(b).
+ *   n_commit <= n_cols: the state moves on over the first n_commit columns alone (see pa_delta_decode).
+ *   d_qkv, d_out: f32 [n_cols][stride], 16-byte aligned, strides multiples of 4;  d_conv_w: f32 [channels][conv_width], 16-byte aligned;
+ *   d_conv_b: f32 [channels], 16-byte aligned, or NULL;  d_a, d_b: f32 [n_cols][ab_stride];  d_a_log, d_dt_bias: f32 [n_v_heads];
+ *   d_g, d_beta: f32 [n_cols][gate_stride].  Outputs share no memory with inputs. */
+int pa_delta_glue(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const float* d_qkv, uint32_t qkv_stride, const float* d_conv_w, const float* d_conv_b,
+                  const float* d_a, const float* d_b, uint32_t ab_stride, const float* d_a_log, const float* d_dt_bias, uint32_t n_cols,
+                  uint32_t n_commit, float* d_out, uint32_t out_stride, float* d_g, float* d_beta, uint32_t gate_stride);
+/* pa_delta_decode: one token, or the columns of a draft, token by token.  Every column has the bits of the one-token call at its
+ * place.  A state cannot be cut back to a shorter length as a cache can, so a draft is run with n_commit = 0, which leaves the
+ * state as it was, and again over the accepted columns with n_commit = n_cols and d_out = NULL (or n_commit between, if the
+ * accepted number is known).
+ *   d_q, d_k: f32 [n_cols][stride], 16-byte aligned, strides multiples of 4, a column holds [n_k_heads][head_k];  d_v: [n_v_heads][head_v];
+ *   d_g (natural logarithm of the decay), d_beta: f32 [n_cols][gate_stride];  the three may be parts of one pa_delta_glue column;
+ *   d_out: [n_cols][out_stride] of out_dtype, a column holds [n_v_heads][head_v]; shares no memory with inputs or state; NULL (then d_q is not read): the
+ *          state alone moves on.
+ * pa_delta_prefill: the same for n_cols columns of a prompt, all of them committed, in chunks of 64 on the matrix cores where that is faster (from
+ * 48 columns on).  Its results agree with pa_delta_decode's to f32 rounding. */
+int pa_delta_decode(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const float* d_q, uint32_t q_stride, const float* d_k, uint32_t k_stride, const float* d_v,
+                    uint32_t v_stride, const float* d_g, const float* d_beta, uint32_t gate_stride, uint32_t n_cols, uint32_t n_commit, void* d_out,
+                    uint32_t out_stride, int out_dtype);
+int pa_delta_prefill(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const float* d_q, uint32_t q_stride, const float* d_k, uint32_t k_stride, const float* d_v,
+                     uint32_t v_stride, const float* d_g, const float* d_beta, uint32_t gate_stride, uint32_t n_cols, void* d_out, uint32_t out_stride,
+                     int out_dtype);
+
+/* ---- a mixture-of-experts layer over a few tokens (the reference's router and expert kernels, engine/wgsl/moe.js) ----
+ *   xn = rmsnorm(x) * norm_w;  p = softmax(router xn);  the top_k experts of the largest logits are chosen, the lower index first where two are equal;
+ *   y = x + sum over the chosen e of w_e down_e (silu(gate_e xn) * (up_e xn)),  w_e = p_e, or p_e / sum of the chosen p with PA_MOE_NORM_TOPK,
+ *       + sigmoid(shared_gate . xn) * the same of the shared expert, with PA_MOE_SHARED. */
+#define PA_MOE_NORM_TOPK 1u
+#define PA_MOE_SHARED 2u
+typedef struct pa_moe_config {
+  uint32_t dim, ffn;      /* model width and width of an expert: multiples of 32, at most 8192 */
+  uint32_t n_experts;     /* at most 1024 */
+  uint32_t top_k;         /* at most 16 and n_experts */
+  int kind;               /* PA_W_* of all expert planes */
+  uint32_t flags;         /* PA_MOE_* */
+} pa_moe_config;
+/* host planes in the layouts of pa_weight_create, expert after expert: gate and up [ffn][dim], down [dim][ffn]; scales NULL for PA_W_F32 */
+typedef struct pa_moe_planes {
+  const float* h_router;                                             /* [n_experts][dim] */
+  const void *h_gate, *h_up, *h_down;
+  const uint16_t *h_gate_s, *h_up_s, *h_down_s;
+  const float* h_shared_gate;                                        /* [dim]; this and what follows: PA_MOE_SHARED */
+  const void *h_shared_gate_w, *h_shared_up_w, *h_shared_down_w;     /* the shared expert's planes */
+  const uint16_t *h_shared_gate_s, *h_shared_up_s, *h_shared_down_s;
+} pa_moe_planes;
+typedef struct pa_moe pa_moe;
+/* copies the planes to the device and allocates the workspace of the widest call (max_cols).  Ownership, ordering and capture as pa_delta_create. */
+int pa_moe_create(pa_ctx* ctx, const pa_moe_config* cfg, const pa_moe_planes* planes, pa_moe** out);
+int pa_moe_destroy(pa_ctx* ctx, pa_moe* moe);
+/* n_cols tokens through the layer.  Made for the few tokens of a decode step, a verify block or a narrow pass, where the chosen experts' weights are
+ * the work; any n_cols up to max_cols is served.  A token's results have the same bits whatever other tokens the call holds.
+ *   d_norm_w: f32 [dim], or NULL: xn = x;  eps from pa_config
+ *   d_x: f32 [n_cols][x_stride];  d_y: f32 [n_cols][y_stride]; either d_x itself with the same stride, or no memory shared;  all 16-byte aligned, strides multiples of 4
+ *   d_ids: u32 [n_cols][top_k], the chosen experts, largest logit first, or NULL;  d_weights: f32 [n_cols][top_k], their w, or NULL
+ * A NaN in a token's x makes its y and w NaN; its ids stay in range. */
+int pa_moe_layer(pa_ctx* ctx, pa_moe* moe, const float* d_norm_w, const float* d_x, uint32_t x_stride, uint32_t n_cols, float* d_y, uint32_t y_stride,
+                 uint32_t* d_ids, float* d_weights);
+
 /* library / device description, e.g. "pooled_attn 0.1 gfx950 256CU" (storage owned by the library, one buffer per
  * calling thread) */
 const char* pa_version(void);

@@ -15,6 +15,8 @@ PA_OK, PA_ERR_INVALID, PA_ERR_UNSUPPORTED, PA_ERR_HIP, PA_ERR_NOMEM = 0, 1, 2, 3
 PA_FLAG_QK_NORM, PA_FLAG_GATE, PA_FLAG_KV_Q8, PA_FLAG_VERIFY_EXACT = 1, 2, 4, 8
 PA_W_F32, PA_W_Q8_0, PA_W_Q4_0 = 0, 1, 2
 PA_OUT_F32, PA_OUT_F16 = 0, 1
+PA_DELTA_L2NORM = 1
+PA_MOE_NORM_TOPK, PA_MOE_SHARED = 1, 2
 
 u32, c_int, vp, f32p = ctypes.c_uint32, ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p
 
@@ -28,6 +30,20 @@ class PaConfig(ctypes.Structure):
 class PaPlan(ctypes.Structure):
     _fields_ = [(n, u32) for n in ("kernel", "split_len", "n_splits", "col_groups", "cols_per_group", "waves",
                                    "row_blocks", "slots")]
+
+
+class PaDeltaConfig(ctypes.Structure):
+    _fields_ = [("n_k_heads", u32), ("n_v_heads", u32), ("head_k", u32), ("head_v", u32), ("conv_width", u32), ("n_layers", u32),
+                ("scale", ctypes.c_float), ("eps", ctypes.c_float), ("flags", u32)]
+
+
+class PaMoeConfig(ctypes.Structure):
+    _fields_ = [("dim", u32), ("ffn", u32), ("n_experts", u32), ("top_k", u32), ("kind", c_int), ("flags", u32)]
+
+
+class PaMoePlanes(ctypes.Structure):
+    _fields_ = [(n, vp) for n in ("h_router", "h_gate", "h_up", "h_down", "h_gate_s", "h_up_s", "h_down_s", "h_shared_gate", "h_shared_gate_w",
+                                  "h_shared_up_w", "h_shared_down_w", "h_shared_gate_s", "h_shared_up_s", "h_shared_down_s")]
 
 
 # name -> (restype, argtypes); every symbol include/pooled_attn.h declares
@@ -81,6 +97,19 @@ SYMBOLS = {
     "pa_rmsnorm_f16": (c_int, [vp, f32p, u32, f32p, u32, u32, vp, u32]),
     "pa_gemm": (c_int, [vp, vp, vp, u32, u32, f32p, u32, c_int]),
     "pa_attn_layer_prefill": (c_int, [vp, u32, vp, vp, f32p, f32p, f32p, f32p, u32, u32, u32]),
+    "pa_delta_create": (c_int, [vp, ctypes.POINTER(PaDeltaConfig), ctypes.POINTER(vp)]),
+    "pa_delta_destroy": (c_int, [vp, vp]),
+    "pa_delta_reset": (c_int, [vp, vp, u32]),
+    "pa_delta_read": (c_int, [vp, vp, u32, c_int, vp]),
+    "pa_delta_write": (c_int, [vp, vp, u32, c_int, vp]),
+    "pa_delta_state_bytes": (ctypes.c_size_t, [vp, c_int]),
+    "pa_delta_state_ptr": (vp, [vp, u32, c_int]),
+    "pa_delta_glue": (c_int, [vp, vp, u32, f32p, u32, f32p, f32p, f32p, f32p, u32, f32p, f32p, u32, u32, f32p, u32, f32p, f32p, u32]),
+    "pa_delta_decode": (c_int, [vp, vp, u32, f32p, u32, f32p, u32, f32p, u32, f32p, f32p, u32, u32, u32, vp, u32, c_int]),
+    "pa_delta_prefill": (c_int, [vp, vp, u32, f32p, u32, f32p, u32, f32p, u32, f32p, f32p, u32, u32, vp, u32, c_int]),
+    "pa_moe_create": (c_int, [vp, ctypes.POINTER(PaMoeConfig), ctypes.POINTER(PaMoePlanes), ctypes.POINTER(vp)]),
+    "pa_moe_destroy": (c_int, [vp, vp]),
+    "pa_moe_layer": (c_int, [vp, vp, f32p, f32p, u32, u32, f32p, u32, vp, f32p]),
     "pa_version": (ctypes.c_char_p, []),
 }
 
@@ -164,6 +193,11 @@ class PooledAttn:
             for w in getattr(self, "_weights", []):
                 self.L.pa_weight_destroy(self.ctx, w)
             self._weights = []
+            for d in getattr(self, "_deltas", []):
+                self.L.pa_delta_destroy(self.ctx, d)
+            for m in getattr(self, "_moes", []):
+                self.L.pa_moe_destroy(self.ctx, m)
+            self._deltas, self._moes = [], []
             for b in self._bufs:
                 b.free()
             self._bufs = []
@@ -359,6 +393,103 @@ class PooledAttn:
     def attn_layer_prefill(self, layer, w_qkv, w_o, d_attn_norm_w, d_qw, d_kw, d_x, x_stride, base_pos, n_cols):
         self._chk(self.L.pa_attn_layer_prefill(self.ctx, layer, w_qkv, w_o, d_attn_norm_w.ptr, d_qw.ptr if d_qw else None,
                                                d_kw.ptr if d_kw else None, d_x.ptr, x_stride, base_pos, n_cols))
+
+    # ---- the gated delta rule ----
+    def delta(self, cfg):
+        """A handle with the states of n_layers layers.  cfg keys: n_k_heads, n_v_heads, head_k, head_v, conv_width (0: no pre-step), n_layers, scale
+        (0: 1 / sqrt(head_k)), eps, l2norm."""
+        c = PaDeltaConfig(cfg["n_k_heads"], cfg["n_v_heads"], cfg["head_k"], cfg["head_v"], cfg.get("conv_width", 0), cfg.get("n_layers", 1),
+                          cfg.get("scale", 0.0), cfg.get("eps", 1e-6), PA_DELTA_L2NORM if cfg.get("l2norm", True) else 0)
+        h = vp()
+        self._chk(self.L.pa_delta_create(self.ctx, ctypes.byref(c), ctypes.byref(h)))
+        if not hasattr(self, "_deltas"):
+            self._deltas = []
+        self._deltas.append(h)
+        return h
+
+    def delta_destroy(self, dn):
+        self._chk(self.L.pa_delta_destroy(self.ctx, dn))
+        self._deltas = [d for d in self._deltas if d is not dn]
+
+    def delta_reset(self, dn, layer):
+        self._chk(self.L.pa_delta_reset(self.ctx, dn, layer))
+
+    def delta_read(self, dn, layer, which):
+        """A layer's state, f32, flat: which 0 = [n_v_heads, head_v, head_k], 1 = the convolution's inputs [conv_width - 1, channels]."""
+        out = np.empty(self.L.pa_delta_state_bytes(dn, which) // 4, np.float32)
+        self._chk(self.L.pa_delta_read(self.ctx, dn, layer, which, out.ctypes.data))
+        return out
+
+    def delta_write(self, dn, layer, which, state):
+        a = np.ascontiguousarray(state, dtype=np.float32)
+        if a.nbytes != self.L.pa_delta_state_bytes(dn, which):
+            raise ValueError("delta_write: %d bytes for a state of %d" % (a.nbytes, self.L.pa_delta_state_bytes(dn, which)))
+        self._chk(self.L.pa_delta_write(self.ctx, dn, layer, which, a.ctypes.data))
+
+    def delta_state_ptr(self, dn, layer, which):
+        return self.L.pa_delta_state_ptr(dn, layer, which)
+
+    def delta_glue(self, dn, layer, d_qkv, qkv_stride, d_conv_w, d_conv_b, d_a, d_b, ab_stride, d_a_log, d_dt_bias, n_cols, n_commit, d_out, out_stride,
+                   d_g, d_beta, gate_stride):
+        self._chk(self.L.pa_delta_glue(self.ctx, dn, layer, d_qkv.ptr, qkv_stride, d_conv_w.ptr, d_conv_b.ptr if d_conv_b else None, d_a.ptr, d_b.ptr, ab_stride,
+                                       d_a_log.ptr, d_dt_bias.ptr, n_cols, n_commit, d_out.ptr, out_stride, d_g.ptr, d_beta.ptr, gate_stride))
+
+    def delta_decode(self, dn, layer, d_q, q_stride, d_k, k_stride, d_v, v_stride, d_g, d_beta, gate_stride, n_cols, n_commit, d_out, out_stride, out_dtype=PA_OUT_F32):
+        self._chk(self.L.pa_delta_decode(self.ctx, dn, layer, d_q.ptr if d_q else None, q_stride, d_k.ptr, k_stride, d_v.ptr, v_stride, d_g.ptr, d_beta.ptr, gate_stride,
+                                         n_cols, n_commit, d_out.ptr if d_out else None, out_stride, out_dtype))
+
+    def delta_prefill(self, dn, layer, d_q, q_stride, d_k, k_stride, d_v, v_stride, d_g, d_beta, gate_stride, n_cols, d_out, out_stride, out_dtype=PA_OUT_F32):
+        self._chk(self.L.pa_delta_prefill(self.ctx, dn, layer, d_q.ptr if d_q else None, q_stride, d_k.ptr, k_stride, d_v.ptr, v_stride, d_g.ptr, d_beta.ptr, gate_stride,
+                                          n_cols, d_out.ptr if d_out else None, out_stride, out_dtype))
+
+    # ---- mixture of experts ----
+    def moe(self, cfg, router, experts, shared=None):
+        """Upload a layer's experts.  cfg keys: dim, ffn, n_experts, top_k, kind (PA_W_*), norm_topk.  router f32 [n_experts, dim]; experts: dict of
+        gate, up [n_experts, ffn, dim], down [n_experts, dim, ffn] planes and their scales gate_s, up_s, down_s (f16 bits; None for f32 weights), in
+        weight()'s formats; shared: the same of one expert, with weight f32 [dim] of its gate, or None."""
+        kind, dim, ffn, n = cfg["kind"], cfg["dim"], cfg["ffn"], cfg["n_experts"]
+        keep = []
+
+        def plane(a, values, scales=False):
+            if a is None:
+                return None
+            want = values // 32 * 2 if scales else values * 4 if kind == PA_W_F32 else values if kind == PA_W_Q8_0 else values // 2
+            a = np.ascontiguousarray(a)
+            if a.nbytes != want:
+                raise ValueError("moe: a plane of %d bytes where %d are needed" % (a.nbytes, want))
+            keep.append(a)
+            return a.ctypes.data
+
+        def f32(a, count):
+            a = np.ascontiguousarray(a, dtype=np.float32)
+            if a.size != count:
+                raise ValueError("moe: %d values where %d are needed" % (a.size, count))
+            keep.append(a)
+            return a.ctypes.data
+        c = PaMoeConfig(dim, ffn, n, cfg["top_k"], kind, (PA_MOE_NORM_TOPK if cfg.get("norm_topk", True) else 0) | (PA_MOE_SHARED if shared is not None else 0))
+        pl = PaMoePlanes(h_router=f32(router, n * dim))
+        for name in ("gate", "up", "down"):
+            setattr(pl, "h_" + name, plane(experts[name], n * dim * ffn))
+            setattr(pl, "h_%s_s" % name, plane(experts.get(name + "_s"), n * dim * ffn, True))
+            if shared is not None:
+                setattr(pl, "h_shared_%s_w" % name, plane(shared[name], dim * ffn))
+                setattr(pl, "h_shared_%s_s" % name, plane(shared.get(name + "_s"), dim * ffn, True))
+        if shared is not None:
+            pl.h_shared_gate = f32(shared["weight"], dim)
+        h = vp()
+        self._chk(self.L.pa_moe_create(self.ctx, ctypes.byref(c), ctypes.byref(pl), ctypes.byref(h)))
+        if not hasattr(self, "_moes"):
+            self._moes = []
+        self._moes.append(h)
+        return h
+
+    def moe_destroy(self, moe):
+        self._chk(self.L.pa_moe_destroy(self.ctx, moe))
+        self._moes = [m for m in self._moes if m is not moe]
+
+    def moe_layer(self, moe, d_norm_w, d_x, x_stride, n_cols, d_y, y_stride, d_ids=None, d_weights=None):
+        self._chk(self.L.pa_moe_layer(self.ctx, moe, d_norm_w.ptr if d_norm_w else None, d_x.ptr, x_stride, n_cols, d_y.ptr, y_stride,
+                                      d_ids.ptr if d_ids else None, d_weights.ptr if d_weights else None))
 
     # ---- numpy convenience used by tests / smoke: whole passes from host arrays ----
     def run_glue_kv(self, layer, q_in, k_in, v_in, qw, kw, base_pos):
