@@ -238,9 +238,10 @@ class _Buf:
 
 
 class _Memory:
-    """Device memory of a handle as torch sees it."""
+    """Device memory of a handle as torch sees it; keeps the context alive as long as a view of it lives."""
 
-    def __init__(self, ptr, shape):
+    def __init__(self, pa, ptr, shape):
+        self.pa = pa
         self.__cuda_array_interface__ = dict(shape=shape, typestr="<f4", data=(ptr, False), version=2)
 
 
@@ -281,7 +282,7 @@ def _prepare_own(st):
     h, L = HEADS[case["heads"]], case["layers"]
     dn = st["dn"] = pa.delta(dict(n_k_heads=h["nk"], n_v_heads=h["nv"], head_k=h["hk"], head_v=h["hv"], conv_width=case.get("width", 0), n_layers=L, eps=L2_EPS, l2norm=True))
     which = 1 if case["op"] == "glue" else 0
-    states = [torch.as_tensor(_Memory(pa.delta_state_ptr(dn, l, which), tuple(d["state"][l].shape)), device="cuda") for l in range(L)]
+    states = [torch.as_tensor(_Memory(pa, pa.delta_state_ptr(dn, l, which), tuple(d["state"][l].shape)), device="cuda") for l in range(L)]
     st["out"], st["bufs"] = [], []
     for l in range(L):
         states[l].copy_(d["state"][l])
