@@ -9,6 +9,9 @@
 // in the last-level cache between them, and the workspace does not grow with the prompt
 #define SEGMENT_COLS 2048u
 
+// which form serves a prefill call
+static bool chunked(uint32_t n_cols) { return n_cols >= 48; }
+
 extern "C" int pa_delta_destroy(pa_ctx* ctx, pa_delta* dn) {
   if (!ctx) return PA_ERR_INVALID;
   if (!dn) return PA_OK;
@@ -47,6 +50,7 @@ extern "C" int pa_delta_create(pa_ctx* ctx, const pa_delta_config* cfg, pa_delta
   dn->ws_chunks = (std::min(ctx->cfg.max_cols, SEGMENT_COLS) + 63) / 64;
   hipError_t e = hipMalloc((void**)&dn->state, sbytes);
   if (e == hipSuccess && cbytes) e = hipMalloc((void**)&dn->conv, cbytes);
+  if (e == hipSuccess && chunked(ctx->cfg.max_cols)) e = hipMalloc(&dn->ws, pa_delta_chunk_ws_bytes(dn->ws_chunks, c.n_k_heads, c.n_v_heads, c.head_k));
   if (e == hipSuccess) e = pa_launch_fill_zero(dn->state, sbytes / 4, ctx->stream);
   if (e == hipSuccess && cbytes) e = pa_launch_fill_zero(dn->conv, cbytes / 4, ctx->stream);
   if (e == hipSuccess) e = hipStreamSynchronize(ctx->stream);
@@ -198,6 +202,6 @@ extern "C" int pa_delta_prefill(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const
   int rc = rule_params(ctx, who, dn, layer, d_q, q_stride, d_k, k_stride, d_v, v_stride, d_g, d_beta, gate_stride, n_cols, n_cols, d_out, out_stride, out_dtype, p);
   if (rc) return rc;
   DeviceGuard on(ctx->device);
-  const hipError_t e = pa_launch_delta_step(p, ctx->stream);
+  const hipError_t e = chunked(n_cols) ? pa_launch_delta_chunks(p, dn->ws, dn->ws_chunks, ctx->stream) : pa_launch_delta_step(p, ctx->stream);
   return e == hipSuccess ? PA_OK : block_fail_hip(ctx, e, who);
 }
