@@ -39,7 +39,7 @@ struct DeltaGlueParams {
 
 hipError_t pa_launch_delta_step(const DeltaParams& p, hipStream_t s);
 // in chunks, all columns committed; ws: pa_delta_chunk_ws_bytes(ws_chunks, ..) bytes
-hipError_t pa_launch_delta_chunks(const DeltaParams& p, void* ws, uint32_t ws_chunks, hipStream_t s);
+hipError_t pa_launch_delta_chunks(const DeltaParams& p, void* ws, uint32_t ws_chunks, int n_cu, hipStream_t s);
 size_t pa_delta_chunk_ws_bytes(uint32_t chunks, uint32_t nk, uint32_t nv, uint32_t hk);
 hipError_t pa_launch_delta_glue(const DeltaGlueParams& p, hipStream_t s);
 hipError_t pa_launch_fill_zero(float* p, size_t n, hipStream_t s);

@@ -26,6 +26,7 @@
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 #define CHUNK 64
@@ -59,6 +60,39 @@ static __device__ inline void split(float x, _Float16& hi, _Float16& lo) {
   lo = (_Float16)((x - (float)hi) * LO_SCALE);
 }
 struct Pair8 { h8 hi, lo; };
+struct Pair4 { h4 hi, lo; };
+// two values at a time: the high halves by one packed conversion, the low ones by a multiply-add each that takes the stored high half as it is
+static __device__ inline void split2(float x0, float x1, h2& hi, h2& lo) {
+  asm("" : "+v"(x0), "+v"(x1));      // f32 numbers as they are: fused into the product that made them, the high half would be rounded once here and twice there
+  uint32_t b;
+  const h2 h = {(_Float16)x0, (_Float16)x1};
+  __builtin_memcpy(&b, &h, 4);
+  asm("" : "+v"(b));
+  __builtin_memcpy(&hi, &b, 4);
+  lo = h2{(_Float16)__builtin_fmaf((float)hi[0], -LO_SCALE, x0 * LO_SCALE), (_Float16)__builtin_fmaf((float)hi[1], -LO_SCALE, x1 * LO_SCALE)};
+}
+static __device__ inline Pair4 split4(const f4 x) {
+  h2 h0, h1, l0, l1;
+  split2(x[0], x[1], h0, l0); split2(x[2], x[3], h1, l1);
+  return {h4{h0[0], h0[1], h1[0], h1[1]}, h4{l0[0], l0[1], l1[0], l1[1]}};
+}
+// buffers: a base in scalar registers, one vector offset for all fragments of a lane, reads past the end are zero and writes dropped
+static __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00020000); }
+static __device__ inline f4 load_f4(__amdgpu_buffer_rsrc_t b, uint32_t at, uint32_t base) {
+  const auto v = __builtin_amdgcn_raw_buffer_load_b128(b, (int)at, (int)base, 0);
+  f4 r; __builtin_memcpy(&r, &v, 16); return r;
+}
+static __device__ inline h8 load_h8(__amdgpu_buffer_rsrc_t b, uint32_t at, uint32_t base) {
+  const auto v = __builtin_amdgcn_raw_buffer_load_b128(b, (int)at, (int)base, 0);
+  h8 r; __builtin_memcpy(&r, &v, 16); return r;
+}
+static __device__ inline float load_f1(__amdgpu_buffer_rsrc_t b, uint32_t at, uint32_t base) { return __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(b, (int)at, (int)base, 0)); }
+static __device__ inline void store_f32(__amdgpu_buffer_rsrc_t b, uint32_t at, float x) { __builtin_amdgcn_raw_buffer_store_b32(__float_as_uint(x), b, (int)at, 0, 0); }
+static __device__ inline void store_f16(__amdgpu_buffer_rsrc_t b, uint32_t at, float x) {
+  const _Float16 h = (_Float16)x;
+  uint16_t u; __builtin_memcpy(&u, &h, 2);
+  __builtin_amdgcn_raw_buffer_store_b16(u, b, (int)at, 0, 0);
+}
 static __device__ inline Pair8 split8(const float (&x)[8]) {
   Pair8 r;
 #pragma unroll
@@ -398,253 +432,373 @@ void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
 }
 
 // ---- 2: from chunk to chunk -------------------------------------------------------------------------
-template <int HK>
-__global__ __launch_bounds__(256)
-void pa_delta_scan_kernel(DeltaParams p, DeltaWs ws) {
+// A workgroup has the state of NT x 16 value columns of a head and twelve wavefronts of three roles.  In a chunk's first phase the four KEYS multiply K by S and make X; in the second the
+// four of STATE multiply K'^T by X and move the state on; each requests its operands while the other works, two chunks ahead.  The four QUERIES, which nothing waits for, multiply Q by S
+// and P' by X.  Two barriers a chunk: S is there | X is there.  Every role has a loop of its own, unrolled by two: no register that a load is still filling is ever
+// copied, and no wait is shared.
+//
+// Scales: E_c is the exponent, per value column, that X of chunk c and the state behind it are scaled by.  It comes from the sums N_c of |S| in front of the chunk before and the
+// sums V of beta |v|: |S| in front of chunk c <= N_(c-1) + V_(c-1), so that KEYS find it a chunk ahead (sums of magnitudes are no smaller than norms, and they neither over- nor
+// underflow before their terms do).  NO_SCALE in its place sends the chunk the slow way.
+enum { KEYS, STATE, QUERIES };
+#define NO_SCALE 10000
+
+template <int HK, int NT> struct ScanLds {
+  static constexpr int KS = HK / 32, MT = HK / 64, COLS = 16 * NT;
+  _Float16 S[NT][2][KS * 512], X[NT][2][2 * 512];                  // pairs, as right operands
+  f4 bv[2][NT][4 * 64], cv[2][16];                                 // beta v, beta e^G of a chunk and the next, in the order of KEYS' lanes
+  f4 norm[2][COLS], val[2][COLS];                                  // N and V, by wavefront
+  int exps[2][COLS];
+  float slow[2][2][4][COLS];
+};
+static __device__ inline float sum4(const f4 x) { return (x[0] + x[1]) + (x[2] + x[3]); }
+static __device__ inline float sum_abs4(const f4 x) { return (fabsf(x[0]) + fabsf(x[1])) + (fabsf(x[2]) + fabsf(x[3])); }
+
+template <int HK, int NT, int ROLE>
+static __device__ __attribute__((always_inline)) void scan_role(const DeltaParams& p, const DeltaWs& ws, ScanLds<HK, NT>& L, const uint32_t w) {
   using F = Frags<HK>;
-  constexpr int KS = F::KS, MW = HK / 64;                          // MW: tiles of 16 state rows (key dimensions) of a wavefront
-  __shared__ __attribute__((aligned(16))) _Float16 Sl[2][KS * 512], Xl[2][2 * 512];
-  __shared__ float norm_s[4][16], value_s[4][16], slow_s[2][2][4][16];
-  const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lg = lane >> 4;
-  const uint32_t h = blockIdx.x % p.nv, v0 = blockIdx.x / p.nv * 16, kh = h / p.group;
-  const uint32_t chunks = (p.n + CHUNK - 1) / CHUNK;
+  using LD = ScanLds<HK, NT>;
+  constexpr int KS = LD::KS, MT = LD::MT, COLS = LD::COLS;
+  const uint32_t tid = threadIdx.x, lane = tid & 63, l16 = lane & 15, lg = lane >> 4;
+  const uint32_t h = blockIdx.x % p.nv, v0 = blockIdx.x / p.nv * COLS, kh = h / p.group;
+  const uint32_t chunks = (p.n + CHUNK - 1) / CHUNK, last = chunks - 1;
   const bool out = p.out != nullptr;
+  const uint32_t ot = p.out_f16 ? 2 : 4;
+  const float* const scal = ws.scal + (size_t)h * SCAL_FLOATS;
+  const size_t scal_step = (size_t)p.nv * SCAL_FLOATS;
+  auto rows_of = [&](uint32_t c) { return min((uint32_t)CHUNK, p.n - c * CHUNK); };
 
-  // state rows 16 (wave MW + x) + 4 lg + r of value column v0 + l16
-  float* const sp = p.state + ((size_t)h * p.hv + v0 + l16) * HK + wave * MW * 16 + 4 * lg;
-  f4 S[MW];
+  // ---- state rows 16 (w MT + m) + 4 lg + r of value columns v0 + 16 t + l16
+  f4 S[NT][MT];
+  float* const sp = p.state + ((size_t)h * p.hv + v0 + l16) * HK + w * MT * 16 + 4 * lg;
+  if constexpr (ROLE == STATE) {
 #pragma unroll
-  for (int x = 0; x < MW; x++) S[x] = *(const f4*)(sp + 16 * x);
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int m = 0; m < MT; m++) S[t][m] = *(const f4*)(sp + t * 16 * HK + m * 16);
+  }
 
-  // Operands of the wavefront, requested a chunk ahead.  The last chunk requests itself again instead of branching round the loads: a short conditional block between a matrix
+  // ---- requests.  Past the last chunk the last one's is made again instead of branching round the loads: a short conditional block between a matrix
   // instruction and the first use of its result makes this compiler (22.0.0git, ROCm 7.2.0) leave out the wait states on the path round the block, and the use then reads the old
-  // registers (seen as states 1e-4 off after a last chunk).
-  h8 kf[KS][2], qf[KS][2], pf[2][2], tf[MW][2][2];
-  struct Rows { f4 sb, sc, se, sq, v; float decay, kscale; uint32_t mark; } now, next;
-  auto load_k = [&](uint32_t c) {
-    const _Float16* b = ws.kq + ((size_t)c * p.nk + kh) * 2 * F::KQ + wave * KS * 512 + lane * 8;
+  // registers (seen as states 1e-4 off after a last chunk).  No dword is loaded that is not used: its register would be taken for something else, and that would wait for the load.
+  // Rows behind the last column read as zero and are not written: the buffers end with the last column.
+  struct KF { h8 x[KS][2]; };
+  struct GF { h8 x[MT][2][2]; };
+  struct PF { h8 x[2][2]; };
+  struct StateRows { f4 a, b, v[NT]; float decay, kscale; };       // beta, beta e^G, values
+  struct QueryRows { f4 a, b; };                                   // e^G, factor of the output
+  const uint32_t at = lane * 16;
+  auto load_k = [&](KF& d, uint32_t c) __attribute__((always_inline)) {
+    const auto b = buffer(ws.kq + (((size_t)min(c, last) * p.nk + kh) * 2 + (ROLE == QUERIES ? 1 : 0)) * F::KQ, F::KQ * 2);
 #pragma unroll
-    for (int s = 0; s < KS; s++) { kf[s][0] = *(const h8*)(b + s * 512); kf[s][1] = *(const h8*)(b + F::KQ / 2 + s * 512); }
+    for (int s = 0; s < KS; s++)
+#pragma unroll
+      for (int e = 0; e < 2; e++) d.x[s][e] = load_h8(b, at + s * 1024, w * KS * 1024 + e * F::KQ);
   };
-  auto load_q = [&](uint32_t c) {
-    const _Float16* b = ws.kq + ((size_t)c * p.nk + kh) * 2 * F::KQ + F::KQ + wave * KS * 512 + lane * 8;
+  auto load_g = [&](GF& d, uint32_t c) __attribute__((always_inline)) {
+    const auto b = buffer(ws.kt + ((size_t)min(c, last) * p.nv + h) * F::KT, F::KT * 2);
 #pragma unroll
-    for (int s = 0; s < KS; s++) { qf[s][0] = *(const h8*)(b + s * 512); qf[s][1] = *(const h8*)(b + F::KQ / 2 + s * 512); }
+    for (int m = 0; m < MT; m++)
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+#pragma unroll
+        for (int e = 0; e < 2; e++) d.x[m][s][e] = load_h8(b, at + s * 1024, (w * MT + m) * 2048 + e * F::KT);
   };
-  auto load_t = [&](uint32_t c) {
-    const _Float16* b = ws.kt + ((size_t)c * p.nv + h) * F::KT + wave * MW * 2 * 512 + lane * 8;
+  auto load_p = [&](PF& d, uint32_t c) __attribute__((always_inline)) {
+    const auto b = buffer(ws.pp + ((size_t)min(c, last) * p.nv + h) * F::P, F::P * 2);
 #pragma unroll
-    for (int x = 0; x < MW; x++)
+    for (int s = 0; s < 2; s++)
 #pragma unroll
-      for (int s = 0; s < 2; s++) { tf[x][s][0] = *(const h8*)(b + (x * 2 + s) * 512); tf[x][s][1] = *(const h8*)(b + F::KT / 2 + (x * 2 + s) * 512); }
+      for (int e = 0; e < 2; e++) d.x[s][e] = load_h8(b, at + s * 1024, w * 2048 + e * F::P);
   };
-  auto load_p = [&](uint32_t c) {
-    const _Float16* b = ws.pp + ((size_t)c * p.nv + h) * F::P + wave * 2 * 512 + lane * 8;
+  uint32_t row_at[4];                                              // STATE: of the values, QUERIES: of the output
+  if constexpr (ROLE != KEYS) {
 #pragma unroll
-    for (int s = 0; s < 2; s++) { pf[s][0] = *(const h8*)(b + s * 512); pf[s][1] = *(const h8*)(b + F::P / 2 + s * 512); }
+    for (int r = 0; r < 4; r++) row_at[r] = (w * 16 + 4 * lg + r) * (ROLE == STATE ? p.v_stride * 4 : p.out_stride * ot) + l16 * (ROLE == STATE ? 4 : ot);
+  }
+  const uint32_t gate_at = (w * 16 + 4 * lg) * 4;
+  auto load_rows = [&](StateRows& d, uint32_t c) __attribute__((always_inline)) {
+    c = min(c, last);
+    const auto b = buffer(scal + c * scal_step, SCAL_FLOATS * 4);
+    const auto x = buffer(p.v + (size_t)c * CHUNK * p.v_stride + (size_t)h * p.hv + v0, ((rows_of(c) - 1) * p.v_stride + COLS) * 4);
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) d.v[t][r] = load_f1(x, row_at[r] + t * 64, 0);
+    d.a = load_f4(b, gate_at, 0); d.b = load_f4(b, gate_at, 256);
+    d.decay = load_f1(b, 0, SCAL_DECAY * 4); d.kscale = load_f1(b, 0, SCAL_KSCALE * 4);
   };
-  auto load_rows = [&](uint32_t c) {                               // the wavefront's 16 rows of values, and their gates
-    const uint32_t i0 = c * CHUNK + wave * 16 + 4 * lg;
-    const float* sg = ws.scal + ((size_t)c * p.nv + h) * SCAL_FLOATS;
-    Rows w;
-#pragma unroll
-    for (int r = 0; r < 4; r++) w.v[r] = i0 + r < p.n ? p.v[(size_t)(i0 + r) * p.v_stride + (size_t)h * p.hv + v0 + l16] : 0.f;
-    w.sb = *(const f4*)(sg + wave * 16 + 4 * lg);
-    w.sc = *(const f4*)(sg + 64 + wave * 16 + 4 * lg);
-    w.se = *(const f4*)(sg + 128 + wave * 16 + 4 * lg);
-    w.sq = *(const f4*)(sg + 192 + wave * 16 + 4 * lg);
-    w.decay = sg[SCAL_DECAY]; w.kscale = sg[SCAL_KSCALE]; w.mark = __float_as_uint(sg[SCAL_MARK]);
-    return w;
+  auto load_query_rows = [&](QueryRows& d, uint32_t c) __attribute__((always_inline)) {
+    const auto b = buffer(scal + min(c, last) * scal_step, SCAL_FLOATS * 4);
+    d.a = load_f4(b, gate_at, 512); d.b = load_f4(b, gate_at, 768);
   };
-  // S as pairs scaled by `sigma`, its column sums |S| (no smaller than the norm, and they neither over- nor underflow before their terms do) and the
-  // coming chunk's sums of beta |v|, for everyone
-  auto publish = [&](float sigma, const Rows& w) {
-    float ss = 0.f, sv = 0.f;
+  auto load_mark = [&](uint32_t c) __attribute__((always_inline)) { return load_f1(buffer(scal + min(c, last) * scal_step, SCAL_FLOATS * 4), 0, SCAL_MARK * 4); };
+
+  // ---- what STATE and KEYS leave for the others
+  auto put_norm = [&](uint32_t c) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < MW; x++) {
-      h4 hi, lo;
+    for (int t = 0; t < NT; t++) {
+      float x = 0.f;
 #pragma unroll
-      for (int r = 0; r < 4; r++) {
-        ss += fabsf(S[x][r]);
-        _Float16 a, b;
-        split(S[x][r] * sigma, a, b);
-        hi[r] = a; lo[r] = b;
-      }
-      const uint32_t d0 = (wave * MW + x) * 16 + 4 * lg, off = (d0 >> 5) * 512 + (l16 + 16 * ((d0 & 31) >> 3)) * 8 + (d0 & 7);
-      *(h4*)(&Sl[0][off]) = hi; *(h4*)(&Sl[1][off]) = lo;
+      for (int m = 0; m < MT; m++) x += sum_abs4(S[t][m]);
+      x = rows4_sum(x);
+      if (lg == 0) L.norm[c & 1][t * 16 + l16][w] = x;
     }
+  };
+  auto put_state = [&](const float (&to)[NT]) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < 4; r++) sv += fabsf(w.sb[r] * w.v[r]);
-    ss = rows4_sum(ss); sv = rows4_sum(sv);
-    if (lg == 0) { norm_s[wave][l16] = ss; value_s[wave][l16] = sv; }
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int m = 0; m < MT; m++) {
+        const Pair4 s = split4(S[t][m] * to[t]);
+        const uint32_t d0 = (w * MT + m) * 16 + 4 * lg, off = (d0 >> 5) * 512 + (l16 + 16 * ((d0 & 31) >> 3)) * 8 + (d0 & 7);
+        *(h4*)(&L.S[t][0][off]) = s.hi; *(h4*)(&L.S[t][1][off]) = s.lo;
+      }
+  };
+  auto put_rows = [&](const StateRows& d, uint32_t c) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const f4 x = d.a * d.v[t];
+      L.bv[c & 1][t][w * 64 + lane] = x;
+      const float y = rows4_sum(sum_abs4(x));
+      if (lg == 0) L.val[c & 1][t * 16 + l16][w] = y;
+    }
+    if (l16 == 0) L.cv[c & 1][w * 4 + lg] = d.b;
+  };
+  auto put_exponent = [&](uint32_t c, bool fresh, float mark) __attribute__((always_inline)) {      // E_c; fresh: the sums of |S| in front of chunk c itself are there
+    const bool marked = __builtin_amdgcn_readfirstlane(__float_as_uint(mark)) != 0;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const float before = fresh ? sum4(L.norm[c & 1][t * 16 + l16]) : 1.01f * (sum4(L.norm[(c - 1) & 1][t * 16 + l16]) + sum4(L.val[(c - 1) & 1][t * 16 + l16]));
+      const float bound = 1.02f * __builtin_fmaf(2.1f, before, sum4(L.val[c & 1][t * 16 + l16]));
+      const bool fine = !marked && (bound == 0.f || (bound >= 0x1p-90f && bound < 0x1p90f));
+      if (w == 0 && lg == 0) L.exps[c & 1][t * 16 + l16] = fine ? scale_exponent(bound) : NO_SCALE;
+    }
+  };
+  auto own_exponents = [&](uint32_t c, int (&e)[NT]) __attribute__((always_inline)) {               // of S in front of chunk c, from itself
+    if constexpr (ROLE == STATE) put_norm(c);
+    lds_barrier();
+#pragma unroll
+    for (int t = 0; t < NT; t++) e[t] = scale_exponent(sum4(L.norm[c & 1][t * 16 + l16]));
   };
 
-  now = load_rows(0);
-  load_k(0); load_t(0);
-  if (out) { load_q(0); load_p(0); }
-  // the first scale from S itself
-  float sigma = 1.f, sigma_inv = 1.f;
+  // ---- in front of the first chunk
+  KF k0, k1;
+  GF g0, g1;
+  PF p0;
+  StateRows rows1;                                                 // of the coming chunk
+  QueryRows q0, q1;
+  float m0 = 0.f, m1 = 0.f;
+  if constexpr (ROLE == KEYS) { m0 = load_mark(0); m1 = load_mark(1); load_k(k0, 0); load_k(k1, 1); }
+  if constexpr (ROLE == STATE) { load_rows(rows1, 0); load_g(g0, 0); put_rows(rows1, 0); }
+  if constexpr (ROLE == QUERIES) { load_query_rows(q0, 0); load_query_rows(q1, 1); load_k(k0, 0); load_p(p0, 0); }
+  float decay = 0.f, kscale = 0.f, next_decay = 0.f, next_kscale = 0.f;
+  if constexpr (ROLE == STATE) { decay = rows1.decay; kscale = rows1.kscale; load_rows(rows1, 1); }
+  float sigma_inv[NT];
   {
-    float ss = 0.f;
+    int e[NT];
+    float to[NT];
+    own_exponents(0, e);
 #pragma unroll
-    for (int x = 0; x < MW; x++)
-#pragma unroll
-      for (int r = 0; r < 4; r++) ss = fmaxf(ss, fabsf(S[x][r]));
-#pragma unroll
-    for (int o = 16; o < 64; o *= 2) ss = fmaxf(ss, __shfl_xor(ss, o));
-    if (lg == 0) norm_s[wave][l16] = ss;
-    lds_barrier();
-    const float m = fmaxf(fmaxf(norm_s[0][l16], norm_s[1][l16]), fmaxf(norm_s[2][l16], norm_s[3][l16]));
-    const int e = scale_exponent(m);
-    sigma = pow2(13 - e); sigma_inv = pow2(e - 13);
-    lds_barrier();
+    for (int t = 0; t < NT; t++) { sigma_inv[t] = pow2(e[t] - 13); to[t] = pow2(13 - e[t]); }
+    if constexpr (ROLE == STATE) put_state(to);
+    if constexpr (ROLE == KEYS) put_exponent(0, true, m0);
   }
-  publish(sigma, now);
 
-  for (uint32_t c = 0; c < chunks; c++) {
+  auto chunk = [&](const uint32_t c, KF& kf, GF& gf, GF& gf_next, QueryRows& qr, float& mark, const float mark_next) __attribute__((always_inline)) {
     lds_barrier();
-    // bound of X and of the next S, per column; a column that has none sends the chunk the slow way
-    const float bound = 1.02f * (2.1f * ((norm_s[0][l16] + norm_s[1][l16]) + (norm_s[2][l16] + norm_s[3][l16])) +
-                                 ((value_s[0][l16] + value_s[1][l16]) + (value_s[2][l16] + value_s[3][l16])));
-    const bool none = !(bound == 0.f || (bound >= 0x1p-90f && bound < 0x1p90f));
-    const uint32_t cn = min(c + 1, chunks - 1);
-    const int be = scale_exponent(bound);
-    const float to = pow2(13 - be), to_inv = pow2(be - 13);
-    next = load_rows(cn);
-    if (!now.mark && !__any(none)) {
-      // R = K S, X = beta v - beta e^G R
-      f4 r0 = {0.f, 0.f, 0.f, 0.f}, r1 = r0, o0 = r0, o1 = r0;
-      h8 sh[KS], sl[KS];
+    int e[NT];
+    bool none = false;
 #pragma unroll
-      for (int s = 0; s < KS; s++) { sh[s] = *(const h8*)(&Sl[0][s * 512 + lane * 8]); sl[s] = *(const h8*)(&Sl[1][s * 512 + lane * 8]); }
+    for (int t = 0; t < NT; t++) { e[t] = L.exps[c & 1][t * 16 + l16]; none = none || e[t] == NO_SCALE; }
+    const bool slow = __any(none);
+    uint32_t rows = rows_of(c);
+    if (slow) {
+      // token by token, in f32: dot products over the key dimensions of the four wavefronts of STATE, one exchange each.  What the matrix instructions below make of this chunk is dropped.
+      const float* const sg = scal + c * scal_step;
+      for (uint32_t i = 0; i < rows; i++) {
+        const size_t col = (size_t)c * CHUNK + i;
+        f4 k[MT], q[MT];
+        if constexpr (ROLE == STATE) {
+          const float dec = expf(p.g[col * p.gate_stride + h]);
 #pragma unroll
-      for (int s = 0; s < KS; s++) mfma_pair(kf[s][0], kf[s][1], sh[s], sl[s], r0, r1);
-      load_k(cn);
-      {
-        h4 hi, lo;
+          for (int m = 0; m < MT; m++) {
+            const uint32_t d = kh * HK + (w * MT + m) * 16 + 4 * lg;
+            k[m] = *(const f4*)(p.k + col * p.k_stride + d) * sg[4 * 64 + i];
+            q[m] = out ? *(const f4*)(p.q + col * p.q_stride + d) * sg[5 * 64 + i] : k[m];
+          }
 #pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const float x = __builtin_fmaf(-now.sc[r], (r0[r] + r1[r] * LO_INV) * (sigma_inv * UNIT_INV), now.sb[r] * now.v[r]);
-          _Float16 a, b;
-          split(x * to, a, b);
-          hi[r] = a; lo[r] = b;
+          for (int t = 0; t < NT; t++) {
+            float a = 0.f;
+#pragma unroll
+            for (int m = 0; m < MT; m++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) { S[t][m][r] *= dec; a = __builtin_fmaf(S[t][m][r], k[m][r], a); }
+            a = rows4_sum(a);
+            if (lg == 0) L.slow[0][i & 1][w][t * 16 + l16] = a;
+          }
         }
-        const uint32_t i0 = wave * 16 + 4 * lg, off = (i0 >> 5) * 512 + (l16 + 16 * ((i0 & 31) >> 3)) * 8 + (i0 & 7);
-        *(h4*)(&Xl[0][off]) = hi; *(h4*)(&Xl[1][off]) = lo;
-      }
-      if (out) {
+        lds_barrier();
+        if constexpr (ROLE == STATE) {
+          const float b = p.beta[col * p.gate_stride + h];
 #pragma unroll
-        for (int s = 0; s < KS; s++) mfma_pair(qf[s][0], qf[s][1], sh[s], sl[s], o0, o1);
-        load_q(cn);
-      }
-      lds_barrier();
-      h8 xh[2], xl[2];
+          for (int t = 0; t < NT; t++) {
+            const auto& x = L.slow[0][i & 1];
+            const uint32_t j = t * 16 + l16;
+            const float u = b * (p.v[col * p.v_stride + (size_t)h * p.hv + v0 + j] - ((x[0][j] + x[1][j]) + (x[2][j] + x[3][j])));
+            float o = 0.f;
 #pragma unroll
-      for (int s = 0; s < 2; s++) { xh[s] = *(const h8*)(&Xl[0][s * 512 + lane * 8]); xl[s] = *(const h8*)(&Xl[1][s * 512 + lane * 8]); }
-      f4 n0[MW], n1[MW];
+            for (int m = 0; m < MT; m++)
 #pragma unroll
-      for (int x = 0; x < MW; x++) {
-        n0[x] = n1[x] = f4{0.f, 0.f, 0.f, 0.f};
+              for (int r = 0; r < 4; r++) { S[t][m][r] = __builtin_fmaf(u, k[m][r], S[t][m][r]); o = __builtin_fmaf(S[t][m][r], q[m][r], o); }
+            o = rows4_sum(o);
+            if (lg == 0) L.slow[1][i & 1][w][j] = o;
+          }
+        }
+        lds_barrier();
+        if constexpr (ROLE == QUERIES) {
+          if (out && w == 0 && lg == 0) {
 #pragma unroll
-        for (int s = 0; s < 2; s++) mfma_pair(tf[x][s][0], tf[x][s][1], xh[s], xl[s], n0[x], n1[x]);
-      }
-      load_t(cn);
-      const float back = to_inv * now.kscale;
-#pragma unroll
-      for (int x = 0; x < MW; x++)
-#pragma unroll
-        for (int r = 0; r < 4; r++) S[x][r] = __builtin_fmaf(S[x][r], now.decay, (n0[x][r] + n1[x][r] * LO_INV) * back);
-      publish(to, next);
-      if (out) {
-        f4 u0 = {0.f, 0.f, 0.f, 0.f}, u1 = u0;
-#pragma unroll
-        for (int s = 0; s < 2; s++) mfma_pair(pf[s][0], pf[s][1], xh[s], xl[s], u0, u1);
-        load_p(cn);
-        const uint32_t i0 = c * CHUNK + wave * 16 + 4 * lg;
-#pragma unroll
-        for (int r = 0; r < 4; r++) {
-          const float o = now.sq[r] * __builtin_fmaf(now.se[r], (o0[r] + o1[r] * LO_INV) * (sigma_inv * UNIT_INV), (u0[r] + u1[r] * LO_INV) * (to_inv * UNIT_INV));
-          if (i0 + r < p.n) {
-            const size_t at = (size_t)(i0 + r) * p.out_stride + (size_t)h * p.hv + v0 + l16;
-            if (p.out_f16) ((_Float16*)p.out)[at] = (_Float16)o; else ((float*)p.out)[at] = o;
+            for (int t = 0; t < NT; t++) {
+              const auto& x = L.slow[1][i & 1];
+              const uint32_t j = t * 16 + l16;
+              const float o = p.scale * ((x[0][j] + x[1][j]) + (x[2][j] + x[3][j]));
+              const size_t to = col * p.out_stride + (size_t)h * p.hv + v0 + j;
+              if (p.out_f16) ((_Float16*)p.out)[to] = (_Float16)o; else ((float*)p.out)[to] = o;
+            }
           }
         }
       }
-      sigma_inv = to_inv;
+      rows = 0;
+      own_exponents(c + 1, e);
+    }
+    float to[NT], to_inv[NT];
+#pragma unroll
+    for (int t = 0; t < NT; t++) { to[t] = pow2(13 - e[t]); to_inv[t] = pow2(e[t] - 13); }
+    f4 held[NT], fq;                                               // QUERIES: the start state's part of the output, all factors in
+    if constexpr (ROLE != STATE) {
+      f4 cv;
+      if constexpr (ROLE == KEYS) cv = L.cv[c & 1][w * 4 + lg];
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        f4 r0 = {0.f, 0.f, 0.f, 0.f}, r1 = r0, r2 = r0, r;
+#pragma unroll
+        for (int s = 0; s < KS; s++) {
+          const h8 sh = *(const h8*)(&L.S[t][0][s * 512 + lane * 8]), sl = *(const h8*)(&L.S[t][1][s * 512 + lane * 8]);
+          r0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.x[s][0], sh, r0, 0, 0, 0);
+          r1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.x[s][0], sl, r1, 0, 0, 0);
+          r2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.x[s][1], sh, r2, 0, 0, 0);
+        }
+        const float back = sigma_inv[t] * UNIT_INV;
+#pragma unroll
+        for (int i = 0; i < 4; i++) r[i] = __builtin_fmaf(r1[i] + r2[i], LO_INV, r0[i]) * back;
+        if constexpr (ROLE == KEYS) {                              // X = beta v - beta e^G K S
+          const f4 bv = L.bv[c & 1][t][w * 64 + lane];
+          f4 x;
+#pragma unroll
+          for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(-cv[i], r[i], bv[i]);
+          const Pair4 s = split4(x * to[t]);
+          const uint32_t i0 = w * 16 + 4 * lg, off = (i0 >> 5) * 512 + (l16 + 16 * ((i0 & 31) >> 3)) * 8 + (i0 & 7);
+          *(h4*)(&L.X[t][0][off]) = s.hi; *(h4*)(&L.X[t][1][off]) = s.lo;
+        } else {
+          held[t] = qr.b * (qr.a * r);
+        }
+      }
+      if constexpr (ROLE == QUERIES) { fq = qr.b; load_k(kf, c + 1); load_query_rows(qr, c + 2); }
     } else {
-      // token by token, in f32: dot products over the key dimensions of all four wavefronts, one exchange each
-      const float* const sg = ws.scal + ((size_t)c * p.nv + h) * SCAL_FLOATS;
-      const uint32_t rows = min((uint32_t)CHUNK, p.n - c * CHUNK);
-      for (uint32_t t = 0; t < rows; t++) {
-        const size_t col = (size_t)c * CHUNK + t;
-        const uint32_t d0 = kh * HK + wave * MW * 16 + 4 * lg;
-        const float ki = sg[4 * 64 + t], qi = sg[5 * 64 + t];
-        const float dec = expf(p.g[col * p.gate_stride + h]), b = p.beta[col * p.gate_stride + h], vt = p.v[col * p.v_stride + (size_t)h * p.hv + v0 + l16];
-        f4 k[MW];
-        float a = 0.f;
+      if constexpr (NT == 1) load_g(gf_next, c + 1);
+      put_rows(rows1, c + 1);
+      next_decay = rows1.decay; next_kscale = rows1.kscale;
+      load_rows(rows1, c + 2);
+    }
+    lds_barrier();
+    if constexpr (ROLE == KEYS) {
+      load_k(kf, c + 2);
+      mark = load_mark(c + 2);
+      put_exponent(c + 1, slow, mark_next);
+    } else {
+      f4 n[NT][MT];
 #pragma unroll
-        for (int x = 0; x < MW; x++) {
-          k[x] = *(const f4*)(p.k + col * p.k_stride + d0 + 16 * x) * ki;
+      for (int t = 0; t < NT; t++)
 #pragma unroll
-          for (int r = 0; r < 4; r++) { S[x][r] *= dec; a = __builtin_fmaf(S[x][r], k[x][r], a); }
-        }
-        a = rows4_sum(a);
-        if (lg == 0) slow_s[0][t & 1][wave][l16] = a;
-        lds_barrier();
-        const float u = b * (vt - ((slow_s[0][t & 1][0][l16] + slow_s[0][t & 1][1][l16]) + (slow_s[0][t & 1][2][l16] + slow_s[0][t & 1][3][l16])));
+        for (int m = 0; m < (ROLE == STATE ? MT : 1); m++) {
+          f4 n0 = {0.f, 0.f, 0.f, 0.f}, n1 = n0, n2 = n0;
 #pragma unroll
-        for (int x = 0; x < MW; x++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) S[x][r] = __builtin_fmaf(u, k[x][r], S[x][r]);
-        if (out) {
-          float o = 0.f;
-#pragma unroll
-          for (int x = 0; x < MW; x++) {
-            const f4 q = *(const f4*)(p.q + col * p.q_stride + d0 + 16 * x) * qi;
-#pragma unroll
-            for (int r = 0; r < 4; r++) o = __builtin_fmaf(S[x][r], q[r], o);
+          for (int s = 0; s < 2; s++) {
+            const h8 xh = *(const h8*)(&L.X[t][0][s * 512 + lane * 8]), xl = *(const h8*)(&L.X[t][1][s * 512 + lane * 8]);
+            const h8 ah = ROLE == STATE ? gf.x[m][s][0] : p0.x[s][0], al = ROLE == STATE ? gf.x[m][s][1] : p0.x[s][1];
+            n0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, xh, n0, 0, 0, 0);
+            n1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, xl, n1, 0, 0, 0);
+            n2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, xh, n2, 0, 0, 0);
           }
-          o = rows4_sum(o);
-          if (lg == 0) slow_s[1][t & 1][wave][l16] = o;
-          lds_barrier();
-          if (tid < 16) {
-            o = p.scale * ((slow_s[1][t & 1][0][l16] + slow_s[1][t & 1][1][l16]) + (slow_s[1][t & 1][2][l16] + slow_s[1][t & 1][3][l16]));
-            const size_t at = col * p.out_stride + (size_t)h * p.hv + v0 + l16;
-            if (p.out_f16) ((_Float16*)p.out)[at] = (_Float16)o; else ((float*)p.out)[at] = o;
+#pragma unroll
+          for (int i = 0; i < 4; i++) n[t][m][i] = __builtin_fmaf(n1[i] + n2[i], LO_INV, n0[i]);
+        }
+      if constexpr (ROLE == STATE) {
+        if constexpr (NT > 1) load_g(gf, c + 1);                   // no room for two chunks' operands
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          const float fs = to_inv[t] * kscale;
+#pragma unroll
+          for (int m = 0; m < MT; m++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+              const float x = __builtin_fmaf(S[t][m][i], decay, n[t][m][i] * fs);
+              S[t][m][i] = slow ? S[t][m][i] : x;
+            }
+        }
+        put_state(to);
+        put_norm(c + 1);
+        decay = next_decay; kscale = next_kscale;
+      } else {
+        const auto b = buffer((unsigned char*)p.out + ((size_t)c * CHUNK * p.out_stride + (size_t)h * p.hv + v0) * ot, out && rows ? ((rows - 1) * p.out_stride + COLS) * ot : 0);
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+          const f4 fx = fq * (to_inv[t] * UNIT_INV);
+          f4 o;
+#pragma unroll
+          for (int r = 0; r < 4; r++) o[r] = __builtin_fmaf(fx[r], n[t][0][r], held[t][r]);
+          if (p.out_f16) {
+#pragma unroll
+            for (int r = 0; r < 4; r++) store_f16(b, row_at[r] + t * 32, o[r]);
+          } else {
+#pragma unroll
+            for (int r = 0; r < 4; r++) store_f32(b, row_at[r] + t * 64, o[r]);
           }
         }
-      }
-      {
-        load_k(cn); load_t(cn);
-        if (out) { load_q(cn); load_p(cn); }
-        // a scale from S itself, as at the start
-        float m = 0.f;
-#pragma unroll
-        for (int x = 0; x < MW; x++)
-#pragma unroll
-          for (int r = 0; r < 4; r++) m = fmaxf(m, fabsf(S[x][r]));
-#pragma unroll
-        for (int o = 16; o < 64; o *= 2) m = fmaxf(m, __shfl_xor(m, o));
-        lds_barrier();                                             // everyone has read this chunk's norms
-        if (lg == 0) norm_s[wave][l16] = m;
-        lds_barrier();
-        m = fmaxf(fmaxf(norm_s[0][l16], norm_s[1][l16]), fmaxf(norm_s[2][l16], norm_s[3][l16]));
-        const int e = scale_exponent(m);
-        sigma = pow2(13 - e); sigma_inv = pow2(e - 13);
-        lds_barrier();
-        publish(sigma, next);
+        load_p(p0, c + 1);
       }
     }
-    now = next;
-  }
 #pragma unroll
-  for (int x = 0; x < MW; x++) *(f4*)(sp + 16 * x) = S[x];
+    for (int t = 0; t < NT; t++) sigma_inv[t] = to_inv[t];
+  };
+  for (uint32_t c = 0; c < chunks; c += 2) {
+    chunk(c, k0, g0, g1, q0, m0, m1);
+    if (c + 1 < chunks) chunk(c + 1, ROLE == QUERIES ? k0 : k1, NT > 1 ? g0 : g1, g0, q1, m1, m0);
+  }
+  if constexpr (ROLE == STATE) {
+#pragma unroll
+    for (int t = 0; t < NT; t++)
+#pragma unroll
+      for (int m = 0; m < MT; m++) *(f4*)(sp + t * 16 * HK + m * 16) = S[t][m];
+  }
+}
+
+template <int HK, int NT>
+__global__ __launch_bounds__(768)
+void pa_delta_scan_kernel(DeltaParams p, DeltaWs ws) {
+  __shared__ __attribute__((aligned(16))) ScanLds<HK, NT> lds;
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (wave < 4) scan_role<HK, NT, KEYS>(p, ws, lds, wave);
+  else if (wave < 8) scan_role<HK, NT, STATE>(p, ws, lds, wave - 4);
+  else scan_role<HK, NT, QUERIES>(p, ws, lds, wave - 8);
 }
 
 template <int HK>
-static hipError_t launch_chunks(const DeltaParams& p, void* mem, uint32_t ws_chunks, hipStream_t s) {
+static hipError_t launch_chunks(const DeltaParams& p, void* mem, uint32_t ws_chunks, int n_cu, hipStream_t s) {
   const DeltaWs ws = ws_at<HK>(mem, ws_chunks, p.nk, p.nv, nullptr);
   const uint32_t seg = ws_chunks * CHUNK;
+  const bool wide = p.hv % 32 == 0 && p.nv * (p.hv / 16) > (uint32_t)n_cu;
   for (uint32_t c0 = 0; c0 < p.n; c0 += seg) {
     DeltaParams r = p;
     r.n = std::min(seg, p.n - c0); r.commit = r.n;
@@ -652,11 +806,13 @@ static hipError_t launch_chunks(const DeltaParams& p, void* mem, uint32_t ws_chu
     r.g += (size_t)c0 * p.gate_stride; r.beta += (size_t)c0 * p.gate_stride;
     if (r.out) r.out = (unsigned char*)p.out + (size_t)c0 * p.out_stride * (p.out_f16 ? 2 : 4);
     hipLaunchKernelGGL(pa_delta_prep_kernel<HK>, dim3(p.nv, (r.n + CHUNK - 1) / CHUNK), dim3(256), 0, s, r, ws);
-    hipLaunchKernelGGL(pa_delta_scan_kernel<HK>, dim3(p.nv * (p.hv / 16)), dim3(256), 0, s, r, ws);
+    const dim3 threads(768);
+    if (wide) hipLaunchKernelGGL((pa_delta_scan_kernel<HK, 2>), dim3(p.nv * (p.hv / 32)), threads, 0, s, r, ws);
+    else hipLaunchKernelGGL((pa_delta_scan_kernel<HK, 1>), dim3(p.nv * (p.hv / 16)), threads, 0, s, r, ws);
   }
   return hipGetLastError();
 }
 
-hipError_t pa_launch_delta_chunks(const DeltaParams& p, void* ws, uint32_t ws_chunks, hipStream_t s) {
-  return p.hk == 64 ? launch_chunks<64>(p, ws, ws_chunks, s) : launch_chunks<128>(p, ws, ws_chunks, s);
+hipError_t pa_launch_delta_chunks(const DeltaParams& p, void* ws, uint32_t ws_chunks, int n_cu, hipStream_t s) {
+  return p.hk == 64 ? launch_chunks<64>(p, ws, ws_chunks, n_cu, s) : launch_chunks<128>(p, ws, ws_chunks, n_cu, s);
 }

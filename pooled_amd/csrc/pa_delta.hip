@@ -202,6 +202,7 @@ extern "C" int pa_delta_prefill(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const
   int rc = rule_params(ctx, who, dn, layer, d_q, q_stride, d_k, k_stride, d_v, v_stride, d_g, d_beta, gate_stride, n_cols, n_cols, d_out, out_stride, out_dtype, p);
   if (rc) return rc;
   DeviceGuard on(ctx->device);
-  const hipError_t e = chunked(n_cols) ? pa_launch_delta_chunks(p, dn->ws, dn->ws_chunks, ctx->stream) : pa_launch_delta_step(p, ctx->stream);
+  // (a chunk's rows of v and of the output are addressed with 32-bit offsets)
+  const hipError_t e = chunked(n_cols) && v_stride <= (1u << 22) && out_stride <= (1u << 22) ? pa_launch_delta_chunks(p, dn->ws, dn->ws_chunks, ctx->n_cu, ctx->stream) : pa_launch_delta_step(p, ctx->stream);
   return e == hipSuccess ? PA_OK : block_fail_hip(ctx, e, who);
 }
