@@ -9,12 +9,12 @@
 // a v head and 16 columns of its values, S in registers: per chunk K S, then X, then K'^T X, and beside them Q S and P' X.  Only decays between a
 // place and a later one occur, never their inverses, so nothing overflows however fast a head forgets; sums of g are kept in 64 bits, because their differences matter.
 //
-// Precision.  The results are f32 and stay as exact as f32 sums: every operand of the f16 matrix instructions is a pair hi + lo / 2048 of f16 values (22 bits), a product is
-// hi hi + (hi lo + lo hi) / 2048 (the dropped lo lo is 2^-22 of it), accumulated in f32.  A pair is exact to 2^-36 of the largest f16 power below it, so it needs operands of known size:
-// rows of q are scaled by a power of two to a norm in [0.5, 1), K' by one for its largest element, and S and X, per value column, by one from a bound: the rule over keys no longer than
-// one with 0 <= beta <= 2, g <= 0 is a contraction, so |S_next| <= |S| + sum beta |v| =: the bound of S_next, and 2 |S| + sum beta |v| that of X.  A chunk whose inputs leave that
-// domain (longer or tiny keys, other gates, infinities, NaN) is marked by the first kernel, or found by the bound, and runs token by token in the second, in f32, with the same
-// S: slower (about 1 us a token), but right for every input.
+// Precision.  The results are f32 and stay as exact as f32 sums: every operand of the f16 matrix instructions is a pair hi + lo of f16 values (22 bits), a product is
+// hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it), accumulated in f32.  A pair is exact to 22 bits down to 2^-3 and to 2^-25 below (S and X, whose low halves are scaled: to 2^-14 and 2^-36), so operands need a known size:
+// rows of q are scaled by a power of two to a norm in [0.5, 1) and, as keys, K' and P', by UNIT more, K' by one for its largest element, and S and X, per value column, by one from a
+// bound: the rule over keys no longer than one with 0 <= beta <= 2, g <= 0 is a contraction, so |S_next| <= |S| + sum beta |v| and |X| <= 2 |S| + beta |v|.  A chunk whose
+// inputs leave that domain (longer or tiny keys, other gates, infinities, NaN) is marked by the first kernel, or found by the bound, and runs token by token in the second, in f32, with
+// the same S: slower (about 1 us a token), but right for every input.
 //
 // What bounds it: a workgroup's chunk reads K, Q, K' (32 KB each at head_k 128) and P' (16 KB): 112 KB through one CU's 64 bytes a clock, 0.73 us, while its 168
 // matrix instructions take 0.3 us of four SIMDs.  The first kernel stores these operands in the order in which lanes load them (a fragment is 1 KB), every
@@ -35,9 +35,10 @@ typedef float f4 __attribute__((ext_vector_type(4)));
 #define SCAL_DECAY 384
 #define SCAL_KSCALE 385
 #define SCAL_MARK 386
+// low halves of S and X are stored times 2048: a column's values may be far below its bound
 #define LO_SCALE 2048.f
 #define LO_INV (1.f / 2048.f)
-// operands of magnitude up to one are stored times 4096, so that their low halves are normal f16 numbers too
+// operands of magnitude up to one are stored times 4096, so that the low halves of all but tiny ones are normal f16 numbers too
 #define UNIT 4096.f
 #define UNIT_INV (1.f / 4096.f)
 
@@ -54,14 +55,10 @@ static __device__ inline float exp_f64(double x) {
   const float hi = (float)x, e = expf(hi);
   return __builtin_fmaf(e, (float)(x - (double)hi), e);
 }
-static __device__ inline void split(float x, _Float16& hi, _Float16& lo) {
-  asm("" : "+v"(x));      // one f32 number: fused into the product that made it, hi would be rounded once and the difference below from a hi rounded twice, a whole step apart at times
-  hi = (_Float16)x;
-  lo = (_Float16)((x - (float)hi) * LO_SCALE);
-}
 struct Pair8 { h8 hi, lo; };
 struct Pair4 { h4 hi, lo; };
 // two values at a time: the high halves by one packed conversion, the low ones by a multiply-add each that takes the stored high half as it is
+template <bool FAR>
 static __device__ inline void split2(float x0, float x1, h2& hi, h2& lo) {
   asm("" : "+v"(x0), "+v"(x1));      // f32 numbers as they are: fused into the product that made them, the high half would be rounded once here and twice there
   uint32_t b;
@@ -69,13 +66,18 @@ static __device__ inline void split2(float x0, float x1, h2& hi, h2& lo) {
   __builtin_memcpy(&b, &h, 4);
   asm("" : "+v"(b));
   __builtin_memcpy(&hi, &b, 4);
-  lo = h2{(_Float16)__builtin_fmaf((float)hi[0], -LO_SCALE, x0 * LO_SCALE), (_Float16)__builtin_fmaf((float)hi[1], -LO_SCALE, x1 * LO_SCALE)};
+  float f = FAR ? -LO_SCALE : -1.f;
+  asm("" : "+s"(f));                 // not a subtraction: the multiply-add reads a half of `hi` in place and writes one of `lo`
+  if constexpr (FAR) { x0 *= LO_SCALE; x1 *= LO_SCALE; }
+  lo = h2{(_Float16)__builtin_fmaf((float)hi[0], f, x0), (_Float16)__builtin_fmaf((float)hi[1], f, x1)};
 }
+template <bool FAR = false>
 static __device__ inline Pair4 split4(const f4 x) {
   h2 h0, h1, l0, l1;
-  split2(x[0], x[1], h0, l0); split2(x[2], x[3], h1, l1);
+  split2<FAR>(x[0], x[1], h0, l0); split2<FAR>(x[2], x[3], h1, l1);
   return {h4{h0[0], h0[1], h1[0], h1[1]}, h4{l0[0], l0[1], l1[0], l1[1]}};
 }
+static __device__ inline h8 join(const h4 a, const h4 b) { return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7); }
 // buffers: a base in scalar registers, one vector offset for all fragments of a lane, reads past the end are zero and writes dropped
 static __device__ inline __amdgpu_buffer_rsrc_t buffer(const void* p, uint32_t bytes) { return __builtin_amdgcn_make_buffer_rsrc((void*)p, 0, (int)bytes, 0x00020000); }
 static __device__ inline f4 load_f4(__amdgpu_buffer_rsrc_t b, uint32_t at, uint32_t base) {
@@ -92,18 +94,6 @@ static __device__ inline void store_f16(__amdgpu_buffer_rsrc_t b, uint32_t at, f
   const _Float16 h = (_Float16)x;
   uint16_t u; __builtin_memcpy(&u, &h, 2);
   __builtin_amdgcn_raw_buffer_store_b16(u, b, (int)at, 0, 0);
-}
-static __device__ inline Pair8 split8(const float (&x)[8]) {
-  Pair8 r;
-#pragma unroll
-  for (int e = 0; e < 8; e++) { _Float16 h, l; split(x[e], h, l); r.hi[e] = h; r.lo[e] = l; }
-  return r;
-}
-// hi hi into `a`, hi lo + lo hi into `b`: the product is a + b / 2048
-static __device__ inline void mfma_pair(const h8 ahi, const h8 alo, const h8 bhi, const h8 blo, f4& a, f4& b) {
-  a = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahi, bhi, a, 0, 0, 0);
-  b = __builtin_amdgcn_mfma_f32_16x16x32_f16(ahi, blo, b, 0, 0, 0);
-  b = __builtin_amdgcn_mfma_f32_16x16x32_f16(alo, bhi, b, 0, 0, 0);
 }
 static __device__ inline float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }          // -126 <= e <= 127
 // largest magnitude `m` -> the exponent e with m 2^(13 - e) in [2^13, 2^14), as far as f32 has the powers
@@ -139,184 +129,202 @@ size_t pa_delta_chunk_ws_bytes(uint32_t chunks, uint32_t nk, uint32_t nv, uint32
 }
 
 // ---- 1: what does not depend on the state ----------------------------------------------------------
-#define TS 68      // floats of a row of A and T in LDS
-// LDS, first pair of regions for the products of rows, then the second: K | Q fragments; A | T (f32) | P fragments | T^T fragments
-#define PREP_A 0
-#define PREP_T (CHUNK * TS * 4)
-#define PREP_P (2 * CHUNK * TS * 4)
-#define PREP_TT (PREP_P + 16384)
-#define PREP_LDS (PREP_TT + 16384)
+// A wavefront has 16 rows of the chunk ("its tile").  Every product below is laid out so that a result, as the matrix instructions leave it (lane: column l16, rows 4 lg + r), is the
+// next product's operand as it stands: contractions run over 4 lg + r, not over 8 lg + j.  So A and P stay in registers from K K^T and K Q^T on; LDS holds the keys, which every
+// tile meets, and the blocks of T, which every wavefront needs.
+#define TS 20      // floats of a row of a 16 x 16 block in LDS
+template <int HK> struct PrepLds {
+  union {
+    _Float16 k[Frags<HK>::KQ];                                     // keys: [plane][tile][k step][lane][8]
+    struct {
+      float a[4][16 * TS], t[10][16 * TS];                         // diagonal blocks of A; blocks (i, j) of T at i (i + 1) / 2 + j
+      h4 tt[10][2][64];                                            // blocks of T as pairs, in the lanes' order
+    };
+  };
+  double G[CHUNK];
+  float beta[CHUNK], kfac[CHUNK], row[CHUNK], col[4][48], top[4];
+};
 
 template <int HK>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(256, 4)
 void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
   using F = Frags<HK>;
   constexpr int KS = F::KS, DT = HK / 64;                          // DT: tiles of 16 key dimensions of a wavefront
-  __shared__ __attribute__((aligned(16))) unsigned char lds[PREP_LDS];
-  __shared__ double Gs[CHUNK];
-  __shared__ float beta_s[CHUNK], kfac_s[CHUNK], kinv_s[CHUNK], max_s[4];
+  __shared__ __attribute__((aligned(16))) PrepLds<HK> L;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lg = lane >> 4;
   const uint32_t h = blockIdx.x, chunk = blockIdx.y, kh = h / p.group, c0 = chunk * CHUNK;
+  const uint32_t w = (wave + chunk + h) & 3;                       // its tile: later tiles are more work, and wavefront i of every workgroup runs on the same SIMD
   _Float16* const kq = ws.kq + ((size_t)chunk * p.nk + kh) * 2 * F::KQ;
   float* const scal = ws.scal + ((size_t)chunk * p.nv + h) * SCAL_FLOATS;
-  _Float16* const kl = (_Float16*)lds;
-  _Float16* const ql = kl + F::KQ;
+  const f4 zero = {0.f, 0.f, 0.f, 0.f};
   bool bad = false;
 
-  // -- rows: lengths, scaled pairs, fragments.  Four lanes a row, eight values each per k step
+  // -- gates: sums of g in 64 bits by one wavefront
+  if (w == 0) {
+    const bool valid = c0 + lane < p.n;
+    const size_t c = min(c0 + lane, p.n - 1);
+    const float g = valid ? p.g[c * p.gate_stride + h] : 0.f, b = valid ? p.beta[c * p.gate_stride + h] : 0.f;
+    bad = !(g <= 0.f) || !(b >= 0.f && b <= 2.f);
+    double G = g > -1e5f ? (double)g : -1e5;                        // exp(-1e5) is 0 as exp(-infinity) is, and differences stay numbers
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) { const double o = __shfl_up(G, d); if (lane >= (uint32_t)d) G += o; }
+    L.G[lane] = G;
+    L.beta[lane] = b;
+  }
+  // -- rows: lengths, scaled pairs.  Lane: row l16 of the tile, values 8 lg .. + 7 of every k step
+  Pair8 kf[KS], qf[KS];
   {
-    const uint32_t row = tid >> 2, part = tid & 3;
+    const uint32_t row = w * 16 + l16;
     const bool valid = c0 + row < p.n;
     const size_t c = min(c0 + row, p.n - 1);
-    const float* kp = p.k + c * p.k_stride + (size_t)kh * HK + 8 * part;
-    const float* qp = p.q + c * p.q_stride + (size_t)kh * HK + 8 * part;
-    float k[KS][8], q[KS][8], kk = 0.f, qq = 0.f;
+    const float* kp = p.k + c * p.k_stride + (size_t)kh * HK + 8 * lg;
+    const float* qp = p.q + c * p.q_stride + (size_t)kh * HK + 8 * lg;
+    f4 k[KS][2], q[KS][2];
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
-      for (int e = 0; e < 2; e++) {
-        const f4 a = *(const f4*)(kp + 32 * s + 4 * e), b = *(const f4*)(qp + 32 * s + 4 * e);
-#pragma unroll
-        for (int j = 0; j < 4; j++) { k[s][4 * e + j] = valid ? a[j] : 0.f; q[s][4 * e + j] = valid ? b[j] : 0.f; }
-      }
+      for (int e = 0; e < 2; e++) { k[s][e] = *(const f4*)(kp + 32 * s + 4 * e); q[s][e] = *(const f4*)(qp + 32 * s + 4 * e); }
+    float kk = 0.f, qq = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; s++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) { kk = __builtin_fmaf(k[s][e], k[s][e], kk); qq = __builtin_fmaf(q[s][e], q[s][e], qq); }
-    kk += dpp_f32<0xB1>(kk); kk += dpp_f32<0x4E>(kk);
-    qq += dpp_f32<0xB1>(qq); qq += dpp_f32<0x4E>(qq);
+      for (int e = 0; e < 2; e++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) { kk = __builtin_fmaf(k[s][e][j], k[s][e][j], kk); qq = __builtin_fmaf(q[s][e][j], q[s][e][j], qq); }
+    kk = valid ? rows4_sum(kk) : 0.f;
+    qq = valid ? rows4_sum(qq) : 0.f;
     const float kinv = p.l2norm && valid ? 1.0f / sqrtf(kk + p.eps) : 1.f;
     const float qinv = p.l2norm && valid ? 1.0f / sqrtf(qq + p.eps) : 1.f;
     const float kn = kk * kinv * kinv, qn = qq * qinv * qinv;      // squares of the lengths that the rule sees
     // lengths whose pairs keep their bits: keys in [2^-10, 1], or 0; q of any size whose square is a normal number, or 0
-    bad = !(kn <= 1.00002f) || (kn < 0x1p-20f && !(kk == 0.f)) || !(qn < 0x1p100f) || (qn < 0x1p-100f && !(qq == 0.f));
+    bad = bad || !(kn <= 1.00002f) || (kn < 0x1p-20f && !(kk == 0.f)) || !(qn < 0x1p100f) || (qn < 0x1p-100f && !(qq == 0.f));
     const int qe = qn >= 0x1p-100f && qn < 0x1p100f ? (exponent(qn) >> 1) + 1 : 0;   // |q| 2^-qe in [0.5, 1)
-    const float qs = qinv * pow2(-qe);
-    if (part == 0) {
-      kinv_s[row] = valid ? kinv : 0.f;
+    if (lg == 0) {
+      L.kfac[row] = valid ? kinv : 0.f;
       scal[4 * 64 + row] = kinv;
       scal[5 * 64 + row] = qinv;
       scal[3 * 64 + row] = p.scale * pow2(qe);
     }
-    const uint32_t frag = (row >> 4) * KS, at = (part * 16 + (row & 15)) * 8;
-    const bool first = h == kh * p.group;                          // one v head of the group stores the k head's fragments
+    const float ks = valid ? kinv * UNIT : 0.f, qs = valid ? qinv * pow2(-qe) * UNIT : 0.f;
+    const bool store_k = h == kh * p.group, store_q = h == kh * p.group + (p.group > 1 ? 1 : 0);      // the k head's fragments are stored by one or two v heads of its group
 #pragma unroll
     for (int s = 0; s < KS; s++) {
-#pragma unroll
-      for (int e = 0; e < 8; e++) { k[s][e] *= kinv * UNIT; q[s][e] *= qs * UNIT; }
-      const Pair8 kp8 = split8(k[s]), qp8 = split8(q[s]);
-      const uint32_t off = (frag + s) * 512 + at;
-      *(h8*)(kl + off) = kp8.hi; *(h8*)(kl + F::KQ / 2 + off) = kp8.lo;
-      *(h8*)(ql + off) = qp8.hi; *(h8*)(ql + F::KQ / 2 + off) = qp8.lo;
-      if (first) {
-        *(h8*)(kq + off) = kp8.hi; *(h8*)(kq + F::KQ / 2 + off) = kp8.lo;
-        *(h8*)(kq + F::KQ + off) = qp8.hi; *(h8*)(kq + F::KQ + F::KQ / 2 + off) = qp8.lo;
-      }
+      const Pair4 k0 = split4(k[s][0] * ks), k1 = split4(k[s][1] * ks), q0 = split4(q[s][0] * qs), q1 = split4(q[s][1] * qs);      // (rows behind the last: a finite one times zero, or the chunk is marked)
+      kf[s].hi = join(k0.hi, k1.hi); kf[s].lo = join(k0.lo, k1.lo);
+      qf[s].hi = join(q0.hi, q1.hi); qf[s].lo = join(q0.lo, q1.lo);
+      const uint32_t off = (w * KS + s) * 512 + lane * 8;
+      *(h8*)(L.k + off) = kf[s].hi; *(h8*)(L.k + F::KQ / 2 + off) = kf[s].lo;
+      if (store_k) { *(h8*)(kq + off) = kf[s].hi; *(h8*)(kq + F::KQ / 2 + off) = kf[s].lo; }
+      if (store_q) { *(h8*)(kq + F::KQ + off) = qf[s].hi; *(h8*)(kq + F::KQ + F::KQ / 2 + off) = qf[s].lo; }
     }
-  }
-  // -- gates: sums of g in 64 bits by the first wavefront
-  if (wave == 0) {
-    const bool valid = c0 + lane < p.n;
-    const size_t c = min(c0 + lane, p.n - 1);
-    const float g = valid ? p.g[c * p.gate_stride + h] : 0.f, b = valid ? p.beta[c * p.gate_stride + h] : 0.f;
-    bad = bad || !(g <= 0.f) || !(b >= 0.f && b <= 2.f);
-    double G = g > -1e5f ? (double)g : -1e5;                        // exp(-1e5) is 0 as exp(-infinity) is, and differences stay numbers
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) { const double o = __shfl_up(G, d); if (lane >= (uint32_t)d) G += o; }
-    Gs[lane] = G;
-    beta_s[lane] = b;
   }
   const bool mark = __syncthreads_or(bad);
+  // decays: of a row from the end of the tile before its own (row), from a row to the end of a later tile's predecessor (col), to the chunk's end (kfac)
   if (tid < 64) {
-    const float eG = exp_f64(Gs[tid]);
-    scal[tid] = beta_s[tid];
-    scal[64 + tid] = beta_s[tid] * eG;
-    kfac_s[tid] = kinv_s[tid] * exp_f64(Gs[63] - Gs[tid]);
+    const double G = L.G[tid];
+    const float eG = exp_f64(G);
+    scal[tid] = L.beta[tid];
+    scal[64 + tid] = L.beta[tid] * eG;
+    scal[2 * 64 + tid] = eG;
     if (tid == 63) { scal[SCAL_DECAY] = eG; scal[SCAL_MARK] = __uint_as_float(mark ? 1u : 0u); }
-  } else if (tid < 128) {
-    const uint32_t r = tid - 64;
-    scal[2 * 64 + r] = exp_f64(Gs[r]);                             // times the factor of P' X, in the second kernel
+    L.row[tid] = tid >= 16 ? exp_f64(G - L.G[(tid & 48) - 1]) : eG;
+  } else {
+    const uint32_t t = tid >> 6, m = tid & 63;
+    if (m < 16 * t) L.col[t][m] = exp_f64(L.G[16 * t - 1] - L.G[m]);
+    if (t == 1) L.kfac[m] *= exp_f64(L.G[63] - L.G[m]);
   }
   if (mark) return;                                                // the chunk runs token by token
+  __syncthreads();
 
-  // -- products of rows: tiles (mt <= nt) of K K^T and K Q^T, keys m in rows, keys / queries i in columns; ten tiles dealt to the wavefronts
-  f4 ga[3], gp[3];
+  // -- tiles (m, w): K K^T and K Q^T, keys m in rows, the wavefront's keys and queries i in columns
+  f4 A[4];                                                         // A_im of the tile, i = l16
+  h4 Ph[4], Pl[4];                                                 // P_im, as pairs
+  const uint32_t i = w * 16 + l16;
 #pragma unroll
-  for (int s = 0; s < 3; s++) {
-    const uint32_t id = wave + 4 * s;
-    ga[s] = gp[s] = f4{0.f, 0.f, 0.f, 0.f};
-    if (id < 10) {
-      const uint32_t nt = id >= 6 ? 3 : id >= 3 ? 2 : id >= 1 ? 1 : 0, mt = id - nt * (nt + 1) / 2;
-      f4 a1 = ga[s], p1 = ga[s];
+  for (int m = 0; m < 4; m++) {
+    A[m] = zero;
+    Ph[m] = Pl[m] = h4{0, 0, 0, 0};
+    if ((uint32_t)m <= w) {
+      f4 a = zero, q = zero;
 #pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        const uint32_t m = (mt * KS + ks) * 512 + lane * 8, i = (nt * KS + ks) * 512 + lane * 8;
-        const h8 mh = *(const h8*)(kl + m), ml = *(const h8*)(kl + F::KQ / 2 + m);
-        mfma_pair(mh, ml, *(const h8*)(kl + i), *(const h8*)(kl + F::KQ / 2 + i), ga[s], a1);
-        mfma_pair(mh, ml, *(const h8*)(ql + i), *(const h8*)(ql + F::KQ / 2 + i), gp[s], p1);
+      for (int s = 0; s < KS; s++) {
+        const uint32_t off = (m * KS + s) * 512 + lane * 8;
+        const h8 mh = *(const h8*)(L.k + off), ml = *(const h8*)(L.k + F::KQ / 2 + off);
+        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(mh, kf[s].hi, a, 0, 0, 0);
+        q = __builtin_amdgcn_mfma_f32_16x16x32_f16(mh, qf[s].hi, q, 0, 0, 0);
+        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(mh, kf[s].lo, a, 0, 0, 0);
+        q = __builtin_amdgcn_mfma_f32_16x16x32_f16(mh, qf[s].lo, q, 0, 0, 0);
+        a = __builtin_amdgcn_mfma_f32_16x16x32_f16(ml, kf[s].hi, a, 0, 0, 0);
+        q = __builtin_amdgcn_mfma_f32_16x16x32_f16(ml, qf[s].hi, q, 0, 0, 0);
       }
-      ga[s] = (ga[s] + a1 * LO_INV) * (UNIT_INV * UNIT_INV);
-      gp[s] = (gp[s] + p1 * LO_INV) * (UNIT_INV * UNIT_INV);
-    }
-  }
-  __syncthreads();                                                 // K and Q have been read: their LDS is A, T and P's now
-  float* const As = (float*)(lds + PREP_A);
-  float* const Tf = (float*)(lds + PREP_T);
-  _Float16* const pl = (_Float16*)(lds + PREP_P);
-  _Float16* const tt = (_Float16*)(lds + PREP_TT);
-  constexpr uint32_t LOP = 4096;                                   // halves from a plane to the other, of P, P' and T^T
+      const uint32_t m0 = m * 16 + 4 * lg;
+      f4 d;
+      if ((uint32_t)m < w) {
+        d = *(const f4*)(&L.col[w][m0]) * L.row[i];
+      } else {
+        const double Gi = L.G[i];
 #pragma unroll
-  for (int s = 0; s < 3; s++) {
-    const uint32_t id = wave + 4 * s;
-    if (id < 10) {
-      const uint32_t nt = id >= 6 ? 3 : id >= 3 ? 2 : id >= 1 ? 1 : 0, mt = id - nt * (nt + 1) / 2;
-      const uint32_t i = nt * 16 + l16, m0 = mt * 16 + 4 * lg;
-      const double Gi = Gs[i];
-      const float b = beta_s[i];
-      f4 a;
-      h4 hi, lo;
+        for (int r = 0; r < 4; r++) d[r] = m0 + r <= i ? exp_f64(Gi - L.G[m0 + r]) : 0.f;
+      }
+      d *= UNIT_INV * UNIT_INV;
+      const float b = L.beta[i];
+      f4 pm;
 #pragma unroll
       for (int r = 0; r < 4; r++) {
-        const float d = m0 + r <= i ? exp_f64(Gi - Gs[m0 + r]) : 0.f;
-        a[r] = m0 + r < i ? b * d * ga[s][r] : 0.f;
-        _Float16 x, y;
-        split(d * gp[s][r] * UNIT, x, y);
-        hi[r] = x; lo[r] = y;
+        A[m][r] = m0 + r < i ? b * d[r] * a[r] : 0.f;
+        pm[r] = d[r] * UNIT * q[r];
       }
-      *(f4*)(As + i * TS + m0) = a;
-      const uint32_t off = (nt * 2 + (mt >> 1)) * 512 + (l16 + 16 * ((m0 & 31) >> 3)) * 8 + (m0 & 7);
-      *(h4*)(pl + off) = hi; *(h4*)(pl + LOP + off) = lo;
+      const Pair4 s = split4(pm);
+      Ph[m] = s.hi; Pl[m] = s.lo;
     }
   }
-  if (wave < 2) {                                                  // the zero halves of fragments that cross the diagonal: tiles (1, 0) and (3, 2)
-    const uint32_t nt = 2 * wave, m0 = (nt + 1) * 16 + 4 * lg, off = (nt * 2 + (nt >> 1)) * 512 + (l16 + 16 * ((m0 & 31) >> 3)) * 8 + (m0 & 7);
-    *(h4*)(pl + off) = h4{0, 0, 0, 0}; *(h4*)(pl + LOP + off) = h4{0, 0, 0, 0};
-  }
-  __syncthreads();
-  // -- T = (1 + A)^-1: each wavefront its diagonal block by substitution, a lane a column (the four lane groups do the same)
+  __syncthreads();                                                 // the keys have been read: their LDS is A and T's now
+  // -- K~ = e^(G_64 - G_i) k_i, right operand: column d, contraction over the chunk's rows.  Requested here, used behind T
+  float kt[DT][2][8];
+#pragma unroll
+  for (int x = 0; x < DT; x++)
+#pragma unroll
+    for (int ks = 0; ks < 2; ks++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) kt[x][ks][e] = p.k[(size_t)min(c0 + 32 * ks + 16 * (e >> 2) + 4 * lg + (e & 3), p.n - 1) * p.k_stride + (size_t)kh * HK + (w * DT + x) * 16 + l16];
+
+  // -- T = (1 + A)^-1.  The diagonal block by substitution, a lane a column (the four lane groups do the same)
+  auto put_block = [&](uint32_t bi, uint32_t bj, const f4 v) {
+    const uint32_t b = bi * (bi + 1) / 2 + bj;
+#pragma unroll
+    for (int r = 0; r < 4; r++) L.t[b][(4 * lg + r) * TS + l16] = v[r];
+    const Pair4 s = split4(v * UNIT);
+    L.tt[b][0][lane] = s.hi; L.tt[b][1][lane] = s.lo;
+  };
   {
+    float* const a = L.a[w];
+    f4 mine = zero;
+#pragma unroll
+    for (int m = 0; m < 4; m++) if ((uint32_t)m == w) mine = A[m];
+    *(f4*)(a + l16 * TS + 4 * lg) = mine;
+    wave_lds_fence();
     float t[16];
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-      float s = l16 == (uint32_t)i ? 1.f : 0.f;
+    for (int r = 0; r < 16; r++) {
+      float s = l16 == (uint32_t)r ? 1.f : 0.f;
 #pragma unroll
-      for (int m4 = 0; m4 < i; m4 += 4) {
-        const f4 a = *(const f4*)(As + (wave * 16 + i) * TS + wave * 16 + m4);
+      for (int m4 = 0; m4 < r; m4 += 4) {
+        const f4 x = *(const f4*)(a + r * TS + m4);
 #pragma unroll
-        for (int m = 0; m < 4; m++) if (m4 + m < i) s = __builtin_fmaf(-a[m], t[m4 + m], s);
+        for (int m = 0; m < 4; m++) if (m4 + m < r) s = __builtin_fmaf(-x[m], t[m4 + m], s);
       }
-      t[i] = s;
+      t[r] = s;
     }
-    if (lg == 0) {
+    f4 v;
 #pragma unroll
-      for (int i = 0; i < 16; i++) Tf[(wave * 16 + i) * TS + wave * 16 + l16] = t[i];
-    }
+    for (int r = 0; r < 4; r++) v[r] = lg < 2 ? (lg == 0 ? t[r] : t[4 + r]) : (lg == 2 ? t[8 + r] : t[12 + r]);
+    put_block(w, w, v);
   }
   __syncthreads();
-  // 16 x 16 products in f32; the contraction runs over 4 lg + r, so that a result is the next product's right operand as it stands
-  auto left = [&](const float* m, uint32_t br, uint32_t bc) { return *(const f4*)(m + (br * 16 + l16) * TS + bc * 16 + 4 * lg); };
-  auto right = [&](const float* m, uint32_t br, uint32_t bc) {
-    const float* x = m + (br * 16 + 4 * lg) * TS + bc * 16 + l16;
+  // block rows from the top: T_ij = -T_ii sum_k A_ik T_kj, products of 16 x 16 in f32
+  auto left = [&](uint32_t b) { return *(const f4*)(&L.t[b * (b + 1) / 2 + b][l16 * TS + 4 * lg]); };                 // T_bb
+  auto right = [&](uint32_t bi, uint32_t bj) {
+    const float* x = &L.t[bi * (bi + 1) / 2 + bj][4 * lg * TS + l16];
     return f4{x[0], x[TS], x[2 * TS], x[3 * TS]};
   };
   auto mul = [&](const f4 a, const f4 b, f4 c) {
@@ -324,110 +332,91 @@ void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
     for (int r = 0; r < 4; r++) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[r], b[r], c, 0, 0, 0);
     return c;
   };
-  auto put = [&](uint32_t br, uint32_t bc, const f4 v) {
-    float* x = Tf + (br * 16 + 4 * lg) * TS + bc * 16 + l16;
-#pragma unroll
-    for (int r = 0; r < 4; r++) x[r * TS] = -v[r];
-  };
-  const f4 zero = {0.f, 0.f, 0.f, 0.f};
-  if (wave < 2) {
-    const uint32_t j = 2 * wave, i = j + 1;
-    put(i, j, mul(left(Tf, i, i), mul(left(As, i, j), right(Tf, j, j), zero), zero));
+  f4 m0 = zero, m1 = zero;
+  if (w == 1) put_block(1, 0, -mul(left(1), mul(A[0], right(0, 0), zero), zero));
+  if (w == 2) {
+    m0 = mul(A[0], right(0, 0), zero);
+    put_block(2, 1, -mul(left(2), mul(A[1], right(1, 1), zero), zero));
+  }
+  if (w == 3) {
+    m0 = mul(A[0], right(0, 0), zero);
+    m1 = mul(A[1], right(1, 1), zero);
+    put_block(3, 2, -mul(left(3), mul(A[2], right(2, 2), zero), zero));
   }
   __syncthreads();
-  {
-    const uint32_t j = wave & 1, i = 2 + (wave >> 1);
-    auto inner = [&](uint32_t row) {                               // row of A T over the first two blocks
-      f4 m = mul(left(As, row, j), right(Tf, j, j), zero);
-      return j == 0 ? mul(left(As, row, 1), right(Tf, 1, 0), m) : m;
-    };
-    const f4 m2 = inner(2);
-    f4 r;
-    if (i == 2) r = mul(left(Tf, 2, 2), m2, zero);
-    else r = mul(left(Tf, 3, 3), inner(3), mul(left(Tf, 3, 2), m2, zero));
-    put(i, j, r);                                                  // blocks that no other wavefront reads here
+  if (w == 2) put_block(2, 0, -mul(left(2), mul(A[1], right(1, 0), m0), zero));
+  if (w == 3) {
+    m0 = mul(A[1], right(1, 0), m0);
+    put_block(3, 1, -mul(left(3), mul(A[2], right(2, 1), m1), zero));
   }
   __syncthreads();
-  // -- T^T as fragments: rows j, contraction over i
+  if (w == 3) put_block(3, 0, -mul(left(3), mul(A[2], right(2, 0), m0), zero));
+  // (K~ into pairs while the last block is made)
+  Pair8 kb[DT][2];
 #pragma unroll
-  for (int e = 0; e < 2; e++) {
-    const uint32_t f = wave * 2 + e, jt = f >> 1, ks = f & 1, j = jt * 16 + l16, i0 = ks * 32 + 8 * lg;
-    float x[8];
+  for (int ks = 0; ks < 2; ks++) {
+    const f4 f0 = *(const f4*)(&L.kfac[32 * ks + 4 * lg]), f1 = *(const f4*)(&L.kfac[32 * ks + 16 + 4 * lg]);
 #pragma unroll
-    for (int m = 0; m < 8; m++) x[m] = i0 + m >= j ? Tf[(i0 + m) * TS + j] * UNIT : 0.f;
-    const Pair8 s = split8(x);
-    *(h8*)(tt + f * 512 + lane * 8) = s.hi; *(h8*)(tt + LOP + f * 512 + lane * 8) = s.lo;
-  }
-  __syncthreads();
-  // -- K' [j][d] = sum_i T_ij e^(G_64 - G_i) k_i[d]
-  f4 kt[DT][4];
-  float top = 0.f;
-#pragma unroll
-  for (int x = 0; x < DT; x++) {
-    const uint32_t d = (wave * DT + x) * 16 + l16;
-    Pair8 b[2];
-#pragma unroll
-    for (int ks = 0; ks < 2; ks++) {
-      float v[8];
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const uint32_t i = ks * 32 + 8 * lg + e;
-        v[e] = p.k[(size_t)min(c0 + i, p.n - 1) * p.k_stride + (size_t)kh * HK + d] * (kfac_s[i] * UNIT);
-      }
-      b[ks] = split8(v);
-    }
-#pragma unroll
-    for (int jt = 0; jt < 4; jt++) {
-      f4 a0 = zero, a1 = zero;
-#pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        if (ks < jt / 2) continue;
-        const uint32_t f = (jt * 2 + ks) * 512 + lane * 8;
-        mfma_pair(*(const h8*)(tt + f), *(const h8*)(tt + LOP + f), b[ks].hi, b[ks].lo, a0, a1);
-      }
-      kt[x][jt] = (a0 + a1 * LO_INV) * (UNIT_INV * UNIT_INV);
-#pragma unroll
-      for (int r = 0; r < 4; r++) top = fmaxf(top, fabsf(kt[x][jt][r]));
+    for (int x = 0; x < DT; x++) {
+      const float* k = kt[x][ks];
+      const Pair4 a = split4(f4{k[0], k[1], k[2], k[3]} * (f0 * UNIT)), b = split4(f4{k[4], k[5], k[6], k[7]} * (f1 * UNIT));
+      kb[x][ks].hi = join(a.hi, b.hi); kb[x][ks].lo = join(a.lo, b.lo);
     }
   }
-  // -- P'^T [j][i] = sum_m T_mj P_im: a wavefront a tile of 16 queries
-  _Float16* const pp = ws.pp + ((size_t)chunk * p.nv + h) * F::P;
+  __syncthreads();
+
+  // -- K' [j][d] = sum_i T_ij K~ [i][d] and P'^T [j][i] = sum_m T_mj P_im: T^T the left operand of both
+  f4 kr[DT][4], pr[4];
+  const h4 none = {0, 0, 0, 0};
+  auto t_block = [&](int bi, int bj, int plane) { return bi >= bj ? L.tt[bi * (bi + 1) / 2 + bj][plane][lane] : none; };
 #pragma unroll
   for (int jt = 0; jt < 4; jt++) {
-    f4 a0 = zero, a1 = zero;
-    if ((uint32_t)jt <= wave) {
+    pr[jt] = zero;
 #pragma unroll
-      for (int ks = 0; ks < 2; ks++) {
-        if (ks < jt / 2 || ks > (int)(wave >> 1)) continue;
-        const uint32_t f = (jt * 2 + ks) * 512 + lane * 8, g = (wave * 2 + ks) * 512 + lane * 8;
-        mfma_pair(*(const h8*)(tt + f), *(const h8*)(tt + LOP + f), *(const h8*)(pl + g), *(const h8*)(pl + LOP + g), a0, a1);
-      }
+    for (int x = 0; x < DT; x++) kr[x][jt] = zero;
+#pragma unroll
+    for (int ks = jt / 2; ks < 2; ks++) {
+      const h8 th = join(t_block(2 * ks, jt, 0), t_block(2 * ks + 1, jt, 0)), tl = join(t_block(2 * ks, jt, 1), t_block(2 * ks + 1, jt, 1));
+      const h8 ph = join(Ph[2 * ks], Ph[2 * ks + 1]), pl = join(Pl[2 * ks], Pl[2 * ks + 1]);
+#pragma unroll
+      for (int x = 0; x < DT; x++) kr[x][jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, kb[x][ks].hi, kr[x][jt], 0, 0, 0);
+      pr[jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, ph, pr[jt], 0, 0, 0);
+#pragma unroll
+      for (int x = 0; x < DT; x++) kr[x][jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, kb[x][ks].lo, kr[x][jt], 0, 0, 0);
+      pr[jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, pl, pr[jt], 0, 0, 0);
+#pragma unroll
+      for (int x = 0; x < DT; x++) kr[x][jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tl, kb[x][ks].hi, kr[x][jt], 0, 0, 0);
+      pr[jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tl, ph, pr[jt], 0, 0, 0);
     }
-    h4 hi, lo;
-#pragma unroll
-    for (int r = 0; r < 4; r++) { _Float16 x, y; split((a0[r] + a1[r] * LO_INV) * UNIT_INV, x, y); hi[r] = x; lo[r] = y; }
-    const uint32_t j0 = jt * 16 + 4 * lg, off = (wave * 2 + (jt >> 1)) * 512 + (l16 + 16 * ((j0 & 31) >> 3)) * 8 + (j0 & 7);
-    *(h4*)(pp + off) = hi; *(h4*)(pp + LOP + off) = lo;
   }
-  // -- K'^T in the order of the second kernel's loads, scaled by the power of two of its largest element
+  // -- P' and K'^T in the order of the second kernel's loads, K' scaled by the power of two of its largest element
+  float top = 0.f;
 #pragma unroll
-  for (int o = 32; o; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
-  if (lane == 0) max_s[wave] = top;
+  for (int x = 0; x < DT; x++)
+#pragma unroll
+    for (int jt = 0; jt < 4; jt++) top = fmaxf(fmaxf(top, fmaxf(fabsf(kr[x][jt][0]), fabsf(kr[x][jt][1]))), fmaxf(fabsf(kr[x][jt][2]), fabsf(kr[x][jt][3])));
+  top = fmaxf(top, dpp_f32<0xB1>(top)); top = fmaxf(top, dpp_f32<0x4E>(top)); top = fmaxf(top, dpp_f32<0x141>(top)); top = fmaxf(top, dpp_f32<0x140>(top));
+  top = fmaxf(fmaxf(readlane_f32(top, 0), readlane_f32(top, 16)), fmaxf(readlane_f32(top, 32), readlane_f32(top, 48)));
+  if (lane == 0) L.top[w] = top;
+  _Float16* const pp = ws.pp + ((size_t)chunk * p.nv + h) * F::P;
+  auto frag_at = [&](uint32_t tile, int jt) { return (tile * 2 + (jt >> 1)) * 512 + (l16 + 16 * (2 * (jt & 1) + (lg >> 1))) * 8 + 4 * (lg & 1); };
+#pragma unroll
+  for (int jt = 0; jt < 4; jt++) {
+    const Pair4 s = split4(pr[jt] * UNIT_INV);
+    *(h4*)(pp + frag_at(w, jt)) = s.hi; *(h4*)(pp + F::P / 2 + frag_at(w, jt)) = s.lo;
+  }
   __syncthreads();
-  top = fmaxf(fmaxf(max_s[0], max_s[1]), fmaxf(max_s[2], max_s[3]));
+  top = fmaxf(fmaxf(L.top[0], L.top[1]), fmaxf(L.top[2], L.top[3])) * (UNIT_INV * UNIT_INV);
   const int ke = top >= 0x1p-100f ? exponent(top) : 13;
-  const float ksc = pow2(13 - ke);
+  const float ksc = pow2(13 - ke) * (UNIT_INV * UNIT_INV);
   if (tid == 0) scal[SCAL_KSCALE] = pow2(ke - 13);
   _Float16* const kto = ws.kt + ((size_t)chunk * p.nv + h) * F::KT;
 #pragma unroll
   for (int x = 0; x < DT; x++)
 #pragma unroll
     for (int jt = 0; jt < 4; jt++) {
-      h4 hi, lo;
-#pragma unroll
-      for (int r = 0; r < 4; r++) { _Float16 a, b; split(kt[x][jt][r] * ksc, a, b); hi[r] = a; lo[r] = b; }
-      const uint32_t j0 = jt * 16 + 4 * lg, off = ((wave * DT + x) * 2 + (jt >> 1)) * 512 + (l16 + 16 * ((j0 & 31) >> 3)) * 8 + (j0 & 7);
-      *(h4*)(kto + off) = hi; *(h4*)(kto + F::KT / 2 + off) = lo;
+      const Pair4 s = split4(kr[x][jt] * ksc);
+      *(h4*)(kto + frag_at(w * DT + x, jt)) = s.hi; *(h4*)(kto + F::KT / 2 + frag_at(w * DT + x, jt)) = s.lo;
     }
 }
 
@@ -550,7 +539,7 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
     for (int t = 0; t < NT; t++)
 #pragma unroll
       for (int m = 0; m < MT; m++) {
-        const Pair4 s = split4(S[t][m] * to[t]);
+        const Pair4 s = split4<true>(S[t][m] * to[t]);
         const uint32_t d0 = (w * MT + m) * 16 + 4 * lg, off = (d0 >> 5) * 512 + (l16 + 16 * ((d0 & 31) >> 3)) * 8 + (d0 & 7);
         *(h4*)(&L.S[t][0][off]) = s.hi; *(h4*)(&L.S[t][1][off]) = s.lo;
       }
@@ -681,7 +670,7 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
       if constexpr (ROLE == KEYS) cv = L.cv[c & 1][w * 4 + lg];
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        f4 r0 = {0.f, 0.f, 0.f, 0.f}, r1 = r0, r2 = r0, r;
+        f4 r0 = {0.f, 0.f, 0.f, 0.f}, r1 = r0, r2 = r0, r;          // hi hi | hi lo, 2048 times | lo hi
 #pragma unroll
         for (int s = 0; s < KS; s++) {
           const h8 sh = *(const h8*)(&L.S[t][0][s * 512 + lane * 8]), sl = *(const h8*)(&L.S[t][1][s * 512 + lane * 8]);
@@ -691,13 +680,13 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
         }
         const float back = sigma_inv[t] * UNIT_INV;
 #pragma unroll
-        for (int i = 0; i < 4; i++) r[i] = __builtin_fmaf(r1[i] + r2[i], LO_INV, r0[i]) * back;
+        for (int i = 0; i < 4; i++) r[i] = __builtin_fmaf(r1[i], LO_INV, r0[i] + r2[i]) * back;
         if constexpr (ROLE == KEYS) {                              // X = beta v - beta e^G K S
           const f4 bv = L.bv[c & 1][t][w * 64 + lane];
           f4 x;
 #pragma unroll
           for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(-cv[i], r[i], bv[i]);
-          const Pair4 s = split4(x * to[t]);
+          const Pair4 s = split4<true>(x * to[t]);
           const uint32_t i0 = w * 16 + 4 * lg, off = (i0 >> 5) * 512 + (l16 + 16 * ((i0 & 31) >> 3)) * 8 + (i0 & 7);
           *(h4*)(&L.X[t][0][off]) = s.hi; *(h4*)(&L.X[t][1][off]) = s.lo;
         } else {
@@ -732,7 +721,7 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
             n2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, xh, n2, 0, 0, 0);
           }
 #pragma unroll
-          for (int i = 0; i < 4; i++) n[t][m][i] = __builtin_fmaf(n1[i] + n2[i], LO_INV, n0[i]);
+          for (int i = 0; i < 4; i++) n[t][m][i] = __builtin_fmaf(n1[i], LO_INV, n0[i] + n2[i]);
         }
       if constexpr (ROLE == STATE) {
         if constexpr (NT > 1) load_g(gf, c + 1);                   // no room for two chunks' operands

@@ -23,102 +23,127 @@ static __device__ inline float row16_sum(float v) {
   return v + dpp_f32<0x140>(v);
 }
 
-// V4: float4 of a row per lane (head_k = 64 V4)
-template <int V4>
+// V4: float4 of a row per lane (head_k = 64 V4).  The leading arguments are those that every load needs: they arrive in scalar registers before the wave starts.
+template <int V4, bool OUT, bool NORM>
 __global__ __launch_bounds__(256)
-void pa_delta_step_kernel(DeltaParams p) {
+void pa_delta_step_kernel(const float* a_k, const float* a_q, const float* a_v, float* a_state, const float* a_g, const float* a_beta, DeltaParams p) {
   constexpr int AHEAD = 4;
   constexpr uint32_t HK = 64 * V4;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, j = lane & 15;
   const uint32_t tiles = p.hv / 16;
   const uint32_t h = blockIdx.x / tiles, row = (blockIdx.x % tiles) * 16 + wave * 4 + (lane >> 4), kh = h / p.group;
-  float* const srow = p.state + ((size_t)h * p.hv + row) * HK + 4 * j;
+  float* const srow = a_state + ((size_t)h * p.hv + row) * HK + 4 * j;
   f4 S[V4];
 #pragma unroll
   for (int i = 0; i < V4; i++) S[i] = *(const f4*)(srow + 64 * i);
-  const float* const kp = p.k + (size_t)kh * HK + 4 * j;
-  const float* const qp = p.q + (size_t)kh * HK + 4 * j;
-  const float* const vp = p.v + (size_t)h * p.hv + row;
-  const bool out = p.out != nullptr;
+  const float* kp = a_k + (size_t)kh * HK + 4 * j;
+  const float* qp = a_q + (size_t)kh * HK + 4 * j;
+  const float* vp = a_v + (size_t)h * p.hv + row;
 
   f4 kr[AHEAD][V4], qr[AHEAD][V4];
-  float vr[AHEAD], gr[AHEAD], br[AHEAD];
-  auto request = [&](int s, uint32_t t) __attribute__((always_inline)) {
+  float vr[AHEAD];
+  auto request = [&](int s) __attribute__((always_inline)) {       // the next column
 #pragma unroll
-    for (int i = 0; i < V4; i++) kr[s][i] = *(const f4*)(kp + (size_t)t * p.k_stride + 64 * i);
-    vr[s] = vp[(size_t)t * p.v_stride];
-    gr[s] = p.g[(size_t)t * p.gate_stride + h];
-    br[s] = p.beta[(size_t)t * p.gate_stride + h];
-    if (out) {
+    for (int i = 0; i < V4; i++) kr[s][i] = *(const f4*)(kp + 64 * i);
+    if constexpr (OUT) {
 #pragma unroll
-      for (int i = 0; i < V4; i++) qr[s][i] = *(const f4*)(qp + (size_t)t * p.q_stride + 64 * i);
+      for (int i = 0; i < V4; i++) qr[s][i] = *(const f4*)(qp + 64 * i);
     }
+    vr[s] = *vp;
+    kp += p.k_stride; qp += p.q_stride; vp += p.v_stride;
   };
+  // gates of sixteen columns at a time, one a lane: their exponentials are one instruction sequence, and a column takes its own by a lane read
+  float gate = 0.f, beta = 0.f;
+  auto request_gates = [&](uint32_t t0) __attribute__((always_inline)) {
+    const size_t t = min(t0 + j, p.n - 1);
+    gate = a_g[t * p.gate_stride + h];
+    beta = a_beta[t * p.gate_stride + h];
+  };
+  request_gates(0);
 #pragma unroll
-  for (int s = 0; s < AHEAD; s++) if ((uint32_t)s < p.n) request(s, s);
+  for (int s = 0; s < AHEAD; s++) if ((uint32_t)s < p.n) request(s);
 
-  for (uint32_t t0 = 0; t0 < p.n; t0 += AHEAD) {
+  for (uint32_t t0 = 0; t0 < p.n; t0 += 16) {
+    const float decays = expf(gate), betas = beta;
+    if (t0 + 16 < p.n) request_gates(t0 + 16);
+    float keep = 0.f;                                              // lane j: the output of column t0 + j
 #pragma unroll
-    for (int s = 0; s < AHEAD; s++) {
-      const uint32_t t = t0 + s;
-      if (t < p.n) {
-        float kk = 0.f, qq = 0.f, inv_k = 1.f, scale_q = p.scale;
-        if (p.l2norm) {                                             // off the chain: needs k_t and q_t alone
+    for (int b = 0; b < 4; b++) {
+      if (t0 + 4 * b >= p.n) break;
 #pragma unroll
-          for (int i = 0; i < V4; i++)
+      for (int s = 0; s < AHEAD; s++) {
+        const uint32_t t = t0 + 4 * b + s;
+        if (t >= p.n) break;
+        const float decay = readlane_f32(decays, 4 * b + s), bt = readlane_f32(betas, 4 * b + s);
+        // with k^ = k / |k|: S' k^ = (S' k) / |k| and u k^ = (u / |k|) k, so the row is used as it came
+        float inv_k = 1.f, x = 0.f, y = 0.f;
+        if constexpr (NORM) {                                      // off the chain: needs k_t alone
 #pragma unroll
-            for (int e = 0; e < 4; e++) kk = __builtin_fmaf(kr[s][i][e], kr[s][i][e], kk);
-          inv_k = 1.0f / sqrtf(row16_sum(kk) + p.eps);
+          for (int i = 0; i < V4; i++) {
+            x = __builtin_fmaf(kr[s][i][0], kr[s][i][0], x); y = __builtin_fmaf(kr[s][i][1], kr[s][i][1], y);
+            x = __builtin_fmaf(kr[s][i][2], kr[s][i][2], x); y = __builtin_fmaf(kr[s][i][3], kr[s][i][3], y);
+          }
+          inv_k = __builtin_amdgcn_rsqf(row16_sum(x + y) + p.eps);
         }
-        const float decay = expf(gr[s]);
-        f4 k[V4];
-        float a = 0.f, b = 0.f;
+        x = y = 0.f;
 #pragma unroll
         for (int i = 0; i < V4; i++) {
-          k[i] = kr[s][i] * inv_k;
           S[i] = S[i] * decay;
-          a = __builtin_fmaf(S[i][0], k[i][0], a); b = __builtin_fmaf(S[i][1], k[i][1], b);
-          a = __builtin_fmaf(S[i][2], k[i][2], a); b = __builtin_fmaf(S[i][3], k[i][3], b);
+          x = __builtin_fmaf(S[i][0], kr[s][i][0], x); y = __builtin_fmaf(S[i][1], kr[s][i][1], y);
+          x = __builtin_fmaf(S[i][2], kr[s][i][2], x); y = __builtin_fmaf(S[i][3], kr[s][i][3], y);
         }
-        const float u = br[s] * (vr[s] - row16_sum(a + b));
+        const float sk = row16_sum(x + y);
+        const float u = bt * (NORM ? __builtin_fmaf(-sk, inv_k, vr[s]) : vr[s] - sk) * inv_k;
 #pragma unroll
         for (int i = 0; i < V4; i++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) S[i][e] = __builtin_fmaf(u, k[i][e], S[i][e]);
-        if (out) {
-          if (p.l2norm) {
+          for (int e = 0; e < 4; e++) S[i][e] = __builtin_fmaf(u, kr[s][i][e], S[i][e]);
+        if constexpr (OUT) {
+          float scale = p.scale;
+          x = y = 0.f;
+          if constexpr (NORM) {
 #pragma unroll
-            for (int i = 0; i < V4; i++)
-#pragma unroll
-              for (int e = 0; e < 4; e++) qq = __builtin_fmaf(qr[s][i][e], qr[s][i][e], qq);
-            scale_q = p.scale / sqrtf(row16_sum(qq) + p.eps);
+            for (int i = 0; i < V4; i++) {
+              x = __builtin_fmaf(qr[s][i][0], qr[s][i][0], x); y = __builtin_fmaf(qr[s][i][1], qr[s][i][1], y);
+              x = __builtin_fmaf(qr[s][i][2], qr[s][i][2], x); y = __builtin_fmaf(qr[s][i][3], qr[s][i][3], y);
+            }
+            scale *= __builtin_amdgcn_rsqf(row16_sum(x + y) + p.eps);
+            x = y = 0.f;
           }
-          float c = 0.f, d = 0.f;
 #pragma unroll
           for (int i = 0; i < V4; i++) {
-            c = __builtin_fmaf(S[i][0], qr[s][i][0], c); d = __builtin_fmaf(S[i][1], qr[s][i][1], d);
-            c = __builtin_fmaf(S[i][2], qr[s][i][2], c); d = __builtin_fmaf(S[i][3], qr[s][i][3], d);
+            x = __builtin_fmaf(S[i][0], qr[s][i][0], x); y = __builtin_fmaf(S[i][1], qr[s][i][1], y);
+            x = __builtin_fmaf(S[i][2], qr[s][i][2], x); y = __builtin_fmaf(S[i][3], qr[s][i][3], y);
           }
-          const float o = row16_sum(c + d) * scale_q;
-          if (j == 0) {
-            const size_t at = (size_t)t * p.out_stride + (size_t)h * p.hv + row;
-            if (p.out_f16) ((_Float16*)p.out)[at] = (_Float16)o; else ((float*)p.out)[at] = o;
-          }
+          const float o = row16_sum(x + y) * scale;
+          keep = j == (uint32_t)(4 * b + s) ? o : keep;
         }
         if (t + 1 == p.commit) {
 #pragma unroll
           for (int i = 0; i < V4; i++) *(f4*)(srow + 64 * i) = S[i];
         }
-        if (t + AHEAD < p.n) request(s, t + AHEAD);
+        if (t + AHEAD < p.n) request(s);
+      }
+    }
+    if constexpr (OUT) {
+      if (t0 + j < p.n) {
+        const size_t at = (size_t)(t0 + j) * p.out_stride + (size_t)h * p.hv + row;
+        if (p.out_f16) ((_Float16*)p.out)[at] = (_Float16)keep; else ((float*)p.out)[at] = keep;
       }
     }
   }
 }
 
-hipError_t pa_launch_delta_step(const DeltaParams& p, hipStream_t s) {
+template <int V4>
+static void launch_step(const DeltaParams& p, hipStream_t s) {
   const dim3 grid(p.nv * (p.hv / 16)), block(256);
-  if (p.hk == 64) hipLaunchKernelGGL(pa_delta_step_kernel<1>, grid, block, 0, s, p);
-  else hipLaunchKernelGGL(pa_delta_step_kernel<2>, grid, block, 0, s, p);
+#define STEP(OUT, NORM) hipLaunchKernelGGL((pa_delta_step_kernel<V4, OUT, NORM>), grid, block, 0, s, p.k, p.q, p.v, p.state, p.g, p.beta, p)
+  if (p.out) { if (p.l2norm) STEP(true, true); else STEP(true, false); }
+  else { if (p.l2norm) STEP(false, true); else STEP(false, false); }
+#undef STEP
+}
+hipError_t pa_launch_delta_step(const DeltaParams& p, hipStream_t s) {
+  if (p.hk == 64) launch_step<1>(p, s); else launch_step<2>(p, s);
   return hipGetLastError();
 }
 
