@@ -5,13 +5,17 @@
 // With a few tokens the work is the stream of the chosen experts' weights: one token of 8 experts of 512 x 2048 and a shared one reads 16 MB of Q4_0
 // planes and 2 MB of router and computes 58 MFLOP.  Three launches, because each needs all of the one before: logits, h, y.
 //   1. router: a wavefront a row (expert) and token, over the raw x; the norm's factor is taken out of the sum, so sum of squares and dot run together.
-//      Further wavefronts write xn, one a token.
-//   2. gate and up: a workgroup a (token, place in the choice, slice of rows).  Which expert that is, every wavefront finds for itself from the token's
-//      logits (a maximum over the 64 lanes per place), while xn is on its way.
+//      One more wavefront a token writes xn.
+//   2. gate and up: a workgroup 16 rows of an expert.  With a few tokens it finds which expert that is by itself, from the token's logits (a maximum over the 64 lanes per place),
+//      while xn is on its way; with more of them the choice is a launch of its own, and for f32 weights a workgroup serves up to four tokens that share an expert.
 //   3. down: the experts of a token lie behind one another as ONE input of slots x ffn values, so a wavefront's row is one dot product over it.
 // A lane owns whole 32-value blocks of the input (one 16-byte load of Q4_0), for all rows of its wavefront; activations are kept in the order
 // in which lanes load them, so that every load is 1 KB of consecutive bytes.  Arithmetic is f32, every sum in an order that depends on the layer's sizes alone:
 // no atomics, and a token's bits do not depend on the other tokens of the call.
+//
+// Measured with 256 experts of 512 x 2048, 8 chosen and one shared (router, choice, gate and up, down, in us): 1 token of Q4_0 5 + 7 + 5, each a launch's latency and one trip to memory;
+// 5 of Q8_0 6 + 23 + 15 for 131 MB of distinct weights, gate and up at 4 TB/s (a large copy runs at 4.9); 16 of Q4_0 8 + 5 + 29 + 20 for 182 MB, gate and up at 4.2 TB/s.
+// f32, 27 tokens, 61 experts of 352 x 1056, 5 chosen: 5 + 5 + 41 + 26 for 245 MB.
 #include "blocks_internal.h"
 #include "glue_math.h"
 
@@ -30,76 +34,94 @@ static __device__ inline uint32_t wave_max_u32(uint32_t v) {
 }
 
 // ---- weights: what a lane holds of a row at a time -----------------------------------------------
-// F32: four values, Q8_0 and Q4_0: a block of 32 with its scale.  F4: float4 of activation that go with it.
-template <int KIND> struct Piece { static constexpr int F4 = 8, VALUES = 32; u4 w[KIND == PA_W_Q8_0 ? 2 : 1]; uint16_t sc; };
-template <> struct Piece<PA_W_F32> { static constexpr int F4 = 1, VALUES = 4; f4 w; };
-
-template <int KIND>
-static __device__ inline void load_piece(Piece<KIND>& r, const unsigned char* plane, const uint16_t* scales, size_t at) {
-  if constexpr (KIND == PA_W_F32) {
-    r.w = *(const f4*)(plane + at * 16);
-  } else if constexpr (KIND == PA_W_Q8_0) {
-    const u4* s = (const u4*)(plane + at * 32);
-    r.w[0] = s[0]; r.w[1] = s[1]; r.sc = scales[at];
-  } else {
-    r.w[0] = *(const u4*)(plane + at * 16); r.sc = scales[at];
-  }
-}
+// Q8_0 and Q4_0: a block of 32 values with its scale; F32: two times four values, 64 lanes apart.  X: the float4 of activation that go with it.
+// Dequantisation is what bounds a pass of several tokens, so it is kept to 0.6 (Q4_0) and 0.75 (Q8_0) instructions a weight beside the multiply-add: the bits of an unsigned weight u in the low bits of an
+// f16 ARE the number u 2^-24 (subnormal), and the mixed-precision multiply-add takes an f16 as it is.  A Q4_0 word gives its eight nibbles as four masked pairs, every other
+// one 16 times too large in place: the activations that meet those (elements 16 to 31 of a block) are kept divided by 16.  Q8_0 bytes are made unsigned by flipping their sign bit and spread over
+// halves by byte permutes.  The offsets, 8 and 128, come off as the offset times the block's sum of activations, which is kept beside them.
+template <int KIND> struct Piece { static constexpr int F4 = 8; static constexpr uint32_t STEP = 64; u4 w[KIND == PA_W_Q8_0 ? 2 : 1]; uint16_t sc; };
+template <> struct Piece<PA_W_F32> { static constexpr int F4 = 2; static constexpr uint32_t STEP = 128; f4 w[2]; };
+template <int KIND> struct Act { f4 x[Piece<KIND>::F4]; float sum; uint32_t have; };   // have: how many of the lane's loads lie in the row
+template <int KIND> static __device__ inline uint32_t pieces(uint32_t values) { return KIND == PA_W_F32 ? values / 4 : values / 32; }
 
 static __device__ inline float f16_bits_f32(uint16_t b) { _Float16 h; __builtin_memcpy(&h, &b, 2); return (float)h; }
+static __device__ inline float half_of(uint32_t w, int i) { h2v v; __builtin_memcpy(&v, &w, 4); return (float)v[i]; }
 
 // acc + f * (piece . x)
 template <int KIND>
-static __device__ inline float dot_piece(const Piece<KIND>& r, const f4 (&x)[Piece<KIND>::F4], float f, float acc) {
-  float a = 0.f;
+static __device__ inline float dot_piece(const Piece<KIND>& r, const Act<KIND>& act, float f, float acc) {
+  const auto& x = act.x;
+  float a = 0.f, b = 0.f;
   if constexpr (KIND == PA_W_F32) {
 #pragma unroll
-    for (int j = 0; j < 4; j++) a = __builtin_fmaf(r.w[j], x[0][j], a);
-    return __builtin_fmaf(a, f, acc);
+    for (int i = 0; i < 2; i++) {
+      if (i >= (int)act.have) break;
+      a = __builtin_fmaf(r.w[i][0], x[i][0], a); b = __builtin_fmaf(r.w[i][1], x[i][1], b);
+      a = __builtin_fmaf(r.w[i][2], x[i][2], a); b = __builtin_fmaf(r.w[i][3], x[i][3], b);
+    }
+    return __builtin_fmaf(a + b, f, acc);
   } else if constexpr (KIND == PA_W_Q8_0) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const int word = (int)r.w[i >> 2][i & 3];
-#pragma unroll
-      for (int j = 0; j < 4; j++) a = __builtin_fmaf((float)((word << (24 - 8 * j)) >> 24), x[i][j], a);
+      const uint32_t word = r.w[i >> 2][i & 3] ^ 0x80808080u;
+      const uint32_t lo = __builtin_amdgcn_perm(0u, word, 0x0c010c00u), hi = __builtin_amdgcn_perm(0u, word, 0x0c030c02u);
+      a = __builtin_fmaf(half_of(lo, 0), x[i][0], a); b = __builtin_fmaf(half_of(lo, 1), x[i][1], b);
+      a = __builtin_fmaf(half_of(hi, 0), x[i][2], a); b = __builtin_fmaf(half_of(hi, 1), x[i][3], b);
     }
-    return __builtin_fmaf(a, f * f16_bits_f32(r.sc), acc);
+    return __builtin_fmaf(__builtin_fmaf(a + b, 16777216.0f, -128.0f * act.sum), f * f16_bits_f32(r.sc), acc);
   } else {
-    // byte j of the block = elements j (low nibble) and j + 16 (high).  Two nibbles of a word under the f16 exponent of 1024 are 1024 + n, less 1032 exactly
-    // n - 8; the mixed-precision fma takes the f16 as it is.
-    const h2v off = {(_Float16)1032.f, (_Float16)1032.f};
+    // byte j of the block = elements j (low nibble) and j + 16 (high)
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-      const uint32_t word = r.w[0][k];
-#pragma unroll
-      for (int t = 0; t < 4; t++) {
-        const uint32_t pr = ((word >> (4 * t)) & 0x000F000Fu) | 0x64006400u;      // nibbles t and t + 4 of the word
-        h2v v; __builtin_memcpy(&v, &pr, 4);
-        v = v - off;
-        const int i = k + 4 * (t & 1), j = t >> 1;                                // element 4 i + j, and two on
-        a = __builtin_fmaf((float)v[0], x[i][j], a);
-        a = __builtin_fmaf((float)v[1], x[i][j + 2], a);
-      }
+      const uint32_t w0 = r.w[0][k], w1 = w0 >> 8;
+      const uint32_t p0 = w0 & 0x000F000Fu, p1 = w0 & 0x00F000F0u, p2 = w1 & 0x000F000Fu, p3 = w1 & 0x00F000F0u;
+      a = __builtin_fmaf(half_of(p0, 0), x[k][0], a); b = __builtin_fmaf(half_of(p1, 0), x[k + 4][0], b);
+      a = __builtin_fmaf(half_of(p0, 1), x[k][2], a); b = __builtin_fmaf(half_of(p1, 1), x[k + 4][2], b);
+      a = __builtin_fmaf(half_of(p2, 0), x[k][1], a); b = __builtin_fmaf(half_of(p3, 0), x[k + 4][1], b);
+      a = __builtin_fmaf(half_of(p2, 1), x[k][3], a); b = __builtin_fmaf(half_of(p3, 1), x[k + 4][3], b);
     }
-    return __builtin_fmaf(a, f * f16_bits_f32(r.sc), acc);
+    return __builtin_fmaf(__builtin_fmaf(a + b, 16777216.0f, -8.0f * act.sum), f * f16_bits_f32(r.sc), acc);
   }
 }
 
-// where value e of an activation lies in reading order
+// Activations in reading order: for quantised weights groups of 64 blocks, in a group eight times 64 lanes x 4 values, then 64 sums of each half of a block; for f32
+// weights as they are.
+#define GROUP_FLOATS MOE_GROUP_FLOATS
+// value e of an activation, written where its reader looks for it
 template <int KIND>
 static __device__ inline uint32_t act_at(uint32_t e) {
   if constexpr (KIND == PA_W_F32) return e;
   const uint32_t b = e / 32;
-  return ((((b / 64) * 8 + (e % 32) / 4) * 64) + b % 64) * 4 + e % 4;
+  return (b / 64) * GROUP_FLOATS + (((e % 32) / 4) * 64 + b % 64) * 4 + e % 4;
 }
-// the float4 of activation of piece q (lane q % 64)
+static __device__ inline uint32_t sum_at(uint32_t e) { return (e / 2048) * GROUP_FLOATS + 2048 + ((e / 16) % 2) * 64 + (e / 32) % 64; }   // of the 16 values from e on
+template <int KIND> static __device__ inline float stored(uint32_t e, float v) { return KIND == PA_W_Q4_0 && (e & 16) ? v * 0.0625f : v; }
+
+// piece q of an activation and of a row (f32: the four from q on); past the end (q >= n) the last one again, which nothing uses
 template <int KIND>
-static __device__ inline void load_act(f4 (&x)[Piece<KIND>::F4], const float* act, uint32_t q) {
+static __device__ inline void load_act(Act<KIND>& d, const float* act, uint32_t q, uint32_t n) {
   if constexpr (KIND == PA_W_F32) {
-    x[0] = ((const f4*)act)[q];
-  } else {
 #pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = ((const f4*)act)[((q / 64) * 8 + i) * 64 + q % 64];
+    for (int i = 0; i < 2; i++) d.x[i] = ((const f4*)act)[min(q + 64 * i, n - 1)];
+    d.have = (q < n) + (q + 64 < n);
+  } else {
+    const uint32_t c = min(q, n - 1);
+    const float* g = act + (c / 64) * GROUP_FLOATS;
+#pragma unroll
+    for (int i = 0; i < 8; i++) d.x[i] = ((const f4*)g)[i * 64 + c % 64];
+    d.sum = g[2048 + c % 64] + g[2112 + c % 64];
+  }
+}
+template <int KIND>
+static __device__ inline void load_piece(Piece<KIND>& r, const unsigned char* plane, const uint16_t* scales, size_t row, uint32_t q, uint32_t n) {
+  if constexpr (KIND == PA_W_F32) {
+#pragma unroll
+    for (int i = 0; i < 2; i++) r.w[i] = ((const f4*)plane)[row * n + min(q + 64 * i, n - 1)];
+  } else {
+    const size_t at = row * n + min(q, n - 1);
+    if constexpr (KIND == PA_W_Q8_0) { const u4* s = (const u4*)(plane + at * 32); r.w[0] = s[0]; r.w[1] = s[1]; }
+    else r.w[0] = *(const u4*)(plane + at * 16);
+    r.sc = scales[at];
   }
 }
 
@@ -108,11 +130,11 @@ template <int KIND>
 __global__ __launch_bounds__(256)
 void pa_moe_router_kernel(MoeParams p, uint32_t rows) {
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y, n4 = p.dim / 4;
-  const uint32_t row = blockIdx.x * 4 + wave;
+  const uint32_t at = blockIdx.x * 4 + wave;                       // 0: xn, the longest way, first; otherwise logit at - 1
   const f4* x = (const f4*)(p.x + (size_t)t * p.x_stride);
   const f4* nw = (const f4*)p.norm_w;
-  if (row > rows) return;
-  const f4* r = (const f4*)(p.router + (size_t)min(row, rows - 1) * p.dim);
+  if (at > rows) return;
+  const f4* r = (const f4*)(p.router + (size_t)(at ? at - 1 : 0) * p.dim);
   float ss = 0.f, a = 0.f, b = 0.f;
   for (uint32_t i0 = 0; i0 < n4; i0 += 512) {
     f4 xv[8], rv[8], wv[8];
@@ -136,15 +158,24 @@ void pa_moe_router_kernel(MoeParams p, uint32_t rows) {
   }
   ss = wave_sum_f32(ss);
   const float inv = nw ? 1.0f / sqrtf(ss / (float)p.dim + p.eps) : 1.f;
-  if (row < rows) {
+  if (at) {
     a = wave_sum_f32(a + b) * inv;
-    if (lane == 0) p.logits[(size_t)t * p.logit_stride + row] = a;
+    if (lane == 0) p.logits[(size_t)t * p.logit_stride + at - 1] = a;
     return;
   }
-  float* xn = p.xn + (size_t)t * p.xn_floats;                     // row == rows: the token's normed activations
-  for (uint32_t q = lane; q < n4; q += 64) {
-    const f4 v = nw ? (x[q] * inv) * nw[q] : x[q];
-    *(f4*)(xn + act_at<KIND>(4 * q)) = v;
+  float* xn = p.xn + (size_t)t * p.xn_floats;
+  for (uint32_t q0 = 0; q0 < n4; q0 += 64) {
+    const uint32_t q = q0 + lane;
+    f4 v = {0.f, 0.f, 0.f, 0.f};
+    if (q < n4) v = nw ? (x[q] * inv) * nw[q] : x[q];
+    float sum = (v[0] + v[1]) + (v[2] + v[3]);                     // of half a block: four lanes'
+    sum += dpp_f32<0xB1>(sum); sum += dpp_f32<0x4E>(sum);
+    if (q < n4) {
+#pragma unroll
+      for (int j = 0; j < 4; j++) v[j] = stored<KIND>(4 * q, v[j]);
+      *(f4*)(xn + act_at<KIND>(4 * q)) = v;
+      if (KIND != PA_W_F32 && (lane & 3) == 0) xn[sum_at(4 * q)] = sum;
+    }
   }
 }
 
@@ -163,9 +194,10 @@ struct Choice {
       key[i] = e < n ? k : 0u;
     }
   }
-  // the largest key, the lowest expert among equals; taken out
-  __device__ uint32_t next(uint32_t lane) {
-    uint32_t m = key[0];
+  static __device__ float logit(uint32_t k) { return k == 1u ? __uint_as_float(0x7FC00000u) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k); }
+  // the expert of the largest key m, the lowest among equals; taken out
+  __device__ uint32_t next(uint32_t lane, uint32_t& m) {
+    m = key[0];
 #pragma unroll
     for (int i = 1; i < NE; i++) m = max(m, key[i]);
     m = wave_max_u32(m);
@@ -188,13 +220,17 @@ static __device__ void write_choice(const MoeParams& p, uint32_t t, uint32_t lan
   const float* l = p.logits + (size_t)t * p.logit_stride;
   Choice<NE> c;
   c.load(l, p.n_experts, lane);
-  uint32_t mine = 0;                                               // lane r: the expert of place r
-  for (uint32_t r = 0; r < p.top_k; r++) { const uint32_t e = c.next(lane); if (lane == r) mine = e; }
-  const float top = l[__builtin_amdgcn_readlane((int)mine, 0)];    // the largest logit (a NaN only where all are)
+  float v[NE];
+#pragma unroll
+  for (int i = 0; i < NE; i++) v[i] = Choice<NE>::logit(c.key[i]);
+  uint32_t mine = 0, mine_key = 0, m;                              // lane r: the expert of place r
+  for (uint32_t r = 0; r < p.top_k; r++) { const uint32_t e = c.next(lane, m); if (lane == r) { mine = e; mine_key = m; } }
+  const float top = readlane_f32(Choice<NE>::logit(mine_key), 0);  // the largest logit (a NaN only where all are)
   float all = 0.f;
-  for (uint32_t e = lane; e < p.n_experts; e += 64) all += expf(l[e] - top);
+#pragma unroll
+  for (int i = 0; i < NE; i++) if (lane + 64 * i < p.n_experts) all += expf(v[i] - top);
   all = wave_sum_f32(all);
-  const float w = lane < p.top_k ? expf(l[mine] - top) : 0.f;
+  const float w = lane < p.top_k ? expf(Choice<NE>::logit(mine_key) - top) : 0.f;
   float sum = all;
   if (p.norm_topk) { sum = wave_sum_f32(w); if (all != all) sum = all; }
   if (lane < p.top_k) {
@@ -208,77 +244,184 @@ static __device__ void write_choice(const MoeParams& p, uint32_t t, uint32_t lan
   }
 }
 
+// the choice in a launch of its own, a wavefront a token
+template <int NE>
+__global__ __launch_bounds__(64)
+void pa_moe_choice_kernel(MoeParams p) { write_choice<NE>(p, blockIdx.x, threadIdx.x); }
+
 // ---- 2: gate and up ------------------------------------------------------------------------------
-template <int KIND, int NE, int RW>
-__global__ __launch_bounds__(256)
+// A workgroup: 16 rows of h (half a block of the next kernel's input) of one expert, for up to GROUP tokens that chose it.  Pairs (token, place) are grouped in
+// windows of whole tokens, at most MOE_WINDOW pairs: of those with the same expert, every GROUP-th leads, and its workgroups read the weights once for itself and those behind it.
+#define MOE_WINDOW 256
+template <int KIND, int NE, int RW, int GROUP, bool CHOSEN>
+__global__ __launch_bounds__(1024 / RW)
 void pa_moe_gate_up_kernel(MoeParams p) {
-  constexpr int F4 = Piece<KIND>::F4, V = Piece<KIND>::VALUES;
+  constexpr uint32_t STEP = Piece<KIND>::STEP;
+  __shared__ float hs[GROUP][16];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t t = blockIdx.y / p.slots, place = blockIdx.y % p.slots;
-  const uint32_t np = p.dim / V, row0 = (blockIdx.x * 4 + wave) * RW;
-  uint32_t e = p.n_experts;
-  if (place < p.top_k) {
-    Choice<NE> c;
-    c.load(p.logits + (size_t)t * p.logit_stride, p.n_experts, lane);
-    for (uint32_t r = 0; r <= place; r++) e = c.next(lane);
-    e = (uint32_t)__builtin_amdgcn_readfirstlane((int)e);
-  }
-  const float* act = p.xn + (size_t)t * p.xn_floats;
-  float g[RW], u[RW];
+  const uint32_t np = pieces<KIND>(p.dim), first = blockIdx.x * 16, pair = blockIdx.y;
+  uint32_t e = p.n_experts, count = 1, member[GROUP];
+  member[0] = pair;
+  Act<KIND> x[2];
+  load_act<KIND>(x[0], p.xn + (size_t)(pair / p.slots) * p.xn_floats, lane, np);
+  if constexpr (!CHOSEN) {
+    const uint32_t place = pair % p.slots;
+    if (place < p.top_k) {
+      Choice<NE> c;
+      c.load(p.logits + (size_t)(pair / p.slots) * p.logit_stride, p.n_experts, lane);
+      uint32_t m;
+      for (uint32_t r = 0; r <= place; r++) e = c.next(lane, m);
+    }
+  } else if constexpr (GROUP == 1) {
+    e = p.sel[pair];
+  } else {
+    // the window's choices, 64 a register
+    const uint32_t tokens = MOE_WINDOW / p.slots, w0 = pair / p.slots / tokens * tokens * p.slots, w1 = min(w0 + tokens * p.slots, p.n * p.slots), me = pair - w0;
+    uint32_t all[MOE_WINDOW / 64], at = 0;
 #pragma unroll
-  for (int r = 0; r < RW; r++) g[r] = u[r] = 0.f;
-  for (uint32_t q0 = 0; q0 < np; q0 += 64) {
-    const uint32_t q = min(q0 + lane, np - 1);                     // pieces past the end repeat the last one, times zero
-    const float f = q0 + lane < np ? 1.f : 0.f;
-    f4 x[F4];
-    load_act<KIND>(x, act, q);
+    for (int k = 0; k < MOE_WINDOW / 64; k++) all[k] = p.sel[min(w0 + 64 * k + lane, w1 - 1)];
+#pragma unroll
+    for (int k = 0; k < MOE_WINDOW / 64; k++) if (me / 64 == k) at = all[k];
+    e = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)(me & 63));
+    uint64_t after[MOE_WINDOW / 64];
+    uint32_t rank = 0;
+#pragma unroll
+    for (int k = 0; k < MOE_WINDOW / 64; k++) {
+      const uint64_t same = __ballot(all[k] == e && w0 + 64 * k + lane < w1);
+      const uint64_t upto = me >= 64u * k + 63 ? ~0ull : me < 64u * k ? 0ull : (2ull << (me & 63)) - 1;
+      rank += (uint32_t)__popcll(same & upto);
+      after[k] = same & ~upto;
+    }
+    if ((rank - 1) % GROUP) return;                                // rank counts the pair itself
+#pragma unroll
+    for (int j = 1; j < GROUP; j++) {
+      member[j] = pair;
+      bool found = false;
+#pragma unroll
+      for (int k = 0; k < MOE_WINDOW / 64; k++) {
+        if (!found && after[k]) { member[j] = w0 + 64 * k + (uint32_t)__builtin_ctzll(after[k]); after[k] &= after[k] - 1; found = true; count = j + 1; }
+      }
+    }
+  }
+  e = (uint32_t)__builtin_amdgcn_readfirstlane((int)e);
+  const size_t row = (size_t)e * p.ffn + first + wave * RW;
+  float g[GROUP][RW], u[GROUP][RW];
+#pragma unroll
+  for (int j = 0; j < GROUP; j++) {
+#pragma unroll
+    for (int r = 0; r < RW; r++) g[j][r] = u[j][r] = 0.f;
+  }
+  for (uint32_t q0 = 0; q0 < np; q0 += STEP) {
+    const uint32_t q = q0 + lane;
     Piece<KIND> wg[RW], wu[RW];
 #pragma unroll
     for (int r = 0; r < RW; r++) {
-      const size_t at = ((size_t)e * p.ffn + min(row0 + r, p.ffn - 1)) * np + q;
-      load_piece<KIND>(wg[r], p.gate, p.gate_s, at);
-      load_piece<KIND>(wu[r], p.up, p.up_s, at);
+      load_piece<KIND>(wg[r], p.gate, p.gate_s, row + r, q, np);
+      load_piece<KIND>(wu[r], p.up, p.up_s, row + r, q, np);
     }
-    if (f != 0.f) {
+    if (q0) load_act<KIND>(x[0], p.xn + (size_t)(pair / p.slots) * p.xn_floats, q, np);
 #pragma unroll
-      for (int r = 0; r < RW; r++) { g[r] = dot_piece<KIND>(wg[r], x, 1.f, g[r]); u[r] = dot_piece<KIND>(wu[r], x, 1.f, u[r]); }
+    for (int j = 0; j < GROUP; j++) {
+      if (j < (int)count) {
+        if (j + 1 < GROUP && j + 1 < (int)count) load_act<KIND>(x[(j + 1) & 1], p.xn + (size_t)(member[j + 1 < GROUP ? j + 1 : 0] / p.slots) * p.xn_floats, q, np);
+        if (KIND == PA_W_F32 || q < np) {
+#pragma unroll
+          for (int r = 0; r < RW; r++) { g[j][r] = dot_piece<KIND>(wg[r], x[j & 1], 1.f, g[j][r]); u[j][r] = dot_piece<KIND>(wu[r], x[j & 1], 1.f, u[j][r]); }
+        }
+      }
     }
   }
-  float* h = p.h + (size_t)t * p.h_floats;
 #pragma unroll
-  for (int r = 0; r < RW; r++) {
-    const float a = wave_sum_f32(g[r]), b = wave_sum_f32(u[r]);
-    if (lane == 0 && row0 + r < p.ffn) h[act_at<KIND>(place * p.ffn + row0 + r)] = a / (1.0f + expf(-a)) * b;
+  for (int j = 0; j < GROUP; j++) {
+    if (j < (int)count) {
+#pragma unroll
+      for (int r = 0; r < RW; r++) {
+        const float a = wave_sum_f32(g[j][r]), b = wave_sum_f32(u[j][r]);
+        if (lane == 0) hs[j][wave * RW + r] = a / (1.0f + expf(-a)) * b;
+      }
+    }
   }
-  if (blockIdx.x == 0 && place == 0 && wave == 0) write_choice<NE>(p, t, lane);
+  __syncthreads();
+  if (threadIdx.x < count * 16) {
+    uint32_t m = member[0];
+#pragma unroll
+    for (int j = 1; j < GROUP; j++) if (threadIdx.x / 16 == j) m = member[j];
+    float* h = p.h + (size_t)(m / p.slots) * p.h_floats;
+    const uint32_t v = (m % p.slots) * p.ffn + first + threadIdx.x % 16;
+    const float y = hs[threadIdx.x / 16][threadIdx.x % 16];
+    h[act_at<KIND>(v)] = stored<KIND>(v, y);
+    if constexpr (KIND != PA_W_F32) {
+      float s = y;
+      s += dpp_f32<0xB1>(s); s += dpp_f32<0x4E>(s); s += dpp_f32<0x141>(s); s += dpp_f32<0x140>(s);
+      if (threadIdx.x % 16 == 0) h[sum_at(v)] = s;
+    }
+  }
+  if (!CHOSEN && blockIdx.x == 0 && pair % p.slots == 0 && wave == 0) write_choice<NE>(p, pair / p.slots, lane);
 }
 
 // ---- 3: down, weighted sum, residual -------------------------------------------------------------
-template <int KIND, int RW>
+// RW rows of y a wavefront; the next pieces are requested while the present ones are used
+template <int KIND, int RW, bool AHEAD>
 __global__ __launch_bounds__(256)
 void pa_moe_down_kernel(MoeParams p) {
-  constexpr int F4 = Piece<KIND>::F4, V = Piece<KIND>::VALUES;
+  constexpr uint32_t STEP = Piece<KIND>::STEP;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y;
-  const uint32_t np = p.ffn / V, all = p.slots * np, row0 = (blockIdx.x * 4 + wave) * RW;
+  const uint32_t np = pieces<KIND>(p.ffn), all = p.slots * np, row0 = (blockIdx.x * 4 + wave) * RW;
   const float* act = p.h + (size_t)t * p.h_floats;
   const uint32_t* sel = p.sel + (size_t)t * p.slots;
   const float* sel_w = p.sel_w + (size_t)t * p.slots;
   float a[RW];
 #pragma unroll
   for (int r = 0; r < RW; r++) a[r] = 0.f;
-  for (uint32_t q0 = 0; q0 < all; q0 += 64) {
-    const uint32_t q = q0 + lane;
-    if (q < all) {
-      const uint32_t place = q / np, e = sel[place];
-      const float f = sel_w[place];
-      f4 x[F4];
-      load_act<KIND>(x, act, q);
-      Piece<KIND> w[RW];
+  // a lane's place and piece in it, 64 further each time
+  const uint32_t my_sel = sel[min(lane, p.slots - 1)], step_place = 64 / np, step_piece = 64 % np;
+  const float my_w = sel_w[min(lane, p.slots - 1)];
+  uint32_t place = lane / np, piece = lane % np;
+  constexpr int LOADS = KIND == PA_W_F32 ? 2 : 1;
+  struct Batch { Act<KIND> x; Piece<KIND> w[RW]; float f[LOADS]; };
+  auto request = [&](Batch& d, uint32_t q0) __attribute__((always_inline)) {
+    load_act<KIND>(d.x, act, q0 + lane, all);
 #pragma unroll
-      for (int r = 0; r < RW; r++) load_piece<KIND>(w[r], p.down, p.down_s, ((size_t)e * p.dim + min(row0 + r, p.dim - 1)) * np + q % np);
+    for (int i = 0; i < LOADS; i++) {
+      const bool in = q0 + 64 * i + lane < all;
+      const uint32_t pl = in ? place : p.slots - 1, pc = in ? piece : np - 1;
+      const size_t e = (uint32_t)__shfl((int)my_sel, (int)pl);
+      d.f[i] = __shfl(my_w, (int)pl);
+      place += step_place; piece += step_piece;
+      if (piece >= np) { piece -= np; place++; }
 #pragma unroll
-      for (int r = 0; r < RW; r++) a[r] = dot_piece<KIND>(w[r], x, f, a[r]);
+      for (int r = 0; r < RW; r++) {
+        const size_t row = e * p.dim + min(row0 + r, p.dim - 1);
+        if constexpr (KIND == PA_W_F32) d.w[r].w[i] = ((const f4*)p.down)[row * np + pc];
+        else load_piece<KIND>(d.w[r], p.down, p.down_s, row, pc, np);
+      }
     }
+  };
+  auto use = [&](Batch& d, uint32_t q0) __attribute__((always_inline)) {
+    if constexpr (KIND == PA_W_F32) {
+      // a piece's float4 may belong to two experts: their weights go into the activations
+#pragma unroll
+      for (int i = 0; i < LOADS; i++) d.x.x[i] *= d.f[i];
+#pragma unroll
+      for (int r = 0; r < RW; r++) a[r] = dot_piece<KIND>(d.w[r], d.x, 1.f, a[r]);
+    } else if (q0 + lane < all) {
+#pragma unroll
+      for (int r = 0; r < RW; r++) a[r] = dot_piece<KIND>(d.w[r], d.x, d.f[0], a[r]);
+    }
+  };
+  if constexpr (AHEAD) {
+    Batch b0, b1;
+    request(b0, 0);
+    for (uint32_t q0 = 0; q0 < all; q0 += 2 * STEP) {
+      if (q0 + STEP < all) request(b1, q0 + STEP);
+      use(b0, q0);
+      if (q0 + STEP < all) {
+        if (q0 + 2 * STEP < all) request(b0, q0 + 2 * STEP);
+        use(b1, q0 + STEP);
+      }
+    }
+  } else {
+    for (uint32_t q0 = 0; q0 < all; q0 += STEP) { Batch b; request(b, q0); use(b, q0); }
   }
 #pragma unroll
   for (int r = 0; r < RW; r++) {
@@ -287,20 +430,39 @@ void pa_moe_down_kernel(MoeParams p) {
   }
 }
 
+template <int KIND, int NE>
+static void launch_experts(const MoeParams& p, hipStream_t s) {
+  // Tokens that share an expert read its weights together where the bytes are what bounds: f32 (27 tokens, 61 experts, 5 chosen: 80 us without groups, 41 with).  Quantised
+  // weights are bound by their instructions too, which a group does not save (16 tokens of Q4_0, 256 experts, 8 chosen: 29 us without, 38 with).
+  constexpr int GROUP = KIND == PA_W_F32 ? 4 : 1;
+  // Up to so many tokens every workgroup makes its choice itself; more have it made once, in a launch of its own.  Both in us, that launch included, for 4, 8 and 12 tokens (256 experts, 8
+  // chosen; f32: 61 and 5): Q4_0 15.2 and 15.1, 25.8 and 21.3, 36.8 and 27.6; Q8_0 19.0 and 23.6, 34.4 and 37.2, 47.4 and 50.0; f32 14.3 and 17.9, 21.8 and 25.8, 30.0 and 32.4, and 56 and 46 for 27.
+  constexpr uint32_t INLINE = KIND == PA_W_Q4_0 ? 4 : 12;
+  const dim3 grid(p.ffn / 16, p.n * p.slots);
+  if (p.n <= INLINE) {
+    hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, NE, 2, 1, false>), grid, dim3(512), 0, s, p);
+  } else {
+    hipLaunchKernelGGL(pa_moe_choice_kernel<NE>, dim3(p.n), dim3(64), 0, s, p);
+    hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, NE, 4, GROUP, true>), grid, dim3(256), 0, s, p);
+  }
+}
 template <int KIND>
-static hipError_t launch_kind(const MoeParams& p, hipStream_t s) {
+static hipError_t launch_kind(const MoeParams& p, int n_cu, hipStream_t s) {
   const uint32_t rows = p.n_experts + (p.slots > p.top_k ? 1 : 0);
   hipLaunchKernelGGL(pa_moe_router_kernel<KIND>, dim3((rows + 1 + 3) / 4, p.n), dim3(256), 0, s, p, rows);
-  constexpr uint32_t RW = 4;
-  const dim3 gu((p.ffn + 4 * RW - 1) / (4 * RW), p.n * p.slots);
-  if (p.n_experts <= 256) hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, 4, RW>), gu, dim3(256), 0, s, p);
-  else hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, 16, RW>), gu, dim3(256), 0, s, p);
-  hipLaunchKernelGGL((pa_moe_down_kernel<KIND, RW>), dim3((p.dim + 4 * RW - 1) / (4 * RW), p.n), dim3(256), 0, s, p);
+  if (p.n_experts <= 256) launch_experts<KIND, 4>(p, s); else launch_experts<KIND, 16>(p, s);
+  // Rows a wavefront: quantised weights share the activations' loads over as many rows as still give every SIMD of the chip three wavefronts
+  // (16 tokens of Q4_0, 2048 rows: 20.4 us with 8 rows, 24.4 with 4; 5 tokens of Q8_0: 19.0 and 15.1; one token: 5.0 with 2 and the next loads ahead, 5.5 without them, 5.1 with 1);
+  // f32 pieces are short (27 tokens: 26.3 us with 2 rows, 28.8 with 4).
+  auto down = [&](auto* kernel, uint32_t rw) { hipLaunchKernelGGL(kernel, dim3((p.dim + 4 * rw - 1) / (4 * rw), p.n), dim3(256), 0, s, p); };
+  if (p.n == 1) down(pa_moe_down_kernel<KIND, 2, true>, 2);
+  else if (KIND == PA_W_F32) down(pa_moe_down_kernel<KIND, 2, false>, 2);
+  else if ((uint64_t)p.n * (p.dim / 8) >= (uint64_t)n_cu * 12) down(pa_moe_down_kernel<KIND, 8, false>, 8);
+  else down(pa_moe_down_kernel<KIND, 4, false>, 4);
   return hipGetLastError();
 }
 
 hipError_t pa_launch_moe(const MoeParams& p, int n_cu, hipStream_t s) {
-  (void)n_cu;
   // grid rows are tokens x places: at most 65535 of them a launch
   const uint32_t most = 65535u / p.slots;
   for (uint32_t t = 0; t < p.n; t += most) {
@@ -311,7 +473,7 @@ hipError_t pa_launch_moe(const MoeParams& p, int n_cu, hipStream_t s) {
     if (q.weights) q.weights += (size_t)t * p.top_k;
     q.xn += (size_t)t * p.xn_floats; q.h += (size_t)t * p.h_floats; q.logits += (size_t)t * p.logit_stride;
     q.sel += (size_t)t * p.slots; q.sel_w += (size_t)t * p.slots;
-    const hipError_t e = p.kind == PA_W_F32 ? launch_kind<PA_W_F32>(q, s) : p.kind == PA_W_Q8_0 ? launch_kind<PA_W_Q8_0>(q, s) : launch_kind<PA_W_Q4_0>(q, s);
+    const hipError_t e = p.kind == PA_W_F32 ? launch_kind<PA_W_F32>(q, n_cu, s) : p.kind == PA_W_Q8_0 ? launch_kind<PA_W_Q8_0>(q, n_cu, s) : launch_kind<PA_W_Q4_0>(q, n_cu, s);
     if (e != hipSuccess) return e;
   }
   return hipSuccess;
