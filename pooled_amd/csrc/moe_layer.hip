@@ -35,17 +35,19 @@ static __device__ inline uint32_t wave_max_u32(uint32_t v) {
 
 // ---- weights: what a lane holds of a row at a time -----------------------------------------------
 // Q8_0 and Q4_0: a block of 32 values with its scale; F32: two times four values, 64 lanes apart.  X: the float4 of activation that go with it.
-// Dequantisation is what bounds a pass of several tokens, so it is kept to 0.6 (Q4_0) and 0.75 (Q8_0) instructions a weight beside the multiply-add: the bits of an unsigned weight u in the low bits of an
-// f16 ARE the number u 2^-24 (subnormal), and the mixed-precision multiply-add takes an f16 as it is.  A Q4_0 word gives its eight nibbles as four masked pairs, every other
-// one 16 times too large in place: the activations that meet those (elements 16 to 31 of a block) are kept divided by 16.  Q8_0 bytes are made unsigned by flipping their sign bit and spread over
-// halves by byte permutes.  The offsets, 8 and 128, come off as the offset times the block's sum of activations, which is kept beside them.
+// Dequantisation is what bounds a pass of several tokens, so it is kept to 0.6 (Q4_0) and 1 (Q8_0: the conversion of a signed byte in place) instructions a weight beside the multiply-add.
+// Q4_0: the bits of an unsigned weight u in the low bits of an f16 ARE the number u 2^-24 (subnormal), and the mixed-precision multiply-add takes an f16 as it is.  A word gives its eight
+// nibbles as four masked pairs, every other one 16 times too large in place: the activations that meet those (elements 16 to 31 of a block) are kept divided by 16.  The offset of 8 comes
+// off as 8 times the block's sum of activations, which is kept beside them; a block's largest weight is 8 or close to it, so at most a bit of the sum is lost to that.  (For Q8_0 the same with
+// an offset of 128 would lose up to seven bits where a block's weights are small, and was no faster.)
 template <int KIND> struct Piece { static constexpr int F4 = 8; static constexpr uint32_t STEP = 64; u4 w[KIND == PA_W_Q8_0 ? 2 : 1]; uint16_t sc; };
 template <> struct Piece<PA_W_F32> { static constexpr int F4 = 2; static constexpr uint32_t STEP = 128; f4 w[2]; };
 template <int KIND> struct Act { f4 x[Piece<KIND>::F4]; float sum; uint32_t have; };   // have: how many of the lane's loads lie in the row
 template <int KIND> static __device__ inline uint32_t pieces(uint32_t values) { return KIND == PA_W_F32 ? values / 4 : values / 32; }
 
 static __device__ inline float f16_bits_f32(uint16_t b) { _Float16 h; __builtin_memcpy(&h, &b, 2); return (float)h; }
-static __device__ inline float half_of(uint32_t w, int i) { h2v v; __builtin_memcpy(&v, &w, 4); return (float)v[i]; }
+static __device__ inline h2v halves(uint32_t w) { h2v v; __builtin_memcpy(&v, &w, 4); return v; }
+static __device__ inline float half_of(uint32_t w, int i) { return (float)halves(w)[i]; }
 
 // acc + f * (piece . x)
 template <int KIND>
@@ -63,12 +65,11 @@ static __device__ inline float dot_piece(const Piece<KIND>& r, const Act<KIND>& 
   } else if constexpr (KIND == PA_W_Q8_0) {
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-      const uint32_t word = r.w[i >> 2][i & 3] ^ 0x80808080u;
-      const uint32_t lo = __builtin_amdgcn_perm(0u, word, 0x0c010c00u), hi = __builtin_amdgcn_perm(0u, word, 0x0c030c02u);
-      a = __builtin_fmaf(half_of(lo, 0), x[i][0], a); b = __builtin_fmaf(half_of(lo, 1), x[i][1], b);
-      a = __builtin_fmaf(half_of(hi, 0), x[i][2], a); b = __builtin_fmaf(half_of(hi, 1), x[i][3], b);
+      const uint32_t word = r.w[i >> 2][i & 3];
+      a = __builtin_fmaf((float)(int8_t)word, x[i][0], a); b = __builtin_fmaf((float)(int8_t)(word >> 8), x[i][1], b);
+      a = __builtin_fmaf((float)(int8_t)(word >> 16), x[i][2], a); b = __builtin_fmaf((float)(int8_t)(word >> 24), x[i][3], b);
     }
-    return __builtin_fmaf(__builtin_fmaf(a + b, 16777216.0f, -128.0f * act.sum), f * f16_bits_f32(r.sc), acc);
+    return __builtin_fmaf(a + b, f * f16_bits_f32(r.sc), acc);
   } else {
     // byte j of the block = elements j (low nibble) and j + 16 (high)
 #pragma unroll
@@ -109,7 +110,7 @@ static __device__ inline void load_act(Act<KIND>& d, const float* act, uint32_t 
     const float* g = act + (c / 64) * GROUP_FLOATS;
 #pragma unroll
     for (int i = 0; i < 8; i++) d.x[i] = ((const f4*)g)[i * 64 + c % 64];
-    d.sum = g[2048 + c % 64] + g[2112 + c % 64];
+    if constexpr (KIND == PA_W_Q4_0) d.sum = g[2048 + c % 64] + g[2112 + c % 64];
   }
 }
 template <int KIND>
@@ -174,7 +175,7 @@ void pa_moe_router_kernel(MoeParams p, uint32_t rows) {
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] = stored<KIND>(4 * q, v[j]);
       *(f4*)(xn + act_at<KIND>(4 * q)) = v;
-      if (KIND != PA_W_F32 && (lane & 3) == 0) xn[sum_at(4 * q)] = sum;
+      if (KIND == PA_W_Q4_0 && (lane & 3) == 0) xn[sum_at(4 * q)] = sum;
     }
   }
 }
@@ -350,7 +351,7 @@ void pa_moe_gate_up_kernel(MoeParams p) {
     const uint32_t v = (m % p.slots) * p.ffn + first + threadIdx.x % 16;
     const float y = hs[threadIdx.x / 16][threadIdx.x % 16];
     h[act_at<KIND>(v)] = stored<KIND>(v, y);
-    if constexpr (KIND != PA_W_F32) {
+    if constexpr (KIND == PA_W_Q4_0) {
       float s = y;
       s += dpp_f32<0xB1>(s); s += dpp_f32<0x4E>(s); s += dpp_f32<0x141>(s); s += dpp_f32<0x140>(s);
       if (threadIdx.x % 16 == 0) h[sum_at(v)] = s;
