@@ -29,8 +29,8 @@ struct CtxBox { pa_ctx* ctx; };
 static void box_finalize(napi_env, void* data, void*) { CtxBox* b = (CtxBox*)data; if (b) { if (b->ctx) pa_destroy(b->ctx); delete b; } }
 
 struct Args {
-  napi_env env; size_t argc; napi_value argv[16]; bool ok;
-  Args(napi_env e, napi_callback_info info) : env(e), argc(16), ok(true) { if (napi_get_cb_info(e, info, &argc, argv, nullptr, nullptr) != napi_ok) ok = false; }
+  napi_env env; size_t argc; napi_value argv[24]; bool ok;
+  Args(napi_env e, napi_callback_info info) : env(e), argc(24), ok(true) { if (napi_get_cb_info(e, info, &argc, argv, nullptr, nullptr) != napi_ok) ok = false; }
   double num(size_t i) { double d = 0; if (i >= argc || napi_get_value_double(env, argv[i], &d) != napi_ok) ok = false; return d; }
   uint32_t u32(size_t i) { return (uint32_t)num(i); }
   void* ptr(size_t i) {                       // device address as a number; null / undefined -> nullptr
@@ -77,6 +77,18 @@ static double prop_f64(napi_env env, napi_value o, const char* k, double def) {
   if (napi_has_named_property(env, o, k, &has) != napi_ok || !has) return def;
   double d; if (napi_get_named_property(env, o, k, &v) != napi_ok || napi_get_value_double(env, v, &d) != napi_ok) return def;
   return d;
+}
+
+// a TypedArray property of o, or nullptr where it is missing, null or undefined; *bytes: its size
+static void* prop_host(napi_env env, napi_value o, const char* k, size_t* bytes) {
+  *bytes = 0;
+  napi_value v; bool is = false;
+  if (napi_get_named_property(env, o, k, &v) != napi_ok || napi_is_typedarray(env, v, &is) != napi_ok || !is) return nullptr;
+  napi_typedarray_type ty; size_t len, off; napi_value ab; void* data = nullptr;
+  if (napi_get_typedarray_info(env, v, &ty, &len, &data, &ab, &off) != napi_ok) return nullptr;
+  static const size_t esz[] = {1, 1, 1, 2, 2, 4, 4, 4, 8, 8, 8};
+  *bytes = (size_t)ty < sizeof esz / sizeof *esz ? len * esz[ty] : 0;
+  return data;
 }
 
 // create({nH, nKV, hd, nRot, ropeTheta, eps, maxSeq, nLayers, maxCols, flags}) -> handle
@@ -291,6 +303,90 @@ static napi_value AttnLayerPrefill(napi_env env, napi_callback_info info) {
   int rc = pa_attn_layer_prefill(c, layer, wqkv, wo, nw, qw, kw, x, xs, base, n); if (rc) return throw_pa(env, c, rc, "pa_attn_layer_prefill"); return undefined(env);
 }
 
+// ---- the gated delta rule ----
+// deltaCreate(ctx, {nKHeads, nVHeads, headK, headV, convWidth, nLayers, scale, eps, flags}) -> handle (a number)
+static napi_value DeltaCreate(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); if (a.argc < 2) a.ok = false; CHECK_ARGS("deltaCreate");
+  napi_value o = a.argv[1];
+  pa_delta_config d; memset(&d, 0, sizeof d);
+  d.n_k_heads = prop_u32(env, o, "nKHeads", 0); d.n_v_heads = prop_u32(env, o, "nVHeads", 0); d.head_k = prop_u32(env, o, "headK", 0); d.head_v = prop_u32(env, o, "headV", 0);
+  d.conv_width = prop_u32(env, o, "convWidth", 0); d.n_layers = prop_u32(env, o, "nLayers", 1); d.scale = (float)prop_f64(env, o, "scale", 0); d.eps = (float)prop_f64(env, o, "eps", 1e-6);
+  d.flags = prop_u32(env, o, "flags", PA_DELTA_L2NORM);
+  pa_delta* dn = nullptr;
+  int rc = pa_delta_create(c, &d, &dn); if (rc) return throw_pa(env, c, rc, "pa_delta_create"); return num_value(env, (double)(uintptr_t)dn);
+}
+static napi_value DeltaDestroy(napi_env env, napi_callback_info info) { ARGS; pa_ctx* c = a.ctx(0); pa_delta* dn = (pa_delta*)a.ptr(1); CHECK_ARGS("deltaDestroy"); int rc = pa_delta_destroy(c, dn); if (rc) return throw_pa(env, c, rc, "pa_delta_destroy"); return undefined(env); }
+static napi_value DeltaReset(napi_env env, napi_callback_info info) { ARGS; pa_ctx* c = a.ctx(0); pa_delta* dn = (pa_delta*)a.ptr(1); uint32_t l = a.u32(2); CHECK_ARGS("deltaReset"); int rc = pa_delta_reset(c, dn, l); if (rc) return throw_pa(env, c, rc, "pa_delta_reset"); return undefined(env); }
+// deltaRead / deltaWrite(ctx, delta, layer, which, Float32Array)
+static napi_value DeltaRead(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); pa_delta* dn = (pa_delta*)a.ptr(1); uint32_t l = a.u32(2); int which = (int)a.u32(3); size_t n; void* h = a.host(4, &n); CHECK_ARGS("deltaRead");
+  if (n < pa_delta_state_bytes(dn, which)) { napi_throw_range_error(env, nullptr, "deltaRead: array shorter than the state"); return nullptr; }
+  int rc = pa_delta_read(c, dn, l, which, h); if (rc) return throw_pa(env, c, rc, "pa_delta_read"); return undefined(env);
+}
+static napi_value DeltaWrite(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); pa_delta* dn = (pa_delta*)a.ptr(1); uint32_t l = a.u32(2); int which = (int)a.u32(3); size_t n; void* h = a.host(4, &n); CHECK_ARGS("deltaWrite");
+  if (n < pa_delta_state_bytes(dn, which)) { napi_throw_range_error(env, nullptr, "deltaWrite: array shorter than the state"); return nullptr; }
+  int rc = pa_delta_write(c, dn, l, which, h); if (rc) return throw_pa(env, c, rc, "pa_delta_write"); return undefined(env);
+}
+// deltaStateBytes(delta, which), deltaStatePtr(delta, layer, which) -> device address
+static napi_value DeltaStateBytes(napi_env env, napi_callback_info info) { ARGS; pa_delta* dn = (pa_delta*)a.ptr(0); int which = (int)a.u32(1); CHECK_ARGS("deltaStateBytes"); return num_value(env, (double)pa_delta_state_bytes(dn, which)); }
+static napi_value DeltaStatePtr(napi_env env, napi_callback_info info) { ARGS; pa_delta* dn = (pa_delta*)a.ptr(0); uint32_t l = a.u32(1); int which = (int)a.u32(2); CHECK_ARGS("deltaStatePtr"); return num_value(env, (double)(uintptr_t)pa_delta_state_ptr(dn, l, which)); }
+// deltaGlue(ctx, delta, layer, qkv, qkvStride, convW, convB | null, a, b, abStride, aLog, dtBias, nCols, nCommit, out, outStride, g, beta, gateStride)
+static napi_value DeltaGlue(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); pa_delta* dn = (pa_delta*)a.ptr(1); uint32_t layer = a.u32(2); const float* x = (const float*)a.ptr(3); uint32_t xs = a.u32(4);
+  const float* w = (const float*)a.ptr(5); const float* bias = (const float*)a.ptr(6); const float* ga = (const float*)a.ptr(7); const float* gb = (const float*)a.ptr(8); uint32_t abs_ = a.u32(9);
+  const float* al = (const float*)a.ptr(10); const float* dt = (const float*)a.ptr(11); uint32_t n = a.u32(12), commit = a.u32(13); float* out = (float*)a.ptr(14); uint32_t os = a.u32(15);
+  float* g = (float*)a.ptr(16); float* beta = (float*)a.ptr(17); uint32_t gs = a.u32(18); CHECK_ARGS("deltaGlue");
+  int rc = pa_delta_glue(c, dn, layer, x, xs, w, bias, ga, gb, abs_, al, dt, n, commit, out, os, g, beta, gs); if (rc) return throw_pa(env, c, rc, "pa_delta_glue"); return undefined(env);
+}
+// deltaDecode(ctx, delta, layer, q, qStride, k, kStride, v, vStride, g, beta, gateStride, nCols, nCommit, out | null, outStride, outDtype)
+static napi_value DeltaDecode(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); pa_delta* dn = (pa_delta*)a.ptr(1); uint32_t layer = a.u32(2); const float* q = (const float*)a.ptr(3); uint32_t qs = a.u32(4);
+  const float* k = (const float*)a.ptr(5); uint32_t ks = a.u32(6); const float* v = (const float*)a.ptr(7); uint32_t vs = a.u32(8); const float* g = (const float*)a.ptr(9); const float* beta = (const float*)a.ptr(10);
+  uint32_t gs = a.u32(11), n = a.u32(12), commit = a.u32(13); void* out = a.ptr(14); uint32_t os = a.u32(15); int dt = (int)a.u32(16); CHECK_ARGS("deltaDecode");
+  int rc = pa_delta_decode(c, dn, layer, q, qs, k, ks, v, vs, g, beta, gs, n, commit, out, os, dt); if (rc) return throw_pa(env, c, rc, "pa_delta_decode"); return undefined(env);
+}
+// deltaPrefill(ctx, delta, layer, q, qStride, k, kStride, v, vStride, g, beta, gateStride, nCols, out | null, outStride, outDtype)
+static napi_value DeltaPrefill(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); pa_delta* dn = (pa_delta*)a.ptr(1); uint32_t layer = a.u32(2); const float* q = (const float*)a.ptr(3); uint32_t qs = a.u32(4);
+  const float* k = (const float*)a.ptr(5); uint32_t ks = a.u32(6); const float* v = (const float*)a.ptr(7); uint32_t vs = a.u32(8); const float* g = (const float*)a.ptr(9); const float* beta = (const float*)a.ptr(10);
+  uint32_t gs = a.u32(11), n = a.u32(12); void* out = a.ptr(13); uint32_t os = a.u32(14); int dt = (int)a.u32(15); CHECK_ARGS("deltaPrefill");
+  int rc = pa_delta_prefill(c, dn, layer, q, qs, k, ks, v, vs, g, beta, gs, n, out, os, dt); if (rc) return throw_pa(env, c, rc, "pa_delta_prefill"); return undefined(env);
+}
+
+// ---- mixture of experts ----
+// moeCreate(ctx, {dim, ffn, nExperts, topK, kind, flags}, {router, gate, up, down [, gateScales, upScales, downScales]
+//           [, sharedGate, sharedGateW, sharedUpW, sharedDownW, sharedGateScales, sharedUpScales, sharedDownScales]}) -> handle (a number); TypedArrays
+static napi_value MoeCreate(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); if (a.argc < 3) a.ok = false; CHECK_ARGS("moeCreate");
+  napi_value o = a.argv[1], h = a.argv[2];
+  pa_moe_config m; memset(&m, 0, sizeof m);
+  m.dim = prop_u32(env, o, "dim", 0); m.ffn = prop_u32(env, o, "ffn", 0); m.n_experts = prop_u32(env, o, "nExperts", 0); m.top_k = prop_u32(env, o, "topK", 0);
+  m.kind = (int)prop_u32(env, o, "kind", 0); m.flags = prop_u32(env, o, "flags", 0);
+  // u32 x u32 fits in 64 bits; the limits that pa_moe_create checks keep the rest far below that
+  const uint64_t values = (uint64_t)m.dim * m.ffn, wb = m.kind == PA_W_F32 ? values * 4 : m.kind == PA_W_Q8_0 ? values : values / 2, sb = m.kind == PA_W_F32 ? 0 : values / 32 * 2;
+  const uint64_t n = m.n_experts < 65536 ? m.n_experts : 65536, shared = m.flags & PA_MOE_SHARED ? 1 : 0;
+  bool fits = m.dim < 65536 && m.ffn < 65536;
+  auto plane = [&](const char* name, uint64_t need) { size_t have; void* p = prop_host(env, h, name, &have); if (have < need) fits = false; return p; };
+  pa_moe_planes p; memset(&p, 0, sizeof p);
+  p.h_router = (const float*)plane("router", n * m.dim * 4);
+  p.h_gate = plane("gate", n * wb); p.h_up = plane("up", n * wb); p.h_down = plane("down", n * wb);
+  p.h_gate_s = (const uint16_t*)plane("gateScales", n * sb); p.h_up_s = (const uint16_t*)plane("upScales", n * sb); p.h_down_s = (const uint16_t*)plane("downScales", n * sb);
+  p.h_shared_gate = (const float*)plane("sharedGate", shared * m.dim * 4);
+  p.h_shared_gate_w = plane("sharedGateW", shared * wb); p.h_shared_up_w = plane("sharedUpW", shared * wb); p.h_shared_down_w = plane("sharedDownW", shared * wb);
+  p.h_shared_gate_s = (const uint16_t*)plane("sharedGateScales", shared * sb); p.h_shared_up_s = (const uint16_t*)plane("sharedUpScales", shared * sb); p.h_shared_down_s = (const uint16_t*)plane("sharedDownScales", shared * sb);
+  if (!fits) { napi_throw_range_error(env, nullptr, "moeCreate: a plane is missing or shorter than the layer needs"); return nullptr; }
+  pa_moe* moe = nullptr;
+  int rc = pa_moe_create(c, &m, &p, &moe); if (rc) return throw_pa(env, c, rc, "pa_moe_create"); return num_value(env, (double)(uintptr_t)moe);
+}
+static napi_value MoeDestroy(napi_env env, napi_callback_info info) { ARGS; pa_ctx* c = a.ctx(0); pa_moe* m = (pa_moe*)a.ptr(1); CHECK_ARGS("moeDestroy"); int rc = pa_moe_destroy(c, m); if (rc) return throw_pa(env, c, rc, "pa_moe_destroy"); return undefined(env); }
+// moeLayer(ctx, moe, normW | null, x, xStride, nCols, y, yStride, ids | null, weights | null)
+static napi_value MoeLayer(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); pa_moe* m = (pa_moe*)a.ptr(1); const float* nw = (const float*)a.ptr(2); const float* x = (const float*)a.ptr(3); uint32_t xs = a.u32(4), n = a.u32(5);
+  float* y = (float*)a.ptr(6); uint32_t ys = a.u32(7); uint32_t* ids = (uint32_t*)a.ptr(8); float* w = (float*)a.ptr(9); CHECK_ARGS("moeLayer");
+  int rc = pa_moe_layer(c, m, nw, x, xs, n, y, ys, ids, w); if (rc) return throw_pa(env, c, rc, "pa_moe_layer"); return undefined(env);
+}
+
 static napi_value Init(napi_env env, napi_value exports) {
   struct { const char* name; napi_callback fn; } table[] = {
     {"create", Create}, {"destroy", Destroy}, {"lastError", LastError}, {"version", Version}, {"layerAlloc", LayerAlloc}, {"sync", Sync},
@@ -302,6 +398,9 @@ static napi_value Init(napi_env env, napi_value exports) {
     {"slotCreate", SlotCreate}, {"slotExport", SlotExport}, {"slotImport", SlotImport}, {"weightCreate", WeightCreate},
     {"weightDestroy", WeightDestroy}, {"gemv", Gemv}, {"gemvNorm", GemvNorm}, {"attnLayerDecode", AttnLayerDecode},
     {"rmsnormF16", RmsnormF16}, {"gemm", Gemm}, {"attnLayerPrefill", AttnLayerPrefill},
+    {"deltaCreate", DeltaCreate}, {"deltaDestroy", DeltaDestroy}, {"deltaReset", DeltaReset}, {"deltaRead", DeltaRead}, {"deltaWrite", DeltaWrite},
+    {"deltaStateBytes", DeltaStateBytes}, {"deltaStatePtr", DeltaStatePtr}, {"deltaGlue", DeltaGlue}, {"deltaDecode", DeltaDecode},
+    {"deltaPrefill", DeltaPrefill}, {"moeCreate", MoeCreate}, {"moeDestroy", MoeDestroy}, {"moeLayer", MoeLayer},
   };
   for (auto& t : table) {
     napi_value fn;

@@ -12,12 +12,16 @@
 // reference) is accepted and ignored: work is enqueued in order on the context's HIP stream, which is the
 // ordering the engine relies on ("the queue is ordered", engine/dense.js:899-901).
 //
+// The other two blocks of a hybrid model's layers are here as well: initDelta / encodeDelta, the gated delta rule with its
+// short convolution (engine/qwen35.js records it where a layer has no attention), and upMoe / encodeMoe, the experts.
+//
 // There is no CPU path here: if the addon is missing, require() throws.
 "use strict";
 const path = require("path");
 const addon = require(path.join(__dirname, "..", "lib", "pooled_attn.node"));
 
 const PA_FLAG_QK_NORM = 1, PA_FLAG_GATE = 2, PA_FLAG_KV_Q8 = 4, PA_FLAG_VERIFY_EXACT = 8, PA_OUT_F32 = 0, PA_OUT_F16 = 1;
+const PA_DELTA_L2NORM = 1, PA_MOE_NORM_TOPK = 1, PA_MOE_SHARED = 2;
 const PA_W_F32 = 0, PA_W_Q8_0 = 1, PA_W_Q4_0 = 2;             // weight kinds of the projections (include/pooled_attn.h)
 
 class HipAttention {
@@ -70,6 +74,11 @@ class HipAttention {
     for (const k of Object.keys(this.B)) addon.free(this.ctx, this.B[k].ptr);
     for (const L of this.layers) { if (L.qNorm) addon.free(this.ctx, L.qNorm); if (L.kNorm) addon.free(this.ctx, L.kNorm); if (L.attnNorm) addon.free(this.ctx, L.attnNorm); }
     for (const w of this._weights || []) addon.weightDestroy(this.ctx, w);
+    for (const m of this._moes || []) addon.moeDestroy(this.ctx, m);
+    if (this.delta) {
+      for (const L of this.delta.layers) for (const k of Object.keys(L)) if (L[k]) addon.free(this.ctx, L[k]);
+      addon.deltaDestroy(this.ctx, this.delta.handle);
+    }
     addon.free(this.ctx, this._ones);
     addon.destroy(this.ctx);
     this.ctx = null;
@@ -267,6 +276,68 @@ class HipAttention {
     const gate = this.gate ? addon.gateBuffer(this.ctx) : null;
     addon.attnGather(this.ctx, LB.layer, null, 0, gate, this.dims.qDim, sel, selStride, maxRows, nCols, this.B.attnOut.ptr, this._outStride(), this.outDtype);
   }
+
+  // ---- gated-delta-rule layers ----
+  // o: { nKHeads, nVHeads, headK, headV, convWidth, nLayers, scale, eps, l2norm = true }.  States of all such layers (counted from 0, without the
+  // attention layers) and their column buffers: B.dQkv [q | k | v] and B.dA, B.dB in front of the pre-step, B.dOut behind.
+  initDelta(o) {
+    if (this.delta) throw new Error("initDelta: called before");
+    const handle = addon.deltaCreate(this.ctx, { nKHeads: o.nKHeads, nVHeads: o.nVHeads, headK: o.headK, headV: o.headV, convWidth: o.convWidth, nLayers: o.nLayers || 1,
+      scale: o.scale || 0, eps: o.eps === undefined ? 1e-6 : o.eps, flags: o.l2norm === false ? 0 : PA_DELTA_L2NORM });
+    const key = o.nKHeads * o.headK, val = o.nVHeads * o.headV;
+    const al = (n) => Math.ceil(n * 4 / 256) * 256;
+    const mkB = (n) => ({ ptr: addon.malloc(this.ctx, this.NC * al(n)), stride: al(n), n: n });
+    this.delta = { handle: handle, key: key, val: val, channels: 2 * key + val, width: o.convWidth, nVHeads: o.nVHeads, layers: [] };
+    for (let i = 0; i < (o.nLayers || 1); i++) this.delta.layers.push({ convW: 0, convB: 0, aLog: 0, dtBias: 0 });
+    Object.assign(this.B, { dQkv: mkB(this.delta.channels), dConv: mkB(this.delta.channels), dA: mkB(o.nVHeads), dB: mkB(o.nVHeads), dG: mkB(o.nVHeads), dBeta: mkB(o.nVHeads), dOut: mkB(val) });
+  }
+  // w: { convW: [channels][convWidth], convB: [channels] or null, aLog: [nVHeads], dtBias: [nVHeads] }
+  setDeltaLayer(i, w) {
+    const D = this.delta, L = D.layers[i], want = { convW: D.channels * D.width, convB: D.channels, aLog: D.nVHeads, dtBias: D.nVHeads };
+    for (const k of Object.keys(want)) {
+      if (k === "convB" && !w[k]) { if (L[k]) { addon.free(this.ctx, L[k]); L[k] = 0; } continue; }
+      if (w[k].length !== want[k]) throw new Error("setDeltaLayer: " + k + " must have " + want[k] + " elements");
+      if (!L[k]) L[k] = addon.malloc(this.ctx, want[k] * 4);
+      addon.upload(this.ctx, L[k], Float32Array.from(w[k]));
+    }
+  }
+  // nCols columns of B.dQkv, B.dA, B.dB through layer i: B.dOut (f32).  commit: the state moves on over so many of them (default: all).  A verify block
+  // runs with commit 0 and, once its accepted columns are known, again over those with { commit: n, stateOnly: true }: a state cannot be cut back.
+  encodeDelta(p, i, nCols, opts) {
+    const D = this.delta, L = D.layers[i], B = this.B, o = opts || {}, commit = o.commit === undefined ? nCols : o.commit;
+    if (!L.convW) throw new Error("encodeDelta: layer " + i + " has no weights (setDeltaLayer)");
+    if (nCols > this.NC) throw new Error("encodeDelta: " + nCols + " columns > batchCols " + this.NC);
+    addon.deltaGlue(this.ctx, D.handle, i, B.dQkv.ptr, B.dQkv.stride / 4, L.convW, L.convB || null, B.dA.ptr, B.dB.ptr, B.dA.stride / 4, L.aLog, L.dtBias, nCols, commit,
+      B.dConv.ptr, B.dConv.stride / 4, B.dG.ptr, B.dBeta.ptr, B.dG.stride / 4);
+    const c = B.dConv.ptr, st = B.dConv.stride / 4, k = c + D.key * 4, v = c + D.key * 8, gs = B.dG.stride / 4, out = o.stateOnly ? null : B.dOut.ptr, os = B.dOut.stride / 4;
+    if (commit === nCols && nCols > 1 && !this._snapNow) addon.deltaPrefill(this.ctx, D.handle, i, c, st, k, st, v, st, B.dG.ptr, B.dBeta.ptr, gs, nCols, out, os, PA_OUT_F32);
+    else addon.deltaDecode(this.ctx, D.handle, i, c, st, k, st, v, st, B.dG.ptr, B.dBeta.ptr, gs, nCols, commit, out, os, PA_OUT_F32);
+  }
+  resetDelta() { for (let i = 0; i < this.delta.layers.length; i++) addon.deltaReset(this.ctx, this.delta.handle, i); }
+  // a layer's states as a session keeps them: { S: Float32Array, conv: Float32Array }
+  readDelta(i) {
+    const get = (w) => { const a = new Float32Array(addon.deltaStateBytes(this.delta.handle, w) / 4); if (a.length) addon.deltaRead(this.ctx, this.delta.handle, i, w, a); return a; };
+    return { S: get(0), conv: get(1) };
+  }
+  writeDelta(i, st) {
+    [st.S, st.conv].forEach((a, w) => {
+      if (a.byteLength !== addon.deltaStateBytes(this.delta.handle, w)) throw new Error("writeDelta: saved state has the wrong shape");
+      if (a.length) addon.deltaWrite(this.ctx, this.delta.handle, i, w, a);
+    });
+  }
+
+  // ---- mixture-of-experts layers ----
+  // m: { kind: "q4" | "q8" | "f32", dim, ffn, nExperts, topK, normTopk, planes } with planes as the addon's moeCreate takes them (sharedGate present: a shared expert)
+  upMoe(m) {
+    const kind = m.kind === "q4" ? PA_W_Q4_0 : m.kind === "q8" ? PA_W_Q8_0 : m.kind === "f32" ? PA_W_F32 : -1;
+    if (kind < 0) throw new Error("upMoe: unknown weight kind " + m.kind);
+    const flags = (m.normTopk ? PA_MOE_NORM_TOPK : 0) | (m.planes.sharedGate ? PA_MOE_SHARED : 0);
+    const h = addon.moeCreate(this.ctx, { dim: m.dim, ffn: m.ffn, nExperts: m.nExperts, topK: m.topK, kind: kind, flags: flags }, m.planes);
+    (this._moes = this._moes || []).push(h);
+    return { handle: h, dim: m.dim, topK: m.topK };
+  }
+  // X (a column buffer of residuals, residualCols(dim) for one) += the layer, in place; nw: device address of the norm's weights
+  encodeMoe(p, moe, nw, X, nCols) { addon.moeLayer(this.ctx, moe.handle, nw || null, X.ptr, X.stride / 4, nCols, X.ptr, X.stride / 4, null, null); }
 
   // ---- DenseEngine shapes (full RoPE, no gate): the glue writes the cache, then attention ----
   // _encodeAttn(pass, BG, seqLen): BG = { layer }; attention of the token at position seqLen - 1
