@@ -18,7 +18,7 @@
 //
 // What bounds it: a workgroup's chunk reads K, Q, K' (32 KB each at head_k 128) and P' (16 KB): 112 KB through one CU's 64 bytes a clock, 0.73 us, while its 168
 // matrix instructions take 0.3 us of four SIMDs.  The first kernel stores these operands in the order in which lanes load them (a fragment is 1 KB), every
-// fragment goes to one wavefront alone, and each is requested a chunk ahead, right behind its last use: no operand passes through LDS but S and X, which change hands
+// fragment goes to one wavefront alone, and each is requested a chunk or two ahead: no operand passes through LDS but S and X, which change hands
 // between the wavefronts twice a chunk.
 #include "blocks_internal.h"
 #include "glue_math.h"
@@ -128,6 +128,21 @@ size_t pa_delta_chunk_ws_bytes(uint32_t chunks, uint32_t nk, uint32_t nv, uint32
   return b;
 }
 
+// inclusive sums over the lanes: within rows of 16, then the rows' last lanes into the rows behind
+template <int CTRL, int ROWS> static __device__ inline double dpp_or_zero(double x) {
+  uint64_t u; __builtin_memcpy(&u, &x, 8);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xF, false), hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, ROWS, 0xF, false);
+  u = (uint64_t)hi << 32 | lo;
+  __builtin_memcpy(&x, &u, 8);
+  return x;
+}
+static __device__ inline double prefix_sum(double x) {
+  x += dpp_or_zero<0x111, 0xF>(x); x += dpp_or_zero<0x112, 0xF>(x); x += dpp_or_zero<0x114, 0xF>(x); x += dpp_or_zero<0x118, 0xF>(x);      // 1, 2, 4, 8 lanes to the right
+  x += dpp_or_zero<0x142, 0xA>(x);                                 // lane 15 to row 1, 47 to row 3
+  x += dpp_or_zero<0x143, 0xC>(x);                                 // lane 31 to rows 2 and 3
+  return x;
+}
+
 // ---- 1: what does not depend on the state ----------------------------------------------------------
 // A wavefront has 16 rows of the chunk ("its tile").  Every product below is laid out so that a result, as the matrix instructions leave it (lane: column l16, rows 4 lg + r), is the
 // next product's operand as it stands: contractions run over 4 lg + r, not over 8 lg + j.  So A and P stay in registers from K K^T and K Q^T on; LDS holds the keys, which every
@@ -143,6 +158,7 @@ template <int HK> struct PrepLds {
   };
   double G[CHUNK];
   float beta[CHUNK], kfac[CHUNK], row[CHUNK], col[4][48], top[4];
+  int marked;
 };
 
 template <int HK>
@@ -158,20 +174,13 @@ void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
   float* const scal = ws.scal + ((size_t)chunk * p.nv + h) * SCAL_FLOATS;
   const f4 zero = {0.f, 0.f, 0.f, 0.f};
   bool bad = false;
+  if (tid == 0) L.marked = 0;
+  __syncthreads();
 
-  // -- gates: sums of g in 64 bits by one wavefront
-  if (w == 0) {
-    const bool valid = c0 + lane < p.n;
-    const size_t c = min(c0 + lane, p.n - 1);
-    const float g = valid ? p.g[c * p.gate_stride + h] : 0.f, b = valid ? p.beta[c * p.gate_stride + h] : 0.f;
-    bad = !(g <= 0.f) || !(b >= 0.f && b <= 2.f);
-    double G = g > -1e5f ? (double)g : -1e5;                        // exp(-1e5) is 0 as exp(-infinity) is, and differences stay numbers
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) { const double o = __shfl_up(G, d); if (lane >= (uint32_t)d) G += o; }
-    L.G[lane] = G;
-    L.beta[lane] = b;
-  }
   // -- rows: lengths, scaled pairs.  Lane: row l16 of the tile, values 8 lg .. + 7 of every k step
+  const bool gated = c0 + lane < p.n;
+  const size_t gc = (size_t)min(c0 + lane, p.n - 1) * p.gate_stride + h;
+  const float g_in = p.g[gc], b_in = p.beta[gc];                   // of row `lane`; requested in front of the rows, used while those are on their way
   Pair8 kf[KS], qf[KS];
   {
     const uint32_t row = w * 16 + l16;
@@ -184,6 +193,13 @@ void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
     for (int s = 0; s < KS; s++)
 #pragma unroll
       for (int e = 0; e < 2; e++) { k[s][e] = *(const f4*)(kp + 32 * s + 4 * e); q[s][e] = *(const f4*)(qp + 32 * s + 4 * e); }
+    // gates: sums of g in 64 bits by one wavefront
+    if (w == 0) {
+      const float g = gated ? g_in : 0.f, b = gated ? b_in : 0.f;
+      bad = !(g <= 0.f) || !(b >= 0.f && b <= 2.f);
+      L.G[lane] = prefix_sum(g > -1e5f ? (double)g : -1e5);         // exp(-1e5) is 0 as exp(-infinity) is, and differences stay numbers
+      L.beta[lane] = b;
+    }
     float kk = 0.f, qq = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; s++)
@@ -218,7 +234,9 @@ void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
       if (store_q) { *(h8*)(kq + F::KQ + off) = qf[s].hi; *(h8*)(kq + F::KQ + F::KQ / 2 + off) = qf[s].lo; }
     }
   }
-  const bool mark = __syncthreads_or(bad);
+  if (__any(bad) && lane == 0) L.marked = 1;                       // (one barrier; the library's reduction takes three)
+  __syncthreads();
+  const bool mark = L.marked != 0;
   // decays: of a row from the end of the tile before its own (row), from a row to the end of a later tile's predecessor (col), to the chunk's end (kfac)
   if (tid < 64) {
     const double G = L.G[tid];
@@ -422,9 +440,11 @@ void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
 
 // ---- 2: from chunk to chunk -------------------------------------------------------------------------
 // A workgroup has the state of NT x 16 value columns of a head and twelve wavefronts of three roles.  In a chunk's first phase the four KEYS multiply K by S and make X; in the second the
-// four of STATE multiply K'^T by X and move the state on; each requests its operands while the other works, two chunks ahead.  The four QUERIES, which nothing waits for, multiply Q by S
-// and P' by X.  Two barriers a chunk: S is there | X is there.  Every role has a loop of its own, unrolled by two: no register that a load is still filling is ever
-// copied, and no wait is shared.
+// four of STATE multiply K'^T by X and move the state on; each requests its operands while the other works, one to two chunks ahead.  The four QUERIES, which nothing waits for, have the
+// other halves of the phases: Q S while STATE works, P' X of the chunk before while KEYS do, so S and X are there twice.  Two barriers a chunk: S is there | X is there.  Every role has
+// a loop of its own, unrolled by two: no register that a load is still filling is ever copied, and no wait is shared.  (NT = 2 has no registers for second sets of operands.)
+// What bounds it: the operands, 112 KB a chunk for each workgroup whatever its columns, at 64 bytes a cycle of a CU 1750 of about 3000 cycles, and a chunk's two barriers with
+// their exchanges.  2048 columns of 32 heads: 64 us with the operands from the last-level cache, 53 from L2, 42 alone on the chip; of 48 heads (NT = 2): 84.
 //
 // Scales: E_c is the exponent, per value column, that X of chunk c and the state behind it are scaled by.  It comes from the sums N_c of |S| in front of the chunk before and the
 // sums V of beta |v|: |S| in front of chunk c <= N_(c-1) + V_(c-1), so that KEYS find it a chunk ahead (sums of magnitudes are no smaller than norms, and they neither over- nor
@@ -434,7 +454,7 @@ enum { KEYS, STATE, QUERIES };
 
 template <int HK, int NT> struct ScanLds {
   static constexpr int KS = HK / 32, MT = HK / 64, COLS = 16 * NT;
-  _Float16 S[NT][2][KS * 512], X[NT][2][2 * 512];                  // pairs, as right operands
+  _Float16 S[2][NT][2][KS * 512], X[2][NT][2][2 * 512];            // pairs, as right operands, of even and odd chunks
   f4 bv[2][NT][4 * 64], cv[2][16];                                 // beta v, beta e^G of a chunk and the next, in the order of KEYS' lanes
   f4 norm[2][COLS], val[2][COLS];                                  // N and V, by wavefront
   int exps[2][COLS];
@@ -534,14 +554,14 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
       if (lg == 0) L.norm[c & 1][t * 16 + l16][w] = x;
     }
   };
-  auto put_state = [&](const float (&to)[NT]) __attribute__((always_inline)) {
+  auto put_state = [&](uint32_t c, const float (&to)[NT]) __attribute__((always_inline)) {
 #pragma unroll
     for (int t = 0; t < NT; t++)
 #pragma unroll
       for (int m = 0; m < MT; m++) {
         const Pair4 s = split4<true>(S[t][m] * to[t]);
         const uint32_t d0 = (w * MT + m) * 16 + 4 * lg, off = (d0 >> 5) * 512 + (l16 + 16 * ((d0 & 31) >> 3)) * 8 + (d0 & 7);
-        *(h4*)(&L.S[t][0][off]) = s.hi; *(h4*)(&L.S[t][1][off]) = s.lo;
+        *(h4*)(&L.S[c & 1][t][0][off]) = s.hi; *(h4*)(&L.S[c & 1][t][1][off]) = s.lo;
       }
   };
   auto put_rows = [&](const StateRows& d, uint32_t c) __attribute__((always_inline)) {
@@ -574,13 +594,13 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
   // ---- in front of the first chunk
   KF k0, k1;
   GF g0, g1;
-  PF p0;
+  PF p0, p1;
   StateRows rows1;                                                 // of the coming chunk
   QueryRows q0, q1;
   float m0 = 0.f, m1 = 0.f;
   if constexpr (ROLE == KEYS) { m0 = load_mark(0); m1 = load_mark(1); load_k(k0, 0); load_k(k1, 1); }
   if constexpr (ROLE == STATE) { load_rows(rows1, 0); load_g(g0, 0); put_rows(rows1, 0); }
-  if constexpr (ROLE == QUERIES) { load_query_rows(q0, 0); load_query_rows(q1, 1); load_k(k0, 0); load_p(p0, 0); }
+  if constexpr (ROLE == QUERIES) { load_query_rows(q0, 0); load_query_rows(q1, 1); load_k(k0, 0); load_p(NT > 1 ? p0 : p1, 0); }
   float decay = 0.f, kscale = 0.f, next_decay = 0.f, next_kscale = 0.f;
   if constexpr (ROLE == STATE) { decay = rows1.decay; kscale = rows1.kscale; load_rows(rows1, 1); }
   float sigma_inv[NT];
@@ -590,11 +610,63 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
     own_exponents(0, e);
 #pragma unroll
     for (int t = 0; t < NT; t++) { sigma_inv[t] = pow2(e[t] - 13); to[t] = pow2(13 - e[t]); }
-    if constexpr (ROLE == STATE) put_state(to);
+    if constexpr (ROLE == STATE) put_state(0, to);
     if constexpr (ROLE == KEYS) put_exponent(0, true, m0);
   }
 
-  auto chunk = [&](const uint32_t c, KF& kf, GF& gf, GF& gf_next, QueryRows& qr, float& mark, const float mark_next) __attribute__((always_inline)) {
+  // product with the S of chunk c: keys or queries
+  auto times_state = [&](uint32_t c, uint32_t t, const KF& kf, float from) __attribute__((always_inline)) {
+    f4 r0 = {0.f, 0.f, 0.f, 0.f}, r1 = r0, r2 = r0, r;              // hi hi | hi lo, 2048 times | lo hi
+#pragma unroll
+    for (int s = 0; s < KS; s++) {
+      const h8 sh = *(const h8*)(&L.S[c & 1][t][0][s * 512 + lane * 8]), sl = *(const h8*)(&L.S[c & 1][t][1][s * 512 + lane * 8]);
+      r0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.x[s][0], sh, r0, 0, 0, 0);
+      r1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.x[s][0], sl, r1, 0, 0, 0);
+      r2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.x[s][1], sh, r2, 0, 0, 0);
+    }
+    const float back = from * UNIT_INV;
+#pragma unroll
+    for (int i = 0; i < 4; i++) r[i] = __builtin_fmaf(r1[i], LO_INV, r0[i] + r2[i]) * back;
+    return r;
+  };
+  // product of a pair of left operands with the X of chunk c
+  auto times_x = [&](uint32_t c, uint32_t t, const h8 (&x)[2][2]) __attribute__((always_inline)) {
+    f4 n0 = {0.f, 0.f, 0.f, 0.f}, n1 = n0, n2 = n0, n;
+#pragma unroll
+    for (int s = 0; s < 2; s++) {
+      const h8 xh = *(const h8*)(&L.X[c & 1][t][0][s * 512 + lane * 8]), xl = *(const h8*)(&L.X[c & 1][t][1][s * 512 + lane * 8]);
+      n0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s][0], xh, n0, 0, 0, 0);
+      n1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s][0], xl, n1, 0, 0, 0);
+      n2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s][1], xh, n2, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) n[i] = __builtin_fmaf(n1[i], LO_INV, n0[i] + n2[i]);
+    return n;
+  };
+  // QUERIES: the start state's part of a chunk's output, all factors in, the factor of the other part, and the rows to store; P' X of that chunk comes a phase later
+  f4 held[NT], fx[NT];
+  uint32_t held_rows = 0;
+#pragma unroll
+  for (int t = 0; t < NT; t++) held[t] = fx[t] = f4{0.f, 0.f, 0.f, 0.f};
+  auto put_out = [&](uint32_t c, const PF& pf) __attribute__((always_inline)) {
+    const auto b = buffer((unsigned char*)p.out + ((size_t)c * CHUNK * p.out_stride + (size_t)h * p.hv + v0) * ot, out && held_rows ? ((held_rows - 1) * p.out_stride + COLS) * ot : 0);
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const f4 n = times_x(c, t, pf.x);
+      f4 o;
+#pragma unroll
+      for (int r = 0; r < 4; r++) o[r] = __builtin_fmaf(fx[t][r], n[r], held[t][r]);
+      if (p.out_f16) {
+#pragma unroll
+        for (int r = 0; r < 4; r++) store_f16(b, row_at[r] + t * 32, o[r]);
+      } else {
+#pragma unroll
+        for (int r = 0; r < 4; r++) store_f32(b, row_at[r] + t * 64, o[r]);
+      }
+    }
+  };
+
+  auto chunk = [&](const uint32_t c, KF& kf, GF& gf, GF& gf_next, KF& kf_next, PF& pf, PF& pf_next, QueryRows& qr, float& mark, const float mark_next) __attribute__((always_inline)) {
     lds_barrier();
     int e[NT];
     bool none = false;
@@ -664,36 +736,22 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
     float to[NT], to_inv[NT];
 #pragma unroll
     for (int t = 0; t < NT; t++) { to[t] = pow2(13 - e[t]); to_inv[t] = pow2(e[t] - 13); }
-    f4 held[NT], fq;                                               // QUERIES: the start state's part of the output, all factors in
-    if constexpr (ROLE != STATE) {
-      f4 cv;
-      if constexpr (ROLE == KEYS) cv = L.cv[c & 1][w * 4 + lg];
+    if constexpr (ROLE == KEYS) {
+      const f4 cv = L.cv[c & 1][w * 4 + lg];
 #pragma unroll
       for (int t = 0; t < NT; t++) {
-        f4 r0 = {0.f, 0.f, 0.f, 0.f}, r1 = r0, r2 = r0, r;          // hi hi | hi lo, 2048 times | lo hi
+        const f4 r = times_state(c, t, kf, sigma_inv[t]), bv = L.bv[c & 1][t][w * 64 + lane];
+        f4 x;                                                      // X = beta v - beta e^G K S
 #pragma unroll
-        for (int s = 0; s < KS; s++) {
-          const h8 sh = *(const h8*)(&L.S[t][0][s * 512 + lane * 8]), sl = *(const h8*)(&L.S[t][1][s * 512 + lane * 8]);
-          r0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.x[s][0], sh, r0, 0, 0, 0);
-          r1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.x[s][0], sl, r1, 0, 0, 0);
-          r2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf.x[s][1], sh, r2, 0, 0, 0);
-        }
-        const float back = sigma_inv[t] * UNIT_INV;
-#pragma unroll
-        for (int i = 0; i < 4; i++) r[i] = __builtin_fmaf(r1[i], LO_INV, r0[i] + r2[i]) * back;
-        if constexpr (ROLE == KEYS) {                              // X = beta v - beta e^G K S
-          const f4 bv = L.bv[c & 1][t][w * 64 + lane];
-          f4 x;
-#pragma unroll
-          for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(-cv[i], r[i], bv[i]);
-          const Pair4 s = split4<true>(x * to[t]);
-          const uint32_t i0 = w * 16 + 4 * lg, off = (i0 >> 5) * 512 + (l16 + 16 * ((i0 & 31) >> 3)) * 8 + (i0 & 7);
-          *(h4*)(&L.X[t][0][off]) = s.hi; *(h4*)(&L.X[t][1][off]) = s.lo;
-        } else {
-          held[t] = qr.b * (qr.a * r);
-        }
+        for (int i = 0; i < 4; i++) x[i] = __builtin_fmaf(-cv[i], r[i], bv[i]);
+        const Pair4 s = split4<true>(x * to[t]);
+        const uint32_t i0 = w * 16 + 4 * lg, off = (i0 >> 5) * 512 + (l16 + 16 * ((i0 & 31) >> 3)) * 8 + (i0 & 7);
+        *(h4*)(&L.X[c & 1][t][0][off]) = s.hi; *(h4*)(&L.X[c & 1][t][1][off]) = s.lo;
       }
-      if constexpr (ROLE == QUERIES) { fq = qr.b; load_k(kf, c + 1); load_query_rows(qr, c + 2); }
+    } else if constexpr (ROLE == QUERIES) {
+      if constexpr (NT == 1) load_p(pf_next, c);
+      put_out(max(c, 1u) - 1, pf);                                 // (no rows yet in front of the first chunk)
+      if constexpr (NT > 1) load_p(pf, c);
     } else {
       if constexpr (NT == 1) load_g(gf_next, c + 1);
       put_rows(rows1, c + 1);
@@ -705,66 +763,46 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
       load_k(kf, c + 2);
       mark = load_mark(c + 2);
       put_exponent(c + 1, slow, mark_next);
-    } else {
+    } else if constexpr (ROLE == STATE) {
       f4 n[NT][MT];
 #pragma unroll
       for (int t = 0; t < NT; t++)
 #pragma unroll
-        for (int m = 0; m < (ROLE == STATE ? MT : 1); m++) {
-          f4 n0 = {0.f, 0.f, 0.f, 0.f}, n1 = n0, n2 = n0;
+        for (int m = 0; m < MT; m++) n[t][m] = times_x(c, t, gf.x[m]);
+      if constexpr (NT > 1) load_g(gf, c + 1);                     // no room for two chunks' operands
 #pragma unroll
-          for (int s = 0; s < 2; s++) {
-            const h8 xh = *(const h8*)(&L.X[t][0][s * 512 + lane * 8]), xl = *(const h8*)(&L.X[t][1][s * 512 + lane * 8]);
-            const h8 ah = ROLE == STATE ? gf.x[m][s][0] : p0.x[s][0], al = ROLE == STATE ? gf.x[m][s][1] : p0.x[s][1];
-            n0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, xh, n0, 0, 0, 0);
-            n1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ah, xl, n1, 0, 0, 0);
-            n2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(al, xh, n2, 0, 0, 0);
+      for (int t = 0; t < NT; t++) {
+        const float fs = to_inv[t] * kscale;
+#pragma unroll
+        for (int m = 0; m < MT; m++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const float x = __builtin_fmaf(S[t][m][i], decay, n[t][m][i] * fs);
+            S[t][m][i] = slow ? S[t][m][i] : x;
           }
-#pragma unroll
-          for (int i = 0; i < 4; i++) n[t][m][i] = __builtin_fmaf(n1[i], LO_INV, n0[i] + n2[i]);
-        }
-      if constexpr (ROLE == STATE) {
-        if constexpr (NT > 1) load_g(gf, c + 1);                   // no room for two chunks' operands
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          const float fs = to_inv[t] * kscale;
-#pragma unroll
-          for (int m = 0; m < MT; m++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-              const float x = __builtin_fmaf(S[t][m][i], decay, n[t][m][i] * fs);
-              S[t][m][i] = slow ? S[t][m][i] : x;
-            }
-        }
-        put_state(to);
-        put_norm(c + 1);
-        decay = next_decay; kscale = next_kscale;
-      } else {
-        const auto b = buffer((unsigned char*)p.out + ((size_t)c * CHUNK * p.out_stride + (size_t)h * p.hv + v0) * ot, out && rows ? ((rows - 1) * p.out_stride + COLS) * ot : 0);
-#pragma unroll
-        for (int t = 0; t < NT; t++) {
-          const f4 fx = fq * (to_inv[t] * UNIT_INV);
-          f4 o;
-#pragma unroll
-          for (int r = 0; r < 4; r++) o[r] = __builtin_fmaf(fx[r], n[t][0][r], held[t][r]);
-          if (p.out_f16) {
-#pragma unroll
-            for (int r = 0; r < 4; r++) store_f16(b, row_at[r] + t * 32, o[r]);
-          } else {
-#pragma unroll
-            for (int r = 0; r < 4; r++) store_f32(b, row_at[r] + t * 64, o[r]);
-          }
-        }
-        load_p(p0, c + 1);
       }
+      put_state(c + 1, to);
+      put_norm(c + 1);
+      decay = next_decay; kscale = next_kscale;
+    } else {
+      if constexpr (NT == 1) load_k(kf_next, c + 1);
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        held[t] = qr.b * (qr.a * times_state(c, t, kf, sigma_inv[t]));
+        fx[t] = qr.b * (to_inv[t] * UNIT_INV);
+      }
+      held_rows = rows;
+      if constexpr (NT > 1) load_k(kf, c + 1);
+      load_query_rows(qr, c + 2);
     }
 #pragma unroll
     for (int t = 0; t < NT; t++) sigma_inv[t] = to_inv[t];
   };
   for (uint32_t c = 0; c < chunks; c += 2) {
-    chunk(c, k0, g0, g1, q0, m0, m1);
-    if (c + 1 < chunks) chunk(c + 1, ROLE == QUERIES ? k0 : k1, NT > 1 ? g0 : g1, g0, q1, m1, m0);
+    chunk(c, k0, g0, g1, k1, NT > 1 ? p0 : p1, p0, q0, m0, m1);
+    if (c + 1 < chunks) chunk(c + 1, ROLE == QUERIES && NT > 1 ? k0 : k1, NT > 1 ? g0 : g1, g0, k0, p0, p1, q1, m1, m0);
   }
+  if constexpr (ROLE == QUERIES) { if (NT == 1 && (last & 1)) put_out(last, p1); else put_out(last, p0); }
   if constexpr (ROLE == STATE) {
 #pragma unroll
     for (int t = 0; t < NT; t++)
