@@ -14,7 +14,7 @@
 // rows of q are scaled by a power of two to a norm in [0.5, 1) and, as keys, K' and P', by UNIT more, K' by one for its largest element, and S and X, per value column, by one from a
 // bound: the rule over keys no longer than one with 0 <= beta <= 2, g <= 0 is a contraction, so |S_next| <= |S| + sum beta |v| and |X| <= 2 |S| + beta |v|.  A chunk whose
 // inputs leave that domain (longer or tiny keys, other gates, infinities, NaN) is marked by the first kernel, or found by the bound, and runs token by token in the second, in f32, with
-// the same S: slower (about 1 us a token), but right for every input.
+// the same S: slower (0.43 us a token of 32 heads, 0.04 otherwise), but right for every input.
 //
 // What bounds it: a workgroup's chunk reads K, Q, K' (32 KB each at head_k 128) and P' (16 KB): 112 KB through one CU's 64 bytes a clock, 0.73 us, while its 168
 // matrix instructions take 0.3 us of four SIMDs.  The first kernel stores these operands in the order in which lanes load them (a fragment is 1 KB), every
@@ -458,7 +458,9 @@ template <int HK, int NT> struct ScanLds {
   f4 bv[2][NT][4 * 64], cv[2][16];                                 // beta v, beta e^G of a chunk and the next, in the order of KEYS' lanes
   f4 norm[2][COLS], val[2][COLS];                                  // N and V, by wavefront
   int exps[2][COLS];
-  float slow[2][2][4][COLS];
+  struct {                                                         // a chunk that goes token by token: its rows, scaled, and the wavefronts' partial sums
+    float k[CHUNK][HK], q[CHUNK][HK], v[CHUNK][COLS], decay[CHUNK], beta[CHUNK], part[2][2][4][COLS];
+  } slow;
 };
 static __device__ inline float sum4(const f4 x) { return (x[0] + x[1]) + (x[2] + x[3]); }
 static __device__ inline float sum_abs4(const f4 x) { return (fabsf(x[0]) + fabsf(x[1])) + (fabsf(x[2]) + fabsf(x[3])); }
@@ -675,19 +677,42 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
     const bool slow = __any(none);
     uint32_t rows = rows_of(c);
     if (slow) {
-      // token by token, in f32: dot products over the key dimensions of the four wavefronts of STATE, one exchange each.  What the matrix instructions below make of this chunk is dropped.
+      // token by token, in f32: dot products over the key dimensions of the four wavefronts of STATE, one exchange and one barrier each.  What the matrix instructions below make of this
+      // chunk is dropped.
       const float* const sg = scal + c * scal_step;
-      for (uint32_t i = 0; i < rows; i++) {
-        const size_t col = (size_t)c * CHUNK + i;
-        f4 k[MT], q[MT];
-        if constexpr (ROLE == STATE) {
-          const float dec = expf(p.g[col * p.gate_stride + h]);
+      const size_t first = (size_t)c * CHUNK;
+      auto& Z = L.slow;
+      if constexpr (ROLE == KEYS) {                                // (the others have no registers to spare)
+#pragma unroll 1
+        for (uint32_t x = tid; x < rows * (HK / 4); x += 256) {
+          const uint32_t i = x / (HK / 4), d = x % (HK / 4) * 4;
+          *(f4*)(&Z.k[i][d]) = *(const f4*)(p.k + (first + i) * p.k_stride + kh * HK + d) * sg[4 * 64 + i];
+          if (out) *(f4*)(&Z.q[i][d]) = *(const f4*)(p.q + (first + i) * p.q_stride + kh * HK + d) * sg[5 * 64 + i];
+        }
+#pragma unroll 1
+        for (uint32_t x = tid; x < rows * COLS; x += 256) Z.v[x / COLS][x % COLS] = p.v[(first + x / COLS) * p.v_stride + (size_t)h * p.hv + v0 + x % COLS];
+        if (tid < rows) { Z.decay[tid] = expf(p.g[(first + tid) * p.gate_stride + h]); Z.beta[tid] = p.beta[(first + tid) * p.gate_stride + h]; }
+      }
+      lds_barrier();
+      auto put_token = [&](uint32_t i) __attribute__((always_inline)) {
+        if (out && w == 0 && lg == 0) {
 #pragma unroll
-          for (int m = 0; m < MT; m++) {
-            const uint32_t d = kh * HK + (w * MT + m) * 16 + 4 * lg;
-            k[m] = *(const f4*)(p.k + col * p.k_stride + d) * sg[4 * 64 + i];
-            q[m] = out ? *(const f4*)(p.q + col * p.q_stride + d) * sg[5 * 64 + i] : k[m];
+          for (int t = 0; t < NT; t++) {
+            const auto& x = Z.part[1][i & 1];
+            const uint32_t j = t * 16 + l16;
+            const float o = p.scale * ((x[0][j] + x[1][j]) + (x[2][j] + x[3][j]));
+            const size_t to = (first + i) * p.out_stride + (size_t)h * p.hv + v0 + j;
+            if (p.out_f16) ((_Float16*)p.out)[to] = (_Float16)o; else ((float*)p.out)[to] = o;
           }
+        }
+      };
+#pragma unroll 1
+      for (uint32_t i = 0; i < rows; i++) {
+        f4 k[MT];
+        if constexpr (ROLE == STATE) {
+          const float dec = Z.decay[i];
+#pragma unroll
+          for (int m = 0; m < MT; m++) k[m] = *(const f4*)(&Z.k[i][(w * MT + m) * 16 + 4 * lg]);
 #pragma unroll
           for (int t = 0; t < NT; t++) {
             float a = 0.f;
@@ -696,40 +721,32 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
 #pragma unroll
               for (int r = 0; r < 4; r++) { S[t][m][r] *= dec; a = __builtin_fmaf(S[t][m][r], k[m][r], a); }
             a = rows4_sum(a);
-            if (lg == 0) L.slow[0][i & 1][w][t * 16 + l16] = a;
+            if (lg == 0) Z.part[0][i & 1][w][t * 16 + l16] = a;
           }
         }
         lds_barrier();
         if constexpr (ROLE == STATE) {
-          const float b = p.beta[col * p.gate_stride + h];
+          const float b = Z.beta[i];
 #pragma unroll
           for (int t = 0; t < NT; t++) {
-            const auto& x = L.slow[0][i & 1];
+            const auto& x = Z.part[0][i & 1];
             const uint32_t j = t * 16 + l16;
-            const float u = b * (p.v[col * p.v_stride + (size_t)h * p.hv + v0 + j] - ((x[0][j] + x[1][j]) + (x[2][j] + x[3][j])));
+            const float u = b * (Z.v[i][j] - ((x[0][j] + x[1][j]) + (x[2][j] + x[3][j])));
             float o = 0.f;
 #pragma unroll
-            for (int m = 0; m < MT; m++)
+            for (int m = 0; m < MT; m++) {
+              const f4 q = *(const f4*)(&Z.q[i][(w * MT + m) * 16 + 4 * lg]);
 #pragma unroll
-              for (int r = 0; r < 4; r++) { S[t][m][r] = __builtin_fmaf(u, k[m][r], S[t][m][r]); o = __builtin_fmaf(S[t][m][r], q[m][r], o); }
-            o = rows4_sum(o);
-            if (lg == 0) L.slow[1][i & 1][w][j] = o;
-          }
-        }
-        lds_barrier();
-        if constexpr (ROLE == QUERIES) {
-          if (out && w == 0 && lg == 0) {
-#pragma unroll
-            for (int t = 0; t < NT; t++) {
-              const auto& x = L.slow[1][i & 1];
-              const uint32_t j = t * 16 + l16;
-              const float o = p.scale * ((x[0][j] + x[1][j]) + (x[2][j] + x[3][j]));
-              const size_t to = col * p.out_stride + (size_t)h * p.hv + v0 + j;
-              if (p.out_f16) ((_Float16*)p.out)[to] = (_Float16)o; else ((float*)p.out)[to] = o;
+              for (int r = 0; r < 4; r++) { S[t][m][r] = __builtin_fmaf(u, k[m][r], S[t][m][r]); o = __builtin_fmaf(S[t][m][r], q[r], o); }
             }
+            o = rows4_sum(o);
+            if (lg == 0) Z.part[1][i & 1][w][j] = o;
           }
         }
+        if constexpr (ROLE == KEYS) { if (i) put_token(i - 1); }
       }
+      lds_barrier();
+      if constexpr (ROLE == KEYS) put_token(rows - 1);
       rows = 0;
       own_exponents(c + 1, e);
     }
@@ -825,6 +842,8 @@ template <int HK>
 static hipError_t launch_chunks(const DeltaParams& p, void* mem, uint32_t ws_chunks, int n_cu, hipStream_t s) {
   const DeltaWs ws = ws_at<HK>(mem, ws_chunks, p.nk, p.nv, nullptr);
   const uint32_t seg = ws_chunks * CHUNK;
+  // Two tiles of value columns a workgroup where one each would not fit on the chip at once: the operands are read half as often, but each chunk takes longer.  2048 columns
+  // of 48 heads of 128 values: 84 us with two (192 workgroups), 128 with one (384 on 256 CUs); of 32 heads: 75 with two (128 workgroups), 63 with one (256).
   const bool wide = p.hv % 32 == 0 && p.nv * (p.hv / 16) > (uint32_t)n_cu;
   for (uint32_t c0 = 0; c0 < p.n; c0 += seg) {
     DeltaParams r = p;
