@@ -368,7 +368,8 @@ void* pa_delta_state_ptr(pa_delta* dn, uint32_t layer, int which);
  *   n_commit <= n_cols: the state moves on over the first n_commit columns alone (see pa_delta_decode).
  *   d_qkv, d_out: f32 [n_cols][stride], 16-byte aligned, strides multiples of 4;  d_conv_w: f32 [channels][conv_width], 16-byte aligned;
  *   d_conv_b: f32 [channels], 16-byte aligned, or NULL;  d_a, d_b: f32 [n_cols][ab_stride];  d_a_log, d_dt_bias: f32 [n_v_heads];
- *   d_g, d_beta: f32 [n_cols][gate_stride].  Outputs share no memory with inputs. */
+ *   d_g, d_beta: f32 [n_cols][gate_stride].  Outputs share no memory with inputs or the state, and no input lies in the state (ranges from the first
+ *   column to the last count: columns of an input and an output do not interleave either). */
 int pa_delta_glue(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const float* d_qkv, uint32_t qkv_stride, const float* d_conv_w, const float* d_conv_b,
                   const float* d_a, const float* d_b, uint32_t ab_stride, const float* d_a_log, const float* d_dt_bias, uint32_t n_cols,
                   uint32_t n_commit, float* d_out, uint32_t out_stride, float* d_g, float* d_beta, uint32_t gate_stride);
@@ -378,10 +379,11 @@ int pa_delta_glue(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const float* d_qkv,
  * accepted number is known).
  *   d_q, d_k: f32 [n_cols][stride], 16-byte aligned, strides multiples of 4, a column holds [n_k_heads][head_k];  d_v: [n_v_heads][head_v];
  *   d_g (natural logarithm of the decay), d_beta: f32 [n_cols][gate_stride];  the three may be parts of one pa_delta_glue column;
- *   d_out: [n_cols][out_stride] of out_dtype, a column holds [n_v_heads][head_v]; shares no memory with inputs or state; NULL (then d_q is not read): the
+ *   d_out: [n_cols][out_stride] of out_dtype, a column holds [n_v_heads][head_v]; shares no memory with inputs or state (ranges, as above); NULL (then d_q is not read): the
  *          state alone moves on.
  * pa_delta_prefill: the same for n_cols columns of a prompt, all of them committed, in chunks of 64 on the matrix cores where that is faster (from
- * 48 columns on).  Its results agree with pa_delta_decode's to f32 rounding. */
+ * 48 columns on).  Its results agree with pa_delta_decode's to f32 rounding, as long as the values that meet in a chunk differ by less than 2^27 in size: what one value
+ * column takes in is held to 22 bits down to 2^-27 of the largest there, and to 2^-49 of that below. */
 int pa_delta_decode(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const float* d_q, uint32_t q_stride, const float* d_k, uint32_t k_stride, const float* d_v,
                     uint32_t v_stride, const float* d_g, const float* d_beta, uint32_t gate_stride, uint32_t n_cols, uint32_t n_commit, void* d_out,
                     uint32_t out_stride, int out_dtype);
@@ -412,7 +414,7 @@ typedef struct pa_moe_planes {
   const uint16_t *h_shared_gate_s, *h_shared_up_s, *h_shared_down_s;
 } pa_moe_planes;
 typedef struct pa_moe pa_moe;
-/* copies the planes to the device and allocates the workspace of the widest call (max_cols).  Ownership, ordering and capture as pa_delta_create. */
+/* copies the planes to the device and allocates the workspace (of at most 512 tokens; a wider call takes them in turn).  Ownership, ordering and capture as pa_delta_create. */
 int pa_moe_create(pa_ctx* ctx, const pa_moe_config* cfg, const pa_moe_planes* planes, pa_moe** out);
 int pa_moe_destroy(pa_ctx* ctx, pa_moe* moe);
 /* n_cols tokens through the layer.  Made for the few tokens of a decode step, a verify block or a narrow pass, where the chosen experts' weights are

@@ -53,7 +53,7 @@ struct pa_moe {
   float* router = nullptr;         // [n_experts (+ 1: the shared expert's gate)][dim]
   unsigned char* gate = nullptr; unsigned char* up = nullptr; unsigned char* down = nullptr;
   uint16_t* gate_s = nullptr; uint16_t* up_s = nullptr; uint16_t* down_s = nullptr;
-  float* scratch = nullptr;        // of max_cols tokens: see MoeParams
+  float* scratch = nullptr;        // see MoeParams
 };
 
 struct MoeParams {
@@ -64,6 +64,7 @@ struct MoeParams {
   // router logits [n][logit_stride], the experts of a token and their weights [n][slots]
   float* xn; float* h; float* logits; uint32_t* sel; float* sel_w;
   uint32_t xn_floats, h_floats, logit_stride;
+  uint32_t batch;                  // tokens that the scratch holds
   uint32_t x_stride, y_stride, n, dim, ffn, n_experts, top_k, slots;
   float eps;
   uint32_t norm_topk;

@@ -23,6 +23,12 @@ static __device__ inline float row16_sum(float v) {
   return v + dpp_f32<0x140>(v);
 }
 
+// 1 / sqrt(x), also where x is subnormal, which the instruction takes for zero (eps may be 0)
+static __device__ inline float inverse_root(float x) {
+  const bool tiny = x < 0x1p-100f;
+  return __builtin_amdgcn_rsqf(tiny ? x * 0x1p100f : x) * (tiny ? 0x1p50f : 1.f);
+}
+
 // V4: float4 of a row per lane (head_k = 64 V4).  The leading arguments are those that every load needs: they arrive in scalar registers before the wave starts.
 template <int V4, bool OUT, bool NORM>
 __global__ __launch_bounds__(256)
@@ -83,7 +89,7 @@ void pa_delta_step_kernel(const float* a_k, const float* a_q, const float* a_v, 
             x = __builtin_fmaf(kr[s][i][0], kr[s][i][0], x); y = __builtin_fmaf(kr[s][i][1], kr[s][i][1], y);
             x = __builtin_fmaf(kr[s][i][2], kr[s][i][2], x); y = __builtin_fmaf(kr[s][i][3], kr[s][i][3], y);
           }
-          inv_k = __builtin_amdgcn_rsqf(row16_sum(x + y) + p.eps);
+          inv_k = inverse_root(row16_sum(x + y) + p.eps);
         }
         x = y = 0.f;
 #pragma unroll
@@ -107,7 +113,7 @@ void pa_delta_step_kernel(const float* a_k, const float* a_q, const float* a_v, 
               x = __builtin_fmaf(qr[s][i][0], qr[s][i][0], x); y = __builtin_fmaf(qr[s][i][1], qr[s][i][1], y);
               x = __builtin_fmaf(qr[s][i][2], qr[s][i][2], x); y = __builtin_fmaf(qr[s][i][3], qr[s][i][3], y);
             }
-            scale *= __builtin_amdgcn_rsqf(row16_sum(x + y) + p.eps);
+            scale *= inverse_root(row16_sum(x + y) + p.eps);
             x = y = 0.f;
           }
 #pragma unroll

@@ -18,6 +18,7 @@
 // f32, 27 tokens, 61 experts of 352 x 1056, 5 chosen: 5 + 5 + 41 + 26 for 245 MB.
 #include "blocks_internal.h"
 #include "glue_math.h"
+#include <algorithm>
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
@@ -464,16 +465,12 @@ static hipError_t launch_kind(const MoeParams& p, int n_cu, hipStream_t s) {
 }
 
 hipError_t pa_launch_moe(const MoeParams& p, int n_cu, hipStream_t s) {
-  // grid rows are tokens x places: at most 65535 of them a launch
-  const uint32_t most = 65535u / p.slots;
-  for (uint32_t t = 0; t < p.n; t += most) {
+  for (uint32_t t = 0; t < p.n; t += p.batch) {                    // at most 512 x 17 grid rows
     MoeParams q = p;
-    q.n = p.n - t < most ? p.n - t : most;
+    q.n = std::min(p.n - t, p.batch);
     q.x += (size_t)t * p.x_stride; q.y += (size_t)t * p.y_stride;
     if (q.ids) q.ids += (size_t)t * p.top_k;
     if (q.weights) q.weights += (size_t)t * p.top_k;
-    q.xn += (size_t)t * p.xn_floats; q.h += (size_t)t * p.h_floats; q.logits += (size_t)t * p.logit_stride;
-    q.sel += (size_t)t * p.slots; q.sel_w += (size_t)t * p.slots;
     const hipError_t e = p.kind == PA_W_F32 ? launch_kind<PA_W_F32>(q, n_cu, s) : p.kind == PA_W_Q8_0 ? launch_kind<PA_W_Q8_0>(q, n_cu, s) : launch_kind<PA_W_Q4_0>(q, n_cu, s);
     if (e != hipSuccess) return e;
   }

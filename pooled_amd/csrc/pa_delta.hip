@@ -143,6 +143,8 @@ extern "C" int pa_delta_glue(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const fl
                      {pa_delta_state_ptr(dn, layer, 1), pa_delta_state_bytes(dn, 1)}};
   const Span res[] = {cols(d_out, n_cols, out_stride, dn->channels, 4), cols(d_g, n_cols, gate_stride, c.n_v_heads, 4), cols(d_beta, n_cols, gate_stride, c.n_v_heads, 4)};
   for (const Span& o : res) for (const Span& i : in) if (overlap(o, i)) return block_fail(ctx, PA_ERR_INVALID, who, "an output shares memory with an input");
+  const Span& state = in[sizeof in / sizeof *in - 1];
+  for (const Span& i : in) if (&i != &state && overlap(state, i)) return block_fail(ctx, PA_ERR_INVALID, who, "an input lies in the layer's state");
   DeltaGlueParams p; memset(&p, 0, sizeof p);
   p.x = d_qkv; p.w = d_conv_w; p.bias = d_conv_b; p.a = d_a; p.b = d_b; p.a_log = d_a_log; p.dt_bias = d_dt_bias;
   p.conv = (float*)pa_delta_state_ptr(dn, layer, 1); p.out = d_out; p.g = d_g; p.beta = d_beta;
@@ -171,12 +173,14 @@ static int rule_params(pa_ctx* ctx, const char* who, pa_delta* dn, uint32_t laye
   if (!aligned(d_k, 16) || (k_stride & 3) || (d_out && (!aligned(d_q, 16) || (q_stride & 3))))
     return block_fail(ctx, PA_ERR_INVALID, who, "q and k must be 16-byte aligned, their strides multiples of 4");
   if (!aligned(d_v, 4) || !aligned(d_g, 4) || !aligned(d_beta, 4) || !aligned(d_out, elem)) return block_fail(ctx, PA_ERR_INVALID, who, "unaligned column");
-  if (d_out) {
-    const Span o = cols(d_out, n_cols, out_stride, vd, elem);
-    const Span in[] = {cols(d_q, n_cols, q_stride, kd, 4), cols(d_k, n_cols, k_stride, kd, 4), cols(d_v, n_cols, v_stride, vd, 4), cols(d_g, n_cols, gate_stride, c.n_v_heads, 4),
-                       cols(d_beta, n_cols, gate_stride, c.n_v_heads, 4), {pa_delta_state_ptr(dn, layer, 0), pa_delta_state_bytes(dn, 0)}};
-    for (const Span& i : in) if (overlap(o, i)) return block_fail(ctx, PA_ERR_INVALID, who, "the output shares memory with an input or the state");
+  const Span o = cols(d_out, n_cols, out_stride, vd, elem), state = {pa_delta_state_ptr(dn, layer, 0), pa_delta_state_bytes(dn, 0)};
+  const Span in[] = {cols(d_out ? d_q : nullptr, n_cols, q_stride, kd, 4), cols(d_k, n_cols, k_stride, kd, 4), cols(d_v, n_cols, v_stride, vd, 4),
+                     cols(d_g, n_cols, gate_stride, c.n_v_heads, 4), cols(d_beta, n_cols, gate_stride, c.n_v_heads, 4)};
+  for (const Span& i : in) {
+    if (overlap(o, i)) return block_fail(ctx, PA_ERR_INVALID, who, "the output shares memory with an input");
+    if (overlap(state, i)) return block_fail(ctx, PA_ERR_INVALID, who, "an input lies in the layer's state");
   }
+  if (overlap(o, state)) return block_fail(ctx, PA_ERR_INVALID, who, "the output shares memory with the state");
   memset(&p, 0, sizeof p);
   p.q = d_out ? d_q : d_k; p.k = d_k; p.v = d_v; p.g = d_g; p.beta = d_beta; p.state = (float*)pa_delta_state_ptr(dn, layer, 0); p.out = d_out;
   p.q_stride = d_out ? q_stride : k_stride; p.k_stride = k_stride; p.v_stride = v_stride; p.gate_stride = gate_stride; p.out_stride = out_stride;

@@ -21,6 +21,10 @@ extern "C" int pa_moe_destroy(pa_ctx* ctx, pa_moe* moe) {
   return PA_OK;
 }
 
+// tokens that the scratch holds; a wider call takes them in turn (35 KB a token with 9 experts of 512 x 2048: 18 MB, where 65535 columns would be 2.3 GB a layer)
+#define BATCH_TOKENS 512u
+static uint32_t batch_of(const pa_ctx* ctx) { return ctx->cfg.max_cols < BATCH_TOKENS ? ctx->cfg.max_cols : BATCH_TOKENS; }
+
 static size_t plane_bytes(int kind, size_t values) { return kind == PA_W_F32 ? values * 4 : kind == PA_W_Q8_0 ? values : values / 2; }
 
 // scratch of n tokens, every part 256-byte aligned: sets p's pointers behind `base` and returns the bytes
@@ -76,7 +80,7 @@ extern "C" int pa_moe_create(pa_ctx* ctx, const pa_moe_config* cfg, const pa_moe
   put((void**)&m->up_s, h.h_up_s, h.h_shared_up_s, sb);
   put((void**)&m->down_s, h.h_down_s, h.h_shared_down_s, sb);
   MoeParams p;
-  const size_t scratch = lay_scratch(m, ctx->cfg.max_cols, nullptr, p);
+  const size_t scratch = lay_scratch(m, batch_of(ctx), nullptr, p);
   if (e == hipSuccess) e = hipMalloc((void**)&m->scratch, scratch);
   const hipError_t s = hipStreamSynchronize(ctx->stream);        // the host planes are the caller's again, whatever happened
   if (e == hipSuccess) e = s;
@@ -104,7 +108,8 @@ extern "C" int pa_moe_layer(pa_ctx* ctx, pa_moe* moe, const float* d_norm_w, con
   MoeParams p; memset(&p, 0, sizeof p);
   p.router = moe->router; p.gate = moe->gate; p.up = moe->up; p.down = moe->down; p.gate_s = moe->gate_s; p.up_s = moe->up_s; p.down_s = moe->down_s;
   p.norm_w = d_norm_w; p.x = d_x; p.y = d_y; p.ids = d_ids; p.weights = d_weights;
-  lay_scratch(moe, ctx->cfg.max_cols, (unsigned char*)moe->scratch, p);
+  p.batch = batch_of(ctx);
+  lay_scratch(moe, p.batch, (unsigned char*)moe->scratch, p);
   p.x_stride = x_stride; p.y_stride = y_stride; p.n = n_cols; p.dim = c.dim; p.ffn = c.ffn; p.n_experts = c.n_experts; p.top_k = c.top_k; p.slots = moe->slots;
   p.eps = ctx->cfg.eps; p.norm_topk = (c.flags & PA_MOE_NORM_TOPK) != 0; p.kind = c.kind;
   DeviceGuard on(ctx->device);
