@@ -69,7 +69,7 @@ def test_inputs_in_the_state_are_refused():
         assert e.value.code == PA_ERR_INVALID
         pa.delta_decode(dn, 1, Part(buf, 0), 64, S, 64, buf, 64, buf, buf, 2, 2, 1, out, 64)      # another layer's state is memory like any other
         with pytest.raises(PaError) as e:
-            pa.delta_glue(dn, 0, conv, 192, buf, None, buf, buf, 2, buf, buf, 2, 2, out, 192, Part(out, 2048), Part(out, 3072), 2)
+            pa.delta_glue(dn, 0, conv, 192, buf, None, buf, buf, 2, buf, buf, 2, 2, out, 192, Part(out, 2048), Part(out, 2560), 2)
         assert e.value.code == PA_ERR_INVALID and "state" in str(e.value)
 
 
