@@ -130,13 +130,13 @@ static __device__ inline void load_piece(Piece<KIND>& r, const unsigned char* pl
 // ---- 1: router logits and normed activations -----------------------------------------------------
 template <int KIND>
 __global__ __launch_bounds__(256)
-void pa_moe_router_kernel(MoeParams p, uint32_t rows) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y, n4 = p.dim / 4;
+void pa_moe_router_kernel(const float* a_x, const float* a_router, const float* a_norm, uint32_t dim, uint32_t x_stride, uint32_t rows, MoeParams p) {
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y, n4 = dim / 4;
   const uint32_t at = blockIdx.x * 4 + wave;                       // 0: xn, the longest way, first; otherwise logit at - 1
-  const f4* x = (const f4*)(p.x + (size_t)t * p.x_stride);
-  const f4* nw = (const f4*)p.norm_w;
+  const f4* x = (const f4*)(a_x + (size_t)t * x_stride);
+  const f4* nw = (const f4*)a_norm;
   if (at > rows) return;
-  const f4* r = (const f4*)(p.router + (size_t)(at ? at - 1 : 0) * p.dim);
+  const f4* r = (const f4*)(a_router + (size_t)(at ? at - 1 : 0) * dim);
   float ss = 0.f, a = 0.f, b = 0.f;
   for (uint32_t i0 = 0; i0 < n4; i0 += 512) {
     f4 xv[8], rv[8], wv[8];
@@ -159,7 +159,7 @@ void pa_moe_router_kernel(MoeParams p, uint32_t rows) {
     }
   }
   ss = wave_sum_f32(ss);
-  const float inv = nw ? 1.0f / sqrtf(ss / (float)p.dim + p.eps) : 1.f;
+  const float inv = nw ? 1.0f / sqrtf(ss / (float)dim + p.eps) : 1.f;
   if (at) {
     a = wave_sum_f32(a + b) * inv;
     if (lane == 0) p.logits[(size_t)t * p.logit_stride + at - 1] = a;
@@ -200,15 +200,20 @@ struct Choice {
   // the expert of the largest key m, the lowest among equals; taken out
   __device__ uint32_t next(uint32_t lane, uint32_t& m) {
     m = key[0];
+    uint32_t i0 = 0;                                               // of the lane's largest key, the first
 #pragma unroll
-    for (int i = 1; i < NE; i++) m = max(m, key[i]);
+    for (int i = 1; i < NE; i++) { i0 = key[i] > m ? (uint32_t)i : i0; m = max(m, key[i]); }
+    const uint32_t mine = m;
     m = wave_max_u32(m);
-    uint32_t e = 0;
-    bool found = false;
+    const uint64_t who = __ballot(mine == m);
+    uint32_t e = 64 * (uint32_t)__builtin_amdgcn_readlane((int)i0, __builtin_ctzll(who)) + (uint32_t)__builtin_ctzll(who);
+    if (who & (who - 1)) {                                         // equal keys in several lanes
+      bool found = false;
 #pragma unroll
-    for (int i = 0; i < NE; i++) {
-      const uint64_t who = __ballot(key[i] == m);
-      if (!found && who) { found = true; e = 64 * i + (uint32_t)__builtin_ctzll(who); }
+      for (int i = 0; i < NE; i++) {
+        const uint64_t at = __ballot(key[i] == m);
+        if (!found && at) { found = true; e = 64 * i + (uint32_t)__builtin_ctzll(at); }
+      }
     }
 #pragma unroll
     for (int i = 0; i < NE; i++) if (e == lane + 64 * i) key[i] = 0u;
@@ -257,31 +262,32 @@ void pa_moe_choice_kernel(MoeParams p) { write_choice<NE>(p, blockIdx.x, threadI
 #define MOE_WINDOW 256
 template <int KIND, int NE, int RW, int GROUP, bool CHOSEN>
 __global__ __launch_bounds__(1024 / RW)
-void pa_moe_gate_up_kernel(MoeParams p) {
+void pa_moe_gate_up_kernel(const float* a_logits, const uint32_t* a_sel, const float* a_xn, uint32_t logit_stride, uint32_t xn_floats, uint32_t n_experts, uint32_t top_k, uint32_t slots,
+                           uint32_t dim, MoeParams p) {
   constexpr uint32_t STEP = Piece<KIND>::STEP;
   __shared__ float hs[GROUP][16];
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t np = pieces<KIND>(p.dim), first = blockIdx.x * 16, pair = blockIdx.y;
-  uint32_t e = p.n_experts, count = 1, member[GROUP];
+  const uint32_t np = pieces<KIND>(dim), first = blockIdx.x * 16, pair = blockIdx.y;
+  uint32_t e = n_experts, count = 1, member[GROUP];
   member[0] = pair;
   Act<KIND> x[2];
-  load_act<KIND>(x[0], p.xn + (size_t)(pair / p.slots) * p.xn_floats, lane, np);
+  load_act<KIND>(x[0], a_xn + (size_t)(pair / slots) * xn_floats, lane, np);
   if constexpr (!CHOSEN) {
-    const uint32_t place = pair % p.slots;
-    if (place < p.top_k) {
+    const uint32_t place = pair % slots;
+    if (place < top_k) {
       Choice<NE> c;
-      c.load(p.logits + (size_t)(pair / p.slots) * p.logit_stride, p.n_experts, lane);
+      c.load(a_logits + (size_t)(pair / slots) * logit_stride, n_experts, lane);
       uint32_t m;
       for (uint32_t r = 0; r <= place; r++) e = c.next(lane, m);
     }
   } else if constexpr (GROUP == 1) {
-    e = p.sel[pair];
+    e = a_sel[pair];
   } else {
     // the window's choices, 64 a register
-    const uint32_t tokens = MOE_WINDOW / p.slots, w0 = pair / p.slots / tokens * tokens * p.slots, w1 = min(w0 + tokens * p.slots, p.n * p.slots), me = pair - w0;
+    const uint32_t tokens = MOE_WINDOW / slots, w0 = pair / slots / tokens * tokens * slots, w1 = min(w0 + tokens * slots, p.n * slots), me = pair - w0;
     uint32_t all[MOE_WINDOW / 64], at = 0;
 #pragma unroll
-    for (int k = 0; k < MOE_WINDOW / 64; k++) all[k] = p.sel[min(w0 + 64 * k + lane, w1 - 1)];
+    for (int k = 0; k < MOE_WINDOW / 64; k++) all[k] = a_sel[min(w0 + 64 * k + lane, w1 - 1)];
 #pragma unroll
     for (int k = 0; k < MOE_WINDOW / 64; k++) if (me / 64 == k) at = all[k];
     e = (uint32_t)__builtin_amdgcn_readlane((int)at, (int)(me & 63));
@@ -321,11 +327,11 @@ void pa_moe_gate_up_kernel(MoeParams p) {
       load_piece<KIND>(wg[r], p.gate, p.gate_s, row + r, q, np);
       load_piece<KIND>(wu[r], p.up, p.up_s, row + r, q, np);
     }
-    if (q0) load_act<KIND>(x[0], p.xn + (size_t)(pair / p.slots) * p.xn_floats, q, np);
+    if (q0) load_act<KIND>(x[0], a_xn + (size_t)(pair / slots) * xn_floats, q, np);
 #pragma unroll
     for (int j = 0; j < GROUP; j++) {
       if (j < (int)count) {
-        if (j + 1 < GROUP && j + 1 < (int)count) load_act<KIND>(x[(j + 1) & 1], p.xn + (size_t)(member[j + 1 < GROUP ? j + 1 : 0] / p.slots) * p.xn_floats, q, np);
+        if (j + 1 < GROUP && j + 1 < (int)count) load_act<KIND>(x[(j + 1) & 1], a_xn + (size_t)(member[j + 1 < GROUP ? j + 1 : 0] / slots) * xn_floats, q, np);
         if (KIND == PA_W_F32 || q < np) {
 #pragma unroll
           for (int r = 0; r < RW; r++) { g[j][r] = dot_piece<KIND>(wg[r], x[j & 1], 1.f, g[j][r]); u[j][r] = dot_piece<KIND>(wu[r], x[j & 1], 1.f, u[j][r]); }
@@ -348,8 +354,8 @@ void pa_moe_gate_up_kernel(MoeParams p) {
     uint32_t m = member[0];
 #pragma unroll
     for (int j = 1; j < GROUP; j++) if (threadIdx.x / 16 == j) m = member[j];
-    float* h = p.h + (size_t)(m / p.slots) * p.h_floats;
-    const uint32_t v = (m % p.slots) * p.ffn + first + threadIdx.x % 16;
+    float* h = p.h + (size_t)(m / slots) * p.h_floats;
+    const uint32_t v = (m % slots) * p.ffn + first + threadIdx.x % 16;
     const float y = hs[threadIdx.x / 16][threadIdx.x % 16];
     h[act_at<KIND>(v)] = stored<KIND>(v, y);
     if constexpr (KIND == PA_W_Q4_0) {
@@ -358,26 +364,26 @@ void pa_moe_gate_up_kernel(MoeParams p) {
       if (threadIdx.x % 16 == 0) h[sum_at(v)] = s;
     }
   }
-  if (!CHOSEN && blockIdx.x == 0 && pair % p.slots == 0 && wave == 0) write_choice<NE>(p, pair / p.slots, lane);
+  if (!CHOSEN && blockIdx.x == 0 && pair % slots == 0 && wave == 0) write_choice<NE>(p, pair / slots, lane);
 }
 
 // ---- 3: down, weighted sum, residual -------------------------------------------------------------
 // RW rows of y a wavefront; the next pieces are requested while the present ones are used
 template <int KIND, int RW, bool AHEAD>
 __global__ __launch_bounds__(256)
-void pa_moe_down_kernel(MoeParams p) {
+void pa_moe_down_kernel(const uint32_t* a_sel, const float* a_sel_w, const float* a_h, uint32_t h_floats, uint32_t slots, uint32_t ffn, uint32_t dim, MoeParams p) {
   constexpr uint32_t STEP = Piece<KIND>::STEP;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, t = blockIdx.y;
-  const uint32_t np = pieces<KIND>(p.ffn), all = p.slots * np, row0 = (blockIdx.x * 4 + wave) * RW;
-  const float* act = p.h + (size_t)t * p.h_floats;
-  const uint32_t* sel = p.sel + (size_t)t * p.slots;
-  const float* sel_w = p.sel_w + (size_t)t * p.slots;
+  const uint32_t np = pieces<KIND>(ffn), all = slots * np, row0 = (blockIdx.x * 4 + wave) * RW;
+  const float* act = a_h + (size_t)t * h_floats;
+  const uint32_t* sel = a_sel + (size_t)t * slots;
+  const float* sel_w = a_sel_w + (size_t)t * slots;
   float a[RW];
 #pragma unroll
   for (int r = 0; r < RW; r++) a[r] = 0.f;
   // a lane's place and piece in it, 64 further each time
-  const uint32_t my_sel = sel[min(lane, p.slots - 1)], step_place = 64 / np, step_piece = 64 % np;
-  const float my_w = sel_w[min(lane, p.slots - 1)];
+  const uint32_t my_sel = sel[min(lane, slots - 1)], step_place = 64 / np, step_piece = 64 % np;
+  const float my_w = sel_w[min(lane, slots - 1)];
   uint32_t place = lane / np, piece = lane % np;
   constexpr int LOADS = KIND == PA_W_F32 ? 2 : 1;
   struct Batch { Act<KIND> x; Piece<KIND> w[RW]; float f[LOADS]; };
@@ -386,14 +392,14 @@ void pa_moe_down_kernel(MoeParams p) {
 #pragma unroll
     for (int i = 0; i < LOADS; i++) {
       const bool in = q0 + 64 * i + lane < all;
-      const uint32_t pl = in ? place : p.slots - 1, pc = in ? piece : np - 1;
+      const uint32_t pl = in ? place : slots - 1, pc = in ? piece : np - 1;
       const size_t e = (uint32_t)__shfl((int)my_sel, (int)pl);
       d.f[i] = __shfl(my_w, (int)pl);
       place += step_place; piece += step_piece;
       if (piece >= np) { piece -= np; place++; }
 #pragma unroll
       for (int r = 0; r < RW; r++) {
-        const size_t row = e * p.dim + min(row0 + r, p.dim - 1);
+        const size_t row = e * dim + min(row0 + r, dim - 1);
         if constexpr (KIND == PA_W_F32) d.w[r].w[i] = ((const f4*)p.down)[row * np + pc];
         else load_piece<KIND>(d.w[r], p.down, p.down_s, row, pc, np);
       }
@@ -428,7 +434,7 @@ void pa_moe_down_kernel(MoeParams p) {
 #pragma unroll
   for (int r = 0; r < RW; r++) {
     const float s = wave_sum_f32(a[r]);
-    if (lane == 0 && row0 + r < p.dim) p.y[(size_t)t * p.y_stride + row0 + r] = p.x[(size_t)t * p.x_stride + row0 + r] + s;
+    if (lane == 0 && row0 + r < dim) p.y[(size_t)t * p.y_stride + row0 + r] = p.x[(size_t)t * p.x_stride + row0 + r] + s;
   }
 }
 
@@ -442,21 +448,21 @@ static void launch_experts(const MoeParams& p, hipStream_t s) {
   constexpr uint32_t INLINE = KIND == PA_W_Q4_0 ? 4 : 12;
   const dim3 grid(p.ffn / 16, p.n * p.slots);
   if (p.n <= INLINE) {
-    hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, NE, 2, 1, false>), grid, dim3(512), 0, s, p);
+    hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, NE, 2, 1, false>), grid, dim3(512), 0, s, p.logits, p.sel, p.xn, p.logit_stride, p.xn_floats, p.n_experts, p.top_k, p.slots, p.dim, p);
   } else {
     hipLaunchKernelGGL(pa_moe_choice_kernel<NE>, dim3(p.n), dim3(64), 0, s, p);
-    hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, NE, 4, GROUP, true>), grid, dim3(256), 0, s, p);
+    hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, NE, 4, GROUP, true>), grid, dim3(256), 0, s, p.logits, p.sel, p.xn, p.logit_stride, p.xn_floats, p.n_experts, p.top_k, p.slots, p.dim, p);
   }
 }
 template <int KIND>
 static hipError_t launch_kind(const MoeParams& p, int n_cu, hipStream_t s) {
   const uint32_t rows = p.n_experts + (p.slots > p.top_k ? 1 : 0);
-  hipLaunchKernelGGL(pa_moe_router_kernel<KIND>, dim3((rows + 1 + 3) / 4, p.n), dim3(256), 0, s, p, rows);
+  hipLaunchKernelGGL(pa_moe_router_kernel<KIND>, dim3((rows + 1 + 3) / 4, p.n), dim3(256), 0, s, p.x, p.router, p.norm_w, p.dim, p.x_stride, rows, p);
   if (p.n_experts <= 256) launch_experts<KIND, 4>(p, s); else launch_experts<KIND, 16>(p, s);
   // Rows a wavefront: quantised weights share the activations' loads over as many rows as still give every SIMD of the chip three wavefronts
   // (16 tokens of Q4_0, 2048 rows: 20.4 us with 8 rows, 24.4 with 4; 5 tokens of Q8_0: 19.0 and 15.1; one token: 5.0 with 2 and the next loads ahead, 5.5 without them, 5.1 with 1);
   // f32 pieces are short (27 tokens: 26.3 us with 2 rows, 28.8 with 4).
-  auto down = [&](auto* kernel, uint32_t rw) { hipLaunchKernelGGL(kernel, dim3((p.dim + 4 * rw - 1) / (4 * rw), p.n), dim3(256), 0, s, p); };
+  auto down = [&](auto* kernel, uint32_t rw) { hipLaunchKernelGGL(kernel, dim3((p.dim + 4 * rw - 1) / (4 * rw), p.n), dim3(256), 0, s, p.sel, p.sel_w, p.h, p.h_floats, p.slots, p.ffn, p.dim, p); };
   if (p.n == 1) down(pa_moe_down_kernel<KIND, 2, true>, 2);
   else if (KIND == PA_W_F32) down(pa_moe_down_kernel<KIND, 2, false>, 2);
   else if ((uint64_t)p.n * (p.dim / 8) >= (uint64_t)n_cu * 12) down(pa_moe_down_kernel<KIND, 8, false>, 8);
