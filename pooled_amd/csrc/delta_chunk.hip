@@ -163,12 +163,13 @@ template <int HK> struct PrepLds {
 
 template <int HK>
 __global__ __launch_bounds__(256, 4)
-void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
+void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, const float* a_beta, uint32_t n, uint32_t k_stride, uint32_t q_stride, uint32_t gate_stride, uint32_t group,
+                          DeltaParams p, DeltaWs ws) {
   using F = Frags<HK>;
   constexpr int KS = F::KS, DT = HK / 64;                          // DT: tiles of 16 key dimensions of a wavefront
   __shared__ __attribute__((aligned(16))) PrepLds<HK> L;
   const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l16 = lane & 15, lg = lane >> 4;
-  const uint32_t h = blockIdx.x, chunk = blockIdx.y, kh = h / p.group, c0 = chunk * CHUNK;
+  const uint32_t h = blockIdx.x, chunk = blockIdx.y, kh = h / group, c0 = chunk * CHUNK;
   const uint32_t w = (wave + chunk + h) & 3;                       // its tile: later tiles are more work, and wavefront i of every workgroup runs on the same SIMD
   _Float16* const kq = ws.kq + ((size_t)chunk * p.nk + kh) * 2 * F::KQ;
   float* const scal = ws.scal + ((size_t)chunk * p.nv + h) * SCAL_FLOATS;
@@ -178,16 +179,16 @@ void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
   __syncthreads();
 
   // -- rows: lengths, scaled pairs.  Lane: row l16 of the tile, values 8 lg .. + 7 of every k step
-  const bool gated = c0 + lane < p.n;
-  const size_t gc = (size_t)min(c0 + lane, p.n - 1) * p.gate_stride + h;
-  const float g_in = p.g[gc], b_in = p.beta[gc];                   // of row `lane`; requested in front of the rows, used while those are on their way
+  const bool gated = c0 + lane < n;
+  const size_t gc = (size_t)min(c0 + lane, n - 1) * gate_stride + h;
+  const float g_in = a_g[gc], b_in = a_beta[gc];                   // of row `lane`; requested in front of the rows, used while those are on their way
   Pair8 kf[KS], qf[KS];
   {
     const uint32_t row = w * 16 + l16;
-    const bool valid = c0 + row < p.n;
-    const size_t c = min(c0 + row, p.n - 1);
-    const float* kp = p.k + c * p.k_stride + (size_t)kh * HK + 8 * lg;
-    const float* qp = p.q + c * p.q_stride + (size_t)kh * HK + 8 * lg;
+    const bool valid = c0 + row < n;
+    const size_t c = min(c0 + row, n - 1);
+    const float* kp = a_k + c * k_stride + (size_t)kh * HK + 8 * lg;
+    const float* qp = a_q + c * q_stride + (size_t)kh * HK + 8 * lg;
     f4 k[KS][2], q[KS][2];
 #pragma unroll
     for (int s = 0; s < KS; s++)
@@ -222,7 +223,7 @@ void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
       scal[3 * 64 + row] = p.scale * pow2(qe);
     }
     const float ks = valid ? kinv * UNIT : 0.f, qs = valid ? qinv * pow2(-qe) * UNIT : 0.f;
-    const bool store_k = h == kh * p.group, store_q = h == kh * p.group + (p.group > 1 ? 1 : 0);      // the k head's fragments are stored by one or two v heads of its group
+    const bool store_k = h == kh * group, store_q = h == kh * group + (group > 1 ? 1 : 0);      // the k head's fragments are stored by one or two v heads of its group
 #pragma unroll
     for (int s = 0; s < KS; s++) {
       const Pair4 k0 = split4(k[s][0] * ks), k1 = split4(k[s][1] * ks), q0 = split4(q[s][0] * qs), q1 = split4(q[s][1] * qs);      // (rows behind the last: a finite one times zero, or the chunk is marked)
@@ -304,7 +305,7 @@ void pa_delta_prep_kernel(DeltaParams p, DeltaWs ws) {
 #pragma unroll
     for (int ks = 0; ks < 2; ks++)
 #pragma unroll
-      for (int e = 0; e < 8; e++) kt[x][ks][e] = p.k[(size_t)min(c0 + 32 * ks + 16 * (e >> 2) + 4 * lg + (e & 3), p.n - 1) * p.k_stride + (size_t)kh * HK + (w * DT + x) * 16 + l16];
+      for (int e = 0; e < 8; e++) kt[x][ks][e] = a_k[(size_t)min(c0 + 32 * ks + 16 * (e >> 2) + 4 * lg + (e & 3), n - 1) * k_stride + (size_t)kh * HK + (w * DT + x) * 16 + l16];
 
   // -- T = (1 + A)^-1.  The diagonal block by substitution, a lane a column (the four lane groups do the same)
   auto put_block = [&](uint32_t bi, uint32_t bj, const f4 v) {
@@ -851,7 +852,7 @@ static hipError_t launch_chunks(const DeltaParams& p, void* mem, uint32_t ws_chu
     r.q += (size_t)c0 * p.q_stride; r.k += (size_t)c0 * p.k_stride; r.v += (size_t)c0 * p.v_stride;
     r.g += (size_t)c0 * p.gate_stride; r.beta += (size_t)c0 * p.gate_stride;
     if (r.out) r.out = (unsigned char*)p.out + (size_t)c0 * p.out_stride * (p.out_f16 ? 2 : 4);
-    hipLaunchKernelGGL(pa_delta_prep_kernel<HK>, dim3(p.nv, (r.n + CHUNK - 1) / CHUNK), dim3(256), 0, s, r, ws);
+    hipLaunchKernelGGL(pa_delta_prep_kernel<HK>, dim3(p.nv, (r.n + CHUNK - 1) / CHUNK), dim3(256), 0, s, r.k, r.q, r.g, r.beta, r.n, r.k_stride, r.q_stride, r.gate_stride, r.group, r, ws);
     const dim3 threads(768);
     if (wide) hipLaunchKernelGGL((pa_delta_scan_kernel<HK, 2>), dim3(p.nv * (p.hv / 32)), threads, 0, s, r, ws);
     else hipLaunchKernelGGL((pa_delta_scan_kernel<HK, 1>), dim3(p.nv * (p.hv / 16)), threads, 0, s, r, ws);

@@ -223,38 +223,39 @@ struct Choice {
 
 // one wavefront: all of a token's experts and their weights
 template <int NE>
-static __device__ void write_choice(const MoeParams& p, uint32_t t, uint32_t lane) {
-  const float* l = p.logits + (size_t)t * p.logit_stride;
+static __device__ inline void write_choice(const MoeParams& p, const float* l, uint32_t n_experts, uint32_t top_k, uint32_t t, uint32_t lane) {
   Choice<NE> c;
-  c.load(l, p.n_experts, lane);
+  c.load(l, n_experts, lane);
   float v[NE];
 #pragma unroll
   for (int i = 0; i < NE; i++) v[i] = Choice<NE>::logit(c.key[i]);
   uint32_t mine = 0, mine_key = 0, m;                              // lane r: the expert of place r
-  for (uint32_t r = 0; r < p.top_k; r++) { const uint32_t e = c.next(lane, m); if (lane == r) { mine = e; mine_key = m; } }
+  for (uint32_t r = 0; r < top_k; r++) { const uint32_t e = c.next(lane, m); if (lane == r) { mine = e; mine_key = m; } }
   const float top = readlane_f32(Choice<NE>::logit(mine_key), 0);  // the largest logit (a NaN only where all are)
   float all = 0.f;
 #pragma unroll
-  for (int i = 0; i < NE; i++) if (lane + 64 * i < p.n_experts) all += expf(v[i] - top);
+  for (int i = 0; i < NE; i++) if (lane + 64 * i < n_experts) all += expf(v[i] - top);
   all = wave_sum_f32(all);
-  const float w = lane < p.top_k ? expf(Choice<NE>::logit(mine_key) - top) : 0.f;
+  const float w = lane < top_k ? expf(Choice<NE>::logit(mine_key) - top) : 0.f;
   float sum = all;
   if (p.norm_topk) { sum = wave_sum_f32(w); if (all != all) sum = all; }
-  if (lane < p.top_k) {
+  if (lane < top_k) {
     p.sel[(size_t)t * p.slots + lane] = mine;
     p.sel_w[(size_t)t * p.slots + lane] = w / sum;
-    if (p.ids) p.ids[(size_t)t * p.top_k + lane] = mine;
-    if (p.weights) p.weights[(size_t)t * p.top_k + lane] = w / sum;
+    if (p.ids) p.ids[(size_t)t * top_k + lane] = mine;
+    if (p.weights) p.weights[(size_t)t * top_k + lane] = w / sum;
   } else if (lane < p.slots) {
-    p.sel[(size_t)t * p.slots + lane] = p.n_experts;
-    p.sel_w[(size_t)t * p.slots + lane] = 1.0f / (1.0f + expf(-l[p.n_experts]));
+    p.sel[(size_t)t * p.slots + lane] = n_experts;
+    p.sel_w[(size_t)t * p.slots + lane] = 1.0f / (1.0f + expf(-l[n_experts]));
   }
 }
 
 // the choice in a launch of its own, a wavefront a token
 template <int NE>
 __global__ __launch_bounds__(64)
-void pa_moe_choice_kernel(MoeParams p) { write_choice<NE>(p, blockIdx.x, threadIdx.x); }
+void pa_moe_choice_kernel(const float* a_logits, uint32_t logit_stride, uint32_t n_experts, uint32_t top_k, MoeParams p) {
+  write_choice<NE>(p, a_logits + (size_t)blockIdx.x * logit_stride, n_experts, top_k, blockIdx.x, threadIdx.x);
+}
 
 // ---- 2: gate and up ------------------------------------------------------------------------------
 // A workgroup: 16 rows of h (half a block of the next kernel's input) of one expert, for up to GROUP tokens that chose it.  Pairs (token, place) are grouped in
@@ -364,7 +365,7 @@ void pa_moe_gate_up_kernel(const float* a_logits, const uint32_t* a_sel, const f
       if (threadIdx.x % 16 == 0) h[sum_at(v)] = s;
     }
   }
-  if (!CHOSEN && blockIdx.x == 0 && pair % slots == 0 && wave == 0) write_choice<NE>(p, pair / slots, lane);
+  if (!CHOSEN && blockIdx.x == 0 && pair % slots == 0 && wave == 0) write_choice<NE>(p, a_logits + (size_t)(pair / slots) * logit_stride, n_experts, top_k, pair / slots, lane);
 }
 
 // ---- 3: down, weighted sum, residual -------------------------------------------------------------
@@ -450,7 +451,7 @@ static void launch_experts(const MoeParams& p, hipStream_t s) {
   if (p.n <= INLINE) {
     hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, NE, 2, 1, false>), grid, dim3(512), 0, s, p.logits, p.sel, p.xn, p.logit_stride, p.xn_floats, p.n_experts, p.top_k, p.slots, p.dim, p);
   } else {
-    hipLaunchKernelGGL(pa_moe_choice_kernel<NE>, dim3(p.n), dim3(64), 0, s, p);
+    hipLaunchKernelGGL(pa_moe_choice_kernel<NE>, dim3(p.n), dim3(64), 0, s, p.logits, p.logit_stride, p.n_experts, p.top_k, p);
     hipLaunchKernelGGL((pa_moe_gate_up_kernel<KIND, NE, 4, GROUP, true>), grid, dim3(256), 0, s, p.logits, p.sel, p.xn, p.logit_stride, p.xn_floats, p.n_experts, p.top_k, p.slots, p.dim, p);
   }
 }
