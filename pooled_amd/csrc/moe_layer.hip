@@ -13,9 +13,9 @@
 // in which lanes load them, so that every load is 1 KB of consecutive bytes.  Arithmetic is f32, every sum in an order that depends on the layer's sizes alone:
 // no atomics, and a token's bits do not depend on the other tokens of the call.
 //
-// Measured with 256 experts of 512 x 2048, 8 chosen and one shared (router, choice, gate and up, down, in us): 1 token of Q4_0 5 + 7 + 5, each a launch's latency and one trip to memory;
-// 5 of Q8_0 6 + 23 + 15 for 131 MB of distinct weights, gate and up at 4 TB/s (a large copy runs at 4.9); 16 of Q4_0 8 + 5 + 29 + 20 for 182 MB, gate and up at 4.2 TB/s.
-// f32, 27 tokens, 61 experts of 352 x 1056, 5 chosen: 5 + 5 + 41 + 26 for 245 MB.
+// Measured with 256 experts of 512 x 2048, 8 chosen and one shared (router, choice, gate and up, down, in us): 1 token of Q4_0 4.5 + 7 + 5, each a launch's latency and a trip or two to
+// memory; 5 of Q8_0 5 + 22 + 14 for 131 MB of distinct weights, gate and up at 4 TB/s (a large copy runs at 4.9); 16 of Q4_0 8 + 5 + 29 + 20 for 182 MB, gate and up at
+// 4.2 TB/s.  f32, 27 tokens, 61 experts of 352 x 1056, 5 chosen: 5 + 5 + 41 + 26 for 245 MB.
 #include "blocks_internal.h"
 #include "glue_math.h"
 #include <algorithm>
