@@ -9,12 +9,14 @@
 // a v head and 16 columns of its values, S in registers: per chunk K S, then X, then K'^T X, and beside them Q S and P' X.  Only decays between a
 // place and a later one occur, never their inverses, so nothing overflows however fast a head forgets; sums of g are kept in 64 bits, because their differences matter.
 //
-// Precision.  The results are f32 and stay as exact as f32 sums: every operand of the f16 matrix instructions is a pair hi + lo of f16 values (22 bits), a product is
-// hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it), accumulated in f32.  A pair is exact to 22 bits down to 2^-3 and to 2^-25 below (S and X, whose low halves are scaled: to 2^-14 and 2^-36), so operands need a known size:
-// rows of q are scaled by a power of two to a norm in [0.5, 1) and, as keys, K' and P', by UNIT more, K' by one for its largest element, and S and X, per value column, by one from a
-// bound: the rule over keys no longer than one with 0 <= beta <= 2, g <= 0 is a contraction, so |S_next| <= |S| + sum beta |v| and |X| <= 2 |S| + beta |v|.  A chunk whose
-// inputs leave that domain (longer or tiny keys, other gates, infinities, NaN) is marked by the first kernel, or found by the bound, and runs token by token in the second, in f32, with
-// the same S: slower (0.43 us a token of 32 heads, 0.04 otherwise), but right for every input.
+// Precision.  Every operand of the f16 matrix instructions is a pair hi + lo of f16 values (22 bits), a product is hi hi + hi lo + lo hi (the dropped lo lo is 2^-22 of it), accumulated
+// in f32.  Low halves are stored 2048 times, so that a pair has its 22 bits down to 2^-14 and is exact to 2^-36 below; those of K and Q alone are not (2^-3 and 2^-25).  So operands need a
+// known size: rows of q are scaled by a power of two to a norm in [0.5, 1), these, keys, P', T and P by UNIT, K' by a power of two for its largest element, and S and X, per value column, by one
+// from a bound: the rule over keys no longer than one with 0 <= beta <= 2, g <= 0 is a contraction, so |S_next| <= |S| + sum beta |v| and |X| <= 2 |S| + beta |v|.  What is small beside the
+// bound, by its value or by a decay, loses bits (P' and K' hold decays as S and X hold values), so a chunk with a token that takes in less than HELD = 2^-23 of it goes token by token
+// (put_exponent): every token's results are as exact as f32 leaves what that token takes in.  A chunk whose inputs leave the domain (longer or tiny keys, other gates, infinities, NaN)
+// is marked by the first kernel, or found by the bound, and goes the same way: token by token in the second kernel, in f32, with the same S.  Slower (0.43 us a token of 32 heads, 0.04
+// otherwise), but right for every input.
 //
 // What bounds it: a workgroup's chunk reads K, Q, K' (32 KB each at head_k 128) and P' (16 KB): 112 KB through one CU's 64 bytes a clock, 0.73 us, while its 168
 // matrix instructions take 0.3 us of four SIMDs.  The first kernel stores these operands in the order in which lanes load them (a fragment is 1 KB), every
@@ -30,20 +32,23 @@ typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 #define CHUNK 64
-// per chunk and v head: beta, beta e^G, output factors of Q S and P' X, 1 / |k| and 1 / |q| (or 1), 64 floats each; then e^G_64, the scale of K', the mark
-#define SCAL_FLOATS 448
+// per chunk and v head: beta, beta e^G, output factors of Q S and P' X, 1 / |k| and 1 / |q| (or 1), 64 floats each; then e^G_64, the scale of K', the mark, and 64 times e^g
+#define SCAL_FLOATS 512
 #define SCAL_DECAY 384
 #define SCAL_KSCALE 385
 #define SCAL_MARK 386
-// low halves of S and X are stored times 2048: a column's values may be far below its bound
+#define SCAL_STEP 448
+// low halves are stored times 2048 (all but those of K and Q, whose rows have one size): a column's values may be far below its bound, and a row of P, T or K' by its decay below another
 #define LO_SCALE 2048.f
 #define LO_INV (1.f / 2048.f)
-// operands of magnitude up to one are stored times 4096, so that the low halves of all but tiny ones are normal f16 numbers too
-#define UNIT 4096.f
-#define UNIT_INV (1.f / 4096.f)
+// operands of magnitude up to two are stored times 16384, so that the halves of all but tiny ones are normal f16 numbers
+#define UNIT 16384.f
+#define UNIT_INV (1.f / 16384.f)
+// what a token takes in (see put_exponent) may be this part of the bound of its value columns before its chunk goes token by token
+#define HELD 0x1p-23f
 
 static __device__ inline void lds_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
-// sum / maximum over lanes {i, i ^ 16, i ^ 32, i ^ 48}
+// sum over lanes {i, i ^ 16, i ^ 32, i ^ 48}
 static __device__ inline float rows4_sum(float v) {
   auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
@@ -100,6 +105,13 @@ static __device__ inline float pow2(int e) { return __uint_as_float((uint32_t)(e
 static __device__ inline int exponent(float x);
 static __device__ inline int scale_exponent(float m) { return m >= 0x1p-100f ? min(exponent(m), 100) : m > 0.f ? -100 : 13; }
 static __device__ inline int exponent(float x) { return (int)((__float_as_uint(x) >> 23) & 255) - 127; }   // of a positive normal number
+
+// of a row of 16 lanes: the lane before by so many (CTRL), or `other` where there is none; the sum
+template <int CTRL> static __device__ inline float dpp_or(float other, float v) { return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(other), __float_as_int(v), CTRL, 0xF, 0xF, false)); }
+static __device__ inline float row_sum(float v) {
+  v += dpp_f32<0xB1>(v); v += dpp_f32<0x4E>(v); v += dpp_f32<0x141>(v);
+  return v + dpp_f32<0x140>(v);
+}
 
 // ---- workspace: fragments of 64 lanes x 8 halves (1 KB) --------------------------------------------
 // K, Q of a k head: [plane hi, lo][row tile 4][k step HK / 32];  K'^T: [plane][row tile HK / 16][k step 2];  P': [plane][row tile 4][k step 2]
@@ -245,6 +257,7 @@ void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, 
     scal[tid] = L.beta[tid];
     scal[64 + tid] = L.beta[tid] * eG;
     scal[2 * 64 + tid] = eG;
+    scal[SCAL_STEP + tid] = expf(gated ? g_in : 0.f);
     if (tid == 63) { scal[SCAL_DECAY] = eG; scal[SCAL_MARK] = __uint_as_float(mark ? 1u : 0u); }
     L.row[tid] = tid >= 16 ? exp_f64(G - L.G[(tid & 48) - 1]) : eG;
   } else {
@@ -293,7 +306,7 @@ void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, 
         A[m][r] = m0 + r < i ? b * d[r] * a[r] : 0.f;
         pm[r] = d[r] * UNIT * q[r];
       }
-      const Pair4 s = split4(pm);
+      const Pair4 s = split4<true>(pm);
       Ph[m] = s.hi; Pl[m] = s.lo;
     }
   }
@@ -312,7 +325,7 @@ void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, 
     const uint32_t b = bi * (bi + 1) / 2 + bj;
 #pragma unroll
     for (int r = 0; r < 4; r++) L.t[b][(4 * lg + r) * TS + l16] = v[r];
-    const Pair4 s = split4(v * UNIT);
+    const Pair4 s = split4<true>(v * UNIT);
     L.tt[b][0][lane] = s.hi; L.tt[b][1][lane] = s.lo;
   };
   {
@@ -378,7 +391,7 @@ void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, 
 #pragma unroll
     for (int x = 0; x < DT; x++) {
       const float* k = kt[x][ks];
-      const Pair4 a = split4(f4{k[0], k[1], k[2], k[3]} * (f0 * UNIT)), b = split4(f4{k[4], k[5], k[6], k[7]} * (f1 * UNIT));
+      const Pair4 a = split4<true>(f4{k[0], k[1], k[2], k[3]} * (f0 * UNIT)), b = split4<true>(f4{k[4], k[5], k[6], k[7]} * (f1 * UNIT));
       kb[x][ks].hi = join(a.hi, b.hi); kb[x][ks].lo = join(a.lo, b.lo);
     }
   }
@@ -390,9 +403,10 @@ void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, 
   auto t_block = [&](int bi, int bj, int plane) { return bi >= bj ? L.tt[bi * (bi + 1) / 2 + bj][plane][lane] : none; };
 #pragma unroll
   for (int jt = 0; jt < 4; jt++) {
+    f4 pf = zero, kl[DT];                                          // products with a low half, 2048 times
     pr[jt] = zero;
 #pragma unroll
-    for (int x = 0; x < DT; x++) kr[x][jt] = zero;
+    for (int x = 0; x < DT; x++) kr[x][jt] = kl[x] = zero;
 #pragma unroll
     for (int ks = jt / 2; ks < 2; ks++) {
       const h8 th = join(t_block(2 * ks, jt, 0), t_block(2 * ks + 1, jt, 0)), tl = join(t_block(2 * ks, jt, 1), t_block(2 * ks + 1, jt, 1));
@@ -401,12 +415,18 @@ void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, 
       for (int x = 0; x < DT; x++) kr[x][jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, kb[x][ks].hi, kr[x][jt], 0, 0, 0);
       pr[jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, ph, pr[jt], 0, 0, 0);
 #pragma unroll
-      for (int x = 0; x < DT; x++) kr[x][jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, kb[x][ks].lo, kr[x][jt], 0, 0, 0);
-      pr[jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, pl, pr[jt], 0, 0, 0);
+      for (int x = 0; x < DT; x++) kl[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, kb[x][ks].lo, kl[x], 0, 0, 0);
+      pf = __builtin_amdgcn_mfma_f32_16x16x32_f16(th, pl, pf, 0, 0, 0);
 #pragma unroll
-      for (int x = 0; x < DT; x++) kr[x][jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tl, kb[x][ks].hi, kr[x][jt], 0, 0, 0);
-      pr[jt] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tl, ph, pr[jt], 0, 0, 0);
+      for (int x = 0; x < DT; x++) kl[x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(tl, kb[x][ks].hi, kl[x], 0, 0, 0);
+      pf = __builtin_amdgcn_mfma_f32_16x16x32_f16(tl, ph, pf, 0, 0, 0);
     }
+#pragma unroll
+    for (int r = 0; r < 4; r++) pr[jt][r] = __builtin_fmaf(pf[r], LO_INV, pr[jt][r]);
+#pragma unroll
+    for (int x = 0; x < DT; x++)
+#pragma unroll
+      for (int r = 0; r < 4; r++) kr[x][jt][r] = __builtin_fmaf(kl[x][r], LO_INV, kr[x][jt][r]);
   }
   // -- P' and K'^T in the order of the second kernel's loads, K' scaled by the power of two of its largest element
   float top = 0.f;
@@ -421,7 +441,7 @@ void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, 
   auto frag_at = [&](uint32_t tile, int jt) { return (tile * 2 + (jt >> 1)) * 512 + (l16 + 16 * (2 * (jt & 1) + (lg >> 1))) * 8 + 4 * (lg & 1); };
 #pragma unroll
   for (int jt = 0; jt < 4; jt++) {
-    const Pair4 s = split4(pr[jt] * UNIT_INV);
+    const Pair4 s = split4<true>(pr[jt] * UNIT_INV);
     *(h4*)(pp + frag_at(w, jt)) = s.hi; *(h4*)(pp + F::P / 2 + frag_at(w, jt)) = s.lo;
   }
   __syncthreads();
@@ -434,7 +454,7 @@ void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, 
   for (int x = 0; x < DT; x++)
 #pragma unroll
     for (int jt = 0; jt < 4; jt++) {
-      const Pair4 s = split4(kr[x][jt] * ksc);
+      const Pair4 s = split4<true>(kr[x][jt] * ksc);
       *(h4*)(kto + frag_at(w * DT + x, jt)) = s.hi; *(h4*)(kto + F::KT / 2 + frag_at(w * DT + x, jt)) = s.lo;
     }
 }
@@ -458,6 +478,7 @@ template <int HK, int NT> struct ScanLds {
   _Float16 S[2][NT][2][KS * 512], X[2][NT][2][2 * 512];            // pairs, as right operands, of even and odd chunks
   f4 bv[2][NT][4 * 64], cv[2][16];                                 // beta v, beta e^G of a chunk and the next, in the order of KEYS' lanes
   f4 norm[2][COLS], val[2][COLS];                                  // N and V, by wavefront
+  float low[2][COLS][16];                                          // the lowest beta |v| of four tokens
   int exps[2][COLS];
   struct {                                                         // a chunk that goes token by token: its rows, scaled, and the wavefronts' partial sums
     float k[CHUNK][HK], q[CHUNK][HK], v[CHUNK][COLS], decay[CHUNK], beta[CHUNK], part[2][2][4][COLS];
@@ -544,6 +565,7 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
     const auto b = buffer(scal + min(c, last) * scal_step, SCAL_FLOATS * 4);
     d.a = load_f4(b, gate_at, 512); d.b = load_f4(b, gate_at, 768);
   };
+  auto load_steps = [&](uint32_t c) __attribute__((always_inline)) { return load_f4(buffer(scal + min(c, last) * scal_step, SCAL_FLOATS * 4), l16 * 16, SCAL_STEP * 4); };
   auto load_mark = [&](uint32_t c) __attribute__((always_inline)) { return load_f1(buffer(scal + min(c, last) * scal_step, SCAL_FLOATS * 4), 0, SCAL_MARK * 4); };
 
   // ---- what STATE and KEYS leave for the others
@@ -574,17 +596,80 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
       L.bv[c & 1][t][w * 64 + lane] = x;
       const float y = rows4_sum(sum_abs4(x));
       if (lg == 0) L.val[c & 1][t * 16 + l16][w] = y;
+      f4 z = x;
+      if (c >= last) {                                             // rows behind the last column do not count
+#pragma unroll
+        for (int r = 0; r < 4; r++) z[r] = w * 16 + 4 * lg + r < rows_of(last) ? z[r] : INFINITY;
+      }
+      L.low[c & 1][t * 16 + l16][w * 4 + lg] = fminf(fminf(fabsf(z[0]), fabsf(z[1])), fminf(fabsf(z[2]), fabsf(z[3])));
     }
     if (l16 == 0) L.cv[c & 1][w * 4 + lg] = d.b;
   };
-  auto put_exponent = [&](uint32_t c, bool fresh, float mark) __attribute__((always_inline)) {      // E_c; fresh: the sums of |S| in front of chunk c itself are there
-    const bool marked = __builtin_amdgcn_readfirstlane(__float_as_uint(mark)) != 0;
+  // E_c, by the first of KEYS; fresh: the sums of |S| in front of chunk c itself are there.
+  // M_i = e^g_i M_(i-1) + beta_i |v_i|, from |S| on, is what token i takes in of a value column.  The pairs hold every term of a column to 22 bits or to a fixed part of its bound, whichever
+  // is more, so a chunk with a token whose M, over the columns, is less than HELD of their bounds goes the slow way, and one that leaves such a column.  Nearly always beta_i |v_i| of any two
+  // columns is enough by itself, and for every column that of the last token (looked at four tokens at a time); only where that is not so, M is summed up (in every chunk: 22.0 us instead of 19.2 for the walk over 1001 columns of 8 heads of 64 x 96; without any such check 16.8).
+  float taken[NT];                                                 // M behind the chunk before, of column l16, where it was summed up
+  bool summed = false;
+  auto put_exponent = [&](uint32_t c, bool fresh, float mark) __attribute__((always_inline)) {
+    if (w != 0 || c > last) return;
+    float bound[NT], before[NT];
+    bool enough = true, fine = true;
+    const uint32_t end = (rows_of(c) - 1) / 4;
 #pragma unroll
     for (int t = 0; t < NT; t++) {
-      const float before = fresh ? sum4(L.norm[c & 1][t * 16 + l16]) : 1.01f * (sum4(L.norm[(c - 1) & 1][t * 16 + l16]) + sum4(L.val[(c - 1) & 1][t * 16 + l16]));
-      const float bound = 1.02f * __builtin_fmaf(2.1f, before, sum4(L.val[c & 1][t * 16 + l16]));
-      const bool fine = !marked && (bound == 0.f || (bound >= 0x1p-90f && bound < 0x1p90f));
-      if (w == 0 && lg == 0) L.exps[c & 1][t * 16 + l16] = fine ? scale_exponent(bound) : NO_SCALE;
+      const uint32_t j = t * 16 + l16;
+      before[t] = fresh ? sum4(L.norm[c & 1][j]) : 1.01f * (sum4(L.norm[(c - 1) & 1][j]) + sum4(L.val[(c - 1) & 1][j]));
+      bound[t] = 1.02f * __builtin_fmaf(2.1f, before[t], sum4(L.val[c & 1][j]));
+      f4 low = *(const f4*)(&L.low[c & 1][j][4 * lg]);
+      enough = enough && L.low[c & 1][j][end] >= HELD * bound[t];
+#pragma unroll
+      for (int r = 0; r < 4; r++) low[r] += dpp_f32<0xB1>(low[r]);  // no more than any of the four tokens' sum over the column and its neighbour (l16 ^ 1)
+      enough = enough && fminf(fminf(low[0], low[1]), fminf(low[2], low[3])) >= HELD * (bound[t] + dpp_f32<0xB1>(bound[t]));
+    }
+    if (!__all(enough)) {                                          // a lane: four tokens (4 l16 ..) of the columns lg, 4 + lg, 8 + lg, 12 + lg of each tile
+      const f4 step = load_steps(c);
+      float d[5], all[4] = {0.f, 0.f, 0.f, 0.f}, floors = 0.f;     // decays over the lane's tokens, and those of 1, 3, 7, 15 lanes before it too
+      d[0] = (step[0] * step[1]) * (step[2] * step[3]);
+      d[1] = d[0] * dpp_or<0x111>(1.f, d[0]); d[2] = d[1] * dpp_or<0x112>(1.f, d[1]); d[3] = d[2] * dpp_or<0x114>(1.f, d[2]); d[4] = d[3] * dpp_or<0x118>(1.f, d[3]);
+#pragma unroll
+      for (int t = 0; t < NT; t++) {
+        float next = 0.f, front = taken[t];
+        if (!summed) front = fabsf(L.bv[(c - 1) & 1][t][15 * 16 + l16][3]);                          // at least the last token of the chunk before
+        if (fresh) front = before[t] * (HK == 64 ? 0.125f : 0.0884f);  // a 2-norm is at least the sum over the root of its length
+#pragma unroll 1
+        for (int i = 0; i < 4; i++) {
+          const int col = 4 * i + lg;
+          const f4 v = L.bv[c & 1][t][l16 * 16 + col];
+          float m = fabsf(v[0]);
+#pragma unroll
+          for (int r = 1; r < 4; r++) m = __builtin_fmaf(m, step[r], fabsf(v[r]));
+          m = __builtin_fmaf(dpp_or<0x111>(0.f, m), d[0], m); m = __builtin_fmaf(dpp_or<0x112>(0.f, m), d[1], m);
+          m = __builtin_fmaf(dpp_or<0x114>(0.f, m), d[2], m); m = __builtin_fmaf(dpp_or<0x118>(0.f, m), d[3], m);
+          m = __builtin_fmaf(dpp_or<0x111>(1.f, d[4]), __shfl(front, col), dpp_or<0x111>(0.f, m));
+#pragma unroll
+          for (int r = 0; r < 4; r++) { m = __builtin_fmaf(m, step[r], fabsf(v[r])); all[r] += m; }
+          const float x = __shfl(m, 16 * (l16 & 3) + 15);          // of column 4 i + l16 % 4
+          if ((l16 >> 2) == (uint32_t)i) next = x;
+        }
+        const float floor = HELD * bound[t];
+        taken[t] = next;
+        floors += floor;
+        fine = fine && (next >= floor || next == 0.f);
+      }
+      floors = row_sum(floors);
+#pragma unroll
+      for (int r = 0; r < 4; r++) { const float m = rows4_sum(all[r]); fine = fine && (m >= floors || m == 0.f); }
+      fine = __all(fine);
+      summed = true;
+    } else {
+      summed = false;
+    }
+    fine = fine && __float_as_uint(mark) == 0;
+#pragma unroll
+    for (int t = 0; t < NT; t++) {
+      const bool in = fine && (bound[t] == 0.f || (bound[t] >= 0x1p-90f && bound[t] < 0x1p90f));
+      if (lg == 0) L.exps[c & 1][t * 16 + l16] = in ? scale_exponent(bound[t]) : NO_SCALE;
     }
   };
   auto own_exponents = [&](uint32_t c, int (&e)[NT]) __attribute__((always_inline)) {               // of S in front of chunk c, from itself
@@ -634,16 +719,16 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
   };
   // product of a pair of left operands with the X of chunk c
   auto times_x = [&](uint32_t c, uint32_t t, const h8 (&x)[2][2]) __attribute__((always_inline)) {
-    f4 n0 = {0.f, 0.f, 0.f, 0.f}, n1 = n0, n2 = n0, n;
+    f4 n0 = {0.f, 0.f, 0.f, 0.f}, n1 = n0, n;                       // hi hi | hi lo + lo hi, 2048 times
 #pragma unroll
     for (int s = 0; s < 2; s++) {
       const h8 xh = *(const h8*)(&L.X[c & 1][t][0][s * 512 + lane * 8]), xl = *(const h8*)(&L.X[c & 1][t][1][s * 512 + lane * 8]);
       n0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s][0], xh, n0, 0, 0, 0);
       n1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s][0], xl, n1, 0, 0, 0);
-      n2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s][1], xh, n2, 0, 0, 0);
+      n1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s][1], xh, n1, 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < 4; i++) n[i] = __builtin_fmaf(n1[i], LO_INV, n0[i] + n2[i]);
+    for (int i = 0; i < 4; i++) n[i] = __builtin_fmaf(n1[i], LO_INV, n0[i]);
     return n;
   };
   // QUERIES: the start state's part of a chunk's output, all factors in, the factor of the other part, and the rows to store; P' X of that chunk comes a phase later
