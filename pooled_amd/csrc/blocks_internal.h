@@ -71,7 +71,7 @@ struct MoeParams {
   int kind;
 };
 
-// floats of an activation of so many values in reading order (moe_layer.hip): groups of 64 blocks with their sums; f32 weights: natural order
-#define MOE_GROUP_FLOATS (2048 + 128)
+// floats of an activation of so many values in reading order (moe_layer.hip): groups of 64 blocks; f32 weights: natural order
+#define MOE_GROUP_FLOATS 2048
 static inline uint32_t moe_act_floats(int kind, uint32_t values) { return kind == PA_W_F32 ? values : (values / 32 + 63) / 64 * MOE_GROUP_FLOATS; }
 hipError_t pa_launch_moe(const MoeParams& p, int n_cu, hipStream_t s);

@@ -14,8 +14,8 @@
 // no atomics, and a token's bits do not depend on the other tokens of the call.
 //
 // Measured with 256 experts of 512 x 2048, 8 chosen and one shared (router, choice, gate and up, down, in us): 1 token of Q4_0 4.5 + 7 + 5, each a launch's latency and a trip or two to
-// memory; 5 of Q8_0 5 + 22 + 14 for 131 MB of distinct weights, gate and up at 4 TB/s (a large copy runs at 4.9); 16 of Q4_0 8 + 5 + 29 + 20 for 182 MB, gate and up at
-// 4.2 TB/s.  f32, 27 tokens, 61 experts of 352 x 1056, 5 chosen: 5 + 5 + 41 + 26 for 245 MB.
+// memory; 5 of Q8_0 5 + 22 + 14 for 131 MB of distinct weights, gate and up at 4 TB/s (a large copy runs at 4.9); 16 of Q4_0 7.5 + 5 + 32 + 22 for 182 MB, gate and up at
+// 3.8 TB/s.  f32, 27 tokens, 61 experts of 352 x 1056, 5 chosen: 5 + 5 + 41 + 26 for 245 MB.
 #include "blocks_internal.h"
 #include "glue_math.h"
 #include <algorithm>
@@ -36,19 +36,18 @@ static __device__ inline uint32_t wave_max_u32(uint32_t v) {
 
 // ---- weights: what a lane holds of a row at a time -----------------------------------------------
 // Q8_0 and Q4_0: a block of 32 values with its scale; F32: two times four values, 64 lanes apart.  X: the float4 of activation that go with it.
-// Dequantisation is what bounds a pass of several tokens, so it is kept to 0.6 (Q4_0) and 1 (Q8_0: the conversion of a signed byte in place) instructions a weight beside the multiply-add.
+// Dequantisation is what bounds a pass of several tokens, so it is kept to 1.1 (Q4_0) and 1 (Q8_0: the conversion of a signed byte in place) instructions a weight beside the multiply-add.
 // Q4_0: the bits of an unsigned weight u in the low bits of an f16 ARE the number u 2^-24 (subnormal), and the mixed-precision multiply-add takes an f16 as it is.  A word gives its eight
 // nibbles as four masked pairs, every other one 16 times too large in place: the activations that meet those (elements 16 to 31 of a block) are kept divided by 16.  The offset of 8 comes
-// off as 8 times the block's sum of activations, which is kept beside them; a block's largest weight is 8 or close to it, so at most a bit of the sum is lost to that.  (For Q8_0 the same with
-// an offset of 128 would lose up to seven bits where a block's weights are small, and was no faster.)
+// off each pair by a packed f16 addition, which is exact there, before the activation is met: taken off the sum instead, as 8 times the block's sum of activations, it needs half an instruction
+// a weight less (16 tokens: gate and up 28 us instead of 32, down 20 instead of 22), but an activation much larger than its neighbours that meets a weight of zero then costs them their bits.
 template <int KIND> struct Piece { static constexpr int F4 = 8; static constexpr uint32_t STEP = 64; u4 w[KIND == PA_W_Q8_0 ? 2 : 1]; uint16_t sc; };
 template <> struct Piece<PA_W_F32> { static constexpr int F4 = 2; static constexpr uint32_t STEP = 128; f4 w[2]; };
-template <int KIND> struct Act { f4 x[Piece<KIND>::F4]; float sum; uint32_t have; };   // have: how many of the lane's loads lie in the row
+template <int KIND> struct Act { f4 x[Piece<KIND>::F4]; uint32_t have; };   // have: how many of the lane's loads lie in the row
 template <int KIND> static __device__ inline uint32_t pieces(uint32_t values) { return KIND == PA_W_F32 ? values / 4 : values / 32; }
 
 static __device__ inline float f16_bits_f32(uint16_t b) { _Float16 h; __builtin_memcpy(&h, &b, 2); return (float)h; }
 static __device__ inline h2v halves(uint32_t w) { h2v v; __builtin_memcpy(&v, &w, 4); return v; }
-static __device__ inline float half_of(uint32_t w, int i) { return (float)halves(w)[i]; }
 
 // acc + f * (piece . x)
 template <int KIND>
@@ -73,21 +72,21 @@ static __device__ inline float dot_piece(const Piece<KIND>& r, const Act<KIND>& 
     return __builtin_fmaf(a + b, f * f16_bits_f32(r.sc), acc);
   } else {
     // byte j of the block = elements j (low nibble) and j + 16 (high)
+    const h2v low = halves(0x80088008u), high = halves(0x80808080u);   // -8 2^-24, -8 x 16 2^-24
 #pragma unroll
     for (int k = 0; k < 4; k++) {
       const uint32_t w0 = r.w[0][k], w1 = w0 >> 8;
-      const uint32_t p0 = w0 & 0x000F000Fu, p1 = w0 & 0x00F000F0u, p2 = w1 & 0x000F000Fu, p3 = w1 & 0x00F000F0u;
-      a = __builtin_fmaf(half_of(p0, 0), x[k][0], a); b = __builtin_fmaf(half_of(p1, 0), x[k + 4][0], b);
-      a = __builtin_fmaf(half_of(p0, 1), x[k][2], a); b = __builtin_fmaf(half_of(p1, 1), x[k + 4][2], b);
-      a = __builtin_fmaf(half_of(p2, 0), x[k][1], a); b = __builtin_fmaf(half_of(p3, 0), x[k + 4][1], b);
-      a = __builtin_fmaf(half_of(p2, 1), x[k][3], a); b = __builtin_fmaf(half_of(p3, 1), x[k + 4][3], b);
+      const h2v p0 = halves(w0 & 0x000F000Fu) + low, p1 = halves(w0 & 0x00F000F0u) + high, p2 = halves(w1 & 0x000F000Fu) + low, p3 = halves(w1 & 0x00F000F0u) + high;
+      a = __builtin_fmaf((float)p0[0], x[k][0], a); b = __builtin_fmaf((float)p1[0], x[k + 4][0], b);
+      a = __builtin_fmaf((float)p0[1], x[k][2], a); b = __builtin_fmaf((float)p1[1], x[k + 4][2], b);
+      a = __builtin_fmaf((float)p2[0], x[k][1], a); b = __builtin_fmaf((float)p3[0], x[k + 4][1], b);
+      a = __builtin_fmaf((float)p2[1], x[k][3], a); b = __builtin_fmaf((float)p3[1], x[k + 4][3], b);
     }
-    return __builtin_fmaf(__builtin_fmaf(a + b, 16777216.0f, -8.0f * act.sum), f * f16_bits_f32(r.sc), acc);
+    return __builtin_fmaf(a + b, f * f16_bits_f32(r.sc) * 16777216.0f, acc);
   }
 }
 
-// Activations in reading order: for quantised weights groups of 64 blocks, in a group eight times 64 lanes x 4 values, then 64 sums of each half of a block; for f32
-// weights as they are.
+// Activations in reading order: for quantised weights groups of 64 blocks, in a group eight times 64 lanes x 4 values; for f32 weights as they are.
 #define GROUP_FLOATS MOE_GROUP_FLOATS
 // value e of an activation, written where its reader looks for it
 template <int KIND>
@@ -96,7 +95,6 @@ static __device__ inline uint32_t act_at(uint32_t e) {
   const uint32_t b = e / 32;
   return (b / 64) * GROUP_FLOATS + (((e % 32) / 4) * 64 + b % 64) * 4 + e % 4;
 }
-static __device__ inline uint32_t sum_at(uint32_t e) { return (e / 2048) * GROUP_FLOATS + 2048 + ((e / 16) % 2) * 64 + (e / 32) % 64; }   // of the 16 values from e on
 template <int KIND> static __device__ inline float stored(uint32_t e, float v) { return KIND == PA_W_Q4_0 && (e & 16) ? v * 0.0625f : v; }
 
 // piece q of an activation and of a row (f32: the four from q on); past the end (q >= n) the last one again, which nothing uses
@@ -111,7 +109,6 @@ static __device__ inline void load_act(Act<KIND>& d, const float* act, uint32_t 
     const float* g = act + (c / 64) * GROUP_FLOATS;
 #pragma unroll
     for (int i = 0; i < 8; i++) d.x[i] = ((const f4*)g)[i * 64 + c % 64];
-    if constexpr (KIND == PA_W_Q4_0) d.sum = g[2048 + c % 64] + g[2112 + c % 64];
   }
 }
 template <int KIND>
@@ -170,13 +167,10 @@ void pa_moe_router_kernel(const float* a_x, const float* a_router, const float* 
     const uint32_t q = q0 + lane;
     f4 v = {0.f, 0.f, 0.f, 0.f};
     if (q < n4) v = nw ? (x[q] * inv) * nw[q] : x[q];
-    float sum = (v[0] + v[1]) + (v[2] + v[3]);                     // of half a block: four lanes'
-    sum += dpp_f32<0xB1>(sum); sum += dpp_f32<0x4E>(sum);
     if (q < n4) {
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] = stored<KIND>(4 * q, v[j]);
       *(f4*)(xn + act_at<KIND>(4 * q)) = v;
-      if (KIND == PA_W_Q4_0 && (lane & 3) == 0) xn[sum_at(4 * q)] = sum;
     }
   }
 }
@@ -359,11 +353,6 @@ void pa_moe_gate_up_kernel(const float* a_logits, const uint32_t* a_sel, const f
     const uint32_t v = (m % slots) * p.ffn + first + threadIdx.x % 16;
     const float y = hs[threadIdx.x / 16][threadIdx.x % 16];
     h[act_at<KIND>(v)] = stored<KIND>(v, y);
-    if constexpr (KIND == PA_W_Q4_0) {
-      float s = y;
-      s += dpp_f32<0xB1>(s); s += dpp_f32<0x4E>(s); s += dpp_f32<0x141>(s); s += dpp_f32<0x140>(s);
-      if (threadIdx.x % 16 == 0) h[sum_at(v)] = s;
-    }
   }
   if (!CHOSEN && blockIdx.x == 0 && pair % slots == 0 && wave == 0) write_choice<NE>(p, a_logits + (size_t)(pair / slots) * logit_stride, n_experts, top_k, pair / slots, lane);
 }
@@ -442,10 +431,10 @@ void pa_moe_down_kernel(const uint32_t* a_sel, const float* a_sel_w, const float
 template <int KIND, int NE>
 static void launch_experts(const MoeParams& p, hipStream_t s) {
   // Tokens that share an expert read its weights together where the bytes are what bounds: f32 (27 tokens, 61 experts, 5 chosen: 80 us without groups, 41 with).  Quantised
-  // weights are bound by their instructions too, which a group does not save (16 tokens of Q4_0, 256 experts, 8 chosen: 29 us without, 38 with).
+  // weights are bound by their instructions too, which a group does not save (16 tokens of Q4_0, 256 experts, 8 chosen: 32 us without, 42 with; 6: 15.5 and 19.3).
   constexpr int GROUP = KIND == PA_W_F32 ? 4 : 1;
   // Up to so many tokens every workgroup makes its choice itself; more have it made once, in a launch of its own.  Both in us, that launch included, for 4, 8 and 12 tokens (256 experts, 8
-  // chosen; f32: 61 and 5): Q4_0 15.2 and 15.1, 25.8 and 21.3, 36.8 and 27.6; Q8_0 19.0 and 23.6, 34.4 and 37.2, 47.4 and 50.0; f32 14.3 and 17.9, 21.8 and 25.8, 30.0 and 32.4, and 56 and 46 for 27.
+  // chosen; f32: 61 and 5): Q4_0 14.4 and 15.9, 24.5 and 22.9, 35.1 and 30.2; Q8_0 19.0 and 23.6, 34.4 and 37.2, 47.4 and 50.0; f32 14.3 and 17.9, 21.8 and 25.8, 30.0 and 32.4, and 56 and 46 for 27.
   constexpr uint32_t INLINE = KIND == PA_W_Q4_0 ? 4 : 12;
   const dim3 grid(p.ffn / 16, p.n * p.slots);
   if (p.n <= INLINE) {
@@ -461,7 +450,8 @@ static hipError_t launch_kind(const MoeParams& p, int n_cu, hipStream_t s) {
   hipLaunchKernelGGL(pa_moe_router_kernel<KIND>, dim3((rows + 1 + 3) / 4, p.n), dim3(256), 0, s, p.x, p.router, p.norm_w, p.dim, p.x_stride, rows, p);
   if (p.n_experts <= 256) launch_experts<KIND, 4>(p, s); else launch_experts<KIND, 16>(p, s);
   // Rows a wavefront: quantised weights share the activations' loads over as many rows as still give every SIMD of the chip three wavefronts
-  // (16 tokens of Q4_0, 2048 rows: 20.4 us with 8 rows, 24.4 with 4; 5 tokens of Q8_0: 19.0 and 15.1; one token: 5.0 with 2 and the next loads ahead, 5.5 without them, 5.1 with 1);
+  // (16 tokens of Q4_0, 2048 rows: 22.0 us with 8 rows, 26.9 with 4; 6 tokens: 12.5 and 11.6; 5 of Q8_0: 19.0 and 15.1; one token, with 2 and the next loads ahead, without them, with 1 and them: Q4_0 5.1, 5.1, 4.8,
+  // Q8_0 5.3, 5.4, 5.0, f32 4.2, 5.0, 3.8, a launch's own spread being 0.5);
   // f32 pieces are short (27 tokens: 26.3 us with 2 rows, 28.8 with 4).
   auto down = [&](auto* kernel, uint32_t rw) { hipLaunchKernelGGL(kernel, dim3((p.dim + 4 * rw - 1) / (4 * rw), p.n), dim3(256), 0, s, p.sel, p.sel_w, p.h, p.h_floats, p.slots, p.ffn, p.dim, p); };
   if (p.n == 1) down(pa_moe_down_kernel<KIND, 2, true>, 2);
