@@ -156,9 +156,23 @@ void pa_moe_router_kernel(const float* a_x, const float* a_router, const float* 
     }
   }
   ss = wave_sum_f32(ss);
-  const float inv = nw ? 1.0f / sqrtf(ss / (float)dim + p.eps) : 1.f;
+  const float mean = ss / (float)dim + p.eps;
+  const float inv = nw ? 1.0f / sqrtf(mean) : 1.f;
+  // a token whose squares leave f32's range (from 2^50 a value on; or tiny, without eps): sums and factor again, in 64 bits
+  const bool far = nw && !(mean >= 0x1p-80f && mean < 0x1p100f);
+  double far_inv = 1.0;
+  if (at) a = wave_sum_f32(a + b) * inv;
+  if (far) {
+    double squares = 0.0, dot = 0.0;
+    for (uint32_t q = lane; q < n4; q += 64) {
+      const f4 xv = x[q], rv = r[q], wv = nw[q];
+#pragma unroll
+      for (int j = 0; j < 4; j++) { squares += (double)xv[j] * (double)xv[j]; dot += (double)xv[j] * (double)wv[j] * (double)rv[j]; }
+    }
+    far_inv = 1.0 / sqrt(wave_sum_f64(squares) / (double)dim + (double)p.eps);
+    a = (float)(wave_sum_f64(dot) * far_inv);
+  }
   if (at) {
-    a = wave_sum_f32(a + b) * inv;
     if (lane == 0) p.logits[(size_t)t * p.logit_stride + at - 1] = a;
     return;
   }
@@ -166,7 +180,15 @@ void pa_moe_router_kernel(const float* a_x, const float* a_router, const float* 
   for (uint32_t q0 = 0; q0 < n4; q0 += 64) {
     const uint32_t q = q0 + lane;
     f4 v = {0.f, 0.f, 0.f, 0.f};
-    if (q < n4) v = nw ? (x[q] * inv) * nw[q] : x[q];
+    if (q < n4) {
+      v = x[q];
+      if (far) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) v[j] = (float)((double)v[j] * far_inv) * nw[q][j];
+      } else if (nw) {
+        v = (v * inv) * nw[q];
+      }
+    }
     if (q < n4) {
 #pragma unroll
       for (int j = 0; j < 4; j++) v[j] = stored<KIND>(4 * q, v[j]);

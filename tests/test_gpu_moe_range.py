@@ -1,6 +1,7 @@
 """The mixture-of-experts layer where one value is far larger than those beside it, against the 64-bit oracle.  Tolerance: test_gpu_moe's, RTOL of the 2-norm of what the layer adds."""
 import numpy as np
 import pytest
+from oracle import blocks_oracle as B
 from pooled_amd.capi import PooledAttn, PA_W_Q4_0, PA_W_Q8_0
 from test_gpu_moe import CTX, RTOL, Layer
 
@@ -57,3 +58,21 @@ def test_a_large_expert_value_without_weight(kind, at, n):
     no_weight(L, "down", at)
     x = L.rng.standard_normal((n, L.dim)).astype(np.float32)
     check(L, x, slice(None))
+
+
+@pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("size,eps", [(1e15, 1e-6), (1e19, 1e-6), (1e25, 1e-6), (1e37, 1e-6), (1e-12, 0.0), (1e-20, 0.0), (1e-30, 0.0)])
+def test_residuals_whose_squares_leave_f32(size, eps, n):
+    """The norm takes the size out: choices, weights and what is added are those of a residual of ordinary size."""
+    L = Layer(dim=1056, ffn=64, E=12, top_k=3, kind=PA_W_Q4_0, seed=int(abs(np.log10(size))))
+    x = (L.rng.standard_normal((n, L.dim)) * size).astype(np.float32)
+    with PooledAttn(dict(CTX, eps=eps), 64, max_cols=max(n, 2)) as pa:
+        y, ids, w = L.call(pa, L.handle(pa), x)
+    ref, rids, rw = B.moe_layer(x, L.norm, L.router, L.ex, L.top_k, L.kind, L.renorm, L.shared, eps=eps)
+    assert np.array_equal(ids, rids)
+    assert np.all(np.abs(w - rw) <= RTOL * rw * 20)                  # as in test_gpu_moe
+    # test_gpu_moe's condition times the norm of what is added: that is nothing in 64 bits beside the largest residuals
+    d = np.sqrt(((y.astype(np.float64) - ref) ** 2).sum(-1))
+    room = RTOL * np.sqrt(((ref - x) ** 2).sum(-1)) + 2.0 ** -24 * np.sqrt((ref ** 2).sum(-1))
+    print("error %.2e of %.2e" % (d.max(), room.min()))
+    assert np.all(d <= room)
