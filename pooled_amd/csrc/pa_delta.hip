@@ -183,7 +183,7 @@ static int rule_params(pa_ctx* ctx, const char* who, pa_delta* dn, uint32_t laye
   if (overlap(o, state)) return block_fail(ctx, PA_ERR_INVALID, who, "the output shares memory with the state");
   memset(&p, 0, sizeof p);
   p.q = d_out ? d_q : d_k; p.k = d_k; p.v = d_v; p.g = d_g; p.beta = d_beta; p.state = (float*)pa_delta_state_ptr(dn, layer, 0); p.out = d_out;
-  p.q_stride = d_out ? q_stride : k_stride; p.k_stride = k_stride; p.v_stride = v_stride; p.gate_stride = gate_stride; p.out_stride = out_stride;
+  p.q_stride = d_out ? q_stride : k_stride; p.k_stride = k_stride; p.v_stride = v_stride; p.gate_stride = gate_stride; p.out_stride = d_out ? out_stride : 0;
   p.n = n_cols; p.commit = n_commit; p.nk = c.n_k_heads; p.nv = c.n_v_heads; p.hk = c.head_k; p.hv = c.head_v; p.group = c.n_v_heads / c.n_k_heads;
   p.scale = dn->scale; p.eps = c.eps; p.l2norm = c.flags & PA_DELTA_L2NORM; p.out_f16 = out_dtype == PA_OUT_F16;
   return PA_OK;
