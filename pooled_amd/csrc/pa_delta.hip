@@ -210,6 +210,6 @@ extern "C" int pa_delta_prefill(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const
   if (rc) return rc;
   DeviceGuard on(ctx->device);
   // (a chunk's rows of v and of the output are addressed with 32-bit offsets)
-  const hipError_t e = chunked(n_cols) && v_stride <= (1u << 22) && out_stride <= (1u << 22) ? pa_launch_delta_chunks(p, dn->ws, dn->ws_chunks, ctx->n_cu, ctx->stream) : pa_launch_delta_step(p, ctx->stream);
+  const hipError_t e = chunked(n_cols) && p.v_stride <= (1u << 22) && p.out_stride <= (1u << 22) ? pa_launch_delta_chunks(p, dn->ws, dn->ws_chunks, ctx->n_cu, ctx->stream) : pa_launch_delta_step(p, ctx->stream);
   return e == hipSuccess ? PA_OK : block_fail_hip(ctx, e, who);
 }
