@@ -369,7 +369,7 @@ void* pa_delta_state_ptr(pa_delta* dn, uint32_t layer, int which);
  *   d_qkv, d_out: f32 [n_cols][stride], 16-byte aligned, strides multiples of 4;  d_conv_w: f32 [channels][conv_width], 16-byte aligned;
  *   d_conv_b: f32 [channels], 16-byte aligned, or NULL;  d_a, d_b: f32 [n_cols][ab_stride];  d_a_log, d_dt_bias: f32 [n_v_heads];
  *   d_g, d_beta: f32 [n_cols][gate_stride].  Outputs share no memory with inputs or the state, and no input lies in the state (ranges from the first
- *   column to the last count: columns of an input and an output do not interleave either). */
+ *   column to the last count: columns of an input and an output do not interleave either); those of two outputs may lie between one another, but share nothing. */
 int pa_delta_glue(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const float* d_qkv, uint32_t qkv_stride, const float* d_conv_w, const float* d_conv_b,
                   const float* d_a, const float* d_b, uint32_t ab_stride, const float* d_a_log, const float* d_dt_bias, uint32_t n_cols,
                   uint32_t n_commit, float* d_out, uint32_t out_stride, float* d_g, float* d_beta, uint32_t gate_stride);

@@ -1,6 +1,7 @@
-// What the host sides of the blocks beside attention share: errors, the context's device, memory ranges.
+// What the host sides of the blocks beside attention share: errors, the context's device; with spans.h, memory ranges.
 #pragma once
 #include "pa_internal.h"
+#include "spans.h"
 #include <algorithm>
 
 // the message of a failing call; an allocation that fails on the way leaves the old message
@@ -23,10 +24,3 @@ struct DeviceGuard {
   DeviceGuard(const DeviceGuard&) = delete;
   DeviceGuard& operator=(const DeviceGuard&) = delete;
 };
-
-static inline bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
-struct Span { const void* p; size_t bytes; };
-static inline Span cols(const void* p, uint32_t n, uint32_t stride, uint32_t col, size_t elem) { return {p, ((size_t)(n - 1) * stride + col) * elem}; }
-static inline bool overlap(const Span& a, const Span& b) {
-  return a.p && b.p && a.bytes && b.bytes && (uintptr_t)a.p < (uintptr_t)b.p + b.bytes && (uintptr_t)b.p < (uintptr_t)a.p + a.bytes;
-}

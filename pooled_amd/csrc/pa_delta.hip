@@ -143,6 +143,8 @@ extern "C" int pa_delta_glue(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const fl
                      {pa_delta_state_ptr(dn, layer, 1), pa_delta_state_bytes(dn, 1)}};
   const Span res[] = {cols(d_out, n_cols, out_stride, dn->channels, 4), cols(d_g, n_cols, gate_stride, c.n_v_heads, 4), cols(d_beta, n_cols, gate_stride, c.n_v_heads, 4)};
   for (const Span& o : res) for (const Span& i : in) if (overlap(o, i)) return block_fail(ctx, PA_ERR_INVALID, who, "an output shares memory with an input");
+  const Columns res_cols[] = {{d_out, out_stride * 4ul, dn->channels * 4ul}, {d_g, gate_stride * 4ul, c.n_v_heads * 4ul}, {d_beta, gate_stride * 4ul, c.n_v_heads * 4ul}};
+  for (int i = 0; i < 3; i++) for (int j = 0; j < i; j++) if (columns_meet(res_cols[i], res_cols[j], n_cols)) return block_fail(ctx, PA_ERR_INVALID, who, "two outputs share memory");
   const Span& state = in[sizeof in / sizeof *in - 1];
   for (const Span& i : in) if (&i != &state && overlap(state, i)) return block_fail(ctx, PA_ERR_INVALID, who, "an input lies in the layer's state");
   DeltaGlueParams p; memset(&p, 0, sizeof p);
