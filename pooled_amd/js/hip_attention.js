@@ -320,10 +320,9 @@ class HipAttention {
     return { S: get(0), conv: get(1) };
   }
   writeDelta(i, st) {
-    [st.S, st.conv].forEach((a, w) => {
-      if (a.byteLength !== addon.deltaStateBytes(this.delta.handle, w)) throw new Error("writeDelta: saved state has the wrong shape");
-      if (a.length) addon.deltaWrite(this.ctx, this.delta.handle, i, w, a);
-    });
+    const parts = [st.S, st.conv];                              // both are looked at before either is written
+    parts.forEach((a, w) => { if (a.byteLength !== addon.deltaStateBytes(this.delta.handle, w)) throw new Error("writeDelta: saved state has the wrong shape"); });
+    parts.forEach((a, w) => { if (a.length) addon.deltaWrite(this.ctx, this.delta.handle, i, w, a); });
   }
 
   // ---- mixture-of-experts layers ----
