@@ -477,7 +477,7 @@ static hipError_t launch_kind(const MoeParams& p, int n_cu, hipStream_t s) {
   // f32 pieces are short (27 tokens: 26.3 us with 2 rows, 28.8 with 4).
   auto down = [&](auto* kernel, uint32_t rw) { hipLaunchKernelGGL(kernel, dim3((p.dim + 4 * rw - 1) / (4 * rw), p.n), dim3(256), 0, s, p.sel, p.sel_w, p.h, p.h_floats, p.slots, p.ffn, p.dim, p); };
   if (p.n == 1) down(pa_moe_down_kernel<KIND, 2, true>, 2);
-  else if (KIND == PA_W_F32) down(pa_moe_down_kernel<KIND, 2, false>, 2);
+  else if constexpr (KIND == PA_W_F32) down(pa_moe_down_kernel<KIND, 2, false>, 2);
   else if ((uint64_t)p.n * (p.dim / 8) >= (uint64_t)n_cu * 12) down(pa_moe_down_kernel<KIND, 8, false>, 8);
   else down(pa_moe_down_kernel<KIND, 4, false>, 4);
   return hipGetLastError();
