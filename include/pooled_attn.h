@@ -332,8 +332,10 @@ int pa_attn_layer_prefill(pa_ctx* ctx, uint32_t layer, const pa_weight* w_qkv, c
  *      cache rows, such a layer keeps per v head h a matrix S [head_v][head_k], and the last conv_width - 1 inputs of a short
  *      convolution.  With k head h / (n_v_heads / n_k_heads), a token t is
  *        S' = exp(g) S;  u = beta (v - S' k);  S = S' + u k^T;  o = scale S q
- *      and, with PA_DELTA_L2NORM, q and k are first divided by sqrt(sum of their squares + eps).  All in f32.
- *      g and beta may be any numbers: g = -inf empties a head's state in front of the token, beta = 0 leaves a token out. ---- */
+ *      and, with PA_DELTA_L2NORM, q and k are first divided by sqrt(sum of their squares + eps).  All in f32, the sums of squares
+ *      too: lengths of q and k stay below 2^63.
+ *      g and beta may be any numbers: g = -inf empties a head's state in front of the token, beta = 0 leaves a token out (0 times what
+ *      is not finite is NaN here as in the formulas: a state to be emptied, and k and v of a token to be left out, are finite). ---- */
 #define PA_DELTA_L2NORM 1u
 typedef struct pa_delta_config {
   uint32_t n_k_heads;    /* q and k heads */

@@ -465,7 +465,8 @@ void pa_delta_prep_kernel(const float* a_k, const float* a_q, const float* a_g, 
 // other halves of the phases: Q S while STATE works, P' X of the chunk before while KEYS do, so S and X are there twice.  Two barriers a chunk: S is there | X is there.  Every role has
 // a loop of its own, unrolled by two: no register that a load is still filling is ever copied, and no wait is shared.  (NT = 2 has no registers for second sets of operands.)
 // What bounds it: the operands, 112 KB a chunk for each workgroup whatever its columns, at 64 bytes a cycle of a CU 1750 of about 3000 cycles, and a chunk's two barriers with
-// their exchanges.  2048 columns of 32 heads: 64 us with the operands from the last-level cache, 53 from L2, 42 alone on the chip; of 48 heads (NT = 2): 84.
+// their exchanges.  2048 columns of 32 heads: 64 us with the operands from the last-level cache, of 48 heads (NT = 2) 87; before the check of a chunk's range
+// 63 and 84, and with 32 heads 53 from L2 and 42 alone on the chip.
 //
 // Scales: E_c is the exponent, per value column, that X of chunk c and the state behind it are scaled by.  It comes from the sums N_c of |S| in front of the chunk before and the
 // sums V of beta |v|: |S| in front of chunk c <= N_(c-1) + V_(c-1), so that KEYS find it a chunk ahead (sums of magnitudes are no smaller than norms, and they neither over- nor
@@ -513,7 +514,7 @@ static __device__ __attribute__((always_inline)) void scan_role(const DeltaParam
 
   // ---- requests.  Past the last chunk the last one's is made again instead of branching round the loads: a short conditional block between a matrix
   // instruction and the first use of its result makes this compiler (22.0.0git, ROCm 7.2.0) leave out the wait states on the path round the block, and the use then reads the old
-  // registers (seen as states 1e-4 off after a last chunk).  No dword is loaded that is not used: its register would be taken for something else, and that would wait for the load.
+  // registers (seen as states 1e-4 off after a last chunk; tests/test_wait_states.py looks for it in what was built).  No dword is loaded that is not used: its register would be taken for something else, and that would wait for the load.
   // Rows behind the last column read as zero and are not written: the buffers end with the last column.
   struct KF { h8 x[KS][2]; };
   struct GF { h8 x[MT][2][2]; };
@@ -929,7 +930,7 @@ static hipError_t launch_chunks(const DeltaParams& p, void* mem, uint32_t ws_chu
   const DeltaWs ws = ws_at<HK>(mem, ws_chunks, p.nk, p.nv, nullptr);
   const uint32_t seg = ws_chunks * CHUNK;
   // Two tiles of value columns a workgroup where one each would not fit on the chip at once: the operands are read half as often, but each chunk takes longer.  2048 columns
-  // of 48 heads of 128 values: 84 us with two (192 workgroups), 128 with one (384 on 256 CUs); of 32 heads: 75 with two (128 workgroups), 63 with one (256).
+  // of 48 heads of 128 values: 84 us with two (192 workgroups), 128 with one (384 on 256 CUs); of 32 heads: 75 with two (128 workgroups), 63 with one (256); all before the check of a chunk's range.
   const bool wide = p.hv % 32 == 0 && p.nv * (p.hv / 16) > (uint32_t)n_cu;
   for (uint32_t c0 = 0; c0 < p.n; c0 += seg) {
     DeltaParams r = p;

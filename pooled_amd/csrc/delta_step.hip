@@ -7,8 +7,8 @@
 // four DPP steps each, and nothing is exchanged between wavefronts.  With 32 v heads of 128 x 128 that is 1024 wavefronts, one per SIMD.
 //
 // One token moves 2 x 4 bytes per state value and computes 6 operations on it: it is bound by the state's stream and, at these sizes (2 MB), by the
-// latency of a launch.  A run of columns is bound by the chain dot -> u -> update of each token; the next columns' q, k, v and gates are
-// requested four columns ahead, so the chain alone counts.  Everything is f32.  A column's arithmetic does not depend on how many columns a
+// latency of a launch.  A run of columns is bound by its instructions, some 93 vector instructions a column and wavefront (370 cycles of 580 measured; 0.24 us a column
+// with one wavefront a SIMD, 0.37 with two on half of them), and by the chain dot -> u -> update; the next columns' q, k, v and gates are requested four columns ahead.  Everything is f32.  A column's arithmetic does not depend on how many columns a
 // call has: a verify block gives every column the bits of the one-token call at its place.
 #include "blocks_internal.h"
 #include "glue_math.h"

@@ -6,13 +6,14 @@
 #include <new>
 
 // Columns that pa_delta_prefill takes in one round of its two kernels.  The fragments of a round (2.6 MB a chunk of 64 with 32 v heads of 128 x 128) should stay in the last-level cache
-// between them, and each round costs two launches: 8192 columns of 32 heads take 402 us in rounds of 1024, 362 in rounds of 2048, 404 of 4096, 412 at once.  So the workspace does not
+// between them, and each round costs two launches: 8192 columns of 32 heads take 402 us in rounds of 1024, 362 in rounds of 2048, 404 of 4096, 412 at once (before the check of a chunk's range, 1 us more).  So the workspace does not
 // grow with the prompt either.
 #define SEGMENT_COLS 2048u
 
-// Which form serves a prefill call.  The step kernel takes 0.24 us a column of 32 heads of 128 x 128 (0.37 of 48), the chunked form 16 us for any first chunk.  Both in us, steps
-// and chunks: 32 heads 12.6 and 16.5 for 40 columns, 14.5 and 16.8 for 48, 18.3 and 17.1 for 64; 48 heads 18.0 and 18.0, 20.9 and 18.2, 26.3 and 18.6; 8 heads of
-// 64 x 96 10.4 and 13.1, 12.1 and 13.2, 15.2 and 13.4.
+// Which form serves a prefill call.  The step kernel takes 0.24 us a column of 32 heads of 128 x 128 (0.37 of 48 or 64), the chunked form 13 to 19 us for any first chunk.  Steps and chunks,
+// in us, for 40, 48, 56 and 64 columns: 4 heads 12.0 and 16.2, 13.9 and 16.4, 16.0 and 16.6, 17.9 and 16.8; 8 heads of 64 x 96 10.4 and 13.3, 12.1 and 13.4, 13.7 and 13.5, 15.4 and 13.6; 32 heads 13.1 and
+// 17.2, 14.8 and 17.1, 16.7 and 17.2, 18.5 and 17.4; 48 heads 18.5 and 18.7, 21.2 and 19.0, 24.1 and 19.2, 26.5 and 19.4; 64 heads the same within 0.6.  Equal at 42 to 60 columns: one number
+// for all heads, at 48 at most 2.5 us behind and at most 2.5 ahead.
 static bool chunked(uint32_t n_cols) { return n_cols >= 48; }
 
 extern "C" int pa_delta_destroy(pa_ctx* ctx, pa_delta* dn) {
