@@ -386,7 +386,8 @@ int pa_delta_glue(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const float* d_qkv,
  * pa_delta_prefill: the same for n_cols columns of a prompt, all of them committed, in chunks of 64 on the matrix cores where that is faster (from
  * 48 columns on).  Its results agree with pa_delta_decode's to f32 rounding of what a token takes in, exp(g) of the tokens before
  * and its own beta |v|: chunks whose sizes or decays are further apart than the matrix cores' operands hold (2^23), and those with keys longer than one, gates
- * that grow or numbers that are not finite, are found on the device and go token by token (32 heads of 128 x 128: 0.43 us a column there, 0.04 otherwise). */
+ * that grow or numbers that are not finite, are found on the device and go token by token (32 heads of 128 x 128: 0.43 us a column there, 0.04 otherwise).  f32 arithmetic on every
+ * column, whatever it holds: pa_delta_decode, which takes as many. */
 int pa_delta_decode(pa_ctx* ctx, pa_delta* dn, uint32_t layer, const float* d_q, uint32_t q_stride, const float* d_k, uint32_t k_stride, const float* d_v,
                     uint32_t v_stride, const float* d_g, const float* d_beta, uint32_t gate_stride, uint32_t n_cols, uint32_t n_commit, void* d_out,
                     uint32_t out_stride, int out_dtype);
