@@ -130,6 +130,18 @@ int pa_glue_kv(pa_ctx* ctx, uint32_t layer, const float* d_q_in, uint32_t q_stri
  * attn_glue does (engine/wgsl/qwen35.js:1082-1136; call site engine/qwen35.js:2473-2483). */
 int pa_glue(pa_ctx* ctx, const float* d_q_in, uint32_t q_stride, float* d_k, uint32_t k_stride,
             const float* d_qw, const float* d_kw, uint32_t base_pos, uint32_t n_cols);
+/* pa_glue_kv_at: pa_glue_kv for columns that have positions of their own: column c is rotated by its own positions and its k and v go to cache row
+ * base_row + c.  For the columns of a draft tree, whose positions are their depths', and for prompts with images or video, whose
+ * rotary positions have several axes.  No counterpart in the reference, whose positions are base_pos + c.
+ *   d_pos: u32 [axes][pos_stride]: column c's position on axis a is d_pos[a * pos_stride + c]; pos_stride >= n_cols (not looked at with one axis).  Any number:
+ *          those below max_seq come from the context's table, others are worked out in the kernel (slower; the same bits).
+ * The angle of pair i is f32(position on the pair's axis) * f32(theta^(-2i / n_rot)), rounded to f32 as in pa_glue_kv, so that rows of either call stand side by side in a cache:
+ * where all axes hold base_row + c the results have pa_glue_kv's bits.  The other arguments as there; inputs must not lie in the context's q and gate buffers.
+ * pa_set_rope_axes: the number of axes, 1 to 4, and the axis of each of the n_rot / 2 rotated pairs (NULL: one axis, which is the default).  Copied; host state that
+ * later calls (and graphs recorded later) go by. */
+int pa_set_rope_axes(pa_ctx* ctx, uint32_t n_axes, const uint8_t* h_axis_of_pair);
+int pa_glue_kv_at(pa_ctx* ctx, uint32_t layer, const float* d_q_in, uint32_t q_stride, const float* d_k, uint32_t k_stride, const float* d_v, uint32_t v_stride,
+                  const float* d_qw, const float* d_kw, const uint32_t* d_pos, uint32_t pos_stride, uint32_t base_row, uint32_t n_cols);
 /* pa_kv_store: f16 (round-to-nearest-even) write of already-roped k and raw v rows at base_pos + c.
  * Replaces kv_store (engine/wgsl/qwen35.js:889-906; call site engine/qwen35.js:2488). */
 int pa_kv_store(pa_ctx* ctx, uint32_t layer, const float* d_k, uint32_t k_stride, const float* d_v,
@@ -206,6 +218,17 @@ int pa_attn_decode_step_noalloc(pa_ctx* ctx, uint32_t layer, const float* d_q_in
 int pa_attn_decode_gather(pa_ctx* ctx, uint32_t layer, const float* d_q, uint32_t q_stride, const float* d_gate,
                           uint32_t gate_stride, const uint32_t* d_sel, uint32_t sel_stride, uint32_t max_rows,
                           uint32_t n_cols, void* d_out, uint32_t out_stride, int out_dtype);
+/* pa_attn_tree: attention of a tree of drafted tokens: column c sees the cache rows [0, base_pos) and those rows base_pos + j, j < n_cols, whose bit is set in its mask, so that
+ * several continuations of one context are verified in one pass (pa_attn_decode's verify block is the one whose mask is a triangle).  The columns' rows are in the cache
+ * already (pa_glue_kv_at with the depths' positions, or pa_glue_kv); pa_kv_compact then keeps the accepted path.  No counterpart in the reference, whose drafts are chains.
+ *   d_mask: u32 [n_cols][mask_stride]; bit j % 32 of word j / 32 of a column's words: it sees row base_pos + j (a node's own bit and its ancestors').  Any pattern; bits
+ *           from n_cols on are not looked at; a column that sees nothing (base_pos 0, no bit) gives zeros.  A drafted row with infinities or NaN reaches those columns alone that see it.
+ *   d_q, d_gate, d_out: as in pa_attn_decode, but the output shares no memory with the inputs (refused).
+ * Operands (q, P, int8 rows' values) are f16, products, sums and softmax f32, as in pa_attn_decode; partials of a split context are kept in f16.  Results do not depend on the
+ * mask rows of other columns; they agree with pa_attn_decode's on a chain to rounding.  pa_set_decode_splits applies.  Partials share the context's scratch: a call that grows it
+ * allocates; under stream capture, where it cannot, the context is split into as many parts as there is room for. */
+int pa_attn_tree(pa_ctx* ctx, uint32_t layer, const float* d_q, uint32_t q_stride, const float* d_gate, uint32_t gate_stride, const uint32_t* d_mask,
+                 uint32_t mask_stride, uint32_t base_pos, uint32_t n_cols, void* d_out, uint32_t out_stride, int out_dtype);
 /* which kernel / split / tile shape the table picks (kind: 0 decode/verify, 1 prefill) */
 int pa_plan_query(const pa_ctx* ctx, int kind, uint32_t base_pos, uint32_t n_cols, pa_plan* out);
 /* override the table's split count for decode passes (0 = table); the reference's attnDecodeSplits
@@ -229,6 +252,12 @@ int pa_kv_write(pa_ctx* ctx, uint32_t layer, int which, uint32_t row0, uint32_t 
  * what pa_kv_read / pa_kv_write move per row and pa_slot_export / pa_slot_import per saved position -- the part sizes of
  * the reference's saved states (engine/qwen35.js:121-131).  0 for a tensor the context does not have. */
 size_t pa_kv_row_bytes(const pa_ctx* ctx, int which);
+/* pa_kv_compact: row dst_row + i of every allocated layer's caches (and scales) becomes what row list[i] was, in place, in one call: the accepted path of a draft tree moved to
+ * the end of the context, or a context cut to the rows worth keeping.  The other rows stay as they are.  No counterpart in the reference, whose caches are cut back to a prefix.
+ *   d_sel: u32: the list's length n, then n cache rows, ascending, each once, the first at or behind dst_row (pa_attn_decode_gather's list).  It is on the device, so a draft may be accepted
+ *          there, and is not trusted: n > max_rows is read as max_rows, rows are clamped to the cache; a list in another order leaves unspecified rows of its own at dst_row .. dst_row + n - 1.
+ *   max_rows: the longest list; dst_row + max_rows <= max_seq. */
+int pa_kv_compact(pa_ctx* ctx, uint32_t dst_row, const uint32_t* d_sel, uint32_t max_rows);
 /* device address of a cache (read-only use; the head-major device layout described at pa_layer_alloc) */
 const void* pa_kv_device_ptr(pa_ctx* ctx, uint32_t layer, int which);
 

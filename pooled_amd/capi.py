@@ -62,11 +62,14 @@ SYMBOLS = {
     "pa_glue_kv": (c_int, [vp, u32, f32p, u32, f32p, u32, f32p, u32, f32p, f32p, u32, u32]),
     "pa_glue": (c_int, [vp, f32p, u32, f32p, u32, f32p, f32p, u32, u32]),
     "pa_kv_store": (c_int, [vp, u32, f32p, u32, f32p, u32, u32, u32]),
+    "pa_set_rope_axes": (c_int, [vp, u32, vp]),
+    "pa_glue_kv_at": (c_int, [vp, u32, f32p, u32, f32p, u32, f32p, u32, f32p, f32p, vp, u32, u32, u32]),
     "pa_q_buffer": (vp, [vp]),
     "pa_gate_buffer": (vp, [vp]),
     "pa_attn_decode": (c_int, [vp, u32, f32p, u32, f32p, u32, u32, u32, vp, u32, c_int]),
     "pa_attn_prefill": (c_int, [vp, u32, f32p, u32, f32p, u32, u32, u32, vp, u32, c_int]),
     "pa_attn_decode_gather": (c_int, [vp, u32, f32p, u32, f32p, u32, vp, u32, u32, u32, vp, u32, c_int]),
+    "pa_attn_tree": (c_int, [vp, u32, f32p, u32, f32p, u32, vp, u32, u32, u32, vp, u32, c_int]),
     "pa_attn_decode_step": (c_int, [vp, u32, f32p, f32p, f32p, f32p, f32p, u32, vp, c_int]),
     "pa_attn_decode_step_noalloc": (c_int, [vp, u32, f32p, f32p, f32p, f32p, f32p, u32, vp, c_int]),
     "pa_plan_query": (c_int, [vp, c_int, u32, u32, ctypes.POINTER(PaPlan)]),
@@ -75,6 +78,7 @@ SYMBOLS = {
     "pa_set_weight_cache": (c_int, [vp, ctypes.c_size_t]),
     "pa_kv_read": (c_int, [vp, u32, c_int, u32, u32, vp]),
     "pa_kv_write": (c_int, [vp, u32, c_int, u32, u32, vp]),
+    "pa_kv_compact": (c_int, [vp, u32, vp, u32]),
     "pa_kv_row_bytes": (ctypes.c_size_t, [vp, c_int]),
     "pa_kv_device_ptr": (vp, [vp, u32, c_int]),
     "pa_timer_start": (c_int, [vp]),
@@ -134,6 +138,28 @@ class PaError(RuntimeError):
     def __init__(self, code, msg):
         RuntimeError.__init__(self, "pooled_attn error %d: %s" % (code, msg))
         self.code = code
+
+
+def tree_mask(seen):
+    """A bool matrix [n, n] (row c: the drafted rows that column c sees, itself among them) as pa_attn_tree's mask words, uint32 [n, ceil(n / 32)]."""
+    seen = np.asarray(seen, bool)
+    n = seen.shape[0]
+    bits = np.zeros((n, (n + 31) // 32 * 32), np.uint8)
+    bits[:, :n] = seen
+    return np.packbits(bits, axis=1, bitorder="little").view("<u4").astype(np.uint32)
+
+
+def tree_of_parents(parents):
+    """The bool matrix of a draft tree: parents[c] is the column before c that c continues, or -1 where it continues the context."""
+    n = len(parents)
+    seen = np.zeros((n, n), bool)
+    for c, up in enumerate(parents):
+        if not -1 <= up < c:
+            raise ValueError("tree_of_parents: a column's parent comes before it")
+        if up >= 0:
+            seen[c] = seen[up]
+        seen[c, c] = True
+    return seen
 
 
 class DeviceBuffer:
@@ -255,6 +281,20 @@ class PooledAttn:
         self._chk(self.L.pa_glue_kv(self.ctx, layer, d_q.ptr, q_stride, d_k.ptr, k_stride, d_v.ptr, v_stride,
                                     d_qw.ptr if d_qw else None, d_kw.ptr if d_kw else None, base_pos, n_cols))
 
+    def set_rope_axes(self, axis_of_pair=None):
+        """The axis of each rotated pair (n_rot / 2 numbers, 0 .. 3) for glue_kv_at's positions; None: one axis."""
+        if axis_of_pair is None:
+            return self._chk(self.L.pa_set_rope_axes(self.ctx, 1, None))
+        a = np.asarray(axis_of_pair)
+        if a.size != self.cfg["n_rot"] // 2 or a.min() < 0 or a.max() > 3:
+            raise ValueError("set_rope_axes: %d pairs, each of an axis 0 .. 3" % (self.cfg["n_rot"] // 2))
+        a = np.ascontiguousarray(a, dtype=np.uint8)
+        self._chk(self.L.pa_set_rope_axes(self.ctx, int(a.max()) + 1, a.ctypes.data))
+
+    def glue_kv_at(self, layer, d_q, q_stride, d_k, k_stride, d_v, v_stride, d_qw, d_kw, d_pos, pos_stride, base_row, n_cols):
+        self._chk(self.L.pa_glue_kv_at(self.ctx, layer, d_q.ptr, q_stride, d_k.ptr, k_stride, d_v.ptr, v_stride,
+                                       d_qw.ptr if d_qw else None, d_kw.ptr if d_kw else None, d_pos.ptr, pos_stride, base_row, n_cols))
+
     def glue(self, d_q, q_stride, d_k, k_stride, d_qw, d_kw, base_pos, n_cols):
         self._chk(self.L.pa_glue(self.ctx, d_q.ptr, q_stride, d_k.ptr, k_stride, d_qw.ptr if d_qw else None,
                                  d_kw.ptr if d_kw else None, base_pos, n_cols))
@@ -267,6 +307,14 @@ class PooledAttn:
         qp = d_q if isinstance(d_q, (int, type(None))) else d_q.ptr
         gp = d_gate if isinstance(d_gate, (int, type(None))) else d_gate.ptr
         self._chk(fn(self.ctx, layer, qp, q_stride, gp, gate_stride, base_pos, n_cols, d_out.ptr, out_stride, out_dtype))
+
+    def attn_tree(self, layer, d_q, q_stride, d_gate, gate_stride, d_mask, mask_stride, base_pos, n_cols, d_out, out_stride, out_dtype=PA_OUT_F32):
+        qp = d_q if isinstance(d_q, (int, type(None))) else d_q.ptr
+        gp = d_gate if isinstance(d_gate, (int, type(None))) else d_gate.ptr
+        self._chk(self.L.pa_attn_tree(self.ctx, layer, qp, q_stride, gp, gate_stride, d_mask.ptr, mask_stride, base_pos, n_cols, d_out.ptr, out_stride, out_dtype))
+
+    def kv_compact(self, dst_row, d_sel, max_rows):
+        self._chk(self.L.pa_kv_compact(self.ctx, dst_row, d_sel.ptr, max_rows))
 
     def attn_decode_step(self, layer, d_q_in, d_k, d_v, d_qw, d_kw, pos, d_out, out_dtype=PA_OUT_F32, noalloc=False):
         fn = self.L.pa_attn_decode_step_noalloc if noalloc else self.L.pa_attn_decode_step
@@ -534,6 +582,30 @@ class PooledAttn:
             if b is not None:
                 b.free(); self._bufs.remove(b)
         return out.reshape(n, self.cfg["n_heads"], self.cfg["head_dim"])
+
+    def run_attn_tree(self, layer, q, mask, base_pos, gate=None, out_dtype=PA_OUT_F32):
+        """q [n, nH, hd]; mask bool [n, n] (column c sees row base_pos + j) or its words, uint32 [n, stride] -> out [n, nH, hd]."""
+        n = q.shape[0]
+        words = tree_mask(mask) if mask.dtype == np.bool_ else np.ascontiguousarray(mask, dtype=np.uint32)
+        dq = self.to_device(q.reshape(n, -1).astype(np.float32))
+        dg = self.to_device(gate.reshape(n, -1).astype(np.float32)) if gate is not None else None
+        dm = self.to_device(words)
+        dout = self.alloc(n * self.q_dim * (4 if out_dtype == PA_OUT_F32 else 2))
+        self.attn_tree(layer, dq, self.q_dim, dg, self.q_dim if dg else 0, dm, words.shape[1], base_pos, n, dout, self.q_dim, out_dtype)
+        self.sync()
+        out = dout.download(np.float32 if out_dtype == PA_OUT_F32 else np.float16, n * self.q_dim)
+        for b in (dq, dg, dm, dout):
+            if b is not None:
+                b.free(); self._bufs.remove(b)
+        return out.reshape(n, self.cfg["n_heads"], self.cfg["head_dim"])
+
+    def run_kv_compact(self, dst_row, rows, max_rows=None):
+        """Rows dst_row + i of every cache become the rows of the list, which ascends from dst_row on."""
+        rows = np.asarray(rows, np.uint32)
+        sel = self.to_device(np.concatenate([np.array([rows.size], np.uint32), rows]))
+        self.kv_compact(dst_row, sel, max_rows or max(rows.size, 1))
+        self.sync()
+        sel.free(); self._bufs.remove(sel)
 
     def run_attn(self, kind, layer, q, base_pos, gate=None, out_dtype=PA_OUT_F32):
         """q [n, nH, hd] f32 (None: the context's q buffer, n from gate or 1) -> out [n, nH, hd]."""

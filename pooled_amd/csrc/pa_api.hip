@@ -706,6 +706,17 @@ static int prof_aux_pair(pa_ctx* ctx, const PaTiming& main, PaTiming* t) {
   return PA_OK;
 }
 
+int pa_ctx_grow(pa_ctx* ctx, void** buf, size_t* have, size_t need) {
+  try { return grow_scratch(ctx, buf, have, need); } catch (const std::bad_alloc&) { return PA_ERR_NOMEM; }
+}
+int pa_ctx_timing(pa_ctx* ctx, PaTiming* main, PaTiming* merge, bool has_merge) {
+  *merge = PaTiming();
+  try {
+    const int rc = prof_pair(ctx, main);
+    return rc || !has_merge ? rc : prof_aux_pair(ctx, *main, merge);
+  } catch (const std::bad_alloc&) { return PA_ERR_NOMEM; }
+}
+
 // Where a kv head's one workgroup writes the output itself (plan_one_wg), other kv heads' workgroups may still be reading: an output that shares
 // memory with what the call reads (f16 results into the q buffer, results into the step's k or v) goes through the scratch of the split partials,
 // which that plan does not use, and is copied behind the kernel.

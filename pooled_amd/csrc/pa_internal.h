@@ -228,6 +228,8 @@ struct pa_ctx {
   std::vector<void*> retired;   // outgrown scratch blocks, kept until pa_destroy (a recorded launch may still name them)
   uint32_t decode_splits_override = 0;
   int prefill_tile_mode = 0;    // pa_set_prefill_tile: 0 table, 1 always the matrix-core kernel, 2 never
+  uint32_t rope_axes = 1;       // pa_set_rope_axes: axes of pa_glue_kv_at's positions ...
+  uint32_t axis_of_pair[8] = {};   // ... and the axis of every rotated pair, two bits each
   // timing
   hipEvent_t t0 = nullptr, t1 = nullptr;
   bool profiling = false;
@@ -237,3 +239,7 @@ struct pa_ctx {
   size_t prof_aux_used = 0;
   std::string err;
 };
+
+// ---- the context's scratch and event pairs, for host files other than pa_api.hip ----
+int pa_ctx_grow(pa_ctx* ctx, void** buf, size_t* have, size_t need);                       // scratch of at least `need` bytes; what it replaces is kept (recorded launches name it)
+int pa_ctx_timing(pa_ctx* ctx, PaTiming* main, PaTiming* merge, bool has_merge);           // the event pairs of a profiled call's kernels; empty without profiling

@@ -1,0 +1,52 @@
+// Declarations shared by the host side of the drafted-tree calls (pa_tree.hip) and their gfx950 kernels.
+#pragma once
+#include "pa_internal.h"
+
+// ---- attention of a tree of drafted tokens (attn_tree.hip) ----
+struct TreeParams {
+  const float* q; const float* gate;            // f32 [n_cols][stride], heads of head_dim
+  const void* k_cache; const void* v_cache;     // f16 or int8, [nKV][max_seq + 32][hd]
+  const float* k_scale; const float* v_scale;   // int8 caches: one f32 scale per 32 values
+  const uint32_t* mask;                         // [n_cols][mask_stride]: bit j: the column sees row base_pos + j
+  uint16_t* part_o; float2* part_ml;            // per (column, head, split): O / l as f16 [hd], and (m, l)
+  void* out;                                    // [n_cols][out_stride]
+  uint32_t q_stride, gate_stride, mask_stride, out_stride;
+  uint32_t n_heads, n_kv_heads, group;          // group = nH / nKV
+  uint32_t base_pos, n_cols, max_seq;
+  uint32_t n_splits, split_tiles;               // splits of the context, 32-row tiles of each
+  uint32_t n_groups, group_rows;                // groups of stacked rows of a kv head (row = column x G + head), rows of each
+  int out_f16;
+  float scale;                                  // 1 / sqrt(hd)
+};
+// what a call runs as: rows a wave holds (16 nb), waves of a workgroup, groups of rows, splits
+struct TreePlan { uint32_t nb, waves, n_groups, group_rows, n_splits, split_tiles; };
+hipError_t pa_launch_tree(const TreeParams& p, const TreePlan& pl, uint32_t hd, hipStream_t s, const PaTiming* t);
+hipError_t pa_launch_tree_merge(const TreeParams& p, uint32_t hd, hipStream_t s, const PaTiming* t);
+
+// ---- pre-step with positions of each column's own (glue_at.hip) ----
+struct GlueAtParams {
+  const float* q_in; const float* k_in; const float* v_in;
+  const float* qw; const float* kw;             // norm weights [hd]
+  const float* inv_freq; const float2* rope_tab;  // [n_rot / 2]; [tab_rows][n_rot / 2] (cos, sin) or nullptr
+  const uint32_t* pos;                          // [axes][pos_stride]
+  float* q_out; float* gate_out;                // [n_cols][nH * hd]
+  void* k_cache; void* v_cache;                 // f16 or int8 [nKV][head_rows][hd]
+  float* ks_cache; float* vs_cache;
+  uint32_t head_rows, tab_rows;
+  uint32_t q_stride, k_stride, v_stride, pos_stride;
+  uint32_t n_heads, n_kv_heads, head_dim, n_rot;
+  uint32_t base_row, n_cols, flags;
+  float eps;
+  uint32_t axis_of_pair[8];                     // two bits a pair, sixteen pairs a word
+};
+hipError_t pa_launch_glue_at(const GlueAtParams& p, hipStream_t s);
+
+// ---- compaction of the caches to a list of rows (kv_compact.hip) ----
+#define PA_COMPACT_TENSORS 128u
+struct CompactParams {
+  void* t[PA_COMPACT_TENSORS];                  // [planes][head_rows][row_bytes of the tensor]; even and odd tensors are K and V, or their scales
+  const uint32_t* sel;                          // n, then n rows, ascending
+  uint32_t n_tensors, n_planes, head_rows, row_bytes;
+  uint32_t dst_row, max_rows, max_seq;
+};
+hipError_t pa_launch_compact(const CompactParams& p, hipStream_t s);
