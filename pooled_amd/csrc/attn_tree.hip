@@ -33,23 +33,72 @@ template <int HD, int W> struct TreeShape {
   static_assert(NP8 * W * 64 == 2 * PIECES && PIECES % 64 == 0, "an int8 tile divides evenly over the threads, a wave's pieces are of one tensor");
 };
 
-static __device__ inline bool not_finite(_Float16 v) {
-  unsigned short b;
-  __builtin_memcpy(&b, &v, 2);
-  return (b & 0x7C00u) == 0x7C00u;
+static __device__ inline bool not_finite2(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }   // any of two f16
+
+// What the drafted rows that column `col` sees hold that is not finite, added to eight dims of its output: rows of v head g, dims d ..
+static __device__ inline void add_not_finite(const TreeParams& p, uint32_t hd, uint32_t col, uint32_t g, uint32_t d, float (&o)[8]) {
+  const uint32_t* words = p.mask + (size_t)col * p.mask_stride;
+#pragma unroll 1
+  for (uint32_t j = 0; j < p.n_cols; j++) {
+    if (!(words[j / 32] >> (j % 32) & 1)) continue;
+    const size_t row = (size_t)g * ((size_t)p.max_seq + 32) + p.base_pos + j;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      const float v = p.v_scale ? (float)((const signed char*)p.v_cache)[row * hd + d + e] * p.v_scale[row * (hd / 32) + d / 32] : (float)((const _Float16*)p.v_cache)[row * hd + d + e];
+      o[e] += __builtin_fabsf(v) < 65520.f ? 0.f : __builtin_fabsf(v) < __builtin_inff() ? __builtin_copysignf(__builtin_inff(), v) : v;     // (int8 values that f16 does not hold)
+    }
+  }
 }
 
 template <int N> static __device__ inline void wait_and_meet() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory"); }
 
-template <int HD, int NB, int W, bool Q8, int D>
-__global__ __launch_bounds__(W * 64, W / 4) void pa_tree_kernel(TreeParams p) {
+// orders a wave's LDS accesses for the compiler (the hardware executes them in order)
+static __device__ inline void wave_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+static __device__ inline void wait_and_meet_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+#define TREE_W 8              // waves of a workgroup, two a SIMD: one wave a SIMD gets half of what the LDS delivers
+
+// LDS behind the ring: mask words of WIN tiles, and a flag of each wave
+template <int NB> struct TreeLds { static constexpr int WIN = 4 / NB, bytes = WIN * 16 * NB * TREE_W * 4 + TREE_W * 4; };
+
+// eight dims of an output column; with the gate
+static __device__ inline void store8(const TreeParams& p, uint32_t col, uint32_t d, const float (&o)[8]) {
+  if (p.out_f16) {
+    _Float16* out = (_Float16*)p.out + (size_t)col * p.out_stride + d;
+    *(h4*)out = (h4){ (_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3] };        // (columns of f16 are 8 bytes aligned)
+    *(h4*)(out + 4) = (h4){ (_Float16)o[4], (_Float16)o[5], (_Float16)o[6], (_Float16)o[7] };
+  } else {
+    float* out = (float*)p.out + (size_t)col * p.out_stride + d;
+    *(f4*)out = (f4){ o[0], o[1], o[2], o[3] };
+    *(f4*)(out + 4) = (f4){ o[4], o[5], o[6], o[7] };
+  }
+}
+static __device__ inline void store_row8(const TreeParams& p, uint32_t col, uint32_t d, float (&o)[8]) {
+  if (p.gate) {
+    const float* gate = p.gate + (size_t)col * p.gate_stride + d;
+    const f4 a = *(const f4*)gate, b = *(const f4*)(gate + 4);
+#pragma unroll
+    for (int i = 0; i < 4; i++) { o[i] *= 1.f / (1.f + __expf(-a[i])); o[4 + i] *= 1.f / (1.f + __expf(-b[i])); }
+  }
+  store8(p, col, d, o);
+}
+template <int HD, int NB, bool Q8, int D>
+__global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreeParams p) {
+  constexpr int W = TREE_W, ROWS = 16 * NB * W;
   typedef TreeShape<HD, W> S;
-  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];     // [D][K tile | V tile]
+  extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];     // [D][K tile | V tile], mask words [WIN][ROWS], a flag of each wave
+  constexpr int RING = D * 2 * S::TILE, WIN = TreeLds<NB>::WIN;
+  uint32_t* win_lds = (uint32_t*)(smem + RING);
+  uint32_t* bad_lds = win_lds + WIN * ROWS;
   // work items are (kv head, split, group of rows), the group fastest; dispatch id i runs on XCD i % 8, which owns a contiguous range of items, so the groups that
   // read the same rows share an L2
   const uint32_t total = p.n_groups * p.n_kv_heads * p.n_splits, per = (total + 7) / 8;
   const uint32_t item = (blockIdx.x % 8) * per + blockIdx.x / 8;
-  if (blockIdx.x / 8 >= per || item >= total) return;
+  if (item >= total) return;
   const uint32_t grp = item % p.n_groups, gs = item / p.n_groups, sp = gs % p.n_splits, g = gs / p.n_splits;
   const uint32_t tid = threadIdx.x, lane = tid & 63, ln = lane & 15, kg = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -57,24 +106,37 @@ __global__ __launch_bounds__(W * 64, W / 4) void pa_tree_kernel(TreeParams p) {
   const uint32_t x0 = grp * p.group_rows, R = min(p.group_rows, p.n_cols * G - x0);     // the group's stacked rows [x0, x0 + R)
   const uint32_t end = p.base_pos + p.n_cols;
   const uint32_t tile0 = sp * p.split_tiles, n_tiles = min(p.split_tiles, (end + 31) / 32 - tile0);
+  const uint32_t draft0 = max(p.base_pos / 32, tile0) - tile0;              // the split's first tile that reaches the drafted rows, if it is below n_tiles
   const size_t head_rows = (size_t)p.max_seq + 32;
 
-  // ---- staging ----
+  // ---- staging: tile i goes to buffer i % D ----
   auto k_slot = [](uint32_t row, uint32_t chunk) __attribute__((always_inline)) { return chunk ^ (row & 15); };      // conflict-free 16-byte fragment reads
   auto v_slot = [](uint32_t row, uint32_t chunk) __attribute__((always_inline)) { return chunk ^ (4 * (row & 3)) ^ (2 * ((row >> 2) & 1)); };   // 2-way for the transpose reads, their best
-  auto kbuf = [&](uint32_t i) __attribute__((always_inline)) { return smem + (i % D) * 2 * S::TILE; };
+  auto buf = [&](uint32_t i) __attribute__((always_inline)) { return smem + (i % D) * 2 * S::TILE; };
   // f16 rows: load j of wave w fills the 1 KB block j W + w of a buffer, rows (j W + w) RPB ..; lane l lands at (row l / CPR, slot l % CPR) and fetches the chunk that belongs there
+  const unsigned char* kb0 = (const unsigned char*)p.k_cache + (size_t)g * head_rows * S::ROWB;
+  const unsigned char* vb0 = (const unsigned char*)p.v_cache + (size_t)g * head_rows * S::ROWB;
+  constexpr bool ONE_OFF = S::RPB * W % 16 == 0;     // the swizzle, and with it a lane's offset in a load's rows, is the same for all of a wave's loads
+  static_assert(ONE_OFF, "rows of two loads of a wave are a multiple of 16 apart");
+  const uint32_t ld_row = wave * S::RPB + lane / S::CPR, ld_c = lane % S::CPR;
+  const uint32_t k_off = ld_row * S::ROWB + k_slot(ld_row, ld_c) * 16, v_off = ld_row * S::ROWB + v_slot(ld_row, ld_c) * 16;
   auto issue = [&](uint32_t i) __attribute__((always_inline)) {
     const uint32_t tp = (tile0 + i) * 32;
-    const unsigned char* kb = (const unsigned char*)p.k_cache + (size_t)g * head_rows * S::ROWB;
-    const unsigned char* vb = (const unsigned char*)p.v_cache + (size_t)g * head_rows * S::ROWB;
-    unsigned char* dst = kbuf(i);
+    unsigned char* dst = buf(i);
+    if (tp + 32 <= end) {
+      const unsigned char *kt = kb0 + (size_t)tp * S::ROWB, *vt = vb0 + (size_t)tp * S::ROWB;
 #pragma unroll
-    for (int j = 0; j < S::NLD; j++) {
-      const uint32_t r = (j * W + wave) * S::RPB + lane / S::CPR, c = lane % S::CPR;
-      const uint32_t row = tp + r < end ? tp + r : p.max_seq;                // (rows behind the last one: the cache's zero padding)
-      PF_GLL(kb + (size_t)row * S::ROWB + k_slot(r, c) * 16, dst + (j * W + wave) * 1024);
-      PF_GLL(vb + (size_t)row * S::ROWB + v_slot(r, c) * 16, dst + S::TILE + (j * W + wave) * 1024);
+      for (int j = 0; j < S::NLD; j++) PF_GLL_S(kt + j * W * S::RPB * S::ROWB, k_off, dst + (j * W + wave) * 1024);
+#pragma unroll
+      for (int j = 0; j < S::NLD; j++) PF_GLL_S(vt + j * W * S::RPB * S::ROWB, v_off, dst + S::TILE + (j * W + wave) * 1024);
+    } else {                                        // rows behind the last one: the cache's zero padding
+#pragma unroll 1
+      for (int j = 0; j < S::NLD; j++) {
+        const uint32_t r = j * W * S::RPB + ld_row;
+        const size_t row = tp + r < end ? tp + r : p.max_seq;
+        PF_GLL(kb0 + row * S::ROWB + k_slot(r, ld_c) * 16, dst + (j * W + wave) * 1024);
+        PF_GLL(vb0 + row * S::ROWB + v_slot(r, ld_c) * 16, dst + S::TILE + (j * W + wave) * 1024);
+      }
     }
   };
   // int8 rows: a thread's 16-byte pieces of a tile, K's and then V's, and their scales; two tiles in registers
@@ -92,8 +154,9 @@ __global__ __launch_bounds__(W * 64, W / 4) void pa_tree_kernel(TreeParams p) {
     }
   };
   auto widen = [&](u4 raw, float sc, unsigned char* row, uint32_t s0, uint32_t s1) __attribute__((always_inline)) {
-    // int8 -> f16 through the bit pattern 0x6400 | (v + 128) = 1152 + v, exactly, then times the f16-rounded scale
-    const h2 s2 = { (_Float16)sc, (_Float16)sc }, off = { (_Float16)1152.f, (_Float16)1152.f };
+    // int8 -> f16 through the bit pattern 0x6400 | (v + 128) = 1152 + v, exactly, then times the scale, which is given as the f16 nearest to it and the rest: rounded once
+    const _Float16 hi = (_Float16)sc, lo = (_Float16)(sc - (float)hi);
+    const h2 sh = { hi, hi }, sl = { lo, lo }, off = { (_Float16)1152.f, (_Float16)1152.f };
     h2 o[8];
 #pragma unroll
     for (int d = 0; d < 4; d++) {
@@ -102,15 +165,17 @@ __global__ __launch_bounds__(W * 64, W / 4) void pa_tree_kernel(TreeParams p) {
       h2 xa, xb;
       __builtin_memcpy(&xa, &a, 4);
       __builtin_memcpy(&xb, &b, 4);
-      o[2 * d] = (xa - off) * s2;
-      o[2 * d + 1] = (xb - off) * s2;
+      xa -= off;
+      xb -= off;
+      o[2 * d] = __builtin_elementwise_fma(xa, sh, xa * sl);
+      o[2 * d + 1] = __builtin_elementwise_fma(xb, sh, xb * sl);
     }
     *(h8*)(row + s0 * 16) = (h8){ o[0][0], o[0][1], o[1][0], o[1][1], o[2][0], o[2][1], o[3][0], o[3][1] };
     *(h8*)(row + s1 * 16) = (h8){ o[4][0], o[4][1], o[5][0], o[5][1], o[6][0], o[6][1], o[7][0], o[7][1] };
   };
   auto stage8 = [&](uint32_t i, auto AT) __attribute__((always_inline)) {
     constexpr int at = decltype(AT)::value;
-    unsigned char* dst = kbuf(i);
+    unsigned char* dst = buf(i);
 #pragma unroll
     for (int j = 0; j < S::NP8; j++) {
       const uint32_t e = tid + j * W * 64, of_v = (wave * 64 + j * W * 64) / S::PIECES, r = e % S::PIECES / (HD / 16), c = e % (HD / 16) * 2;
@@ -119,75 +184,133 @@ __global__ __launch_bounds__(W * 64, W / 4) void pa_tree_kernel(TreeParams p) {
   };
   typedef std::integral_constant<int, 0> I0;
   typedef std::integral_constant<int, 1> I1;
+  // the rows' words of the mask at WIN tiles from the split's draft tile d on
+  auto fill_windows = [&](uint32_t d) __attribute__((always_inline)) {
+#pragma unroll 1
+    for (uint32_t e = tid; e < WIN * ROWS; e += W * 64) {
+      const uint32_t r = e % ROWS, i = draft0 + d + e / ROWS, x = x0 + min(r, R - 1);
+      if (i < n_tiles) win_lds[e] = mask_window(p.mask + (size_t)(x / G) * p.mask_stride, (int)((tile0 + i) * 32 - p.base_pos), p.n_cols);
+    }
+  };
+
+  // ---- start: the first tile goes out, then what the wave's rows need; the other tiles behind them, since loads return in order ----
+  // (block nb of a wave is rows 16 (nb W + wave) ..: the blocks of a group spread over the SIMDs evenly)
+  auto row_of = [&](uint32_t nb, uint32_t r) __attribute__((always_inline)) -> uint32_t { return (nb * W + wave) * 16 + r; };
+  const uint32_t blocks = R > wave * 16 ? (R - wave * 16 + W * 16 - 1) / (W * 16) : 0;      // the wave's live blocks
+  if constexpr (Q8) fetch8(0, I0{}); else issue(0);
+  // ---- what follows is one program for the waves of two live blocks, of one, and of none, which pass the same barriers ----
+  auto run = [&](auto BLOCKS) __attribute__((always_inline)) {
+  constexpr int LIVE = decltype(BLOCKS)::value, NL = LIVE ? LIVE : 1, KD = NL == 1 ? 4 : 3, VD = NL == 1 ? 4 : 3;      // K and V^T fragments (NL products each) fetched ahead
+  // Q: whole rows as they lie in memory, through a wave-private part of the ring's last buffer (taken by a tile only behind the first barrier), eight rows at a time, to the fragments: row ln of block nb, dims 32 ks + 8 kg .. + 7
+  h8 qf[NL][S::KS];
+  if constexpr (LIVE == 0) { if (draft0 < n_tiles) fill_windows(0); } else {
+    constexpr int LPQ = HD / 4, RPL = 64 / LPQ, QL = 8 / RPL;               // lanes of a row, rows of a load, loads of eight rows
+    unsigned char* qs = smem + (D - 1) * 2 * S::TILE + wave * 8 * S::ROWB;
+    static_assert(8 * W * S::ROWB <= 2 * S::TILE, "eight rows of each wave fit a buffer");
+    f4 qv[2 * NL][QL];
+#pragma unroll
+    for (int b = 0; b < 2 * NL; b++)
+#pragma unroll
+      for (int j = 0; j < QL; j++) {
+        const uint32_t x = x0 + min(row_of(b / 2, b % 2 * 8 + j * RPL + lane / LPQ), R - 1), col = x / G;
+        qv[b][j] = *(const f4*)(p.q + (size_t)col * p.q_stride + (size_t)(g * G + x - col * G) * HD + lane % LPQ * 4);
+      }
+    if (draft0 < n_tiles) fill_windows(0);
+#pragma unroll
+    for (int b = 0; b < 2 * NL; b++) {
+#pragma unroll
+      for (int j = 0; j < QL; j++) {
+        const uint32_t r = j * RPL + lane / LPQ, c = lane % LPQ;
+        *(h4*)(qs + r * S::ROWB + ((c / 2) ^ r) * 16 + c % 2 * 8) = (h4){ (_Float16)qv[b][j][0], (_Float16)qv[b][j][1], (_Float16)qv[b][j][2], (_Float16)qv[b][j][3] };
+      }
+      wave_fence();
+#pragma unroll
+      for (int ks = 0; ks < S::KS; ks++) {
+        const h8 f = *(const h8*)(qs + (ln & 7) * S::ROWB + ((ks * 4 + kg) ^ (ln & 7)) * 16);
+        if (b % 2 == 0) qf[b / 2][ks] = f;
+        else qf[b / 2][ks] = ln < 8 ? qf[b / 2][ks] : f;
+      }
+      wave_fence();
+    }
+  }
   if constexpr (Q8) {
-    fetch8(0, I0{});
     if (n_tiles > 1) fetch8(1, I1{});
   } else {
 #pragma unroll
-    for (int i = 0; i < D - 1; i++) if ((uint32_t)i < n_tiles) issue(i);
+    for (int i = 1; i < D - 1; i++) if ((uint32_t)i < n_tiles) issue(i);
   }
-
-  // ---- the wave's rows: Q fragments (row ln of block nb, dims 32 ks + 8 kg .. + 7) ----
-  const uint32_t wrow0 = wave * 16 * NB;
-  const bool live = wrow0 < R;
-  h8 qf[NB][S::KS];
+  f4 acc[S::DB][NL];
+  float m_ref[NL], l_run[NL];
 #pragma unroll
-  for (int nb = 0; nb < NB; nb++) {
-    const uint32_t x = x0 + min(wrow0 + nb * 16 + ln, R - 1), col = x / G;
-    const float* qrow = p.q + (size_t)col * p.q_stride + (size_t)(g * G + x - col * G) * HD + 8 * kg;
-#pragma unroll
-    for (int ks = 0; ks < S::KS; ks++) {
-      const f4 a = *(const f4*)(qrow + 32 * ks), b = *(const f4*)(qrow + 32 * ks + 4);
-      qf[nb][ks] = (h8){ (_Float16)a[0], (_Float16)a[1], (_Float16)a[2], (_Float16)a[3], (_Float16)b[0], (_Float16)b[1], (_Float16)b[2], (_Float16)b[3] };
-    }
-  }
-  f4 acc[S::DB][NB];
-  float m_ref[NB], l_run[NB];
-#pragma unroll
-  for (int nb = 0; nb < NB; nb++) {
+  for (int nb = 0; nb < NL; nb++) {
 #pragma unroll
     for (int db = 0; db < S::DB; db++) acc[db][nb] = (f4){0.f, 0.f, 0.f, 0.f};
     m_ref[nb] = NEG_INF;
     l_run[nb] = 0.f;
   }
   bool unseen = true;                               // a row of the wave has no reference yet
+  bool bad = false;                                 // a drafted row holds what is not finite
   const float c1 = p.scale * 1.4426950408889634f;   // scores -> log2 domain
   const uint32_t k_rd = ln * S::ROWB + (kg ^ ln) * 16;                                                                        // K fragment of k-step ks at k_rd ^ 64 ks
   const uint32_t v_rd = (4 * kg + (ln >> 2)) * S::ROWB + (((ln & 3) >> 1) ^ (4 * (ln >> 2)) ^ (2 * (kg & 1))) * 16 + (ln & 1) * 8;   // V fragment of block db at v_rd ^ 32 db
 
-  auto tile = [&](const unsigned char* kb, const uint32_t tp) __attribute__((always_inline)) {
-    const unsigned char* vb = kb + S::TILE;
-    f4 s[2][NB];
-    h8 pf[NB];
-    uint32_t win[NB];
+  f4 s[2][NL];                                      // a tile's scores: a lane holds row ln of each block, positions tp + 16 pb + 4 kg + i
+  h8 pf[NL];
+  // one tile: scores, softmax, product
+  auto turn = [&](uint32_t i) __attribute__((always_inline)) {
+    constexpr int NF = 2 * S::KS;
+    const unsigned char *kb = buf(i), *vb = kb + S::TILE;
+    // ---- S^T = K Q^T ----
+    {
+      h8 ka[KD];
+      auto at = [&](int f) __attribute__((always_inline)) { return kb + (k_rd ^ (f / 2 % 4 * 64)) + f / 8 * 256 + f % 2 * 16 * S::ROWB; };
 #pragma unroll
-    for (int pb = 0; pb < 2; pb++)
+      for (int f = 0; f < KD; f++) ka[f] = *(const h8*)at(f);
 #pragma unroll
-      for (int nb = 0; nb < NB; nb++) s[pb][nb] = (f4){0.f, 0.f, 0.f, 0.f};
-    // ---- S^T = K Q^T; a lane then holds row ln of each block, positions tp + 16 pb + 4 kg + i ----
+      for (int pb = 0; pb < 2; pb++)
 #pragma unroll
-    for (int f = 0; f < 2 * S::KS; f++) {
-      const h8 a = *(const h8*)(kb + (k_rd ^ (f / 2 % 4 * 64)) + f / 8 * 256 + f % 2 * 16 * S::ROWB);
+        for (int nb = 0; nb < NL; nb++) s[pb][nb] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int nb = 0; nb < NB; nb++) s[f % 2][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[nb][f / 2], s[f % 2][nb], 0, 0, 0);
+      for (int f = 0; f < NF; f++) {
+        const h8 a = ka[f % KD];
+        if (f + KD < NF) ka[f % KD] = *(const h8*)at(f + KD);
+#pragma unroll
+        for (int nb = 0; nb < NL; nb++) s[f % 2][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[nb][f / 2], s[f % 2][nb], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, KD, 0);
+#pragma unroll
+      for (int f = 0; f < NF; f++) {
+        __builtin_amdgcn_sched_group_barrier(0x008, NL, 0);
+        if (f + KD < NF) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
     }
-    const bool draft = tp + 32 > p.base_pos;        // the tile reaches the drafted rows
-    if (draft) {
+    // (the first fragments of V^T, with one block on their way during the softmax: with two the registers are full)
+    h4 lo[VD], hi[VD];
+    auto fetch = [&](int f) __attribute__((always_inline)) {
+      const unsigned char* vp = vb + (v_rd ^ (f % 8 * 32)) + f / 8 * 256;
+      lo[f % VD] = lds_read_tr16(vp);
+      hi[f % VD] = lds_read_tr16(vp + 16 * S::ROWB);
+    };
+    if constexpr (NL == 1) {
 #pragma unroll
-      for (int nb = 0; nb < NB; nb++) {
-        const uint32_t x = x0 + min(wrow0 + nb * 16 + ln, R - 1);
-        win[nb] = mask_window(p.mask + (size_t)(x / G) * p.mask_stride, (int)(tp - p.base_pos), p.n_cols);
+      for (int f = 0; f < VD; f++) fetch(f);
+    }
+    if (__builtin_expect(i >= draft0, 0)) {
+#pragma unroll
+      for (int nb = 0; nb < NL; nb++) {
+        const uint32_t win = win_lds[(i - draft0) % WIN * ROWS + row_of(nb, ln)] >> (4 * kg);
 #pragma unroll
         for (int pb = 0; pb < 2; pb++)
 #pragma unroll
-          for (int i = 0; i < 4; i++) s[pb][nb][i] = win[nb] >> (16 * pb + 4 * kg + i) & 1 ? s[pb][nb][i] : NEG_INF;
+          for (int e = 0; e < 4; e++) s[pb][nb][e] = win >> (16 * pb + e) & 1 ? s[pb][nb][e] : NEG_INF;
       }
     }
     // ---- softmax ----
+    // the references of the rows raised to the tile's maxima, O and l rescaled
     auto raise = [&]() __attribute__((always_inline)) {
       bool none = false;
 #pragma unroll
-      for (int nb = 0; nb < NB; nb++) {
+      for (int nb = 0; nb < NL; nb++) {
         float mx = s[0][nb][0];
 #pragma unroll
         for (int j = 1; j < 8; j++) mx = fmaxf(mx, s[j / 4][nb][j % 4]);
@@ -204,10 +327,11 @@ __global__ __launch_bounds__(W * 64, W / 4) void pa_tree_kernel(TreeParams p) {
       }
       unseen = __any(none);
     };
+    // P of the tile against the references; whether one passes them by more than f16 should hold
     auto probs = [&]() __attribute__((always_inline)) -> bool {
       h2 top = { (_Float16)0.f, (_Float16)0.f };
 #pragma unroll
-      for (int nb = 0; nb < NB; nb++) {
+      for (int nb = 0; nb < NL; nb++) {
         const float nmr = m_ref[nb] == NEG_INF ? 0.f : -m_ref[nb];
 #pragma unroll
         for (int j = 0; j < 8; j += 2) {
@@ -224,190 +348,249 @@ __global__ __launch_bounds__(W * 64, W / 4) void pa_tree_kernel(TreeParams p) {
     };
     if (__builtin_expect(unseen, 0)) raise();
     if (__builtin_expect(probs(), 0)) { raise(); probs(); }
+    // ---- O^T += V^T P^T, contraction slot 8 kg + j: position 4 kg + j, or 16 + 4 kg + j - 4; and l += the P that it uses ----
     const h2 ones = { (_Float16)1.f, (_Float16)1.f };
 #pragma unroll
-    for (int nb = 0; nb < NB; nb++)
+    for (int nb = 0; nb < NL; nb++)
 #pragma unroll
       for (int j = 0; j < 8; j += 2) { const h2 pp = { pf[nb][j], pf[nb][j + 1] }; l_run[nb] = __builtin_amdgcn_fdot2(pp, ones, l_run[nb], false); }
-    // ---- O^T += V^T P^T, contraction slot 8 kg + j: position 4 kg + j, or 16 + 4 kg + j - 4 ----
-    auto pv = [&](auto CLEAN) __attribute__((always_inline)) -> bool {
-      bool bad = false;
+    if constexpr (NL > 1) {
 #pragma unroll
-      for (int f = 0; f < S::DB; f++) {
-        const unsigned char* vp = vb + (v_rd ^ (f % 8 * 32)) + f / 8 * 256;
-        const h4 lo = lds_read_tr16(vp), hi = lds_read_tr16(vp + 16 * S::ROWB);
-        h8 a = { lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3] };
-        if constexpr (decltype(CLEAN)::value) {
+      for (int f = 0; f < VD; f++) fetch(f);
+    }
 #pragma unroll
-          for (int j = 0; j < 8; j++) if (not_finite(a[j])) { a[j] = (_Float16)0.f; bad = true; }
-        }
+    for (int f = 0; f < S::DB; f++) {
+      const h4 l = lo[f % VD], h = hi[f % VD];
+      const h8 a = { l[0], l[1], l[2], l[3], h[0], h[1], h[2], h[3] };
+      if (f + VD < S::DB) fetch(f + VD);
 #pragma unroll
-        for (int nb = 0; nb < NB; nb++) acc[f][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pf[nb], acc[f][nb], 0, 0, 0);
-      }
-      return bad;
-    };
-    if (!draft) pv(std::false_type{});
-    else if (__any(pv(std::true_type{}))) {
-      // what is not finite, element by element: to the rows that see it
-      for (uint32_t r = 0; r < 32; r++)
+      for (int nb = 0; nb < NL; nb++) acc[f][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, pf[nb], acc[f][nb], 0, 0, 0);
+    }
+    if constexpr (NL > 1) __builtin_amdgcn_sched_group_barrier(0x100, 2 * VD, 1);
 #pragma unroll
-        for (int db = 0; db < S::DB; db++) {
-          const uint32_t d = 16 * db + 4 * kg;
-          const h4 v = *(const h4*)(vb + r * S::ROWB + v_slot(r, d / 8) * 16 + d % 8 * 2);
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            if (not_finite(v[i])) {
-#pragma unroll
-              for (int nb = 0; nb < NB; nb++) if (win[nb] >> r & 1) acc[db][nb][i] += (float)v[i];
-            }
-        }
+    for (int f = 0; f < S::DB; f++) {
+      __builtin_amdgcn_sched_group_barrier(0x008, NL, 1);
+      if (f + VD < S::DB) __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
     }
   };
+  // A tile that reaches the drafted rows: the next mask words where the ones at hand are through; and what is not finite in V becomes zero in LDS (see the head of the file)
+  auto draft_tile = [&](uint32_t i) __attribute__((always_inline)) {
+    const uint32_t d = i - draft0;
+    if (d && d % WIN == 0) { fill_windows(d); __syncthreads(); }
+    unsigned char* vb = buf(i) + S::TILE + (wave * 64 + lane) * 16;
+    constexpr int NV = S::TILE / (W * 1024);
+    bool any = false;
+    u4 v[NV];
+#pragma unroll
+    for (int j = 0; j < NV; j++) {
+      v[j] = *(const u4*)(vb + j * W * 1024);
+      any |= not_finite2(v[j][0]) || not_finite2(v[j][1]) || not_finite2(v[j][2]) || not_finite2(v[j][3]);
+    }
+    any = __any(any);
+    if (any) {
+#pragma unroll
+      for (int j = 0; j < NV; j++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[j][e] &= ((v[j][e] & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) | ((v[j][e] & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u);
+        *(u4*)(vb + j * W * 1024) = v[j];
+      }
+    }
+    if (lane == 0) bad_lds[wave] = any;
+    __syncthreads();
+    uint32_t all = 0;
+#pragma unroll
+    for (int w = 0; w < W; w++) all |= bad_lds[w];
+    bad |= all != 0;
+  };
 
-  // ---- main loop: tile i is there behind the barrier, and every wave has done tile i - 1, whose buffer takes the load that goes out next ----
+  // ---- main loop: behind turn i's barrier tile i is there for every wave, and every wave has done turn i - 1, so that tile i - 1's buffer takes what comes next ----
   if constexpr (Q8) {
-    static_assert(D == 2, "int8 rows: two buffers");
-    auto turn = [&](uint32_t i, auto AT, auto NEXT) __attribute__((always_inline)) {
-      // registers NEXT hold tile i + 1, registers AT are free
-      if (i + 2 < n_tiles) fetch8(i + 2, AT);
-      asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      if (live) tile(kbuf(i), (tile0 + i) * 32);
-      if (i + 1 < n_tiles) stage8(i + 1, NEXT);
-    };
+    static_assert(D == 2, "int8 rows: a turn's tile and the one that is staged meanwhile");
+    // when turn i begins, the registers of the other parity hold tile i + 1, those of its own tile i + 2
     stage8(0, I0{});
-    uint32_t i = 0;
-    for (; i + 1 < n_tiles; i += 2) { turn(i, I0{}, I1{}); turn(i + 1, I1{}, I0{}); }
-    if (i < n_tiles) turn(i, I0{}, I1{});
-  } else {
-    constexpr int AHEAD = 2 * S::NLD * (D - 2);     // a wave's loads behind tile i's
+    if (n_tiles > 2) fetch8(2, I0{});
     for (uint32_t i = 0; i < n_tiles; i++) {
-      if (i + D - 2 < n_tiles) wait_and_meet<AHEAD>(); else wait_and_meet<0>();
+      wait_and_meet_lds();
+      if (i + 1 < n_tiles) {
+        if (i & 1) { stage8(i + 1, I0{}); if (i + 3 < n_tiles) fetch8(i + 3, I0{}); }
+        else { stage8(i + 1, I1{}); if (i + 3 < n_tiles) fetch8(i + 3, I1{}); }
+      }
+      if (__builtin_expect(i >= draft0, 0)) draft_tile(i);
+      if constexpr (LIVE > 0) turn(i);
+    }
+  } else {
+    constexpr int LOADS = 2 * S::NLD;               // a wave's loads of a tile
+    for (uint32_t i = 0; i < n_tiles; i++) {
+      // tiles up to i + D - 2 were issued: tile i is there when D - 2 tiles' loads are left
+      if (i + D - 2 < n_tiles) wait_and_meet<LOADS * (D - 2)>(); else wait_and_meet<0>();
       if (i + D - 1 < n_tiles) issue(i + D - 1);
-      if (live) tile(kbuf(i), (tile0 + i) * 32);
+      if (__builtin_expect(i >= draft0, 0)) draft_tile(i);
+      if constexpr (LIVE > 0) turn(i);
     }
   }
-  if (!live) return;
 
-  // ---- the split's outputs ----
+  // ---- the split's outputs: through LDS, so that a row leaves in whole lines ----
+  wait_and_meet_lds();                              // every wave has read the last tile
+  if constexpr (LIVE > 0) {
+  constexpr int EROWS = RING / W / (HD * 4) < 16 ? 8 : 16, LPR = HD / 8, RPI = 64 / LPR;      // rows at a time; lanes of a row, rows of the wave at once
+  static_assert(EROWS * HD * 4 * W <= RING, "the rows fit the ring");
+  float* os = (float*)(smem + wave * EROWS * HD * 4);
 #pragma unroll
-  for (int nb = 0; nb < NB; nb++) {
+  for (int nb = 0; nb < NL; nb++) {
     l_run[nb] += __shfl_xor(l_run[nb], 16, 64);
     l_run[nb] += __shfl_xor(l_run[nb], 32, 64);
-    const uint32_t r = wrow0 + nb * 16 + ln;
-    if (r >= R) continue;
-    const uint32_t x = x0 + r, col = x / G, hq = g * G + x - col * G;
     const float inv = l_run[nb] == 0.f ? 0.f : 1.f / l_run[nb];             // a row that sees nothing: zeros
-    if (p.n_splits == 1) {
-      const float* gate = p.gate ? p.gate + (size_t)col * p.gate_stride + (size_t)hq * HD : nullptr;
+    if (p.n_splits > 1 && kg == 0 && row_of(nb, ln) < R) {
+      const uint32_t x = x0 + row_of(nb, ln), col = x / G;
+      // (the sign of l says that a drafted row of the split holds what is not finite; a row of NaN scores may have found no reference)
+      p.part_ml[((size_t)col * nH + g * G + x - col * G) * p.n_splits + sp] = make_float2(l_run[nb] != l_run[nb] ? __builtin_inff() : m_ref[nb], bad ? -l_run[nb] : l_run[nb]);
+    }
 #pragma unroll
-      for (int db = 0; db < S::DB; db++) {
-        const uint32_t d = 16 * db + 4 * kg;
-        f4 o = acc[db][nb] * inv;
-        if (gate) {
-          const f4 gt = *(const f4*)(gate + d);
+    for (int half = 0; half < 16 / EROWS; half++) {
+      if (EROWS == 16 || (int)(ln / 8) == half) {
+        const uint32_t r = ln % EROWS;
 #pragma unroll
-          for (int i = 0; i < 4; i++) o[i] *= 1.f / (1.f + __expf(-gt[i]));
+        for (int db = 0; db < S::DB; db++) *(f4*)(os + r * HD + ((4 * db + kg) ^ r) * 4) = acc[db][nb] * inv;
+      }
+      wave_fence();
+      // eight dims of row r
+      auto row8 = [&](uint32_t r, float (&o)[8]) __attribute__((always_inline)) {
+        const uint32_t c = lane % LPR * 2;
+        const f4 a = *(const f4*)(os + r * HD + (c ^ r) * 4), b = *(const f4*)(os + r * HD + ((c + 1) ^ r) * 4);
+#pragma unroll
+        for (int i = 0; i < 4; i++) { o[i] = a[i]; o[4 + i] = b[i]; }
+      };
+      const uint32_t r0 = row_of(nb, half * EROWS), d = lane % LPR * 8;
+      if (p.n_splits > 1) {
+#pragma unroll
+        for (int it = 0; it < EROWS / RPI; it++) {
+          const uint32_t r = it * RPI + lane / LPR;
+          float o[8];
+          row8(r, o);
+          if (r0 + r < R) {
+            const uint32_t x = x0 + r0 + r, col = x / G, hq = g * G + x - col * G;
+            const h8 v = { (_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3], (_Float16)o[4], (_Float16)o[5], (_Float16)o[6], (_Float16)o[7] };
+            __builtin_nontemporal_store(v, (h8*)((_Float16*)p.part_o + (((size_t)col * nH + hq) * p.n_splits + sp) * HD + d));
+          }
         }
-        if (p.out_f16) *(h4*)((_Float16*)p.out + (size_t)col * p.out_stride + (size_t)hq * HD + d) = (h4){ (_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3] };
-        else *(f4*)((float*)p.out + (size_t)col * p.out_stride + (size_t)hq * HD + d) = o;
+      } else {
+#pragma unroll 1
+        for (int it = 0; it < EROWS / RPI; it++) {
+          const uint32_t r = it * RPI + lane / LPR;
+          if (r0 + r >= R) continue;
+          float o[8];
+          row8(r, o);
+          const uint32_t x = x0 + r0 + r, col = x / G, hq = g * G + x - col * G;
+          if (__builtin_expect(bad, 0)) add_not_finite(p, HD, col, g, d, o);
+          store_row8(p, col, hq * HD + d, o);
+        }
       }
-    } else {
-      const size_t slot = ((size_t)col * nH + hq) * p.n_splits + sp;
-#pragma unroll
-      for (int db = 0; db < S::DB; db++) {
-        const f4 o = acc[db][nb] * inv;
-        *(h4*)((_Float16*)p.part_o + slot * HD + 16 * db + 4 * kg) = (h4){ (_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3] };
-      }
-      if (kg == 0) p.part_ml[slot] = make_float2(m_ref[nb], l_run[nb]);
+      wave_fence();
     }
   }
+  }
+  };
+  if (blocks == 1) run(std::integral_constant<int, 1>{});
+  else if (blocks == 0) run(std::integral_constant<int, 0>{});
+  else if constexpr (NB == 2) run(std::integral_constant<int, 2>{});
 }
 
-// Joins the splits of a (column, head): w_s = l_s 2^(m_s - M), out = sum w_s o_s / sum w_s, times sigmoid(gate).  A wavefront takes one (column, head): HD / 8 lanes of
-// eight dims, 512 / HD groups of lanes over the splits in turn.
-template <int HD>
+// Joins the splits of a (column, head): w_s = l_s 2^(m_s - M), out = sum w_s o_s / sum w_s, times sigmoid(gate).  A wavefront takes LPG x 8 dims of a (column, head): LPG lanes of eight
+// dims, 64 / LPG groups of lanes over the splits in turn, eight splits of a group in one round trip.
+template <int HD, int LPG>
 __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
-  constexpr uint32_t LPR = HD / 8, NG = 64 / LPR, B = 8;
-  const uint32_t lane = threadIdx.x & 63, l8 = lane % LPR, grp = lane / LPR;
-  const uint32_t x = blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr uint32_t NG = 64 / LPG, B = 8, SL = HD / 8 / LPG;
+  const uint32_t lane = threadIdx.x & 63, l8 = lane % LPG, grp = lane / LPG;
+  const uint32_t wv = blockIdx.x * 4 + (threadIdx.x >> 6), x = wv / SL;
   if (x >= p.n_cols * p.n_heads) return;
-  const uint32_t col = x / p.n_heads, h = x - col * p.n_heads, ns = p.n_splits;
+  const uint32_t col = x / p.n_heads, h = x - col * p.n_heads, ns = p.n_splits, d = (wv % SL * LPG + l8) * 8;
   const float2* ml = p.part_ml + (size_t)x * ns;
-  const h8* po = (const h8*)((const _Float16*)p.part_o + (size_t)x * ns * HD) + l8;
+  const _Float16* po = (const _Float16*)p.part_o + (size_t)x * ns * HD + d;
+  float2 m[B];
+  h8 v[B];
+  auto load = [&](uint32_t s0) __attribute__((always_inline)) {
+#pragma unroll
+    for (uint32_t k = 0; k < B; k++) {
+      const uint32_t s = s0 + NG * k, at = min(s, ns - 1);
+      m[k] = ml[at];
+      v[k] = *(const h8*)(po + (size_t)at * HD);
+      if (s >= ns) m[k] = make_float2(NEG_INF, 0.f);
+    }
+  };
+  load(grp);
+  float gt[8];
+  if (p.gate) {
+    const float* gate = p.gate + (size_t)col * p.gate_stride + h * HD + d;
+    const f4 a = *(const f4*)gate, b = *(const f4*)(gate + 4);
+#pragma unroll
+    for (int i = 0; i < 4; i++) { gt[i] = a[i]; gt[4 + i] = b[i]; }
+  }
   float M = NEG_INF;
-  for (uint32_t s = lane; s < ns; s += 64) M = fmaxf(M, ml[s].x);
 #pragma unroll
-  for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
+  for (uint32_t k = 0; k < B; k++) M = fmaxf(M, m[k].x);
+  for (uint32_t s = grp + NG * B; s < ns; s += NG) M = fmaxf(M, ml[s].x);
+#pragma unroll
+  for (uint32_t o = LPG; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
   float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  uint32_t sign = 0;
   if (M != NEG_INF) {
-    for (uint32_t s0 = grp; s0 < ns; s0 += NG * B) {
-      float2 m[B];
-      h8 v[B];
-#pragma unroll
-      for (uint32_t k = 0; k < B; k++) { const uint32_t s = min(s0 + NG * k, ns - 1); m[k] = ml[s]; v[k] = po[(size_t)s * LPR]; }
+    for (uint32_t s0 = grp;;) {
 #pragma unroll
       for (uint32_t k = 0; k < B; k++) {
-        const float w = s0 + NG * k < ns ? m[k].y * __builtin_amdgcn_exp2f(m[k].x - M) : 0.f;
-        if (w != 0.f) {                             // (a split that the row saw nothing of holds zeros)
-          L += w;
+        sign |= __float_as_uint(m[k].y);
+        const float w = m[k].y == 0.f ? 0.f : __builtin_fabsf(m[k].y) * __builtin_amdgcn_exp2f(m[k].x - M);      // (a split that the row saw nothing of holds zeros)
+        L += w;
 #pragma unroll
-          for (int i = 0; i < 8; i++) o[i] += w * (float)v[k][i];
-        }
+        for (int i = 0; i < 8; i++) o[i] = __builtin_fmaf(w, (float)v[k][i], o[i]);
       }
+      s0 += NG * B;
+      if (s0 - grp >= ns) break;
+      load(s0);
     }
   }
 #pragma unroll
-  for (uint32_t k = LPR; k < 64; k <<= 1) {
+  for (uint32_t k = LPG; k < 64; k <<= 1) {
     L += __shfl_xor(L, k, 64);
 #pragma unroll
     for (int i = 0; i < 8; i++) o[i] += __shfl_xor(o[i], k, 64);
   }
+  sign = __any(sign >> 31);
   if (grp) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  const uint32_t d = h * HD + 8 * l8;
+#pragma unroll
+  for (int i = 0; i < 8; i++) o[i] *= inv;
+  if (__builtin_expect(sign, 0)) add_not_finite(p, HD, col, h / p.group, d, o);
   if (p.gate) {
-    const float* gate = p.gate + (size_t)col * p.gate_stride + d;
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] *= inv / (1.f + __expf(-gate[i]));
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; i++) o[i] *= inv;
+    for (int i = 0; i < 8; i++) o[i] *= 1.f / (1.f + __expf(-gt[i]));
   }
-  if (p.out_f16) {
-    _Float16* out = (_Float16*)p.out + (size_t)col * p.out_stride + d;
-    *(h4*)out = (h4){ (_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3] };
-    *(h4*)(out + 4) = (h4){ (_Float16)o[4], (_Float16)o[5], (_Float16)o[6], (_Float16)o[7] };
-  } else {
-    float* out = (float*)p.out + (size_t)col * p.out_stride + d;
-    *(f4*)out = (f4){ o[0], o[1], o[2], o[3] };
-    *(f4*)(out + 4) = (f4){ o[4], o[5], o[6], o[7] };
-  }
+  store8(p, col, h * HD + d, o);
 }
 
-template <int HD, int NB, int W, bool Q8>
+template <int HD, int NB, bool Q8>
 static hipError_t launch_tree_k(const TreeParams& p, hipStream_t s, const PaTiming* t) {
-  typedef TreeShape<HD, W> S;
+  typedef TreeShape<HD, TREE_W> S;
   constexpr int D = Q8 ? 2 : 4;
-  constexpr size_t lds = (size_t)D * 2 * S::TILE;
+  constexpr size_t lds = (size_t)D * 2 * S::TILE + TreeLds<NB>::bytes;
   static_assert(lds <= 160 * 1024, "the ring fits a CU");
-  if (p.n_groups == 0 || p.group_rows == 0 || p.group_rows > 16u * NB * W || (uint64_t)(p.n_groups - 1) * p.group_rows >= (uint64_t)p.n_cols * p.group ||
+  if (p.n_groups == 0 || p.group_rows == 0 || p.group_rows > 16u * NB * TREE_W || (uint64_t)(p.n_groups - 1) * p.group_rows >= (uint64_t)p.n_cols * p.group ||
       (uint64_t)p.n_groups * p.group_rows < (uint64_t)p.n_cols * p.group || p.n_splits == 0 ||
       (uint64_t)(p.n_splits - 1) * p.split_tiles * 32 >= (uint64_t)p.base_pos + p.n_cols || (uint64_t)p.n_splits * p.split_tiles * 32 < (uint64_t)p.base_pos + p.n_cols) return hipErrorInvalidValue;
   const uint64_t total = (uint64_t)p.n_groups * p.n_kv_heads * p.n_splits;
   if (total > 0x7fffff00ull) return hipErrorInvalidValue;
   static PaPerDevice lds_set;
-  const hipError_t e = pa_lds_limit(lds_set, (const void*)pa_tree_kernel<HD, NB, W, Q8, D>, lds);
+  const hipError_t e = pa_lds_limit(lds_set, (const void*)pa_tree_kernel<HD, NB, Q8, D>, lds);
   if (e != hipSuccess) return e;
-  PA_LAUNCH((pa_tree_kernel<HD, NB, W, Q8, D>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(W * 64), lds, s, t, p);
+  PA_LAUNCH((pa_tree_kernel<HD, NB, Q8, D>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(TREE_W * 64), lds, s, t, p);
   return hipGetLastError();
 }
 
 template <int HD, bool Q8>
 static hipError_t launch_tree_hd(const TreeParams& p, const TreePlan& pl, hipStream_t s, const PaTiming* t) {
-  if (pl.waves != 8) return hipErrorInvalidValue;
+  if (pl.waves != TREE_W) return hipErrorInvalidValue;
   switch (pl.nb) {
-    case 1: return launch_tree_k<HD, 1, 8, Q8>(p, s, t);
-    case 2: return launch_tree_k<HD, 2, 8, Q8>(p, s, t);
+    case 1: return launch_tree_k<HD, 1, Q8>(p, s, t);
+    case 2: return launch_tree_k<HD, 2, Q8>(p, s, t);
     default: return hipErrorInvalidValue;
   }
 }
@@ -418,10 +601,20 @@ hipError_t pa_launch_tree(const TreeParams& p, const TreePlan& pl, uint32_t hd, 
   return hipErrorInvalidValue;
 }
 
+// few splits: whole rows a wave, many: narrow slices, so that all of a row's splits are one round trip
+template <int HD>
+static void launch_merge(const TreeParams& p, hipStream_t s, const PaTiming* t) {
+  constexpr uint32_t LPR = HD / 8;
+  const uint32_t rows = p.n_cols * p.n_heads;
+  auto grid = [&](uint32_t lpg) { return dim3((unsigned)(((uint64_t)rows * (LPR / lpg) + 3) / 4)); };
+  if (p.n_splits <= 64 / LPR * 8) PA_LAUNCH((pa_tree_merge_kernel<HD, LPR>), grid(LPR), dim3(256), 0, s, t, p);
+  else if (p.n_splits <= 64) PA_LAUNCH((pa_tree_merge_kernel<HD, 8>), grid(8), dim3(256), 0, s, t, p);
+  else PA_LAUNCH((pa_tree_merge_kernel<HD, 4>), grid(4), dim3(256), 0, s, t, p);
+}
+
 hipError_t pa_launch_tree_merge(const TreeParams& p, uint32_t hd, hipStream_t s, const PaTiming* t) {
-  const dim3 grid((p.n_cols * p.n_heads + 3) / 4);
-  if (hd == 256) PA_LAUNCH(pa_tree_merge_kernel<256>, grid, dim3(256), 0, s, t, p);
-  else if (hd == 128) PA_LAUNCH(pa_tree_merge_kernel<128>, grid, dim3(256), 0, s, t, p);
+  if (hd == 256) launch_merge<256>(p, s, t);
+  else if (hd == 128) launch_merge<128>(p, s, t);
   else return hipErrorInvalidValue;
   return hipGetLastError();
 }

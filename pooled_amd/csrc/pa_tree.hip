@@ -78,9 +78,9 @@ static TreePlan plan_tree(const pa_config& c, uint32_t n_cu, uint32_t base, uint
   TreePlan pl;
   const uint32_t rows = n_cols * (c.n_heads / c.n_kv_heads), tiles = ceil_div(base + n_cols, 32);
   pl.waves = 8;
-  pl.nb = rows > 128 ? 2 : 1;
-  const uint32_t cap = 16 * pl.nb * pl.waves;
-  pl.group_rows = (ceil_div(rows, ceil_div(rows, cap)) + 15) & ~15u;
+  const uint32_t most = getenv("TREE_MOST") && atoi(getenv("TREE_MOST")) ? atoi(getenv("TREE_MOST")) : 128, per = ceil_div(rows, ceil_div(rows, most));
+  pl.group_rows = (per + 15) & ~15u;
+  pl.nb = ceil_div(pl.group_rows, 128);
   pl.n_groups = ceil_div(rows, pl.group_rows);
   const uint64_t wgs = (uint64_t)pl.n_groups * c.n_kv_heads;
   uint32_t want = override_splits ? override_splits : (uint32_t)std::max<uint64_t>(1, n_cu / wgs);

@@ -137,7 +137,7 @@ def test_wait_states_behind_matrix_instructions(tmp_path):
     assert kernels
     for name, code in kernels.items():
         uses = shortest(code)
-        assert len(uses) > 20 and all(op in NEEDED for op, _, _ in uses), name
+        assert len(uses) >= 8 and all(op in NEEDED for op, _, _ in uses), name
         low = min(uses, key=lambda u: u[1] - NEEDED[u[0]])
         assert low[1] >= NEEDED[low[0]], "%s: %d wait states behind %s in front of %s" % (name, low[1], low[0], low[2])
 
