@@ -19,6 +19,7 @@
 #include "pf_common.h"
 #include "tree_mask.h"
 
+#define TREE_ISSUE 4         // waves that send for tiles
 template <int HD, int W> struct TreeShape {
   static constexpr int ROWB = HD * 2;               // bytes of a staged row
   static constexpr int TILE = 32 * ROWB;            // bytes of a staged tile of K or of V
@@ -26,10 +27,10 @@ template <int HD, int W> struct TreeShape {
   static constexpr int DB = HD / 16;                // 16-dim blocks of the output
   static constexpr int CPR = HD / 8;                // 16-byte chunks of a staged row
   static constexpr int RPB = 64 / CPR;              // rows of a 1 KB LDS-direct load
-  static constexpr int NLD = 32 / RPB / W;          // LDS-direct loads of a wave, a tensor and tile
+  static constexpr int NLD = 32 / RPB / TREE_ISSUE; // LDS-direct loads of a wave that issues them, a tensor and tile
   static constexpr int PIECES = 32 * HD / 16;       // int8 rows: 16-byte pieces of a tile of K or of V ...
   static constexpr int NP8 = 2 * PIECES / (W * 64); // ... and a thread's share of both
-  static_assert(NLD * W * RPB == 32, "a tile divides evenly over the waves");
+  static_assert(NLD * TREE_ISSUE * RPB == 32, "a tile divides evenly over the waves");
   static_assert(NP8 * W * 64 == 2 * PIECES && PIECES % 64 == 0, "an int8 tile divides evenly over the threads, a wave's pieces are of one tensor");
 };
 
@@ -116,26 +117,34 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   // f16 rows: load j of wave w fills the 1 KB block j W + w of a buffer, rows (j W + w) RPB ..; lane l lands at (row l / CPR, slot l % CPR) and fetches the chunk that belongs there
   const unsigned char* kb0 = (const unsigned char*)p.k_cache + (size_t)g * head_rows * S::ROWB;
   const unsigned char* vb0 = (const unsigned char*)p.v_cache + (size_t)g * head_rows * S::ROWB;
-  constexpr bool ONE_OFF = S::RPB * W % 16 == 0;     // the swizzle, and with it a lane's offset in a load's rows, is the same for all of a wave's loads
-  static_assert(ONE_OFF, "rows of two loads of a wave are a multiple of 16 apart");
-  const uint32_t ld_row = wave * S::RPB + lane / S::CPR, ld_c = lane % S::CPR;
-  const uint32_t k_off = ld_row * S::ROWB + k_slot(ld_row, ld_c) * 16, v_off = ld_row * S::ROWB + v_slot(ld_row, ld_c) * 16;
+  // Only the last waves, which have the fewest rows, send for tiles: a CU takes in 64 bytes a clock, so a tile's loads hold up who issues them for hundreds of clocks, and one wave of each SIMD computes meanwhile.
+  constexpr int IS = TREE_ISSUE;
+  const bool issuer = wave >= W - IS;
+  const uint32_t iw = wave - (W - IS), ld_row = iw * S::RPB + lane / S::CPR, ld_c = lane % S::CPR;
+  constexpr int NOFF = IS * S::RPB % 16 ? 16 / (IS * S::RPB) : 1;            // loads after which the swizzle, and with it a lane's offset in a load's rows, comes again
+  uint32_t k_off[NOFF], v_off[NOFF];
+#pragma unroll
+  for (int j = 0; j < NOFF; j++) {
+    const uint32_t r = j * IS * S::RPB + ld_row;
+    k_off[j] = ld_row * S::ROWB + k_slot(r, ld_c) * 16;
+    v_off[j] = ld_row * S::ROWB + v_slot(r, ld_c) * 16;
+  }
   auto issue = [&](uint32_t i) __attribute__((always_inline)) {
     const uint32_t tp = (tile0 + i) * 32;
     unsigned char* dst = buf(i);
     if (tp + 32 <= end) {
       const unsigned char *kt = kb0 + (size_t)tp * S::ROWB, *vt = vb0 + (size_t)tp * S::ROWB;
 #pragma unroll
-      for (int j = 0; j < S::NLD; j++) PF_GLL_S(kt + j * W * S::RPB * S::ROWB, k_off, dst + (j * W + wave) * 1024);
+      for (int j = 0; j < S::NLD; j++) PF_GLL_S(kt + j * IS * S::RPB * S::ROWB, k_off[j % NOFF], dst + (j * IS + iw) * 1024);
 #pragma unroll
-      for (int j = 0; j < S::NLD; j++) PF_GLL_S(vt + j * W * S::RPB * S::ROWB, v_off, dst + S::TILE + (j * W + wave) * 1024);
+      for (int j = 0; j < S::NLD; j++) PF_GLL_S(vt + j * IS * S::RPB * S::ROWB, v_off[j % NOFF], dst + S::TILE + (j * IS + iw) * 1024);
     } else {                                        // rows behind the last one: the cache's zero padding
 #pragma unroll 1
       for (int j = 0; j < S::NLD; j++) {
-        const uint32_t r = j * W * S::RPB + ld_row;
+        const uint32_t r = j * IS * S::RPB + ld_row;
         const size_t row = tp + r < end ? tp + r : p.max_seq;
-        PF_GLL(kb0 + row * S::ROWB + k_slot(r, ld_c) * 16, dst + (j * W + wave) * 1024);
-        PF_GLL(vb0 + row * S::ROWB + v_slot(r, ld_c) * 16, dst + S::TILE + (j * W + wave) * 1024);
+        PF_GLL(kb0 + row * S::ROWB + k_slot(r, ld_c) * 16, dst + (j * IS + iw) * 1024);
+        PF_GLL(vb0 + row * S::ROWB + v_slot(r, ld_c) * 16, dst + S::TILE + (j * IS + iw) * 1024);
       }
     }
   };
@@ -197,7 +206,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   // (block nb of a wave is rows 16 (nb W + wave) ..: the blocks of a group spread over the SIMDs evenly)
   auto row_of = [&](uint32_t nb, uint32_t r) __attribute__((always_inline)) -> uint32_t { return (nb * W + wave) * 16 + r; };
   const uint32_t blocks = R > wave * 16 ? (R - wave * 16 + W * 16 - 1) / (W * 16) : 0;      // the wave's live blocks
-  if constexpr (Q8) fetch8(0, I0{}); else issue(0);
+  if constexpr (Q8) fetch8(0, I0{}); else if (issuer) issue(0);
   // ---- what follows is one program for the waves of two live blocks, of one, and of none, which pass the same barriers ----
   auto run = [&](auto BLOCKS) __attribute__((always_inline)) {
   constexpr int LIVE = decltype(BLOCKS)::value, NL = LIVE ? LIVE : 1, KD = NL == 1 ? 4 : 3, VD = NL == 1 ? 4 : 3;      // K and V^T fragments (NL products each) fetched ahead
@@ -237,7 +246,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
     if (n_tiles > 1) fetch8(1, I1{});
   } else {
 #pragma unroll
-    for (int i = 1; i < D - 1; i++) if ((uint32_t)i < n_tiles) issue(i);
+    for (int i = 1; i < D - 1; i++) if (issuer && (uint32_t)i < n_tiles) issue(i);
   }
   f4 acc[S::DB][NL];
   float m_ref[NL], l_run[NL];
@@ -422,8 +431,8 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
     constexpr int LOADS = 2 * S::NLD;               // a wave's loads of a tile
     for (uint32_t i = 0; i < n_tiles; i++) {
       // tiles up to i + D - 2 were issued: tile i is there when D - 2 tiles' loads are left
-      if (i + D - 2 < n_tiles) wait_and_meet<LOADS * (D - 2)>(); else wait_and_meet<0>();
-      if (i + D - 1 < n_tiles) issue(i + D - 1);
+      if (!issuer) wait_and_meet_lds(); else if (i + D - 2 < n_tiles) wait_and_meet<LOADS * (D - 2)>(); else wait_and_meet<0>();
+      if (issuer && i + D - 1 < n_tiles) issue(i + D - 1);
       if (__builtin_expect(i >= draft0, 0)) draft_tile(i);
       if constexpr (LIVE > 0) turn(i);
     }

@@ -159,22 +159,35 @@ extern "C" int pa_kv_compact(pa_ctx* ctx, uint32_t dst_row, const uint32_t* d_se
   DeviceGuard on(ctx->device);
   CompactParams p;
   memset(&p, 0, sizeof p);
+  const uint32_t per = kv_q8(ctx) ? 4 : 2;
   p.sel = d_sel; p.n_planes = c.n_kv_heads; p.head_rows = c.max_seq + 32; p.dst_row = dst_row; p.max_rows = max_rows; p.max_seq = c.max_seq;
-  bool any = false;
-  for (int scales = 0; scales < (kv_q8(ctx) ? 2 : 1); scales++) {
-    p.row_bytes = scales ? c.head_dim / 8 : kv_q8(ctx) ? c.head_dim : c.head_dim * 2;
-    p.n_tensors = 0;
-    auto go = [&]() -> hipError_t { const hipError_t e = p.n_tensors ? pa_launch_compact(p, ctx->stream) : hipSuccess; p.n_tensors = 0; return e; };
-    hipError_t e = hipSuccess;
-    for (const pa_layer& L : ctx->layers) {
-      if (!L.k) continue;
-      any = true;
-      p.t[p.n_tensors++] = L.tensor(2 * scales);
-      p.t[p.n_tensors++] = L.tensor(2 * scales + 1);
-      if (p.n_tensors == PA_COMPACT_TENSORS && (e = go()) != hipSuccess) break;
+  p.row_bytes = kv_q8(ctx) ? c.head_dim : c.head_dim * 2; p.scale_bytes = kv_q8(ctx) ? c.head_dim / 8 : 0;
+  uint32_t layers = 0;
+  for (const pa_layer& L : ctx->layers) layers += L.k != nullptr;
+  if (!layers) return block_fail(ctx, PA_ERR_INVALID, who, "no layer has a cache (call pa_layer_alloc)");
+  p.n_layers = std::min(layers, PA_COMPACT_LAYERS);
+  if (!pa_compact_one_round(p)) {
+    // flags for the segments of a long list; under stream capture, where nothing can be allocated, those of the earlier calls are used or the list is walked without
+    const size_t need = pa_compact_flags(p) * sizeof(uint32_t);
+    if (need > ctx->compact_flags_bytes) {
+      hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+      hipError_t e = hipStreamIsCapturing(ctx->stream, &st);
+      if (e != hipSuccess) return block_fail_hip(ctx, e, who);
+      const int rc = st == hipStreamCaptureStatusNone ? pa_ctx_grow(ctx, (void**)&ctx->compact_flags, &ctx->compact_flags_bytes, need) : PA_OK;
+      if (rc) return rc;
     }
-    if (e == hipSuccess) e = go();
-    if (e != hipSuccess) return block_fail_hip(ctx, e, who);
+    p.flags = need <= ctx->compact_flags_bytes ? ctx->compact_flags : nullptr;
   }
-  return any ? PA_OK : block_fail(ctx, PA_ERR_INVALID, who, "no layer has a cache (call pa_layer_alloc)");
+  p.n_layers = 0;
+  hipError_t e = hipSuccess;
+  for (const pa_layer& L : ctx->layers) {
+    if (!L.k) continue;
+    for (uint32_t w = 0; w < per; w++) p.t[p.n_layers * per + w] = L.tensor((int)w);
+    layers--;
+    if (++p.n_layers == PA_COMPACT_LAYERS || !layers) {
+      if ((e = pa_launch_compact(p, ctx->stream)) != hipSuccess) return block_fail_hip(ctx, e, who);
+      p.n_layers = 0;
+    }
+  }
+  return PA_OK;
 }

@@ -42,11 +42,15 @@ struct GlueAtParams {
 hipError_t pa_launch_glue_at(const GlueAtParams& p, hipStream_t s);
 
 // ---- compaction of the caches to a list of rows (kv_compact.hip) ----
-#define PA_COMPACT_TENSORS 128u
+#define PA_COMPACT_LAYERS 32u
 struct CompactParams {
-  void* t[PA_COMPACT_TENSORS];                  // [planes][head_rows][row_bytes of the tensor]; even and odd tensors are K and V, or their scales
+  void* t[4 * PA_COMPACT_LAYERS];               // a layer's K, V (and their scales): [planes][head_rows][row_bytes or scale_bytes]
   const uint32_t* sel;                          // n, then n rows, ascending
-  uint32_t n_tensors, n_planes, head_rows, row_bytes;
+  uint32_t* flags;                              // a word for each segment, zero; nullptr: none
+  uint32_t n_layers, n_planes, head_rows;
+  uint32_t row_bytes, scale_bytes;              // scale_bytes 0: f16 caches
   uint32_t dst_row, max_rows, max_seq;
 };
+bool pa_compact_one_round(const CompactParams& p);        // a list so short that no segments are needed
+size_t pa_compact_flags(const CompactParams& p);          // words of p.flags
 hipError_t pa_launch_compact(const CompactParams& p, hipStream_t s);

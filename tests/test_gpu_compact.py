@@ -60,6 +60,18 @@ def test_paths_that_stay_and_neighbours():
             check(pa, was, dst, rows)
 
 
+@pytest.mark.parametrize("q8", [False, True])
+def test_long_lists(q8):
+    """Many segments to a plane, kept rows of a tenth to nearly all, one call behind another."""
+    with PooledAttn(dict(SHAPES["qwen38_27b"], kv_q8=q8), 40000, n_layers=2) as pa:
+        was = filled(pa, (0, 1), 5)
+        rng = np.random.default_rng(9)
+        for dst, end, n in ((0, 40000, 36000), (4, 36000, 20000), (1000, 39000, 3800), (0, 40000, 39999)):
+            rows = ascending(rng, dst, end, n)
+            pa.run_kv_compact(dst, rows, max_rows=min(n + 17, 40000 - dst))
+            check(pa, was, dst, rows)
+
+
 def test_many_layers():
     """More tensors than one launch takes."""
     cfg = dict(n_heads=2, n_kv_heads=1, head_dim=128, n_rot=64, rope_theta=1e6, eps=1e-6, qk_norm=True, gate=False)
