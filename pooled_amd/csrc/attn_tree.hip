@@ -100,10 +100,12 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   const uint32_t total = p.n_groups * p.n_kv_heads * p.n_splits, per = (total + 7) / 8;
   const uint32_t item = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (item >= total) return;
-  const uint32_t grp = item % p.n_groups, gs = item / p.n_groups, sp = gs % p.n_splits, g = gs / p.n_splits;
+  const uint32_t gs = p.ng_magic ? __umulhi(item, p.ng_magic) : item, grp = item - gs * p.n_groups;
+  const uint32_t g = p.ns_magic ? __umulhi(gs, p.ns_magic) : gs, sp = gs - g * p.n_splits;
   const uint32_t tid = threadIdx.x, lane = tid & 63, ln = lane & 15, kg = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t G = p.group, nH = p.n_heads;
+  auto col_of = [&](uint32_t x) __attribute__((always_inline)) -> uint32_t { return p.g_magic ? __umulhi(x, p.g_magic) : x; };      // x divided by G
   const uint32_t x0 = grp * p.group_rows, R = min(p.group_rows, p.n_cols * G - x0);     // the group's stacked rows [x0, x0 + R)
   const uint32_t end = p.base_pos + p.n_cols;
   const uint32_t tile0 = sp * p.split_tiles, n_tiles = min(p.split_tiles, (end + 31) / 32 - tile0);
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
 #pragma unroll 1
     for (uint32_t e = tid; e < WIN * ROWS; e += W * 64) {
       const uint32_t r = e % ROWS, i = draft0 + d + e / ROWS, x = x0 + min(r, R - 1);
-      if (i < n_tiles) win_lds[e] = mask_window(p.mask + (size_t)(x / G) * p.mask_stride, (int)((tile0 + i) * 32 - p.base_pos), p.n_cols);
+      if (i < n_tiles) win_lds[e] = mask_window(p.mask + (size_t)col_of(x) * p.mask_stride, (int)((tile0 + i) * 32 - p.base_pos), p.n_cols);
     }
   };
 
@@ -221,7 +223,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
     for (int b = 0; b < 2 * NL; b++)
 #pragma unroll
       for (int j = 0; j < QL; j++) {
-        const uint32_t x = x0 + min(row_of(b / 2, b % 2 * 8 + j * RPL + lane / LPQ), R - 1), col = x / G;
+        const uint32_t x = x0 + min(row_of(b / 2, b % 2 * 8 + j * RPL + lane / LPQ), R - 1), col = col_of(x);
         qv[b][j] = *(const f4*)(p.q + (size_t)col * p.q_stride + (size_t)(g * G + x - col * G) * HD + lane % LPQ * 4);
       }
     if (draft0 < n_tiles) fill_windows(0);
@@ -267,10 +269,10 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   h8 pf[NL];
   // one tile: scores, softmax, product
   auto turn = [&](uint32_t i) __attribute__((always_inline)) {
-    constexpr int NF = 2 * S::KS;
     const unsigned char *kb = buf(i), *vb = kb + S::TILE;
     // ---- S^T = K Q^T ----
     {
+      constexpr int NF = 2 * S::KS;
       h8 ka[KD];
       auto at = [&](int f) __attribute__((always_inline)) { return kb + (k_rd ^ (f / 2 % 4 * 64)) + f / 8 * 256 + f % 2 * 16 * S::ROWB; };
 #pragma unroll
@@ -414,7 +416,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
 
   // ---- main loop: behind turn i's barrier tile i is there for every wave, and every wave has done turn i - 1, so that tile i - 1's buffer takes what comes next ----
   if constexpr (Q8) {
-    static_assert(D == 2, "int8 rows: a turn's tile and the one that is staged meanwhile");
+    static_assert(!Q8 || D == 2, "int8 rows: a turn's tile and the one that is staged meanwhile");
     // when turn i begins, the registers of the other parity hold tile i + 1, those of its own tile i + 2
     stage8(0, I0{});
     if (n_tiles > 2) fetch8(2, I0{});
@@ -428,7 +430,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
       if constexpr (LIVE > 0) turn(i);
     }
   } else {
-    constexpr int LOADS = 2 * S::NLD;               // a wave's loads of a tile
+    constexpr int LOADS = 2 * S::NLD;               // an issuing wave's loads of a tile
     for (uint32_t i = 0; i < n_tiles; i++) {
       // tiles up to i + D - 2 were issued: tile i is there when D - 2 tiles' loads are left
       if (!issuer) wait_and_meet_lds(); else if (i + D - 2 < n_tiles) wait_and_meet<LOADS * (D - 2)>(); else wait_and_meet<0>();
@@ -441,60 +443,59 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   // ---- the split's outputs: through LDS, so that a row leaves in whole lines ----
   wait_and_meet_lds();                              // every wave has read the last tile
   if constexpr (LIVE > 0) {
-  constexpr int EROWS = RING / W / (HD * 4) < 16 ? 8 : 16, LPR = HD / 8, RPI = 64 / LPR;      // rows at a time; lanes of a row, rows of the wave at once
-  static_assert(EROWS * HD * 4 * W <= RING, "the rows fit the ring");
-  float* os = (float*)(smem + wave * EROWS * HD * 4);
+  // partials: O [kv head][split][stacked row][HD], so that what a wave writes is one piece; (m, l) [kv head][stacked row][split]
+  const uint32_t rows_all = p.n_cols * G, c = lane % (HD / 8);
+  constexpr int RPI = 64 / (HD / 8);                // rows of the wave at once, eight dims a lane
 #pragma unroll
   for (int nb = 0; nb < NL; nb++) {
     l_run[nb] += __shfl_xor(l_run[nb], 16, 64);
     l_run[nb] += __shfl_xor(l_run[nb], 32, 64);
     const float inv = l_run[nb] == 0.f ? 0.f : 1.f / l_run[nb];             // a row that sees nothing: zeros
-    if (p.n_splits > 1 && kg == 0 && row_of(nb, ln) < R) {
-      const uint32_t x = x0 + row_of(nb, ln), col = x / G;
+    const uint32_t r0 = row_of(nb, 0);
+    if (p.n_splits > 1) {
       // (the sign of l says that a drafted row of the split holds what is not finite; a row of NaN scores may have found no reference)
-      p.part_ml[((size_t)col * nH + g * G + x - col * G) * p.n_splits + sp] = make_float2(l_run[nb] != l_run[nb] ? __builtin_inff() : m_ref[nb], bad ? -l_run[nb] : l_run[nb]);
-    }
+      if (kg == 0 && r0 + ln < R)
+        p.part_ml[((size_t)g * rows_all + x0 + r0 + ln) * p.n_splits + sp] = make_float2(l_run[nb] != l_run[nb] ? __builtin_inff() : m_ref[nb], bad ? -l_run[nb] : l_run[nb]);
+      unsigned char* os = smem + wave * 16 * S::ROWB;
+      static_assert(16 * W * S::ROWB <= RING, "sixteen rows of each wave fit the ring");
 #pragma unroll
-    for (int half = 0; half < 16 / EROWS; half++) {
-      if (EROWS == 16 || (int)(ln / 8) == half) {
-        const uint32_t r = ln % EROWS;
-#pragma unroll
-        for (int db = 0; db < S::DB; db++) *(f4*)(os + r * HD + ((4 * db + kg) ^ r) * 4) = acc[db][nb] * inv;
+      for (int db = 0; db < S::DB; db++) {
+        const f4 o = acc[db][nb] * inv;
+        *(h4*)(os + ln * S::ROWB + ((2 * db + kg / 2) ^ ln) * 16 + kg % 2 * 8) = (h4){ (_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3] };
       }
       wave_fence();
-      // eight dims of row r
-      auto row8 = [&](uint32_t r, float (&o)[8]) __attribute__((always_inline)) {
-        const uint32_t c = lane % LPR * 2;
-        const f4 a = *(const f4*)(os + r * HD + (c ^ r) * 4), b = *(const f4*)(os + r * HD + ((c + 1) ^ r) * 4);
+      h8* to = (h8*)((_Float16*)p.part_o + (((size_t)g * p.n_splits + sp) * rows_all + x0 + r0) * HD) + lane;
 #pragma unroll
-        for (int i = 0; i < 4; i++) { o[i] = a[i]; o[4 + i] = b[i]; }
-      };
-      const uint32_t r0 = row_of(nb, half * EROWS), d = lane % LPR * 8;
-      if (p.n_splits > 1) {
-#pragma unroll
-        for (int it = 0; it < EROWS / RPI; it++) {
-          const uint32_t r = it * RPI + lane / LPR;
-          float o[8];
-          row8(r, o);
-          if (r0 + r < R) {
-            const uint32_t x = x0 + r0 + r, col = x / G, hq = g * G + x - col * G;
-            const h8 v = { (_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3], (_Float16)o[4], (_Float16)o[5], (_Float16)o[6], (_Float16)o[7] };
-            __builtin_nontemporal_store(v, (h8*)((_Float16*)p.part_o + (((size_t)col * nH + hq) * p.n_splits + sp) * HD + d));
-          }
-        }
-      } else {
-#pragma unroll 1
-        for (int it = 0; it < EROWS / RPI; it++) {
-          const uint32_t r = it * RPI + lane / LPR;
-          if (r0 + r >= R) continue;
-          float o[8];
-          row8(r, o);
-          const uint32_t x = x0 + r0 + r, col = x / G, hq = g * G + x - col * G;
-          if (__builtin_expect(bad, 0)) add_not_finite(p, HD, col, g, d, o);
-          store_row8(p, col, hq * HD + d, o);
-        }
+      for (int it = 0; it < 16 / RPI; it++) {
+        const uint32_t r = it * RPI + lane / (HD / 8);
+        const h8 v = *(const h8*)(os + r * S::ROWB + (c ^ r) * 16);
+        if (r0 + r < R) __builtin_nontemporal_store(v, to + it * 64);
       }
       wave_fence();
+    } else {
+      constexpr int EROWS = RING / W / (HD * 4) < 16 ? 8 : 16;              // f32 rows that a wave's part of the ring holds
+      static_assert(EROWS * HD * 4 * W <= RING, "the rows fit the ring");
+      float* os = (float*)(smem + wave * EROWS * HD * 4);
+#pragma unroll
+      for (int half = 0; half < 16 / EROWS; half++) {
+        if (EROWS == 16 || (int)(ln / 8) == half) {
+          const uint32_t r = ln % EROWS;
+#pragma unroll
+          for (int db = 0; db < S::DB; db++) *(f4*)(os + r * HD + ((4 * db + kg) ^ r) * 4) = acc[db][nb] * inv;
+        }
+        wave_fence();
+#pragma unroll 2
+        for (int it = 0; it < EROWS / RPI; it++) {
+          const uint32_t r = it * RPI + lane / (HD / 8), wr = r0 + half * EROWS + r;
+          if (wr >= R) continue;
+          const f4 a = *(const f4*)(os + r * HD + ((2 * c) ^ r) * 4), b = *(const f4*)(os + r * HD + ((2 * c + 1) ^ r) * 4);
+          float o[8] = { a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3] };
+          const uint32_t x = x0 + wr, col = col_of(x), hq = g * G + x - col * G;
+          if (__builtin_expect(bad, 0)) add_not_finite(p, HD, col, g, 8 * c, o);
+          store_row8(p, col, hq * HD + 8 * c, o);
+        }
+        wave_fence();
+      }
     }
   }
   }
@@ -510,11 +511,13 @@ template <int HD, int LPG>
 __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
   constexpr uint32_t NG = 64 / LPG, B = 8, SL = HD / 8 / LPG;
   const uint32_t lane = threadIdx.x & 63, l8 = lane % LPG, grp = lane / LPG;
-  const uint32_t wv = blockIdx.x * 4 + (threadIdx.x >> 6), x = wv / SL;
-  if (x >= p.n_cols * p.n_heads) return;
-  const uint32_t col = x / p.n_heads, h = x - col * p.n_heads, ns = p.n_splits, d = (wv % SL * LPG + l8) * 8;
-  const float2* ml = p.part_ml + (size_t)x * ns;
-  const _Float16* po = (const _Float16*)p.part_o + (size_t)x * ns * HD + d;
+  const uint32_t wv = blockIdx.x * 4 + (threadIdx.x >> 6), row = wv / SL, rows_all = p.n_cols * p.group, ns = p.n_splits;
+  if (row >= p.n_cols * p.n_heads) return;
+  const uint32_t g = p.rows_magic ? __umulhi(row, p.rows_magic) : row, x = row - g * rows_all;                 // kv head, stacked row
+  const uint32_t col = p.g_magic ? __umulhi(x, p.g_magic) : x, h = g * p.group + x - col * p.group, d = (wv % SL * LPG + l8) * 8;
+  const float2* ml = p.part_ml + (size_t)row * ns;
+  const _Float16* po = (const _Float16*)p.part_o + ((size_t)g * ns * rows_all + x) * HD + d;
+  const size_t step = (size_t)rows_all * HD;
   float2 m[B];
   h8 v[B];
   auto load = [&](uint32_t s0) __attribute__((always_inline)) {
@@ -522,7 +525,7 @@ __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
     for (uint32_t k = 0; k < B; k++) {
       const uint32_t s = s0 + NG * k, at = min(s, ns - 1);
       m[k] = ml[at];
-      v[k] = *(const h8*)(po + (size_t)at * HD);
+      v[k] = __builtin_nontemporal_load((const h8*)(po + at * step));
       if (s >= ns) m[k] = make_float2(NEG_INF, 0.f);
     }
   };
@@ -568,12 +571,24 @@ __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
   const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
   for (int i = 0; i < 8; i++) o[i] *= inv;
-  if (__builtin_expect(sign, 0)) add_not_finite(p, HD, col, h / p.group, d, o);
+  if (__builtin_expect(sign, 0)) add_not_finite(p, HD, col, g, d, o);
   if (p.gate) {
 #pragma unroll
     for (int i = 0; i < 8; i++) o[i] *= 1.f / (1.f + __expf(-gt[i]));
   }
   store8(p, col, h * HD + d, o);
+}
+
+// n / d = mulhi(n, ceil(2^32 / d)) while n d < 2^32: the divisions at the head of the kernels, some thirty instructions each, cost 1 - 2 us a call
+static bool set_magics(TreeParams& p) {
+  bool ok = true;
+  auto magic = [&](uint64_t below, uint32_t d) -> uint32_t { ok = ok && below * d < (1ull << 32); return d > 1 ? (uint32_t)(((1ull << 32) + d - 1) / d) : 0u; };
+  const uint64_t gs = (uint64_t)p.n_kv_heads * p.n_splits;
+  p.ng_magic = magic(gs * p.n_groups + 8, p.n_groups);
+  p.ns_magic = magic(gs + 8, p.n_splits);
+  p.g_magic = magic((uint64_t)p.n_cols * p.group, p.group);
+  p.rows_magic = magic((uint64_t)p.n_cols * p.n_heads, p.n_cols * p.group);
+  return ok;
 }
 
 template <int HD, int NB, bool Q8>
@@ -590,7 +605,9 @@ static hipError_t launch_tree_k(const TreeParams& p, hipStream_t s, const PaTimi
   static PaPerDevice lds_set;
   const hipError_t e = pa_lds_limit(lds_set, (const void*)pa_tree_kernel<HD, NB, Q8, D>, lds);
   if (e != hipSuccess) return e;
-  PA_LAUNCH((pa_tree_kernel<HD, NB, Q8, D>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(TREE_W * 64), lds, s, t, p);
+  TreeParams pk = p;
+  if (!set_magics(pk)) return hipErrorInvalidValue;
+  PA_LAUNCH((pa_tree_kernel<HD, NB, Q8, D>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(TREE_W * 64), lds, s, t, pk);
   return hipGetLastError();
 }
 
@@ -599,7 +616,7 @@ static hipError_t launch_tree_hd(const TreeParams& p, const TreePlan& pl, hipStr
   if (pl.waves != TREE_W) return hipErrorInvalidValue;
   switch (pl.nb) {
     case 1: return launch_tree_k<HD, 1, Q8>(p, s, t);
-    case 2: return launch_tree_k<HD, 2, Q8>(p, s, t);
+    case 2: if constexpr (HD == 128 || !Q8) return launch_tree_k<HD, 2, Q8>(p, s, t); else return hipErrorInvalidValue;
     default: return hipErrorInvalidValue;
   }
 }
@@ -621,7 +638,9 @@ static void launch_merge(const TreeParams& p, hipStream_t s, const PaTiming* t) 
   else PA_LAUNCH((pa_tree_merge_kernel<HD, 4>), grid(4), dim3(256), 0, s, t, p);
 }
 
-hipError_t pa_launch_tree_merge(const TreeParams& p, uint32_t hd, hipStream_t s, const PaTiming* t) {
+hipError_t pa_launch_tree_merge(const TreeParams& p_in, uint32_t hd, hipStream_t s, const PaTiming* t) {
+  TreeParams p = p_in;
+  if (!set_magics(p)) return hipErrorInvalidValue;
   if (hd == 256) launch_merge<256>(p, s, t);
   else if (hd == 128) launch_merge<128>(p, s, t);
   else return hipErrorInvalidValue;

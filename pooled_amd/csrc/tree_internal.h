@@ -8,7 +8,7 @@ struct TreeParams {
   const void* k_cache; const void* v_cache;     // f16 or int8, [nKV][max_seq + 32][hd]
   const float* k_scale; const float* v_scale;   // int8 caches: one f32 scale per 32 values
   const uint32_t* mask;                         // [n_cols][mask_stride]: bit j: the column sees row base_pos + j
-  uint16_t* part_o; float2* part_ml;            // per (column, head, split): O / l as f16 [hd], and (m, l)
+  uint16_t* part_o; float2* part_ml;            // partials of the splits: O / l as f16 and (m, l), see attn_tree.hip
   void* out;                                    // [n_cols][out_stride]
   uint32_t q_stride, gate_stride, mask_stride, out_stride;
   uint32_t n_heads, n_kv_heads, group;          // group = nH / nKV
@@ -17,6 +17,7 @@ struct TreeParams {
   uint32_t n_groups, group_rows;                // groups of stacked rows of a kv head (row = column x G + head), rows of each
   int out_f16;
   float scale;                                  // 1 / sqrt(hd)
+  uint32_t ng_magic, ns_magic, g_magic, rows_magic; // ceil(2^32 / d) of n_groups, n_splits, group and n_cols x group, 0 for one (set by the launchers)
 };
 // what a call runs as: rows a wave holds (16 nb), waves of a workgroup, groups of rows, splits
 struct TreePlan { uint32_t nb, waves, n_groups, group_rows, n_splits, split_tiles; };
