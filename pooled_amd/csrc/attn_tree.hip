@@ -156,12 +156,20 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   auto fetch8 = [&](uint32_t i, auto AT) __attribute__((always_inline)) {
     constexpr int at = decltype(AT)::value;
     const uint32_t tp = (tile0 + i) * 32;
+    const size_t row0 = (size_t)g * head_rows + tp;
 #pragma unroll
     for (int j = 0; j < S::NP8; j++) {
       const uint32_t e = tid + j * W * 64, of_v = (wave * 64 + j * W * 64) / S::PIECES, r = e % S::PIECES / (HD / 16), c = e % (HD / 16);
-      const size_t row = (size_t)g * head_rows + (tp + r < end ? tp + r : p.max_seq);
-      raw8[at][j] = *(const u4*)((const unsigned char*)(of_v ? p.v_cache : p.k_cache) + row * HD + c * 16);
-      sc8[at][j] = (of_v ? p.v_scale : p.k_scale)[row * (HD / 32) + c / 2];
+      const unsigned char* rows = (const unsigned char*)(of_v ? p.v_cache : p.k_cache) + row0 * HD;
+      const float* scales = (of_v ? p.v_scale : p.k_scale) + row0 * (HD / 32);
+      if (tp + 32 <= end) {                         // (one offset a thread for all tiles)
+        raw8[at][j] = *(const u4*)(rows + (e % S::PIECES) * 16);
+        sc8[at][j] = scales[e % S::PIECES / 2];
+      } else {                                      // rows behind the last one: the cache's zero padding
+        const uint32_t rr = tp + r < end ? r : p.max_seq - tp;
+        raw8[at][j] = *(const u4*)(rows + (size_t)rr * HD + c * 16);
+        sc8[at][j] = scales[(size_t)rr * (HD / 32) + c / 2];
+      }
     }
   };
   auto widen = [&](u4 raw, float sc, unsigned char* row, uint32_t s0, uint32_t s1) __attribute__((always_inline)) {
@@ -245,7 +253,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
     }
   }
   if constexpr (Q8) {
-    if (n_tiles > 1) fetch8(1, I1{});
+    fetch8(min(1u, n_tiles - 1), I1{});
   } else {
 #pragma unroll
     for (int i = 1; i < D - 1; i++) if (issuer && (uint32_t)i < n_tiles) issue(i);
@@ -417,18 +425,21 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   // ---- main loop: behind turn i's barrier tile i is there for every wave, and every wave has done turn i - 1, so that tile i - 1's buffer takes what comes next ----
   if constexpr (Q8) {
     static_assert(!Q8 || D == 2, "int8 rows: a turn's tile and the one that is staged meanwhile");
-    // when turn i begins, the registers of the other parity hold tile i + 1, those of its own tile i + 2
+    // When turn i begins, the registers of the other parity hold tile i + 1, those of its own tile i + 2.  Fetches and stores go on behind the last tile (the last one again, which nobody looks at):
+    // under a condition the wait for the older registers would be one for the younger too.
+    const uint32_t last = n_tiles - 1;
     stage8(0, I0{});
-    if (n_tiles > 2) fetch8(2, I0{});
-    for (uint32_t i = 0; i < n_tiles; i++) {
+    fetch8(min(2u, last), I0{});
+    auto step = [&](uint32_t i, auto NEXT) __attribute__((always_inline)) {
       wait_and_meet_lds();
-      if (i + 1 < n_tiles) {
-        if (i & 1) { stage8(i + 1, I0{}); if (i + 3 < n_tiles) fetch8(i + 3, I0{}); }
-        else { stage8(i + 1, I1{}); if (i + 3 < n_tiles) fetch8(i + 3, I1{}); }
-      }
+      stage8(i + 1, NEXT);
+      fetch8(min(i + 3, last), NEXT);
       if (__builtin_expect(i >= draft0, 0)) draft_tile(i);
       if constexpr (LIVE > 0) turn(i);
-    }
+    };
+    uint32_t i = 0;
+    for (; i + 1 < n_tiles; i += 2) { step(i, I1{}); step(i + 1, I0{}); }
+    if (i < n_tiles) step(i, I1{});
   } else {
     constexpr int LOADS = 2 * S::NLD;               // an issuing wave's loads of a tile
     for (uint32_t i = 0; i < n_tiles; i++) {
