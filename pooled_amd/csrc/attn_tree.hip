@@ -100,12 +100,12 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   const uint32_t total = p.n_groups * p.n_kv_heads * p.n_splits, per = (total + 7) / 8;
   const uint32_t item = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (item >= total) return;
-  const uint32_t gs = p.ng_magic ? __umulhi(item, p.ng_magic) : item, grp = item - gs * p.n_groups;
-  const uint32_t g = p.ns_magic ? __umulhi(gs, p.ns_magic) : gs, sp = gs - g * p.n_splits;
+  const uint32_t gs = div_by(item, p.n_groups, p.ng_magic), grp = item - gs * p.n_groups;
+  const uint32_t g = div_by(gs, p.n_splits, p.ns_magic), sp = gs - g * p.n_splits;
   const uint32_t tid = threadIdx.x, lane = tid & 63, ln = lane & 15, kg = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const uint32_t G = p.group, nH = p.n_heads;
-  auto col_of = [&](uint32_t x) __attribute__((always_inline)) -> uint32_t { return p.g_magic ? __umulhi(x, p.g_magic) : x; };      // x divided by G
+  auto col_of = [&](uint32_t x) __attribute__((always_inline)) -> uint32_t { return div_by(x, G, p.g_magic); };
   const uint32_t x0 = grp * p.group_rows, R = min(p.group_rows, p.n_cols * G - x0);     // the group's stacked rows [x0, x0 + R)
   const uint32_t end = p.base_pos + p.n_cols;
   const uint32_t tile0 = sp * p.split_tiles, n_tiles = min(p.split_tiles, (end + 31) / 32 - tile0);
@@ -524,8 +524,8 @@ __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
   const uint32_t lane = threadIdx.x & 63, l8 = lane % LPG, grp = lane / LPG;
   const uint32_t wv = blockIdx.x * 4 + (threadIdx.x >> 6), row = wv / SL, rows_all = p.n_cols * p.group, ns = p.n_splits;
   if (row >= p.n_cols * p.n_heads) return;
-  const uint32_t g = p.rows_magic ? __umulhi(row, p.rows_magic) : row, x = row - g * rows_all;                 // kv head, stacked row
-  const uint32_t col = p.g_magic ? __umulhi(x, p.g_magic) : x, h = g * p.group + x - col * p.group, d = (wv % SL * LPG + l8) * 8;
+  const uint32_t g = div_by(row, rows_all, p.rows_magic), x = row - g * rows_all;                 // kv head, stacked row
+  const uint32_t col = div_by(x, p.group, p.g_magic), h = g * p.group + x - col * p.group, d = (wv % SL * LPG + l8) * 8;
   const float2* ml = p.part_ml + (size_t)row * ns;
   const _Float16* po = (const _Float16*)p.part_o + ((size_t)g * ns * rows_all + x) * HD + d;
   const size_t step = (size_t)rows_all * HD;
@@ -590,16 +590,13 @@ __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
   store8(p, col, h * HD + d, o);
 }
 
-// n / d = mulhi(n, ceil(2^32 / d)) while n d < 2^32: the divisions at the head of the kernels, some thirty instructions each, cost 1 - 2 us a call
-static bool set_magics(TreeParams& p) {
-  bool ok = true;
-  auto magic = [&](uint64_t below, uint32_t d) -> uint32_t { ok = ok && below * d < (1ull << 32); return d > 1 ? (uint32_t)(((1ull << 32) + d - 1) / d) : 0u; };
+// (the divisions at the head of the kernels, some thirty instructions each, cost 1 - 2 us a call)
+static void set_magics(TreeParams& p) {
   const uint64_t gs = (uint64_t)p.n_kv_heads * p.n_splits;
-  p.ng_magic = magic(gs * p.n_groups + 8, p.n_groups);
-  p.ns_magic = magic(gs + 8, p.n_splits);
-  p.g_magic = magic((uint64_t)p.n_cols * p.group, p.group);
-  p.rows_magic = magic((uint64_t)p.n_cols * p.n_heads, p.n_cols * p.group);
-  return ok;
+  p.ng_magic = div_magic(gs * p.n_groups + 8, p.n_groups);
+  p.ns_magic = div_magic(gs + 8, p.n_splits);
+  p.g_magic = div_magic((uint64_t)p.n_cols * p.group, p.group);
+  p.rows_magic = div_magic((uint64_t)p.n_cols * p.n_heads, p.n_cols * p.group);
 }
 
 template <int HD, int NB, bool Q8>
@@ -617,7 +614,7 @@ static hipError_t launch_tree_k(const TreeParams& p, hipStream_t s, const PaTimi
   const hipError_t e = pa_lds_limit(lds_set, (const void*)pa_tree_kernel<HD, NB, Q8, D>, lds);
   if (e != hipSuccess) return e;
   TreeParams pk = p;
-  if (!set_magics(pk)) return hipErrorInvalidValue;
+  set_magics(pk);
   PA_LAUNCH((pa_tree_kernel<HD, NB, Q8, D>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(TREE_W * 64), lds, s, t, pk);
   return hipGetLastError();
 }
@@ -651,7 +648,7 @@ static void launch_merge(const TreeParams& p, hipStream_t s, const PaTiming* t) 
 
 hipError_t pa_launch_tree_merge(const TreeParams& p_in, uint32_t hd, hipStream_t s, const PaTiming* t) {
   TreeParams p = p_in;
-  if (!set_magics(p)) return hipErrorInvalidValue;
+  set_magics(p);
   if (hd == 256) launch_merge<256>(p, s, t);
   else if (hd == 128) launch_merge<128>(p, s, t);
   else return hipErrorInvalidValue;

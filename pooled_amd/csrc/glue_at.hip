@@ -3,7 +3,8 @@
 // Pair i of a head's rotated dims, (x[i], x[i + n_rot / 2]), turns by the angle of the position that the column has on the pair's axis; norm, gate and cache rows as in
 // glue_kv.hip, whose arithmetic (glue_math.h) this shares: where every axis holds base + c, the results have the bits of that kernel at base + c.
 //
-// One wavefront per (head, column), key heads with their value head.
+// A wavefront takes 512 values of query heads of one column (two heads of 256, four of 128), or one key head with its value head; every load of a wave goes out ahead of what depends on
+// one.  Wide chunks are bound by HBM, which the loads of several heads a wave keep busy where one head a wave does not; a draft's columns by the chain position -> (cos, sin) -> rotation.
 #include "tree_internal.h"
 #include "glue_math.h"
 
@@ -24,50 +25,119 @@ static __device__ inline void store_row_q8(const float* src, uint32_t hd, uint32
   }
 }
 
-__global__ __launch_bounds__(64) void pa_glue_at_kernel(GlueAtParams p) {
-  __shared__ float xs[256];
-  const uint32_t hh = blockIdx.x, col = blockIdx.y, lane = threadIdx.x;
-  const uint32_t nH = p.n_heads, hd = p.head_dim, qd = nH * hd, half = p.n_rot / 2;
-  const bool is_q = hh < nH, gated = (p.flags & PA_FLAG_GATE) != 0, norm = (p.flags & PA_FLAG_QK_NORM) != 0;
-  const uint32_t h = is_q ? hh : hh - nH;
-  const float* src = is_q ? p.q_in + (size_t)col * p.q_stride + (size_t)h * (gated ? 2 * hd : hd) : p.k_in + (size_t)col * p.k_stride + (size_t)h * hd;
-  float x[4], w[4] = {0.f, 0.f, 0.f, 0.f};
-  float2 cs[2];
-#pragma unroll
-  for (int j = 0; j < 4; j++) x[j] = lane + 64 * j < hd ? src[lane + 64 * j] : 0.f;
-  if (norm) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) w[j] = lane + 64 * j < hd ? (is_q ? p.qw : p.kw)[lane + 64 * j] : 0.f;
-  }
+// REGS: the pair distance is one that glue_heads_regs serves
+template <int HD, bool REGS>
+__global__ __launch_bounds__(256) void pa_glue_at_kernel(GlueAtParams p) {
+  constexpr int N = 512 / HD, J = HD / 64;          // query heads of a wave; values of a lane and head
+  __shared__ float xs_all[4][N * HD];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), task = blockIdx.x * 4 + wave;
+  const uint32_t nH = p.n_heads, qd = nH * HD, half = p.n_rot / 2, q_tasks = (nH + N - 1) / N, per_col = q_tasks + p.n_kv_heads;
+  const uint32_t col = div_by(task, per_col, p.per_col_magic), u = task - col * per_col;
+  if (col >= p.n_cols) return;
+  const bool is_q = u < q_tasks, gated = (p.flags & PA_FLAG_GATE) != 0, norm = (p.flags & PA_FLAG_QK_NORM) != 0;
+  const uint32_t h0 = is_q ? u * N : u - q_tasks, heads = is_q ? min((uint32_t)N, nH - h0) : 1;
+  float* xs = xs_all[wave];
+  // the positions first: two loads hang on them
+  uint32_t pair[2], pos[2];
 #pragma unroll
   for (int j = 0; j < 2; j++) {
-    const uint32_t i = min(lane + 64 * j, half - 1), axis = p.axis_of_pair[i / 16] >> (i % 16 * 2) & 3;
-    const uint32_t pos = p.pos[(size_t)axis * p.pos_stride + col];
-    if (pos < p.tab_rows) cs[j] = p.rope_tab[(size_t)pos * half + i];
-    else rope_cos_sin(pos, p.inv_freq[i], cs[j].x, cs[j].y);
+    pair[j] = REGS && half == 32 ? lane & 31 : min(lane + 64 * j, half - 1);
+    const uint32_t axis = p.n_axes == 1 ? 0u : p.axis_of_pair[pair[j] / 16] >> (pair[j] % 16 * 2) & 3;
+    pos[j] = p.pos[(size_t)axis * p.pos_stride + col];
   }
-  if (is_q && gated)
-    for (uint32_t i = lane; i < hd; i += 64) p.gate_out[(size_t)col * qd + h * hd + i] = src[hd + i];
-  glue_head_wave(x, w, norm, p.eps, hd, half, cs, xs, lane);
+  const float* src = is_q ? p.q_in + (size_t)col * p.q_stride + (size_t)h0 * (gated ? 2 * HD : HD) : p.k_in + (size_t)col * p.k_stride + (size_t)h0 * HD;
+  const uint32_t step = is_q && gated ? 2 * HD : HD;
+  float x[N][4], gt[N][J], w[4] = {0.f, 0.f, 0.f, 0.f};
   if (is_q) {
-    for (uint32_t i = lane; i < hd; i += 64) p.q_out[(size_t)col * qd + h * hd + i] = xs[i];
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+      const float* s = src + (size_t)min((uint32_t)n, heads - 1) * step;     // (a wave's heads past the last: that one again, not stored)
+#pragma unroll
+      for (int j = 0; j < 4; j++) x[n][j] = j < J ? __builtin_nontemporal_load(s + lane + 64 * j) : 0.f;
+      if (gated)
+#pragma unroll
+        for (int j = 0; j < J; j++) gt[n][j] = __builtin_nontemporal_load(s + HD + lane + 64 * j);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++) x[0][j] = j < J ? src[lane + 64 * j] : 0.f;
+  }
+  float v[J];
+  if (!is_q) {
+#pragma unroll
+    for (int j = 0; j < J; j++) v[j] = p.v_in[(size_t)col * p.v_stride + (size_t)h0 * HD + lane + 64 * j];
+  }
+  if (norm) {
+#pragma unroll
+    for (int j = 0; j < J; j++) w[j] = (is_q ? p.qw : p.kw)[lane + 64 * j];
+  }
+  float2 cs[2];
+#pragma unroll
+  for (int j = 0; j < 2; j++) {
+    if (j && half <= 64) { cs[j] = cs[0]; continue; }                        // (not looked at)
+    if (pos[j] < p.tab_rows) cs[j] = p.rope_tab[(size_t)pos[j] * half + pair[j]];
+    else rope_cos_sin(pos[j], p.inv_freq[pair[j]], cs[j].x, cs[j].y);
+  }
+  if (is_q) {
+    const size_t at = (size_t)col * qd + h0 * HD + lane;
+    if (gated) {
+#pragma unroll
+      for (int n = 0; n < N; n++)
+        if ((uint32_t)n < heads)
+#pragma unroll
+          for (int j = 0; j < J; j++) p.gate_out[at + n * HD + 64 * j] = gt[n][j];
+    }
+    if constexpr (REGS) glue_heads_regs<N>(x, w, norm, p.eps, HD, half, cs, lane);
+    else {
+      glue_heads_wave<N>(x, w, norm, p.eps, HD, half, cs, xs, HD, lane);
+#pragma unroll
+      for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int j = 0; j < J; j++) x[n][j] = xs[n * HD + lane + 64 * j];
+    }
+#pragma unroll
+    for (int n = 0; n < N; n++)
+      if ((uint32_t)n < heads)
+#pragma unroll
+        for (int j = 0; j < J; j++) p.q_out[at + n * HD + 64 * j] = x[n][j];
     return;
   }
-  const float* v = p.v_in + (size_t)col * p.v_stride + (size_t)h * hd;
-  const size_t row = (size_t)h * p.head_rows + p.base_row + col;
+  float x1[1][4] = { { x[0][0], x[0][1], x[0][2], x[0][3] } };
+  if constexpr (REGS) {
+    glue_heads_regs<1>(x1, w, norm, p.eps, HD, half, cs, lane);
+#pragma unroll
+    for (int j = 0; j < J; j++) xs[lane + 64 * j] = x1[0][j];
+  } else glue_heads_wave<1>(x1, w, norm, p.eps, HD, half, cs, xs, HD, lane);
+#pragma unroll
+  for (int j = 0; j < J; j++) xs[HD + lane + 64 * j] = v[j];                 // the value row beside the key row
+  wave_lds_fence();
+  const size_t row = (size_t)h0 * p.head_rows + p.base_row + col;
   if (p.ks_cache) {
-    store_row_q8(xs, hd, lane, (unsigned char*)p.k_cache + row * hd, p.ks_cache + row * (hd / 32));
-    store_row_q8(v, hd, lane, (unsigned char*)p.v_cache + row * hd, p.vs_cache + row * (hd / 32));
+    store_row_q8(xs, HD, lane, (unsigned char*)p.k_cache + row * HD, p.ks_cache + row * (HD / 32));
+    store_row_q8(xs + HD, HD, lane, (unsigned char*)p.v_cache + row * HD, p.vs_cache + row * (HD / 32));
   } else {
-    for (uint32_t i = lane; i < hd / 2; i += 64) {
-      ((uint32_t*)((uint16_t*)p.k_cache + row * hd))[i] = pack_f16x2(xs[2 * i], xs[2 * i + 1]);
-      ((uint32_t*)((uint16_t*)p.v_cache + row * hd))[i] = pack_f16x2(v[2 * i], v[2 * i + 1]);
+#pragma unroll
+    for (int t = 0; t < HD / 128; t++) {
+      const uint32_t i = lane + 64 * t;
+      ((uint32_t*)((uint16_t*)p.k_cache + row * HD))[i] = pack_f16x2(xs[2 * i], xs[2 * i + 1]);
+      ((uint32_t*)((uint16_t*)p.v_cache + row * HD))[i] = pack_f16x2(xs[HD + 2 * i], xs[HD + 2 * i + 1]);
     }
   }
 }
 
-hipError_t pa_launch_glue_at(const GlueAtParams& p, hipStream_t s) {
-  if (!p.n_cols || p.n_cols > 65535u) return hipErrorInvalidValue;
-  hipLaunchKernelGGL(pa_glue_at_kernel, dim3(p.n_heads + p.n_kv_heads, p.n_cols), dim3(64), 0, s, p);
+template <int HD> static hipError_t launch_glue_at(const GlueAtParams& p, uint32_t wgs, hipStream_t s) {
+  if (glue_regs_serves(p.n_rot / 2)) hipLaunchKernelGGL((pa_glue_at_kernel<HD, true>), dim3(wgs), dim3(256), 0, s, p);
+  else hipLaunchKernelGGL((pa_glue_at_kernel<HD, false>), dim3(wgs), dim3(256), 0, s, p);
   return hipGetLastError();
+}
+
+hipError_t pa_launch_glue_at(const GlueAtParams& p_in, hipStream_t s) {
+  GlueAtParams p = p_in;
+  const uint32_t n = p.head_dim ? 512 / p.head_dim : 1;
+  const uint64_t per_col = (uint64_t)(p.n_heads + n - 1) / n + p.n_kv_heads, tasks = per_col * p.n_cols;
+  if (!tasks || tasks > 0x7fffff00ull) return hipErrorInvalidValue;
+  p.per_col_magic = div_magic(tasks + 4, (uint32_t)per_col);
+  if (p.head_dim == 256) return launch_glue_at<256>(p, (uint32_t)((tasks + 3) / 4), s);
+  if (p.head_dim == 128) return launch_glue_at<128>(p, (uint32_t)((tasks + 3) / 4), s);
+  return hipErrorInvalidValue;
 }

@@ -160,7 +160,7 @@ static __device__ inline void glue_heads_wave(const float (&x_in)[N][4], const f
 // register 0, exchanged by a lane-swap instruction; cs[0] must then hold the (cos, sin) of pair lane & 31 in every lane).
 // On return x holds the normed and rotated head, element lane + 64 j in x[n][j].  Same operations on the same values as
 // glue_heads_wave, so the same bits; four dependent LDS round trips shorter.
-static __device__ inline bool glue_regs_serves(uint32_t half) { return half == 0 || half == 32 || (half & 63) == 0; }
+static __host__ __device__ inline bool glue_regs_serves(uint32_t half) { return half == 0 || half == 32 || (half & 63) == 0; }
 template <int N>
 static __device__ inline void glue_heads_regs(float (&x)[N][4], const float (&w)[4], bool norm, float eps, uint32_t hd,
                                               uint32_t half, const float2 (&cs)[2], uint32_t lane) {

@@ -61,6 +61,7 @@ extern "C" int pa_glue_kv_at(pa_ctx* ctx, uint32_t layer, const float* d_q_in, u
   p.q_stride = q_stride; p.k_stride = k_stride; p.v_stride = v_stride;
   p.n_heads = c.n_heads; p.n_kv_heads = c.n_kv_heads; p.head_dim = c.head_dim; p.n_rot = c.n_rot;
   p.base_row = base_row; p.n_cols = n_cols; p.flags = c.flags; p.eps = c.eps;
+  p.n_axes = ctx->rope_axes;
   memcpy(p.axis_of_pair, ctx->axis_of_pair, sizeof p.axis_of_pair);
   DeviceGuard on(ctx->device);
   const hipError_t e = pa_launch_glue_at(p, ctx->stream);
@@ -72,22 +73,46 @@ extern "C" int pa_glue_kv_at(pa_ctx* ctx, uint32_t layer, const float* d_q_in, u
 static size_t part_bytes(const pa_config& c, uint32_t n_cols, uint32_t splits) { return (size_t)n_cols * c.n_heads * splits * c.head_dim * 2; }
 static size_t ml_bytes(const pa_config& c, uint32_t n_cols, uint32_t splits) { return (size_t)n_cols * c.n_heads * splits * 8; }
 
-// Rows of a workgroup: 128 stacked rows, or 256 where there are more.  Splits: until every CU has a workgroup, the tiles of the context permitting.
-// most_splits: what a caller that cannot allocate has room for.
+// What a call takes, in us, fitted to 463 timed calls (16 / 2-, 24 / 4- and 16 / 8-head shapes, 2 - 64 columns at 64 - 65536 rows, f16 and int8 rows, 64 - 256 rows a workgroup, all CUs busy
+// down to an eighth of them; mean error 4 %, nine in ten within 8 %; what it chooses takes 100.8 % of the best plan tried, 109 % at worst).  The launches, the start of a workgroup and its
+// outputs; then its tiles, each so long for the barrier and the chain of one wave and so much for every block of 16 rows, or the stream of the cache if that is more; and the
+// partials, written and read again.
+static double tree_us(const pa_config& c, uint32_t n_cu, uint32_t rows, uint32_t tiles, const TreePlan& pl) {
+  const bool q8 = (c.flags & PA_FLAG_KV_Q8) != 0, wide = c.head_dim == 256;
+  const double fixed = q8 ? (wide ? 10.1 : 7.6) : wide ? 8.6 : 7.2, out = q8 ? (wide ? 0.05 : 0.18) : wide ? 0.29 : 0.19;
+  const double tile = q8 ? (wide ? 0.629 : 0.458) : wide ? 0.356 : 0.358, block = q8 ? (wide ? 0.072 : 0.016) : wide ? 0.063 : 0.019;
+  const double blocks = pl.group_rows / 16.0, wgs = (double)pl.n_groups * c.n_kv_heads * pl.n_splits;
+  const double chain = pl.split_tiles * (tile + block * blocks) * std::ceil(wgs / n_cu);
+  const double stream = 1e-6 / 7.0 * tiles * 32.0 * c.n_kv_heads * c.head_dim * (q8 ? 2.25 : 4.0);
+  const double partials = pl.n_splits > 1 ? 1e-6 * rows * c.n_kv_heads * pl.n_splits * c.head_dim * 2.0 : 0.0;
+  return fixed + std::max(chain, stream) + out * blocks + 0.427 * partials;
+}
+
+// Rows of a workgroup: up to 256, a wave two blocks of 16, or 128, 64 and 32, the groups then sharing the stream through their XCD's L2 (two blocks of int8 rows of head_dim 256 do not fit the
+// registers).  Splits: a workgroup a CU, or fewer, whose partials are less.  most_splits: what a caller that cannot allocate has room for.
 static TreePlan plan_tree(const pa_config& c, uint32_t n_cu, uint32_t base, uint32_t n_cols, uint32_t override_splits, uint32_t most_splits) {
-  TreePlan pl;
   const uint32_t rows = n_cols * (c.n_heads / c.n_kv_heads), tiles = ceil_div(base + n_cols, 32);
-  pl.waves = 8;
-  const uint32_t most = getenv("TREE_MOST") && atoi(getenv("TREE_MOST")) ? atoi(getenv("TREE_MOST")) : 128, per = ceil_div(rows, ceil_div(rows, most));
-  pl.group_rows = (per + 15) & ~15u;
-  pl.nb = ceil_div(pl.group_rows, 128);
-  pl.n_groups = ceil_div(rows, pl.group_rows);
-  const uint64_t wgs = (uint64_t)pl.n_groups * c.n_kv_heads;
-  uint32_t want = override_splits ? override_splits : (uint32_t)std::max<uint64_t>(1, n_cu / wgs);
-  want = std::max(1u, std::min({want, tiles, most_splits}));
-  pl.split_tiles = ceil_div(tiles, want);
-  pl.n_splits = ceil_div(tiles, pl.split_tiles);
-  return pl;
+  const bool narrow = (c.flags & PA_FLAG_KV_Q8) && c.head_dim == 256;
+  TreePlan best{};
+  double best_us = -1.0;
+  for (uint32_t cap = narrow ? 128 : 256; cap >= 32; cap /= 2) {
+    if (cap < 256 && cap / 2 >= rows && cap > 32) continue;                  // the same groups as the next cap's
+    TreePlan pl{};
+    pl.waves = 8;
+    pl.group_rows = (ceil_div(rows, ceil_div(rows, cap)) + 15) & ~15u;
+    pl.nb = ceil_div(pl.group_rows, 128);
+    pl.n_groups = ceil_div(rows, pl.group_rows);
+    const uint32_t full = (uint32_t)std::max<uint64_t>(1, n_cu / ((uint64_t)pl.n_groups * c.n_kv_heads));
+    for (uint32_t part = 1; part <= 8; part *= 2) {
+      const uint32_t want = std::max(1u, std::min({override_splits ? override_splits : std::max(1u, full / part), tiles, most_splits}));
+      pl.split_tiles = ceil_div(tiles, want);
+      pl.n_splits = ceil_div(tiles, pl.split_tiles);
+      const double us = tree_us(c, n_cu, rows, tiles, pl);
+      if (best_us < 0.0 || us < best_us) { best = pl; best_us = us; }
+      if (override_splits || full / part <= 1) break;
+    }
+  }
+  return best;
 }
 
 // the plan of a call, for the tests: {nb, waves, n_groups, group_rows, n_splits, split_tiles}

@@ -2,6 +2,10 @@
 #pragma once
 #include "pa_internal.h"
 
+// n / d for all n below a bound, as mulhi(n, ceil(2^32 / d)), which is exact while bound x d < 2^32; 0 where it is not, or d is 1
+static inline uint32_t div_magic(uint64_t bound, uint32_t d) { return d > 1 && bound * d < (1ull << 32) ? (uint32_t)(((1ull << 32) + d - 1) / d) : 0u; }
+static __device__ inline uint32_t div_by(uint32_t n, uint32_t d, uint32_t magic) { return magic ? __umulhi(n, magic) : d == 1 ? n : n / d; }
+
 // ---- attention of a tree of drafted tokens (attn_tree.hip) ----
 struct TreeParams {
   const float* q; const float* gate;            // f32 [n_cols][stride], heads of head_dim
@@ -17,7 +21,7 @@ struct TreeParams {
   uint32_t n_groups, group_rows;                // groups of stacked rows of a kv head (row = column x G + head), rows of each
   int out_f16;
   float scale;                                  // 1 / sqrt(hd)
-  uint32_t ng_magic, ns_magic, g_magic, rows_magic; // ceil(2^32 / d) of n_groups, n_splits, group and n_cols x group, 0 for one (set by the launchers)
+  uint32_t ng_magic, ns_magic, g_magic, rows_magic; // div_magic of n_groups, n_splits, group and n_cols x group (set by the launchers)
 };
 // what a call runs as: rows a wave holds (16 nb), waves of a workgroup, groups of rows, splits
 struct TreePlan { uint32_t nb, waves, n_groups, group_rows, n_splits, split_tiles; };
@@ -38,6 +42,7 @@ struct GlueAtParams {
   uint32_t n_heads, n_kv_heads, head_dim, n_rot;
   uint32_t base_row, n_cols, flags;
   float eps;
+  uint32_t n_axes, per_col_magic;               // per_col_magic: set by the launcher
   uint32_t axis_of_pair[8];                     // two bits a pair, sixteen pairs a word
 };
 hipError_t pa_launch_glue_at(const GlueAtParams& p, hipStream_t s);
