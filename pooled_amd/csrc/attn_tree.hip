@@ -104,7 +104,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   const uint32_t g = div_by(gs, p.n_splits, p.ns_magic), sp = gs - g * p.n_splits;
   const uint32_t tid = threadIdx.x, lane = tid & 63, ln = lane & 15, kg = lane >> 4;
   const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const uint32_t G = p.group, nH = p.n_heads;
+  const uint32_t G = p.group;
   auto col_of = [&](uint32_t x) __attribute__((always_inline)) -> uint32_t { return div_by(x, G, p.g_magic); };
   const uint32_t x0 = grp * p.group_rows, R = min(p.group_rows, p.n_cols * G - x0);     // the group's stacked rows [x0, x0 + R)
   const uint32_t end = p.base_pos + p.n_cols;
