@@ -190,6 +190,39 @@ static napi_value AttnGather(napi_env env, napi_callback_info info) {
   if (rc) return throw_pa(env, c, rc, "pa_attn_decode_gather");
   return undefined(env);
 }
+// setRopeAxes(ctx, nAxes, Uint8Array of nRot / 2 axes | null)
+static napi_value SetRopeAxes(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); uint32_t n = a.u32(1); size_t bytes = 0; const void* h = nullptr;
+  napi_valuetype t = napi_undefined;
+  if (a.argc > 2) napi_typeof(env, a.argv[2], &t);
+  if (t != napi_null && t != napi_undefined) h = a.host(2, &bytes);
+  CHECK_ARGS("setRopeAxes");
+  uint8_t axis[128];                            // at most 128 pairs; those that the array does not have are of no axis, and refused
+  memset(axis, 255, sizeof axis);
+  if (h) memcpy(axis, h, bytes < sizeof axis ? bytes : sizeof axis);
+  int rc = pa_set_rope_axes(c, n, h ? axis : nullptr); if (rc) return throw_pa(env, c, rc, "pa_set_rope_axes"); return undefined(env);
+}
+// glueKvAt(ctx, layer, dQ, qStride, dK, kStride, dV, vStride, dQw, dKw, dPos, posStride, baseRow, nCols)
+static napi_value GlueKvAt(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0);
+  uint32_t layer = a.u32(1); const float* q = (const float*)a.ptr(2); uint32_t qs = a.u32(3); const float* k = (const float*)a.ptr(4); uint32_t ks = a.u32(5);
+  const float* v = (const float*)a.ptr(6); uint32_t vs = a.u32(7); const float* qw = (const float*)a.ptr(8); const float* kw = (const float*)a.ptr(9);
+  const uint32_t* pos = (const uint32_t*)a.ptr(10); uint32_t ps = a.u32(11), base = a.u32(12), n = a.u32(13); CHECK_ARGS("glueKvAt");
+  int rc = pa_glue_kv_at(c, layer, q, qs, k, ks, v, vs, qw, kw, pos, ps, base, n); if (rc) return throw_pa(env, c, rc, "pa_glue_kv_at"); return undefined(env);
+}
+// attnTree(ctx, layer, q|null, qStride, gate|null, gateStride, mask, maskStride, basePos, nCols, out, outStride, outDtype)
+static napi_value AttnTree(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0);
+  uint32_t layer = a.u32(1); const float* q = (const float*)a.ptr(2); uint32_t qs = a.u32(3);
+  const float* g = (const float*)a.ptr(4); uint32_t gs = a.u32(5); const uint32_t* mask = (const uint32_t*)a.ptr(6);
+  uint32_t ms = a.u32(7), base = a.u32(8), n = a.u32(9); void* out = a.ptr(10); uint32_t os = a.u32(11); int dt = (int)a.u32(12); CHECK_ARGS("attnTree");
+  int rc = pa_attn_tree(c, layer, q, qs, g, gs, mask, ms, base, n, out, os, dt); if (rc) return throw_pa(env, c, rc, "pa_attn_tree"); return undefined(env);
+}
+// kvCompact(ctx, dstRow, sel, maxRows)
+static napi_value KvCompact(napi_env env, napi_callback_info info) {
+  ARGS; pa_ctx* c = a.ctx(0); uint32_t dst = a.u32(1); const uint32_t* sel = (const uint32_t*)a.ptr(2); uint32_t mr = a.u32(3); CHECK_ARGS("kvCompact");
+  int rc = pa_kv_compact(c, dst, sel, mr); if (rc) return throw_pa(env, c, rc, "pa_kv_compact"); return undefined(env);
+}
 // planQuery(ctx, kind, basePos, nCols) -> {kernel, splitLen, nSplits, colGroups, colsPerGroup, waves, rowBlocks, slots}
 static napi_value PlanQuery(napi_env env, napi_callback_info info) {
   ARGS; pa_ctx* c = a.ctx(0); int kind = (int)a.u32(1); uint32_t base = a.u32(2), n = a.u32(3); CHECK_ARGS("planQuery");
@@ -400,6 +433,7 @@ static napi_value Init(napi_env env, napi_value exports) {
     {"rmsnormF16", RmsnormF16}, {"gemm", Gemm}, {"attnLayerPrefill", AttnLayerPrefill},
     {"deltaCreate", DeltaCreate}, {"deltaDestroy", DeltaDestroy}, {"deltaReset", DeltaReset}, {"deltaRead", DeltaRead}, {"deltaWrite", DeltaWrite},
     {"deltaStateBytes", DeltaStateBytes}, {"deltaStatePtr", DeltaStatePtr}, {"deltaGlue", DeltaGlue}, {"deltaDecode", DeltaDecode},
+    {"setRopeAxes", SetRopeAxes}, {"glueKvAt", GlueKvAt}, {"attnTree", AttnTree}, {"kvCompact", KvCompact},
     {"deltaPrefill", DeltaPrefill}, {"moeCreate", MoeCreate}, {"moeDestroy", MoeDestroy}, {"moeLayer", MoeLayer},
   };
   for (auto& t : table) {

@@ -15,6 +15,8 @@
 // The other two blocks of a hybrid model's layers are here as well: initDelta / encodeDelta, the gated delta rule with its
 // short convolution (engine/qwen35.js records it where a layer has no attention), and upMoe / encodeMoe, the experts.
 //
+// Draft trees, which the engines do not have, are draftTree / encodeLayerTree / acceptTree; keepRows cuts the caches to a list of rows.
+//
 // There is no CPU path here: if the addon is missing, require() throws.
 "use strict";
 const path = require("path");
@@ -73,6 +75,7 @@ class HipAttention {
     if (!this.ctx) return;
     for (const k of Object.keys(this.B)) addon.free(this.ctx, this.B[k].ptr);
     for (const L of this.layers) { if (L.qNorm) addon.free(this.ctx, L.qNorm); if (L.kNorm) addon.free(this.ctx, L.kNorm); if (L.attnNorm) addon.free(this.ctx, L.attnNorm); }
+    if (this._tree) for (const k of ["pos", "mask", "sel"]) addon.free(this.ctx, this._tree[k]);
     for (const w of this._weights || []) addon.weightDestroy(this.ctx, w);
     for (const m of this._moes || []) addon.moeDestroy(this.ctx, m);
     if (this.delta) {
@@ -275,6 +278,65 @@ class HipAttention {
   _encAttnQsa(p, LB, sel, selStride, maxRows, nCols) {
     const gate = this.gate ? addon.gateBuffer(this.ctx) : null;
     addon.attnGather(this.ctx, LB.layer, null, 0, gate, this.dims.qDim, sel, selStride, maxRows, nCols, this.B.attnOut.ptr, this._outStride(), this.outDtype);
+  }
+
+  // ---- draft trees: several continuations of one context verified in one pass ----
+  // Rotary positions of several axes (prompts with images or video): the axis of each of the nRot / 2 rotated pairs; null: one axis, the default.
+  setRopeAxes(axisOfPair) {
+    const half = this.dims.nRot / 2;
+    if (axisOfPair && (axisOfPair.length !== half || !Array.from(axisOfPair).every((a) => Number.isInteger(a) && a >= 0 && a < 4))) throw new Error("setRopeAxes: expected " + half + " axes, each 0 .. 3");
+    this._axes = axisOfPair ? Math.max.apply(null, Array.from(axisOfPair)) + 1 : 1;
+    addon.setRopeAxes(this.ctx, this._axes, axisOfPair ? Uint8Array.from(axisOfPair) : null);
+  }
+  _treeBuffers() {
+    if (!this._tree) {
+      const t = { stride: Math.ceil(this.NC / 32), n: 0 };
+      t.pos = addon.malloc(this.ctx, 4 * this.NC * 4); t.mask = addon.malloc(this.ctx, this.NC * t.stride * 4); t.sel = addon.malloc(this.ctx, (this.maxSeq + 1) * 4);
+      this._tree = t;
+    }
+    return this._tree;
+  }
+  // the tree of the next encodeLayerTree calls: parents[c] is the column before c that c continues, -1 where it continues the context.  Column c goes to cache row basePos + c; its rotary
+  // position is pos0 (default basePos) + its depth, on every axis.
+  draftTree(parents, basePos, pos0) {
+    const n = parents.length, t = this._treeBuffers(), depth = new Uint32Array(n), p0 = pos0 === undefined ? basePos : pos0;
+    if (n === 0 || n > this.NC) throw new Error("draftTree: " + n + " columns, batchCols " + this.NC);
+    const mask = new Uint32Array(n * t.stride), pos = new Uint32Array(4 * this.NC);
+    for (let c = 0; c < n; c++) {
+      const up = parents[c];
+      if (!(Number.isInteger(up) && up >= -1 && up < c)) throw new Error("draftTree: a column's parent comes before it");
+      if (up >= 0) { depth[c] = depth[up] + 1; for (let w = 0; w < t.stride; w++) mask[c * t.stride + w] = mask[up * t.stride + w]; }
+      mask[c * t.stride + (c >> 5)] |= 1 << (c & 31);
+      for (let a = 0; a < 4; a++) pos[a * this.NC + c] = p0 + depth[c];
+    }
+    addon.upload(this.ctx, t.mask, mask);
+    addon.upload(this.ctx, t.pos, pos);
+    t.n = n; t.base = basePos; t.parents = Array.from(parents);
+  }
+  // layer i over the tree's columns: B.qFull, B.k, B.v -> the cache's rows behind the context, B.attnOut
+  encodeLayerTree(p, i) {
+    const B = this.B, t = this._tree, w = this._norms(this.layers[i]);
+    if (!t || !t.n) throw new Error("encodeLayerTree: no tree (draftTree)");
+    addon.glueKvAt(this.ctx, i, B.qFull.ptr, this._strideF(B.qFull), B.k.ptr, this._strideF(B.k), B.v.ptr, this._strideF(B.v), w[0], w[1], t.pos, this.NC, t.base, t.n);
+    addon.attnTree(this.ctx, i, null, 0, this.gate ? addon.gateBuffer(this.ctx) : null, this.dims.qDim, t.mask, t.stride, t.base, t.n, B.attnOut.ptr, this._outStride(), this.outDtype);
+  }
+  // the path from a root to column c stays, in every layer's cache, as rows basePos, basePos + 1, ...; returns its columns (c = -1: none).  The next token goes behind them.
+  acceptTree(c) {
+    const t = this._tree, path = [];
+    if (!t || !t.n || !(Number.isInteger(c) && c >= -1 && c < t.n)) throw new Error("acceptTree: no such column");
+    for (let x = c; x >= 0; x = t.parents[x]) path.unshift(x);
+    if (path.length) this.keepRows(t.base, path.map((x) => t.base + x));
+    t.n = 0;
+    return path;
+  }
+  // rows dstRow + i of every layer's caches become the rows of the list, which ascends from dstRow on: a context cut to the rows worth keeping
+  keepRows(dstRow, rows) {
+    if (!rows.length) return;
+    for (let i = 0; i < rows.length; i++)
+      if (!(Number.isInteger(rows[i]) && rows[i] >= (i ? rows[i - 1] + 1 : dstRow) && rows[i] < this.maxSeq)) throw new Error("keepRows: the list ascends from dstRow on, within the cache");
+    const t = this._treeBuffers();
+    addon.upload(this.ctx, t.sel, Uint32Array.from([rows.length].concat(Array.from(rows))));
+    addon.kvCompact(this.ctx, dstRow, t.sel, rows.length);
   }
 
   // ---- gated-delta-rule layers ----
