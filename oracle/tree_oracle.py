@@ -11,10 +11,10 @@ from oracle import attn_oracle as O
 
 
 def tree_attention(q, k, v, base, seen, gate=None):
-    """q [n, nH, hd]; k, v numbers [>= base + n, nKV, hd]; seen bool [n, n] -> (out [n, nH, hd] f64, absolute [n, nH, hd]: sum p |v|, reach [n, nH]: the largest sum |q_i k_i| / sqrt(hd) of a seen row)."""
+    """q [n, nH, hd]; seen bool [n, m] of m drafted rows (n of their columns, or all); k, v numbers [>= base + m, nKV, hd] -> (out [n, nH, hd] f64, absolute [n, nH, hd]: sum p |v|, reach [n, nH]: the largest sum |q_i k_i| / sqrt(hd) of a seen row)."""
     q = np.asarray(q, np.float64)
     n, nH, hd = q.shape
-    T, nKV = base + n, k.shape[1]
+    T, nKV = base + np.shape(seen)[1], k.shape[1]
     k, v = np.asarray(k[:T], np.float64), np.asarray(v[:T], np.float64)
     full = np.concatenate([np.ones((n, base), bool), np.asarray(seen, bool)], 1)
     out, absolute, reach = np.zeros((n, nH, hd)), np.zeros((n, nH, hd)), np.zeros((n, nH))
