@@ -5,7 +5,7 @@
 //             stored.  Workgroups share nothing.  For the accepted path of a draft (one round), and where there is no memory for flags.
 //   segments  a workgroup has 64 KB of a plane's list: it reads its rows into registers, says so in a flag, waits for the flags of the plane's earlier segments and stores.
 //             A segment reads without waiting for anybody and waits only for workgroups of a lower number, which are dispatched before it, so every wait ends; and they
-//             have mostly read when it has.  Whole lines in and out, all CUs busy.
+//             have mostly read when it has.  Whole lines in and out, all CUs busy.  Flags are zero between calls: the plane's last workgroup through its wait clears them.
 // Bound by HBM (two transfers of each row that moves) or, for a few rows, by one launch.
 #include "tree_internal.h"
 
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void pa_compact_walk_kernel(CompactParams p) {
   }
 }
 
-// workgroups: (segment, tensor, plane) of the values, the segment slowest, then those of the scales; flags in the same order
+// workgroups: (segment, tensor, plane) of the values, the segment slowest, then those of the scales; flags in the same order, and behind them how many of a plane are through
 __global__ __launch_bounds__(256) void pa_compact_segment_kernel(CompactParams p, uint32_t value_segs) {
   const uint32_t planes = 2 * p.n_layers * p.n_planes;
   const uint32_t scales = blockIdx.x >= planes * value_segs, wg = scales ? blockIdx.x - planes * value_segs : blockIdx.x;
@@ -72,6 +72,16 @@ __global__ __launch_bounds__(256) void pa_compact_segment_kernel(CompactParams p
   for (uint32_t k = threadIdx.x; k < seg; k += 256)
     while (!__hip_atomic_load(flags + (size_t)k * planes, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT)) __builtin_amdgcn_s_sleep(1);
   __syncthreads();
+  if (threadIdx.x < 64) {
+    const uint32_t live = (n + rows - 1) / rows;
+    uint32_t* through = p.flags + gridDim.x + scales * planes + pl;
+    uint32_t before = 0;
+    if (threadIdx.x == 0) before = __hip_atomic_fetch_add(through, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (__builtin_amdgcn_readfirstlane(before) == live - 1) {
+      for (uint32_t k = threadIdx.x; k < live; k += 64) __hip_atomic_store(flags + (size_t)k * planes, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      if (threadIdx.x == 0) __hip_atomic_store(through, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+  }
 #pragma unroll
   for (int k = 0; k < CT_SEG; k++) {
     const uint32_t i = i0 + k * step + r0;
@@ -79,14 +89,10 @@ __global__ __launch_bounds__(256) void pa_compact_segment_kernel(CompactParams p
   }
 }
 
-__global__ __launch_bounds__(256) void pa_compact_clear_kernel(uint32_t* flags, uint32_t n) {
-  const uint32_t i = blockIdx.x * 256 + threadIdx.x;
-  if (i < n) flags[i] = 0;
-}
-
 static uint32_t segments(const CompactParams& p, uint32_t row_bytes) { return row_bytes ? (uint32_t)(((uint64_t)p.max_rows * row_bytes + 256 * CT_SEG * 16 - 1) / (256 * CT_SEG * 16)) : 0; }
 bool pa_compact_one_round(const CompactParams& p) { return p.max_rows <= 32 * CT_ROUND; }
-size_t pa_compact_flags(const CompactParams& p) { return (size_t)2 * p.n_layers * p.n_planes * ((size_t)segments(p, p.row_bytes) + segments(p, p.scale_bytes)); }
+static size_t segment_wgs(const CompactParams& p) { return (size_t)2 * p.n_layers * p.n_planes * ((size_t)segments(p, p.row_bytes) + segments(p, p.scale_bytes)); }
+size_t pa_compact_flags(const CompactParams& p) { return segment_wgs(p) + (size_t)4 * p.n_layers * p.n_planes; }
 
 hipError_t pa_launch_compact(const CompactParams& p, hipStream_t s) {
   auto power = [](uint32_t b) { return b % 16 == 0 && (b & (b - 1)) == 0; };
@@ -94,12 +100,9 @@ hipError_t pa_launch_compact(const CompactParams& p, hipStream_t s) {
       !p.max_rows || (uint64_t)p.dst_row + p.max_rows > p.max_seq) return hipErrorInvalidValue;
   const uint64_t planes = 2ull * p.n_layers * p.n_planes;
   const bool walk = pa_compact_one_round(p) || !p.flags;
-  const uint64_t wgs = walk ? planes * (p.row_bytes / 128 + (p.scale_bytes ? 1 : 0)) : pa_compact_flags(p);
+  const uint64_t wgs = walk ? planes * (p.row_bytes / 128 + (p.scale_bytes ? 1 : 0)) : segment_wgs(p);
   if (wgs > 0x7fffff00ull) return hipErrorInvalidValue;
   if (walk) hipLaunchKernelGGL(pa_compact_walk_kernel, dim3((unsigned)wgs), dim3(256), 0, s, p);
-  else {
-    hipLaunchKernelGGL(pa_compact_clear_kernel, dim3((unsigned)((wgs + 255) / 256)), dim3(256), 0, s, p.flags, (uint32_t)wgs);
-    hipLaunchKernelGGL(pa_compact_segment_kernel, dim3((unsigned)wgs), dim3(256), 0, s, p, segments(p, p.row_bytes));
-  }
+  else hipLaunchKernelGGL(pa_compact_segment_kernel, dim3((unsigned)wgs), dim3(256), 0, s, p, segments(p, p.row_bytes));
   return hipGetLastError();
 }

@@ -198,8 +198,12 @@ extern "C" int pa_kv_compact(pa_ctx* ctx, uint32_t dst_row, const uint32_t* d_se
       hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
       hipError_t e = hipStreamIsCapturing(ctx->stream, &st);
       if (e != hipSuccess) return block_fail_hip(ctx, e, who);
-      const int rc = st == hipStreamCaptureStatusNone ? pa_ctx_grow(ctx, (void**)&ctx->compact_flags, &ctx->compact_flags_bytes, need) : PA_OK;
-      if (rc) return rc;
+      if (st == hipStreamCaptureStatusNone) {
+        const int rc = pa_ctx_grow(ctx, (void**)&ctx->compact_flags, &ctx->compact_flags_bytes, need);
+        if (rc) return rc;
+        // (zero from here on: a call leaves them as it found them)
+        if ((e = hipMemsetAsync(ctx->compact_flags, 0, ctx->compact_flags_bytes, ctx->stream)) != hipSuccess) { ctx->compact_flags_bytes = 0; return block_fail_hip(ctx, e, who); }
+      }
     }
     p.flags = need <= ctx->compact_flags_bytes ? ctx->compact_flags : nullptr;
   }

@@ -52,7 +52,7 @@ hipError_t pa_launch_glue_at(const GlueAtParams& p, hipStream_t s);
 struct CompactParams {
   void* t[4 * PA_COMPACT_LAYERS];               // a layer's K, V (and their scales): [planes][head_rows][row_bytes or scale_bytes]
   const uint32_t* sel;                          // n, then n rows, ascending
-  uint32_t* flags;                              // a word for each segment, zero; nullptr: none
+  uint32_t* flags;                              // pa_compact_flags words, zero before and after a call; nullptr: none
   uint32_t n_layers, n_planes, head_rows;
   uint32_t row_bytes, scale_bytes;              // scale_bytes 0: f16 caches
   uint32_t dst_row, max_rows, max_seq;

@@ -395,3 +395,35 @@ def test_two_blocks_of_rows_a_wave_without_splits(heads, hd, q8):
     with c.context() as pa:
         c.fill(pa)
         check_some(c, pa.run_attn_tree(0, c.q, c.seen, base), "%d / 1 of %d, one split" % (heads, hd))
+
+
+@pytest.mark.parametrize("q8", [False, True])
+def test_long_lists_one_behind_the_other_and_from_a_graph(q8):
+    """Lists of segments that wait for one another: several lengths and limits in turn, eagerly and replayed, each as if it were the first call."""
+    cfg, seq = dict(SHAPES["qwen36_moe"], kv_q8=q8), 6000
+    c = Case(cfg, seq - 1, 1, seed=8, more=0)
+    G = Graph()
+    with PooledAttn(cfg, seq, n_layers=1, max_cols=1) as pa:
+        pa._chk(pa.L.pa_set_stream(pa.ctx, G.stream))
+        pa.layer_alloc(0)
+        calls = []
+        for dst, n, limit in ((0, 3000, 6000), (7, 300, 400), (100, 2900, 2900), (3, 0, 5000), (1, 5000, 5999), (0, 257, 257)):
+            rows = np.sort(c.rng.choice(seq - dst, n, replace=False)) + dst
+            calls.append((dst, rows, limit, pa.to_device(np.concatenate([[n], rows]).astype(np.uint32))))
+
+        def once(run, dst, rows):
+            for t, part in enumerate(c.parts):
+                pa.kv_write(0, t, 0, part)
+            run()
+            pa.sync()
+            for t, part in enumerate(c.parts):
+                assert pa.kv_read(0, t, 0, seq).tobytes() == T.compact(part, dst, rows).tobytes(), (dst, len(rows), t)
+        for dst, rows, limit, sel in calls + calls[::-1]:
+            once(lambda: pa.kv_compact(dst, sel, limit), dst, rows)
+        recorded = [(G.record(lambda: pa.kv_compact(dst, sel, limit)), dst, rows) for dst, rows, limit, sel in calls]
+        for rep in range(3):
+            for graph, dst, rows in recorded:
+                once(lambda: G.run(graph), dst, rows)
+            dst, rows, limit, sel = calls[rep]
+            once(lambda: pa.kv_compact(dst, sel, limit), dst, rows)
+    G.close()
