@@ -224,8 +224,8 @@ int pa_attn_decode_gather(pa_ctx* ctx, uint32_t layer, const float* d_q, uint32_
  *   d_mask: u32 [n_cols][mask_stride]; bit j % 32 of word j / 32 of a column's words: it sees row base_pos + j (a node's own bit and its ancestors').  Any pattern; bits
  *           from n_cols on are not looked at; a column that sees nothing (base_pos 0, no bit) gives zeros.  A drafted row with infinities or NaN reaches those columns alone that see it.
  *   d_q, d_gate, d_out: as in pa_attn_decode, but the output shares no memory with the inputs (refused).
- * Operands (q, P, int8 rows' values) are f16, products, sums and softmax f32, as in pa_attn_decode; partials of a split context are kept in f16.  Results do not depend on the
- * mask rows of other columns; they agree with pa_attn_decode's on a chain to rounding.  pa_set_decode_splits applies.  Partials share the context's scratch: a call that grows it
+ * Operands (q, P, int8 rows' values) are f16, products, sums and softmax f32, as in pa_attn_decode; partials of a split context are kept in f16.  Other columns' masks
+ * change a column's results in their rounding at most; on a chain they agree with pa_attn_decode's to rounding; the same call gives the same bits.  pa_set_decode_splits applies.  Partials share the context's scratch: a call that grows it
  * allocates; under stream capture, where it cannot, the context is split into as many parts as there is room for. */
 int pa_attn_tree(pa_ctx* ctx, uint32_t layer, const float* d_q, uint32_t q_stride, const float* d_gate, uint32_t gate_stride, const uint32_t* d_mask,
                  uint32_t mask_stride, uint32_t base_pos, uint32_t n_cols, void* d_out, uint32_t out_stride, int out_dtype);
@@ -256,7 +256,8 @@ size_t pa_kv_row_bytes(const pa_ctx* ctx, int which);
  * the end of the context, or a context cut to the rows worth keeping.  The other rows stay as they are.  No counterpart in the reference, whose caches are cut back to a prefix.
  *   d_sel: u32: the list's length n, then n cache rows, ascending, each once, the first at or behind dst_row (pa_attn_decode_gather's list).  It is on the device, so a draft may be accepted
  *          there, and is not trusted: n > max_rows is read as max_rows, rows are clamped to the cache; a list in another order leaves unspecified rows of its own at dst_row .. dst_row + n - 1.
- *   max_rows: the longest list; dst_row + max_rows <= max_seq. */
+ *   max_rows: the longest list; dst_row + max_rows <= max_seq.  Above 256 a call needs a word of scratch for every 64 KB of a cache's rows, which it allocates at its first use; under stream
+ *           capture, where it cannot, the list is gone through in order without (slower by up to 3; one eager call with the same max_rows before the capture is enough). */
 int pa_kv_compact(pa_ctx* ctx, uint32_t dst_row, const uint32_t* d_sel, uint32_t max_rows);
 /* device address of a cache (read-only use; the head-major device layout described at pa_layer_alloc) */
 const void* pa_kv_device_ptr(pa_ctx* ctx, uint32_t layer, int which);

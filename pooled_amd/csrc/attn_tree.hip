@@ -4,8 +4,9 @@
 //   o[c, h] = sum_t softmax_t(q[c, h] . k[t] / sqrt(hd)) v[t]
 // The G query heads of a kv head and all columns are stacked rows (row = column x G + head), so K and V are read once for all of them.
 //
-//   * A workgroup is W wavefronts of 16 NB stacked rows each over one split of the context; every 32-row tile of K and V that it stages in LDS serves
-//     all of its waves.  Tiles go global -> LDS directly, D - 1 of them in flight (int8 rows: through registers, widened on the way); one barrier a tile.
+//   * A workgroup is eight wavefronts, two a SIMD (one a SIMD gets half of what the LDS delivers: four waves of up to three blocks took 174 us where this takes 92), over one split of
+//     the context and up to 256 stacked rows in blocks of 16, block b with wave b % 8; every 32-row tile of K and V that it stages in LDS serves all of them.  Tiles go global -> LDS
+//     directly, three of them in flight in a ring of four; one barrier a tile.  Int8 rows go through registers, two tiles ahead, and are widened on the way to a ring of two.
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: Q fragments stay in registers, K fragments are 16-byte LDS reads, V^T fragments come from the
 //     LDS transpose read.  The accumulator of S^T is the operand of P V, so probabilities never leave registers.
 //   * Online softmax in f32 in the exp2 domain: the reference of a row is raised, and O and l rescaled, only where a P comes out above 2^8 (exact enough in f16); l is
@@ -15,6 +16,11 @@
 //     zeros and are added to the outputs of the columns that see them.
 //   * Splits leave (m, l) and O / l in f16: a convex combination of f16 values loses 2^-12 of itself by that (mean of a rounding of at most 2^-11), below what the f16 P
 //     lose, and the partials are half the bytes; pa_tree_merge_kernel joins them.
+//
+// Measured (24 query and 4 key heads of 256, 65536 rows of f16, 268 MB): 16 columns 52 us = 5.1 TB/s, which is what a large copy reaches; 48 columns 92 us = 840 TFLOP/s (a large matrix
+// product: 1330), and 3 % less with every tile read from the L2, so there the SIMDs' work bounds it: a tile of nine blocks, three of them on one SIMD, takes 1.3 us, of which the matrix
+// instructions are 0.7 at the 2.1 GHz that the part holds.  The merge adds 9 us there (19 MB of partials), 3 - 4 for small drafts, most of it the launch.  Int8: 17 columns at 20003 rows
+// 21.5 us and 6.5: the widening through registers, 1.1 us a tile of seven blocks.  5 columns at 190 rows, 16 and 8 heads of 128: 4.7 us and 3.1, two launches and a trip to memory each.
 #include "tree_internal.h"
 #include "pf_common.h"
 #include "tree_mask.h"

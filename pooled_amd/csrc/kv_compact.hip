@@ -6,7 +6,9 @@
 //   segments  a workgroup has 64 KB of a plane's list: it reads its rows into registers, says so in a flag, waits for the flags of the plane's earlier segments and stores.
 //             A segment reads without waiting for anybody and waits only for workgroups of a lower number, which are dispatched before it, so every wait ends; and they
 //             have mostly read when it has.  Whole lines in and out, all CUs busy.  Flags are zero between calls: the plane's last workgroup through its wait clears them.
-// Bound by HBM (two transfers of each row that moves) or, for a few rows, by one launch.
+// Bound by HBM (two transfers of each row that moves) or, for a few rows, by one launch.  8000 of 16003 rows of six layers of 8 heads of 128 (394 MB read and written): 77 us = 5.1 TB/s,
+// the rate of a large copy; 10001 of 30011 int8 rows of three layers of 4 heads of 256 (138 MB): 38 us, where the scales' 32 bytes a row cost whole lines of 128 (23 MB read for 8).  Five
+// rows in ten layers: 2.9 us.
 #include "tree_internal.h"
 
 typedef unsigned int u4 __attribute__((ext_vector_type(4)));
