@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 from oracle import attn_oracle as O
 from oracle import tree_oracle as T
-from pooled_amd.capi import PooledAttn, PA_OUT_F32, tree_mask, tree_of_parents
+from pooled_amd.capi import PooledAttn, PA_ERR_INVALID, tree_mask, tree_of_parents
 from helpers import SHAPES
 from test_gpu_graph import _hip, _ok
 from test_gpu_tree import Case, random_tree
@@ -427,3 +427,18 @@ def test_long_lists_one_behind_the_other_and_from_a_graph(q8):
             dst, rows, limit, sel = calls[rep]
             once(lambda: pa.kv_compact(dst, sel, limit), dst, rows)
     G.close()
+
+
+def test_inputs_in_the_buffers_that_the_pre_step_writes():
+    cfg, n = SHAPES["qwen36_moe"], 4
+    d = O.make_inputs(cfg, 0, n, 1)
+    with PooledAttn(cfg, 64, n_layers=1, max_cols=n) as pa:
+        pa.layer_alloc(0)
+        w, (q, k, v) = [pa.to_device(d["qw"]), pa.to_device(d["kw"])], (pa.to_device(d[x]) for x in ("qraw", "kraw", "vraw"))
+        p = pa.to_device(np.arange(n, dtype=np.uint32))
+        for buf in (pa.q_buffer_ptr(), pa.gate_buffer_ptr()):
+            for at in range(4):
+                ptrs = [q.ptr, k.ptr, v.ptr, p.ptr]
+                ptrs[at] = buf + 64
+                rc = pa.L.pa_glue_kv_at(pa.ctx, 0, ptrs[0], d["qraw"].shape[1], ptrs[1], d["kraw"].shape[1], ptrs[2], d["vraw"].shape[1], w[0].ptr, w[1].ptr, ptrs[3], n, 0, n)
+                assert rc == PA_ERR_INVALID
