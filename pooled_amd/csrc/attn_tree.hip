@@ -19,7 +19,7 @@
 //
 // Measured (24 query and 4 key heads of 256, 65536 rows of f16, 268 MB): 16 columns 52 us = 5.1 TB/s, which is what a large copy reaches; 48 columns 92 us = 840 TFLOP/s (a large matrix
 // product: 1330), and 3 % less with every tile read from the L2, so there the SIMDs' work bounds it: a tile of nine blocks, three of them on one SIMD, takes 1.3 us, of which the matrix
-// instructions are 0.7 at the 2.1 GHz that the part holds.  The merge adds 9 us there (19 MB of partials), 3 - 4 for small drafts, most of it the launch.  Int8: 17 columns at 20003 rows
+// instructions are 0.7 at the 2.1 GHz that the part holds.  The merge adds 7 us there (19 MB of partials), 3 - 4 for small drafts, most of it the launch.  Int8: 17 columns at 20003 rows
 // 21.5 us and 6.5: the widening through registers, 1.1 us a tile of seven blocks.  5 columns at 190 rows, 16 and 8 heads of 128: 4.7 us and 3.1, two launches and a trip to memory each.
 #include "tree_internal.h"
 #include "pf_common.h"
@@ -641,13 +641,15 @@ hipError_t pa_launch_tree(const TreeParams& p, const TreePlan& pl, uint32_t hd, 
   return hipErrorInvalidValue;
 }
 
-// few splits: whole rows a wave, many: narrow slices, so that all of a row's splits are one round trip
+// few splits: whole rows a wave, many: narrow slices, so that all of a row's splits are one round trip, with no more lanes than they need (1152 rows of 256, 32 splits: 7.0 us with 16 lanes a
+// slice, 8.8 with 8)
 template <int HD>
 static void launch_merge(const TreeParams& p, hipStream_t s, const PaTiming* t) {
   constexpr uint32_t LPR = HD / 8;
   const uint32_t rows = p.n_cols * p.n_heads;
   auto grid = [&](uint32_t lpg) { return dim3((unsigned)(((uint64_t)rows * (LPR / lpg) + 3) / 4)); };
   if (p.n_splits <= 64 / LPR * 8) PA_LAUNCH((pa_tree_merge_kernel<HD, LPR>), grid(LPR), dim3(256), 0, s, t, p);
+  else if (HD == 256 && p.n_splits <= 32) PA_LAUNCH((pa_tree_merge_kernel<256, 16>), grid(16), dim3(256), 0, s, t, p);
   else if (p.n_splits <= 64) PA_LAUNCH((pa_tree_merge_kernel<HD, 8>), grid(8), dim3(256), 0, s, t, p);
   else PA_LAUNCH((pa_tree_merge_kernel<HD, 4>), grid(4), dim3(256), 0, s, t, p);
 }
