@@ -19,7 +19,7 @@
 //
 // Measured (24 query and 4 key heads of 256, 65536 rows of f16, 268 MB): 16 columns 52 us = 5.1 TB/s, which is what a large copy reaches; 48 columns 92 us = 840 TFLOP/s (a large matrix
 // product: 1330), and 3 % less with every tile read from the L2, so there the SIMDs' work bounds it: a tile of nine blocks, three of them on one SIMD, takes 1.3 us, of which the matrix
-// instructions are 0.7 at the 2.1 GHz that the part holds.  The merge adds 7 us there (19 MB of partials), 3 - 4 for small drafts, most of it the launch.  Int8: 17 columns at 20003 rows
+// instructions are 0.8 at the 1.9 GHz that the power limit leaves.  The merge adds 7 us there (19 MB of partials), 3 - 4 for small drafts, most of it the launch.  Int8: 17 columns at 20003 rows
 // 21.5 us and 6.5: the widening through registers, 1.1 us a tile of seven blocks.  5 columns at 190 rows, 16 and 8 heads of 128: 4.7 us and 3.1, two launches and a trip to memory each.
 #include "tree_internal.h"
 #include "pf_common.h"
