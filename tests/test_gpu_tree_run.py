@@ -442,3 +442,29 @@ def test_inputs_in_the_buffers_that_the_pre_step_writes():
                 ptrs[at] = buf + 64
                 rc = pa.L.pa_glue_kv_at(pa.ctx, 0, ptrs[0], d["qraw"].shape[1], ptrs[1], d["kraw"].shape[1], ptrs[2], d["vraw"].shape[1], w[0].ptr, w[1].ptr, ptrs[3], n, 0, n)
                 assert rc == PA_ERR_INVALID
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("gate", [False, True])
+@pytest.mark.parametrize("heads,kv_heads,hd,n_rot", [(5, 5, 128, 128), (6, 3, 128, 64), (7, 1, 128, 96), (3, 1, 256, 64), (9, 3, 256, 256), (1, 1, 256, 16)])
+def test_the_pre_step_of_head_counts_that_fill_no_wave(heads, kv_heads, hd, n_rot, gate, q8):
+    """A wave takes 512 values of heads: the last one of a column may have fewer.  The bits of pa_glue_kv, and nothing beside them written."""
+    cfg = dict(n_heads=heads, n_kv_heads=kv_heads, head_dim=hd, n_rot=n_rot, rope_theta=1e6, eps=1e-6, qk_norm=True, gate=gate, kv_q8=q8)
+    base, n = 11, 13
+    d = O.make_inputs(cfg, 0, n, heads)
+    got = []
+    for at in (False, True):
+        with PooledAttn(cfg, base + n + 3, n_layers=1, max_cols=n + 2) as pa:
+            pa.layer_alloc(0)
+            w, (q, k, v) = [pa.to_device(d["qw"]), pa.to_device(d["kw"])], [pa.to_device(d[x]) for x in ("qraw", "kraw", "vraw")]
+            fill = np.full((n + 2) * pa.q_dim, 7.0, np.float32)
+            for buf in (pa.q_buffer_ptr(), pa.gate_buffer_ptr() if gate else None):
+                if buf:
+                    pa._chk(pa.L.pa_upload(pa.ctx, buf, fill.ctypes.data, fill.nbytes))
+            if at:
+                pa.glue_kv_at(0, q, d["qraw"].shape[1], k, d["kraw"].shape[1], v, d["vraw"].shape[1], *w, pa.to_device((base + np.arange(n)).astype(np.uint32)), n, base, n)
+            else:
+                pa.glue_kv(0, q, d["qraw"].shape[1], k, d["kraw"].shape[1], v, d["vraw"].shape[1], *w, base, n)
+            pa.sync()
+            got.append([pa.read_q_buffer(n + 2).tobytes(), pa.read_gate_buffer(n + 2).tobytes() if gate else b""] + caches(pa, 0, base + n + 3))
+    assert got[0] == got[1]
