@@ -4,8 +4,9 @@
 //   walk      a workgroup has a (tensor, kv head) plane and a slice of its rows' bytes and walks the list in order, each round's rows in registers before one of them is
 //             stored.  Workgroups share nothing.  For the accepted path of a draft (one round), and where there is no memory for flags.
 //   segments  a workgroup has 64 KB of a plane's list: it reads its rows into registers, says so in a flag, waits for the flags of the plane's earlier segments and stores.
-//             A segment reads without waiting for anybody and waits only for workgroups of a lower number, which are dispatched before it, so every wait ends; and they
-//             have mostly read when it has.  Whole lines in and out, all CUs busy.  Flags are zero between calls: the plane's last workgroup through its wait clears them.
+//             A segment reads without waiting for anybody and waits only for segments in front of it in its plane.  Workgroups take segments by ticket, in the order in which they
+//             start, so those in front are with workgroups that run already and every wait ends, whatever else the device runs and in whatever order workgroups start.  Whole
+//             lines in and out, all CUs busy.  Flags and tickets are zero between calls: the plane's last workgroup through its wait clears them.
 // Bound by HBM (two transfers of each row that moves) or, for a few rows, by one launch.  8000 of 16003 rows of six layers of 8 heads of 128 (394 MB read and written): 77 us = 5.1 TB/s,
 // the rate of a large copy; 10001 of 30011 int8 rows of three layers of 4 heads of 256 (138 MB): 38 us, where the scales' 32 bytes a row cost whole lines of 128 (23 MB read for 8).  Five
 // rows in ten layers: 2.9 us.
@@ -48,12 +49,22 @@ __global__ __launch_bounds__(256) void pa_compact_walk_kernel(CompactParams p) {
   }
 }
 
-// workgroups: (segment, tensor, plane) of the values, the segment slowest, then those of the scales; flags in the same order, and behind them how many of a plane are through
+// workgroups: (segment, tensor, plane) of the values, the segment slowest, then those of the scales; flags in the same order, and behind them a line of each plane: tickets taken, and how many
+// are through their waits
+#define CT_LINE 32            // words of a plane's line
 __global__ __launch_bounds__(256) void pa_compact_segment_kernel(CompactParams p, uint32_t value_segs) {
   const uint32_t planes = 2 * p.n_layers * p.n_planes;
-  const uint32_t scales = blockIdx.x >= planes * value_segs, wg = scales ? blockIdx.x - planes * value_segs : blockIdx.x;
-  const uint32_t seg = wg / planes, pl = wg % planes;
+  const uint32_t scales = blockIdx.x >= planes * value_segs, pl = blockIdx.x % planes, segs = scales ? gridDim.x / planes - value_segs : value_segs;
   uint32_t* flags = p.flags + (scales ? planes * value_segs : 0) + pl;       // segment k's: flags[k * planes]
+  uint32_t* line = p.flags + gridDim.x + (scales * planes + pl) * CT_LINE;
+  __shared__ uint32_t ticket;
+  if (threadIdx.x == 0) {
+    const uint32_t t = __hip_atomic_fetch_add(line, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (t == segs - 1) __hip_atomic_store(line, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    ticket = t;
+  }
+  __syncthreads();
+  const uint32_t seg = __builtin_amdgcn_readfirstlane(ticket);
   const CompactPlane c = plane_of(p, pl / p.n_planes, pl % p.n_planes, scales);
   const uint32_t n = min(p.sel[0], p.max_rows), sh = 31 - __clz(c.units), rows = 256 * CT_SEG >> sh, i0 = seg * rows;
   if (i0 >= n) return;
@@ -76,7 +87,7 @@ __global__ __launch_bounds__(256) void pa_compact_segment_kernel(CompactParams p
   __syncthreads();
   if (threadIdx.x < 64) {
     const uint32_t live = (n + rows - 1) / rows;
-    uint32_t* through = p.flags + gridDim.x + scales * planes + pl;
+    uint32_t* through = line + 1;
     uint32_t before = 0;
     if (threadIdx.x == 0) before = __hip_atomic_fetch_add(through, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     if (__builtin_amdgcn_readfirstlane(before) == live - 1) {
@@ -94,7 +105,7 @@ __global__ __launch_bounds__(256) void pa_compact_segment_kernel(CompactParams p
 static uint32_t segments(const CompactParams& p, uint32_t row_bytes) { return row_bytes ? (uint32_t)(((uint64_t)p.max_rows * row_bytes + 256 * CT_SEG * 16 - 1) / (256 * CT_SEG * 16)) : 0; }
 bool pa_compact_one_round(const CompactParams& p) { return p.max_rows <= 32 * CT_ROUND; }
 static size_t segment_wgs(const CompactParams& p) { return (size_t)2 * p.n_layers * p.n_planes * ((size_t)segments(p, p.row_bytes) + segments(p, p.scale_bytes)); }
-size_t pa_compact_flags(const CompactParams& p) { return segment_wgs(p) + (size_t)4 * p.n_layers * p.n_planes; }
+size_t pa_compact_flags(const CompactParams& p) { return segment_wgs(p) + (size_t)4 * p.n_layers * p.n_planes * CT_LINE; }
 
 hipError_t pa_launch_compact(const CompactParams& p, hipStream_t s) {
   auto power = [](uint32_t b) { return b % 16 == 0 && (b & (b - 1)) == 0; };

@@ -468,3 +468,31 @@ def test_the_pre_step_of_head_counts_that_fill_no_wave(heads, kv_heads, hd, n_ro
             pa.sync()
             got.append([pa.read_q_buffer(n + 2).tobytes(), pa.read_gate_buffer(n + 2).tobytes() if gate else b""] + caches(pa, 0, base + n + 3))
     assert got[0] == got[1]
+
+
+def test_two_contexts_cut_long_caches_at_once():
+    """Compactions of more segments than the device runs at a time, of two contexts on two streams, enqueued in turn without a wait between them."""
+    seq, graphs, work = 150000, [Graph(), Graph()], []
+    rng = np.random.default_rng(4)
+    cfgs = [dict(n_heads=h, n_kv_heads=h, head_dim=128, n_rot=128, rope_theta=1e6, eps=1e-6, qk_norm=False, gate=False) for h in (1, 3)]
+    with PooledAttn(cfgs[0], seq, n_layers=1, max_cols=1) as a, PooledAttn(cfgs[1], seq, n_layers=1, max_cols=1) as b:
+        for pa, g in ((a, graphs[0]), (b, graphs[1])):
+            pa._chk(pa.L.pa_set_stream(pa.ctx, g.stream))
+            pa.layer_alloc(0)
+            parts = [rng.integers(0, 1 << 16, (seq, pa.cfg["n_kv_heads"], 128), dtype=np.uint16) for _ in range(2)]
+            for t in range(2):
+                pa.kv_write(0, t, 0, parts[t])
+            lists = [np.sort(rng.choice(n - 5, m, replace=False)) + 5 for n, m in ((seq, 120000), (120000, 100000), (100000, 90000))]
+            work.append((pa, parts, lists, [pa.to_device(np.concatenate([[x.size], x]).astype(np.uint32)) for x in lists]))
+        for i in range(3):
+            for pa, _, lists, sels in work:
+                pa.kv_compact(5, sels[i], lists[i].size)
+        for pa, parts, lists, _ in work:
+            pa.sync()
+            for t in range(2):
+                want = parts[t]
+                for rows in lists:
+                    want = T.compact(want, 5, rows)
+                assert pa.kv_read(0, t, 0, seq).tobytes() == want.tobytes()
+    for g in graphs:
+        g.close()
