@@ -20,7 +20,8 @@
 // Measured (24 query and 4 key heads of 256, 65536 rows of f16, 268 MB): 16 columns 52 us = 5.1 TB/s, which is what a large copy reaches; 48 columns 92 us = 840 TFLOP/s (a large matrix
 // product: 1330), and 3 % less with every tile read from the L2, so there the SIMDs' work bounds it: a tile of nine blocks, three of them on one SIMD, takes 1.3 us, of which the matrix
 // instructions are 0.8 at the 1.9 GHz that the power limit leaves.  The merge adds 7 us there (19 MB of partials), 3 - 4 for small drafts, most of it the launch.  Int8: 17 columns at 20003 rows
-// 21.5 us and 6.5: the widening through registers, 1.1 us a tile of seven blocks.  5 columns at 190 rows, 16 and 8 heads of 128: 4.7 us and 3.1, two launches and a trip to memory each.
+// 21.5 us and 6.5: the widening through registers, 1.1 us a tile of seven blocks.  5 columns at 190 rows, 16 and 8 heads of 128: 7.2 us a call in one launch, 7.8 with
+// seven splits and the merge; at 100 rows 5.9 and 8.3.
 #include "tree_internal.h"
 #include "pf_common.h"
 #include "tree_mask.h"
@@ -72,7 +73,10 @@ static __device__ inline void wait_and_meet_lds() { asm volatile("s_waitcnt lgkm
 // LDS behind the ring: mask words of WIN tiles, and a flag of each wave
 template <int NB> struct TreeLds { static constexpr int WIN = 4 / NB, bytes = WIN * 16 * NB * TREE_W * 4 + TREE_W * 4; };
 
-// eight dims of an output column; with the gate
+// sigmoid; the reciprocal is off by 2^-23 of itself, an exact division is a dozen instructions a value
+static __device__ inline float gate_of(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
+
+// eight dims of an output column
 static __device__ inline void store8(const TreeParams& p, uint32_t col, uint32_t d, const float (&o)[8]) {
   if (p.out_f16) {
     _Float16* out = (_Float16*)p.out + (size_t)col * p.out_stride + d;
@@ -83,15 +87,6 @@ static __device__ inline void store8(const TreeParams& p, uint32_t col, uint32_t
     *(f4*)out = (f4){ o[0], o[1], o[2], o[3] };
     *(f4*)(out + 4) = (f4){ o[4], o[5], o[6], o[7] };
   }
-}
-static __device__ inline void store_row8(const TreeParams& p, uint32_t col, uint32_t d, float (&o)[8]) {
-  if (p.gate) {
-    const float* gate = p.gate + (size_t)col * p.gate_stride + d;
-    const f4 a = *(const f4*)gate, b = *(const f4*)(gate + 4);
-#pragma unroll
-    for (int i = 0; i < 4; i++) { o[i] *= 1.f / (1.f + __expf(-a[i])); o[4 + i] *= 1.f / (1.f + __expf(-b[i])); }
-  }
-  store8(p, col, d, o);
 }
 template <int HD, int NB, bool Q8, int D>
 __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreeParams p) {
@@ -493,6 +488,17 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
       constexpr int EROWS = RING / W / (HD * 4) < 16 ? 8 : 16;              // f32 rows that a wave's part of the ring holds
       static_assert(EROWS * HD * 4 * W <= RING, "the rows fit the ring");
       float* os = (float*)(smem + wave * EROWS * HD * 4);
+      // all of the block's gates ahead (one after the other they are a trip to memory each: 5 columns at 20 rows, 16 / 2 heads of 256, 9.5 us a call, so 8.8, and 7.7 with a reciprocal for the division)
+      f4 gt[16 / RPI][2];
+      if (p.gate) {
+#pragma unroll
+        for (int it = 0; it < 16 / RPI; it++) {
+          const uint32_t x = x0 + min(r0 + it * RPI + lane / (HD / 8), R - 1), col = col_of(x), hq = g * G + x - col * G;
+          const float* gate = p.gate + (size_t)col * p.gate_stride + hq * HD + 8 * c;
+          gt[it][0] = *(const f4*)gate;
+          gt[it][1] = *(const f4*)(gate + 4);
+        }
+      }
 #pragma unroll
       for (int half = 0; half < 16 / EROWS; half++) {
         if (EROWS == 16 || (int)(ln / 8) == half) {
@@ -501,7 +507,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
           for (int db = 0; db < S::DB; db++) *(f4*)(os + r * HD + ((4 * db + kg) ^ r) * 4) = acc[db][nb] * inv;
         }
         wave_fence();
-#pragma unroll 2
+#pragma unroll
         for (int it = 0; it < EROWS / RPI; it++) {
           const uint32_t r = it * RPI + lane / (HD / 8), wr = r0 + half * EROWS + r;
           if (wr >= R) continue;
@@ -509,7 +515,12 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
           float o[8] = { a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3] };
           const uint32_t x = x0 + wr, col = col_of(x), hq = g * G + x - col * G;
           if (__builtin_expect(bad, 0)) add_not_finite(p, HD, col, g, 8 * c, o);
-          store_row8(p, col, hq * HD + 8 * c, o);
+          if (p.gate) {
+            const f4 ga = gt[half * (EROWS / RPI) + it][0], gb = gt[half * (EROWS / RPI) + it][1];
+#pragma unroll
+            for (int i = 0; i < 4; i++) { o[i] *= gate_of(ga[i]); o[4 + i] *= gate_of(gb[i]); }
+          }
+          store8(p, col, hq * HD + 8 * c, o);
         }
         wave_fence();
       }
@@ -591,7 +602,7 @@ __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
   if (__builtin_expect(sign, 0)) add_not_finite(p, HD, col, g, d, o);
   if (p.gate) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] *= 1.f / (1.f + __expf(-gt[i]));
+    for (int i = 0; i < 8; i++) o[i] *= gate_of(gt[i]);
   }
   store8(p, col, h * HD + d, o);
 }

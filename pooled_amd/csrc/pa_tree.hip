@@ -85,12 +85,15 @@ static double tree_us(const pa_config& c, uint32_t n_cu, uint32_t rows, uint32_t
   const double blocks = pl.group_rows / 16.0, wgs = (double)pl.n_groups * c.n_kv_heads * pl.n_splits;
   const double chain = pl.split_tiles * (tile + block * blocks) * std::ceil(wgs / n_cu);
   const double stream = 1e-6 / 7.0 * tiles * 32.0 * c.n_kv_heads * c.head_dim * (q8 ? 2.25 : 4.0);
+  // (a second launch and its trip to memory saved; 168 calls of 1 - 63 columns at 20 - 450 rows: one split is ahead up to some 200 rows of head_dim 128, 130 of 256, 30 - 150 of int8 rows;
+  // 24 columns at 100 rows of 16 / 8 heads of 128 6.2 us against 8.5, at 300 9.2 against 8.7)
+  const double merge = pl.n_splits > 1 ? 0.0 : q8 ? (wide ? 1.3 : 2.6) : wide ? 1.9 : 2.9;
   const double partials = pl.n_splits > 1 ? 1e-6 * rows * c.n_kv_heads * pl.n_splits * c.head_dim * 2.0 : 0.0;
-  return fixed + std::max(chain, stream) + out * blocks + 0.427 * partials;
+  return fixed - merge + std::max(chain, stream) + out * blocks + 0.427 * partials;
 }
 
 // Rows of a workgroup: up to 256, a wave two blocks of 16, or 128, 64 and 32, the groups then sharing the stream through their XCD's L2 (two blocks of int8 rows of head_dim 256 do not fit the
-// registers).  Splits: a workgroup a CU, or fewer, whose partials are less.  most_splits: what a caller that cannot allocate has room for.
+// registers).  Splits: a workgroup a CU, or fewer, whose partials are less, or one, which needs no second launch.  most_splits: what a caller that cannot allocate has room for.
 static TreePlan plan_tree(const pa_config& c, uint32_t n_cu, uint32_t base, uint32_t n_cols, uint32_t override_splits, uint32_t most_splits) {
   const uint32_t rows = n_cols * (c.n_heads / c.n_kv_heads), tiles = ceil_div(base + n_cols, 32);
   const bool narrow = (c.flags & PA_FLAG_KV_Q8) && c.head_dim == 256;
@@ -104,13 +107,13 @@ static TreePlan plan_tree(const pa_config& c, uint32_t n_cu, uint32_t base, uint
     pl.nb = ceil_div(pl.group_rows, 128);
     pl.n_groups = ceil_div(rows, pl.group_rows);
     const uint32_t full = (uint32_t)std::max<uint64_t>(1, n_cu / ((uint64_t)pl.n_groups * c.n_kv_heads));
-    for (uint32_t part = 1; part <= 8; part *= 2) {
+    for (uint32_t part : {1u, 2u, 4u, 8u, full}) {
       const uint32_t want = std::max(1u, std::min({override_splits ? override_splits : std::max(1u, full / part), tiles, most_splits}));
       pl.split_tiles = ceil_div(tiles, want);
       pl.n_splits = ceil_div(tiles, pl.split_tiles);
       const double us = tree_us(c, n_cu, rows, tiles, pl);
       if (best_us < 0.0 || us < best_us) { best = pl; best_us = us; }
-      if (override_splits || full / part <= 1) break;
+      if (override_splits || pl.n_splits == 1) break;
     }
   }
   return best;
