@@ -553,7 +553,9 @@ __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
     for (uint32_t k = 0; k < B; k++) {
       const uint32_t s = s0 + NG * k, at = min(s, ns - 1);
       m[k] = ml[at];
-      v[k] = __builtin_nontemporal_load((const h8*)(po + at * step));
+      u4 o = __builtin_nontemporal_load((const u4*)(po + at * step));
+      o &= s < ns ? 0xffffffffu : 0u;               // (a surplus one is zeros: what is there may be infinite, and 0 x inf is not 0)
+      __builtin_memcpy(&v[k], &o, 16);
       if (s >= ns) m[k] = make_float2(NEG_INF, 0.f);
     }
   };
