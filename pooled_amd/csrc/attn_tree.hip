@@ -13,7 +13,7 @@
 //     the sum of the rounded P, so an output is a convex combination of value rows whatever that rounding did.
 //   * The mask is looked at only in tiles that reach the drafted rows.  There a row's 32 bits are one word, cut out of its mask at the tile's offset with the rows in front
 //     of the draft as ones.  A drafted row that holds what is not finite must reach those columns alone that see it, and 0 x inf is not 0: such elements go into the product as
-//     zeros and are added to the outputs of the columns that see them.
+//     zeros and are added to the outputs of the columns that see them.  Rows of the context, which all columns see, go into it as they are, also those of the draft's first tile.
 //   * Splits leave (m, l) and O / l in f16: a convex combination of f16 values loses 2^-12 of itself by that (mean of a rounding of at most 2^-11), below what the f16 P
 //     lose, and the partials are half the bytes; pa_tree_merge_kernel joins them.
 //
@@ -393,23 +393,25 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
       if (f + VD < S::DB) __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
     }
   };
-  // A tile that reaches the drafted rows: the next mask words where the ones at hand are through; and what is not finite in V becomes zero in LDS (see the head of the file)
+  // A tile that reaches the drafted rows: the next mask words where the ones at hand are through; and what is not finite in V's drafted rows becomes zero in LDS (see the head of the file)
   auto draft_tile = [&](uint32_t i) __attribute__((always_inline)) {
     const uint32_t d = i - draft0;
     if (d && d % WIN == 0) { fill_windows(d); __syncthreads(); }
-    unsigned char* vb = buf(i) + S::TILE + (wave * 64 + lane) * 16;
+    const uint32_t at = (wave * 64 + lane) * 16, context = p.base_pos > (tile0 + i) * 32 ? p.base_pos - (tile0 + i) * 32 : 0;     // the tile's rows in front of the draft
+    unsigned char* vb = buf(i) + S::TILE + at;
     constexpr int NV = S::TILE / (W * 1024);
     bool any = false;
     u4 v[NV];
 #pragma unroll
     for (int j = 0; j < NV; j++) {
       v[j] = *(const u4*)(vb + j * W * 1024);
-      any |= not_finite2(v[j][0]) || not_finite2(v[j][1]) || not_finite2(v[j][2]) || not_finite2(v[j][3]);
+      any |= (at + j * W * 1024) / S::ROWB >= context && (not_finite2(v[j][0]) || not_finite2(v[j][1]) || not_finite2(v[j][2]) || not_finite2(v[j][3]));
     }
     any = __any(any);
     if (any) {
 #pragma unroll
       for (int j = 0; j < NV; j++) {
+        if ((at + j * W * 1024) / S::ROWB < context) continue;
 #pragma unroll
         for (int e = 0; e < 4; e++) v[j][e] &= ((v[j][e] & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) | ((v[j][e] & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u);
         *(u4*)(vb + j * W * 1024) = v[j];
