@@ -37,7 +37,8 @@ def tree_attention(q, k, v, base, seen, gate=None):
 
 def tree_bound(out, absolute, reach, v_max, rows, q8=False, out_f16=False):
     """How far pa_attn_tree may be from tree_attention, by the roundings that it makes (f16: half a step is 2^-11 of the value, or 2^-25 of what is below 2^-14):
-      q is rounded to f16, int8 rows' scales and then their products too (2^-10 together), and a product of hd terms is summed in f32: a score is off by at most
+      q is rounded to f16, and so are int8 rows' values (2^-11 of themselves, and 2^-20 for the parts of the scale: kv, 2^-10, is more than both; those below 2^-14 by up to 2^-24 each,
+      which is not in here), and a product of hd terms is summed in f32: a score is off by at most
         ds = reach (2^-11 + kv + 2^-16)  -- hd 2^-24 <= 2^-16 for the sums
       a weight is off by e^ds and by the rounding of P, numerator and denominator each; exp2 and the f32 sums add less than 2^-16; P below 2^-14 are off by 2^-25 each, of a sum of
         about 1 at the least (a row's reference is one of its own scores, whose weight is in the sum)

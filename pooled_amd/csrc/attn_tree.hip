@@ -43,6 +43,24 @@ template <int HD, int W> struct TreeShape {
 
 static __device__ inline bool not_finite2(uint32_t w) { return (w & 0x7c00u) == 0x7c00u || (w & 0x7c000000u) == 0x7c000000u; }   // any of two f16
 
+// An int8 row's values v as f16: v 2^-k, exactly, times scale 2^k, which is given as the f16 nearest to it and the rest.  k brings the scale to [1, 2) where 2^-24 <= scale < 64 (-5 <= k <= 24), so that
+// the two parts hold it to 2^-24 of itself and the product is rounded once, to what f16 holds of it, subnormal numbers too (the part of the rest, rounded before, adds 2^-21 of a value, or 2^-25).
+// Smaller scales give zeros, larger ones what f16 holds; from 2^21 on they count as infinite.
+// v 2^-k is the bit pattern of 2^(10 - k) + (v + 128) 2^-k, whose upper byte is (25 - k) << 2, less 1152 x 2^-k.
+struct Widen { _Float16 hi, lo, off; uint32_t top; };
+static __device__ inline Widen widen_of(float sc) {
+  const int e = min(max(__builtin_amdgcn_frexp_expf(sc) + 24, 1), 30);     // 25 - k: the exponent field of 1024 x 2^-k
+  const float s = __builtin_amdgcn_ldexpf(sc, 25 - e);
+  Widen w;
+  w.hi = (_Float16)s;
+  const float rest = s - (float)w.hi;
+  w.lo = (_Float16)(__builtin_fabsf(rest) < 64.f ? rest : 0.f);            // (at most 2^-11 of s; where that is infinite there is none)
+  w.top = (uint32_t)e << 2;
+  const uint16_t off = (uint16_t)(e << 10 | 128);
+  __builtin_memcpy(&w.off, &off, 2);
+  return w;
+}
+
 // What the drafted rows that column `col` sees hold that is not finite, added to eight dims of its output: rows of v head g, dims d ..
 static __device__ inline void add_not_finite(const TreeParams& p, uint32_t hd, uint32_t col, uint32_t g, uint32_t d, float (&o)[8]) {
   const uint32_t* words = p.mask + (size_t)col * p.mask_stride;
@@ -52,8 +70,16 @@ static __device__ inline void add_not_finite(const TreeParams& p, uint32_t hd, u
     const size_t row = (size_t)g * ((size_t)p.max_seq + 32) + p.base_pos + j;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      const float v = p.v_scale ? (float)((const signed char*)p.v_cache)[row * hd + d + e] * p.v_scale[row * (hd / 32) + d / 32] : (float)((const _Float16*)p.v_cache)[row * hd + d + e];
-      o[e] += __builtin_fabsf(v) < 65520.f ? 0.f : __builtin_fabsf(v) < __builtin_inff() ? __builtin_copysignf(__builtin_inff(), v) : v;     // (int8 values that f16 does not hold)
+      float v;
+      if (p.v_scale) {                              // (as it was widened: what f16 does not hold is infinite)
+        const Widen w = widen_of(p.v_scale[row * (hd / 32) + d / 32]);
+        uint16_t bits = (uint16_t)(w.top << 8 | ((uint32_t)((const unsigned char*)p.v_cache)[row * hd + d + e] ^ 0x80u));
+        _Float16 x;
+        __builtin_memcpy(&x, &bits, 2);
+        x -= w.off;
+        v = (float)__builtin_elementwise_fma(x, w.hi, x * w.lo);
+      } else v = (float)((const _Float16*)p.v_cache)[row * hd + d + e];
+      o[e] += __builtin_fabsf(v) < __builtin_inff() ? 0.f : v;
     }
   }
 }
@@ -174,14 +200,13 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
     }
   };
   auto widen = [&](u4 raw, float sc, unsigned char* row, uint32_t s0, uint32_t s1) __attribute__((always_inline)) {
-    // int8 -> f16 through the bit pattern 0x6400 | (v + 128) = 1152 + v, exactly, then times the scale, which is given as the f16 nearest to it and the rest: rounded once
-    const _Float16 hi = (_Float16)sc, lo = (_Float16)(sc - (float)hi);
-    const h2 sh = { hi, hi }, sl = { lo, lo }, off = { (_Float16)1152.f, (_Float16)1152.f };
+    const Widen w = widen_of(sc);
+    const h2 sh = { w.hi, w.hi }, sl = { w.lo, w.lo }, off = { w.off, w.off };
     h2 o[8];
 #pragma unroll
     for (int d = 0; d < 4; d++) {
-      const uint32_t w = raw[d] ^ 0x80808080u;
-      const uint32_t a = __builtin_amdgcn_perm(0x64646464u, w, 0x04010400u), b = __builtin_amdgcn_perm(0x64646464u, w, 0x04030402u);
+      const uint32_t u = raw[d] ^ 0x80808080u;
+      const uint32_t a = __builtin_amdgcn_perm(w.top, u, 0x04010400u), b = __builtin_amdgcn_perm(w.top, u, 0x04030402u);
       h2 xa, xb;
       __builtin_memcpy(&xa, &a, 4);
       __builtin_memcpy(&xb, &b, 4);
