@@ -9,6 +9,8 @@
 //     directly, three of them in flight in a ring of four; one barrier a tile.  Int8 rows go through registers, two tiles ahead, and are widened on the way to a ring of two.
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: Q fragments stay in registers, K fragments are 16-byte LDS reads, V^T fragments come from the
 //     LDS transpose read.  The accumulator of S^T is the operand of P V, so probabilities never leave registers.
+//   * q is rounded to f16, for its f16 products.  Up to eight stacked rows in all leave half of their one block free: its rows 8 .. 15 hold what that rounding drops of rows 0 .. 7, and the two
+//     halves' scores are added, so that a small draft's q counts to 2^-22 as it does in a verify block of so many rows.  More rows would need products of their own for it.
 //   * Online softmax in f32 in the exp2 domain: the reference of a row is raised, and O and l rescaled, only where a P comes out above 2^8 (exact enough in f16); l is
 //     the sum of the rounded P, so an output is a convex combination of value rows whatever that rounding did.
 //   * The mask is looked at only in tiles that reach the drafted rows.  There a row's 32 bits are one word, cut out of its mask at the tile's offset with the rows in front
@@ -114,8 +116,11 @@ static __device__ inline void store8(const TreeParams& p, uint32_t col, uint32_t
     *(f4*)(out + 4) = (f4){ o[4], o[5], o[6], o[7] };
   }
 }
-template <int HD, int NB, bool Q8, int D>
+
+// QP: rows 8 .. 15 of the one block are what f16 drops of rows 0 .. 7 (see the head of the file)
+template <int HD, int NB, bool Q8, int D, bool QP>
 __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreeParams p) {
+  static_assert(!QP || NB == 1, "one block of rows");
   constexpr int W = TREE_W, ROWS = 16 * NB * W;
   typedef TreeShape<HD, W> S;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];     // [D][K tile | V tile], mask words [WIN][ROWS], a flag of each wave
@@ -266,7 +271,12 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
 #pragma unroll
       for (int j = 0; j < QL; j++) {
         const uint32_t r = j * RPL + lane / LPQ, c = lane % LPQ;
-        *(h4*)(qs + r * S::ROWB + ((c / 2) ^ r) * 16 + c % 2 * 8) = (h4){ (_Float16)qv[b][j][0], (_Float16)qv[b][j][1], (_Float16)qv[b][j][2], (_Float16)qv[b][j][3] };
+        f4 v = qv[b][j];
+        if (QP && b == 1) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) v[e] = qv[0][j][e] - (float)(_Float16)qv[0][j][e];
+        }
+        *(h4*)(qs + r * S::ROWB + ((c / 2) ^ r) * 16 + c % 2 * 8) = (h4){ (_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3] };
       }
       wave_fence();
 #pragma unroll
@@ -339,6 +349,10 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
     if constexpr (NL == 1) {
 #pragma unroll
       for (int f = 0; f < VD; f++) fetch(f);
+    }
+    if constexpr (QP) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) s[j / 4][0][j % 4] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(s[j / 4][0][j % 4]), 0x128, 0xF, 0xF, false));     // row_ror:8
     }
     if (__builtin_expect(i >= draft0, 0)) {
 #pragma unroll
@@ -645,7 +659,7 @@ static void set_magics(TreeParams& p) {
   p.rows_magic = div_magic((uint64_t)p.n_cols * p.n_heads, p.n_cols * p.group);
 }
 
-template <int HD, int NB, bool Q8>
+template <int HD, int NB, bool Q8, bool QP>
 static hipError_t launch_tree_k(const TreeParams& p, hipStream_t s, const PaTiming* t) {
   typedef TreeShape<HD, TREE_W> S;
   constexpr int D = Q8 ? 2 : 4;
@@ -654,14 +668,15 @@ static hipError_t launch_tree_k(const TreeParams& p, hipStream_t s, const PaTimi
   if (p.n_groups == 0 || p.group_rows == 0 || p.group_rows > 16u * NB * TREE_W || (uint64_t)(p.n_groups - 1) * p.group_rows >= (uint64_t)p.n_cols * p.group ||
       (uint64_t)p.n_groups * p.group_rows < (uint64_t)p.n_cols * p.group || p.n_splits == 0 ||
       (uint64_t)(p.n_splits - 1) * p.split_tiles * 32 >= (uint64_t)p.base_pos + p.n_cols || (uint64_t)p.n_splits * p.split_tiles * 32 < (uint64_t)p.base_pos + p.n_cols) return hipErrorInvalidValue;
+  if (QP && (uint64_t)p.n_cols * p.group > 8) return hipErrorInvalidValue;
   const uint64_t total = (uint64_t)p.n_groups * p.n_kv_heads * p.n_splits;
   if (total > 0x7fffff00ull) return hipErrorInvalidValue;
   static PaPerDevice lds_set;
-  const hipError_t e = pa_lds_limit(lds_set, (const void*)pa_tree_kernel<HD, NB, Q8, D>, lds);
+  const hipError_t e = pa_lds_limit(lds_set, (const void*)pa_tree_kernel<HD, NB, Q8, D, QP>, lds);
   if (e != hipSuccess) return e;
   TreeParams pk = p;
   set_magics(pk);
-  PA_LAUNCH((pa_tree_kernel<HD, NB, Q8, D>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(TREE_W * 64), lds, s, t, pk);
+  PA_LAUNCH((pa_tree_kernel<HD, NB, Q8, D, QP>), dim3((unsigned)((total + 7) / 8 * 8)), dim3(TREE_W * 64), lds, s, t, pk);
   return hipGetLastError();
 }
 
@@ -669,8 +684,8 @@ template <int HD, bool Q8>
 static hipError_t launch_tree_hd(const TreeParams& p, const TreePlan& pl, hipStream_t s, const PaTiming* t) {
   if (pl.waves != TREE_W) return hipErrorInvalidValue;
   switch (pl.nb) {
-    case 1: return launch_tree_k<HD, 1, Q8>(p, s, t);
-    case 2: if constexpr (HD == 128 || !Q8) return launch_tree_k<HD, 2, Q8>(p, s, t); else return hipErrorInvalidValue;
+    case 1: return (uint64_t)p.n_cols * p.group <= 8 ? launch_tree_k<HD, 1, Q8, true>(p, s, t) : launch_tree_k<HD, 1, Q8, false>(p, s, t);
+    case 2: if constexpr (HD == 128 || !Q8) return launch_tree_k<HD, 2, Q8, false>(p, s, t); else return hipErrorInvalidValue;
     default: return hipErrorInvalidValue;
   }
 }

@@ -1,4 +1,4 @@
-"""Numbers that pa_attn_tree holds in f16, on the GPU against the oracle in 64 bits: int8 rows' values from the smallest to the largest scales."""
+"""Numbers that pa_attn_tree holds in f16, on the GPU against the oracle in 64 bits: int8 rows' values from the smallest to the largest scales, and the queries of small drafts."""
 import numpy as np
 import pytest
 from oracle import attn_oracle as O
@@ -66,3 +66,29 @@ def test_an_infinite_int8_scale(base, n, at, splits, value):
         pa.set_decode_splits(splits)
         got = pa.run_attn_tree(0, c.q, c.seen, base, gate=c.gate)
     assert (got[sees][..., 64:96] == value).all() and np.isfinite(got[~sees]).all() and np.isfinite(np.delete(got, np.arange(64, 96), axis=2)).all()
+
+
+@pytest.mark.parametrize("shape", sorted(SHAPES))
+@pytest.mark.parametrize("base,splits", [(0, 0), (3, 0), (40, 1), (59, 2)])
+def test_queries_of_small_drafts(shape, base, splits):
+    """Up to eight stacked rows: q counts to 2^-22 of itself (its f16 and what that leaves), as in a verify block of the same columns.  Long queries at right angles to the keys but for a small
+    part: rounded to f16, their scores would be off by some hundredths.  What is left are P, partials and f32 sums, at most four roundings of half a step, 2^-11, that add in squares (as in
+    test_gpu_tree_run.check_some): 2^-10 of the norm."""
+    cfg = SHAPES[shape]
+    G, hd = cfg["n_heads"] // cfg["n_kv_heads"], cfg["head_dim"]
+    for n in sorted({1, 8 // G}):
+        c = Case(cfg, base, n, seed=base + n)
+        for h in range(cfg["n_heads"]):
+            K = c.k[:, h // G].astype(np.float64)
+            back = np.linalg.pinv(K)
+            for col in range(n):
+                far = 20 * c.rng.standard_normal(hd)
+                c.q[col, h] = far - back @ (K @ far) + back @ (np.sqrt(hd) * c.rng.standard_normal(K.shape[0]))
+        with c.context() as pa:
+            c.fill(pa)
+            pa.set_decode_splits(splits)
+            got = pa.run_attn_tree(0, c.q, c.seen, base, gate=c.gate)
+        ref = T.tree_attention(c.q, c.k, c.v, base, c.seen, c.gate)[0]
+        norm = np.sqrt(((got - ref) ** 2).sum() / (ref ** 2).sum())
+        print("small draft %s base %d n %d: %.2e of the norm" % (shape, base, n, norm), flush=True)
+        assert norm <= 2.0 ** -10
