@@ -224,9 +224,12 @@ int pa_attn_decode_gather(pa_ctx* ctx, uint32_t layer, const float* d_q, uint32_
  *   d_mask: u32 [n_cols][mask_stride]; bit j % 32 of word j / 32 of a column's words: it sees row base_pos + j (a node's own bit and its ancestors').  Any pattern; bits
  *           from n_cols on are not looked at; a column that sees nothing (base_pos 0, no bit) gives zeros.  A drafted row with infinities or NaN reaches those columns alone that see it.
  *   d_q, d_gate, d_out: as in pa_attn_decode, but the output shares no memory with the inputs (refused).
- * Operands (q, P, int8 rows' values) are f16, products, sums and softmax f32, as in pa_attn_decode; partials of a split context are kept in f16.  Other columns' masks
- * change a column's results in their rounding at most; on a chain they agree with pa_attn_decode's to rounding; the same call gives the same bits.  pa_set_decode_splits applies.  Partials share the context's scratch: a call that grows it
- * allocates; under stream capture, where it cannot, the context is split into as many parts as there is room for. */
+ * q, P and int8 rows' values go into the products as f16 (an int8 value that f16 does not hold is infinite); sums and softmax are f32.  With up to eight stacked rows, n_cols n_heads / n_kv_heads,
+ * q counts to 2^-22 of itself, as in pa_attn_decode's blocks of so many.  Partials of a split context are kept in f16 (pa_attn_decode: in f32 but for many splits).  A column's results
+ * change in their rounding with the other columns, their masks and the splits; on a chain they agree with pa_attn_decode's to rounding; the same call gives the same bits, under stream capture too
+ * if the scratch is that of an eager call before.  They are not those of one-column decodes: in a context with PA_FLAG_VERIFY_EXACT the call returns PA_ERR_UNSUPPORTED.
+ * pa_set_decode_splits applies.  Partials share the context's scratch: a call that grows it allocates; under stream capture, where it cannot, the context is split into as many parts as there
+ * is room for. */
 int pa_attn_tree(pa_ctx* ctx, uint32_t layer, const float* d_q, uint32_t q_stride, const float* d_gate, uint32_t gate_stride, const uint32_t* d_mask,
                  uint32_t mask_stride, uint32_t base_pos, uint32_t n_cols, void* d_out, uint32_t out_stride, int out_dtype);
 /* which kernel / split / tile shape the table picks (kind: 0 decode/verify, 1 prefill) */

@@ -135,6 +135,7 @@ extern "C" int pa_attn_tree(pa_ctx* ctx, uint32_t layer, const float* d_q, uint3
   if (rc) return rc;
   const pa_config& c = ctx->cfg;
   const uint32_t qd = c.n_heads * c.head_dim;
+  if (c.flags & PA_FLAG_VERIFY_EXACT) return block_fail(ctx, PA_ERR_UNSUPPORTED, who, "PA_FLAG_VERIFY_EXACT promises the bits of one-column decodes, which a tree's columns do not have");
   if (!d_mask || !d_out) return block_fail(ctx, PA_ERR_INVALID, who, "null mask or output");
   if (out_dtype != PA_OUT_F32 && out_dtype != PA_OUT_F16) return block_fail(ctx, PA_ERR_INVALID, who, "bad out_dtype");
   if (!d_q) { d_q = ctx->q_buf; q_stride = qd; }
