@@ -46,8 +46,9 @@ extern "C" int pa_glue_kv_at(pa_ctx* ctx, uint32_t layer, const float* d_q_in, u
   if (q_stride < qcol || k_stride < kvd || v_stride < kvd) return block_fail(ctx, PA_ERR_INVALID, who, "column stride shorter than a column");
   if (ctx->rope_axes > 1 && pos_stride < n_cols) return block_fail(ctx, PA_ERR_INVALID, who, "pos_stride shorter than an axis's positions");
   if (((uintptr_t)d_q_in | (uintptr_t)d_k | (uintptr_t)d_v | (uintptr_t)d_qw | (uintptr_t)d_kw | (uintptr_t)d_pos) & 3) return block_fail(ctx, PA_ERR_INVALID, who, "pointers must be 4-byte aligned");
-  const Span in[4] = {{d_q_in, cols_bytes(n_cols, q_stride, qcol, 4)}, {d_k, cols_bytes(n_cols, k_stride, kvd, 4)}, {d_v, cols_bytes(n_cols, v_stride, kvd, 4)},
-                      {d_pos, ((size_t)(ctx->rope_axes - 1) * pos_stride + n_cols) * 4}};
+  const size_t norm = (c.flags & PA_FLAG_QK_NORM) ? c.head_dim * 4 : 0;
+  const Span in[6] = {{d_q_in, cols_bytes(n_cols, q_stride, qcol, 4)}, {d_k, cols_bytes(n_cols, k_stride, kvd, 4)}, {d_v, cols_bytes(n_cols, v_stride, kvd, 4)},
+                      {d_pos, ((size_t)(ctx->rope_axes - 1) * pos_stride + n_cols) * 4}, {d_qw, norm}, {d_kw, norm}};
   for (const Span& s : in)
     if (overlap(s, {ctx->q_buf, (size_t)n_cols * qd * 4}) || overlap(s, {ctx->gate_buf, (size_t)n_cols * qd * 4}))
       return block_fail(ctx, PA_ERR_INVALID, who, "an input lies in the context's q or gate buffer, which the call writes");
