@@ -259,8 +259,8 @@ size_t pa_kv_row_bytes(const pa_ctx* ctx, int which);
  * the end of the context, or a context cut to the rows worth keeping.  The other rows stay as they are.  No counterpart in the reference, whose caches are cut back to a prefix.
  *   d_sel: u32: the list's length n, then n cache rows, ascending, each once, the first at or behind dst_row (pa_attn_decode_gather's list).  It is on the device, so a draft may be accepted
  *          there, and is not trusted: n > max_rows is read as max_rows, rows are clamped to the cache; a list in another order leaves unspecified rows of its own at dst_row .. dst_row + n - 1.
- *   max_rows: the longest list; dst_row + max_rows <= max_seq.  Above 256 a call needs a word of scratch for every 64 KB of a cache's rows, which it allocates at its first use; under stream
- *           capture, where it cannot, the list is gone through in order without (up to 2.6 times as long; one eager call with the same max_rows before the capture is enough). */
+ *   max_rows: the longest list; dst_row + max_rows <= max_seq.  Above 256 a call needs a word of scratch for every 64 KB of a cache's rows, which the context keeps for each stream that it is
+ *           called on and allocates when it grows.  Under stream capture, and on hipStreamPerThread, the list is gone through in order without scratch (up to 2.6 times as long). */
 int pa_kv_compact(pa_ctx* ctx, uint32_t dst_row, const uint32_t* d_sel, uint32_t max_rows);
 /* device address of a cache (read-only use; the head-major device layout described at pa_layer_alloc) */
 const void* pa_kv_device_ptr(pa_ctx* ctx, uint32_t layer, int which);

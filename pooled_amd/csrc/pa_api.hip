@@ -145,7 +145,7 @@ extern "C" int pa_destroy(pa_ctx* ctx) {
   if (ctx->part_ml) (void)hipFree(ctx->part_ml);
   if (ctx->proj_buf) (void)hipFree(ctx->proj_buf);
   if (ctx->chunk_buf) (void)hipFree(ctx->chunk_buf);
-  if (ctx->compact_flags) (void)hipFree(ctx->compact_flags);
+  for (auto& f : ctx->compact_flags) if (f.flags) (void)hipFree(f.flags);
   if (ctx->w16_buf) (void)hipFree(ctx->w16_buf);
   if (ctx->wide_k) (void)hipFree(ctx->wide_k);
   if (ctx->wide_v) (void)hipFree(ctx->wide_v);

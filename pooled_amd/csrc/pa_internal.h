@@ -202,6 +202,7 @@ struct pa_weight {
   hipStream_t w16_stream = nullptr;
 };
 
+struct CompactFlags { hipStream_t stream = nullptr; uint32_t* flags = nullptr; size_t bytes = 0; };
 struct pa_ctx {
   pa_config cfg{};
   int device = 0;
@@ -228,8 +229,7 @@ struct pa_ctx {
   std::vector<void*> retired;   // outgrown scratch blocks, kept until pa_destroy (a recorded launch may still name them)
   uint32_t decode_splits_override = 0;
   int prefill_tile_mode = 0;    // pa_set_prefill_tile: 0 table, 1 always the matrix-core kernel, 2 never
-  uint32_t* compact_flags = nullptr;   // pa_kv_compact: flags of a long list's segments
-  size_t compact_flags_bytes = 0;
+  std::vector<CompactFlags> compact_flags;   // pa_kv_compact: flags of a long list's segments, of each stream that had one
   uint32_t rope_axes = 1;       // pa_set_rope_axes: axes of pa_glue_kv_at's positions ...
   uint32_t axis_of_pair[8] = {};   // ... and the axis of every rotated pair, two bits each
   // timing

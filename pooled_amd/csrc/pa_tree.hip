@@ -198,20 +198,29 @@ extern "C" int pa_kv_compact(pa_ctx* ctx, uint32_t dst_row, const uint32_t* d_se
   if (!layers) return block_fail(ctx, PA_ERR_INVALID, who, "no layer has a cache (call pa_layer_alloc)");
   p.n_layers = std::min(layers, PA_COMPACT_LAYERS);
   if (!pa_compact_one_round(p)) {
-    // flags for the segments of a long list; under stream capture, where nothing can be allocated, those of the earlier calls are used or the list is walked without
-    const size_t need = pa_compact_flags(p) * sizeof(uint32_t);
-    if (need > ctx->compact_flags_bytes) {
-      hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-      hipError_t e = hipStreamIsCapturing(ctx->stream, &st);
-      if (e != hipSuccess) return block_fail_hip(ctx, e, who);
-      if (st == hipStreamCaptureStatusNone) {
-        const int rc = pa_ctx_grow(ctx, (void**)&ctx->compact_flags, &ctx->compact_flags_bytes, need);
+    // Flags for the segments of a long list.  A workgroup waits for flags of its launch: two launches at once with the same ones would take one another's tickets, and a wait could be without
+    // end.  So every stream, which runs its launches one behind the other, has flags of its own; and a recorded call, which may be replayed on any stream beside any other call, walks the list
+    // without, as does one on hipStreamPerThread, which is another stream in every thread.  (One stream's flags in turn with events between the calls cost 3 us a call.)
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    hipError_t e = hipStreamIsCapturing(ctx->stream, &st);
+    if (e != hipSuccess) return block_fail_hip(ctx, e, who);
+    if (st == hipStreamCaptureStatusNone && ctx->stream != hipStreamPerThread) {
+      const size_t need = pa_compact_flags(p) * sizeof(uint32_t);
+      CompactFlags* f = nullptr;
+      for (CompactFlags& have : ctx->compact_flags) if (have.stream == ctx->stream) f = &have;
+      if (!f) {
+        try { ctx->compact_flags.push_back(CompactFlags()); } catch (const std::bad_alloc&) { return block_fail(ctx, PA_ERR_NOMEM, who, "out of host memory"); }
+        f = &ctx->compact_flags.back();
+        f->stream = ctx->stream;
+      }
+      if (need > f->bytes) {
+        const int rc = pa_ctx_grow(ctx, (void**)&f->flags, &f->bytes, need);
         if (rc) return rc;
         // (zero from here on: a call leaves them as it found them)
-        if ((e = hipMemsetAsync(ctx->compact_flags, 0, ctx->compact_flags_bytes, ctx->stream)) != hipSuccess) { ctx->compact_flags_bytes = 0; return block_fail_hip(ctx, e, who); }
+        if ((e = hipMemsetAsync(f->flags, 0, f->bytes, ctx->stream)) != hipSuccess) { f->bytes = 0; return block_fail_hip(ctx, e, who); }
       }
+      p.flags = f->flags;
     }
-    p.flags = need <= ctx->compact_flags_bytes ? ctx->compact_flags : nullptr;
   }
   p.n_layers = 0;
   hipError_t e = hipSuccess;
