@@ -15,7 +15,8 @@
 // The other two blocks of a hybrid model's layers are here as well: initDelta / encodeDelta, the gated delta rule with its
 // short convolution (engine/qwen35.js records it where a layer has no attention), and upMoe / encodeMoe, the experts.
 //
-// Draft trees, which the engines do not have, are draftTree / encodeLayerTree / acceptTree; keepRows cuts the caches to a list of rows.
+// Draft trees, which the engines do not have, are draftTree / encodeLayerTree / acceptTree; keepRows cuts the caches to a list of rows.  Columns whose rotary positions are not their rows
+// (prompts with images or video and what follows them, what follows rows that were cut out) are setRopeAxes / setPositions / encodeLayerAt.
 //
 // There is no CPU path here: if the addon is missing, require() throws.
 "use strict";
@@ -76,6 +77,7 @@ class HipAttention {
     for (const k of Object.keys(this.B)) addon.free(this.ctx, this.B[k].ptr);
     for (const L of this.layers) { if (L.qNorm) addon.free(this.ctx, L.qNorm); if (L.kNorm) addon.free(this.ctx, L.kNorm); if (L.attnNorm) addon.free(this.ctx, L.attnNorm); }
     if (this._tree) for (const k of ["pos", "mask", "sel"]) addon.free(this.ctx, this._tree[k]);
+    if (this._at) addon.free(this.ctx, this._at.pos);
     for (const w of this._weights || []) addon.weightDestroy(this.ctx, w);
     for (const m of this._moes || []) addon.moeDestroy(this.ctx, m);
     if (this.delta) {
@@ -280,14 +282,41 @@ class HipAttention {
     addon.attnGather(this.ctx, LB.layer, null, 0, gate, this.dims.qDim, sel, selStride, maxRows, nCols, this.B.attnOut.ptr, this._outStride(), this.outDtype);
   }
 
-  // ---- draft trees: several continuations of one context verified in one pass ----
-  // Rotary positions of several axes (prompts with images or video): the axis of each of the nRot / 2 rotated pairs; null: one axis, the default.
+  // ---- columns at rotary positions of their own ----
+  // The other methods rotate a column by its cache row.  Where that is not its position, it goes through setPositions and encodeLayerAt: in a prompt with images or video (positions on several
+  // axes), in everything behind such a prompt, whose positions fall behind its rows, and behind keepRows where positions go on from before the cut.
+  // The axis of each of the nRot / 2 rotated pairs; null: one axis, the default.
   setRopeAxes(axisOfPair) {
     const half = this.dims.nRot / 2;
     if (axisOfPair && (axisOfPair.length !== half || !Array.from(axisOfPair).every((a) => Number.isInteger(a) && a >= 0 && a < 4))) throw new Error("setRopeAxes: expected " + half + " axes, each 0 .. 3");
-    this._axes = axisOfPair ? Math.max.apply(null, Array.from(axisOfPair)) + 1 : 1;
-    addon.setRopeAxes(this.ctx, this._axes, axisOfPair ? Uint8Array.from(axisOfPair) : null);
+    const axes = axisOfPair ? Math.max.apply(null, Array.from(axisOfPair)) + 1 : 1;
+    addon.setRopeAxes(this.ctx, axes, axisOfPair ? Uint8Array.from(axisOfPair) : null);
+    this._axes = axes;
+    if (this._at) this._at.n = 0;                                 // positions of other axes
   }
+  // the positions of the columns of the next encodeLayerAt calls, of every layer: an array of them for each axis (one axis: [positions])
+  setPositions(positions) {
+    const axes = this._axes || 1, n = positions.length ? positions[0].length : 0;
+    if (positions.length !== axes || !positions.every((a) => a.length === n)) throw new Error("setPositions: expected the columns' positions on " + axes + " axes");
+    if (n === 0 || n > this.NC) throw new Error("setPositions: " + n + " columns, batchCols " + this.NC);
+    if (!positions.every((a) => Array.from(a).every((x) => Number.isInteger(x) && x >= 0 && x <= 0xFFFFFFFF))) throw new Error("setPositions: a position is a whole number");
+    if (!this._at) this._at = { pos: addon.malloc(this.ctx, 4 * this.NC * 4), n: 0 };
+    this._at.n = 0;
+    const all = new Uint32Array(axes * this.NC);
+    positions.forEach((a, axis) => all.set(Array.from(a), axis * this.NC));
+    addon.upload(this.ctx, this._at.pos, all);
+    this._at.n = n;
+  }
+  // layer i over those columns, cache rows baseRow ..: B.qFull, B.k, B.v -> the cache, B.attnOut; each column sees the rows in front of it and its own, as in encodeLayerBatchAttn
+  encodeLayerAt(p, i, baseRow) {
+    const B = this.B, w = this._norms(this.layers[i]), n = this._at ? this._at.n : 0;
+    if (!n) throw new Error("encodeLayerAt: no positions (setPositions)");
+    addon.glueKvAt(this.ctx, i, B.qFull.ptr, this._strideF(B.qFull), B.k.ptr, this._strideF(B.k), B.v.ptr, this._strideF(B.v), w[0], w[1], this._at.pos, this.NC, baseRow, n);
+    const kind = (this.attnPrefillTile && n === this.NC && n > 1 && !this._snapNow) ? 1 : 0;
+    addon.attn(this.ctx, kind, i, null, 0, this.gate ? addon.gateBuffer(this.ctx) : null, this.dims.qDim, baseRow, n, B.attnOut.ptr, this._outStride(), this.outDtype);
+  }
+
+  // ---- draft trees: several continuations of one context verified in one pass ----
   _treeBuffers() {
     if (!this._tree) {
       const t = { stride: Math.ceil(this.NC / 32), n: 0 };
@@ -329,7 +358,8 @@ class HipAttention {
     t.n = 0;
     return path;
   }
-  // rows dstRow + i of every layer's caches become the rows of the list, which ascends from dstRow on: a context cut to the rows worth keeping
+  // rows dstRow + i of every layer's caches become the rows of the list, which ascends from dstRow on: a context cut to the rows worth keeping.  The rows stay turned by the positions that they
+  // had; tokens behind that go on from those take encodeLayerAt, or draftTree's pos0.
   keepRows(dstRow, rows) {
     if (!rows.length) return;
     for (let i = 0; i < rows.length; i++)
