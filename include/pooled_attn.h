@@ -220,7 +220,8 @@ int pa_attn_decode_gather(pa_ctx* ctx, uint32_t layer, const float* d_q, uint32_
                           uint32_t n_cols, void* d_out, uint32_t out_stride, int out_dtype);
 /* pa_attn_tree: attention of a tree of drafted tokens: column c sees the cache rows [0, base_pos) and those rows base_pos + j, j < n_cols, whose bit is set in its mask, so that
  * several continuations of one context are verified in one pass (pa_attn_decode's verify block is the one whose mask is a triangle).  The columns' rows are in the cache
- * already (pa_glue_kv_at with the depths' positions, or pa_glue_kv); pa_kv_compact then keeps the accepted path.  No counterpart in the reference, whose drafts are chains.
+ * already (pa_glue_kv_at with the depths' positions, or pa_glue_kv); pa_kv_compact then keeps the accepted path.  Delta-rule layers take a chain (pa_delta_decode): trees that branch are for models
+ * whose layers are all attention.  No counterpart in the reference, whose drafts are chains.
  *   d_mask: u32 [n_cols][mask_stride]; bit j % 32 of word j / 32 of a column's words: it sees row base_pos + j (a node's own bit and its ancestors').  Any pattern; bits
  *           from n_cols on are not looked at; a column that sees nothing (base_pos 0, no bit) gives zeros.  A drafted row with infinities or NaN reaches those columns alone that see it.
  *   d_q, d_gate, d_out: as in pa_attn_decode, but the output shares no memory with the inputs (refused).

@@ -327,13 +327,21 @@ class HipAttention {
   }
   // the tree of the next encodeLayerTree calls: parents[c] is the column before c that c continues, -1 where it continues the context.  Column c goes to cache row basePos + c; its rotary
   // position is pos0 (default basePos) + its depth, on every axis.
+  // Delta-rule layers take their columns as one chain: with them (initDelta) a tree that branches is refused.  So is any with { verifyExact: true }, whose promise the stacked columns do not keep.
   draftTree(parents, basePos, pos0) {
-    const n = parents.length, t = this._treeBuffers(), depth = new Uint32Array(n), p0 = pos0 === undefined ? basePos : pos0;
+    const n = parents.length, p0 = pos0 === undefined ? basePos : pos0;
+    if (this.verifyExact) throw new Error("draftTree: a tree's columns do not have the bits of one-token passes, which verifyExact promises");
     if (n === 0 || n > this.NC) throw new Error("draftTree: " + n + " columns, batchCols " + this.NC);
-    const mask = new Uint32Array(n * t.stride), pos = new Uint32Array(4 * this.NC);
+    for (let c = 0; c < n; c++) {
+      if (!(Number.isInteger(parents[c]) && parents[c] >= -1 && parents[c] < c)) throw new Error("draftTree: a column's parent comes before it");
+      if (this.delta && parents[c] !== c - 1) throw new Error("draftTree: delta-rule layers take a chain, and this tree branches");
+    }
+    if (!(Number.isInteger(basePos) && basePos >= 0 && basePos + n <= this.maxSeq)) throw new Error("draftTree: the columns' rows exceed maxSeq");
+    if (!(Number.isInteger(p0) && p0 >= 0 && p0 + n - 1 <= 0xFFFFFFFF)) throw new Error("draftTree: pos0 is a whole number");
+    const t = this._treeBuffers(), depth = new Uint32Array(n), mask = new Uint32Array(n * t.stride), pos = new Uint32Array(4 * this.NC);
+    t.n = 0;
     for (let c = 0; c < n; c++) {
       const up = parents[c];
-      if (!(Number.isInteger(up) && up >= -1 && up < c)) throw new Error("draftTree: a column's parent comes before it");
       if (up >= 0) { depth[c] = depth[up] + 1; for (let w = 0; w < t.stride; w++) mask[c * t.stride + w] = mask[up * t.stride + w]; }
       mask[c * t.stride + (c >> 5)] |= 1 << (c & 31);
       for (let a = 0; a < 4; a++) pos[a * this.NC + c] = p0 + depth[c];
@@ -350,6 +358,7 @@ class HipAttention {
     addon.attnTree(this.ctx, i, null, 0, this.gate ? addon.gateBuffer(this.ctx) : null, this.dims.qDim, t.mask, t.stride, t.base, t.n, B.attnOut.ptr, this._outStride(), this.outDtype);
   }
   // the path from a root to column c stays, in every layer's cache, as rows basePos, basePos + 1, ...; returns its columns (c = -1: none).  The next token goes behind them.
+  // (The states of delta-rule layers move on by encodeDelta over the accepted columns, as behind a verify block.)
   acceptTree(c) {
     const t = this._tree, path = [];
     if (!t || !t.n || !(Number.isInteger(c) && c >= -1 && c < t.n)) throw new Error("acceptTree: no such column");
@@ -374,6 +383,7 @@ class HipAttention {
   // attention layers) and their column buffers: B.dQkv [q | k | v] and B.dA, B.dB in front of the pre-step, B.dOut behind.
   initDelta(o) {
     if (this.delta) throw new Error("initDelta: called before");
+    if (this._tree && this._tree.n && this._tree.parents.some((up, c) => up !== c - 1)) throw new Error("initDelta: a tree that branches is on its way");
     const handle = addon.deltaCreate(this.ctx, { nKHeads: o.nKHeads, nVHeads: o.nVHeads, headK: o.headK, headV: o.headV, convWidth: o.convWidth, nLayers: o.nLayers || 1,
       scale: o.scale || 0, eps: o.eps === undefined ? 1e-6 : o.eps, flags: o.l2norm === false ? 0 : PA_DELTA_L2NORM });
     const key = o.nKHeads * o.headK, val = o.nVHeads * o.headV;
