@@ -96,8 +96,6 @@ static __device__ inline void wave_fence() {
 }
 static __device__ inline void wait_and_meet_lds() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
 
-#define TREE_W 8              // waves of a workgroup, two a SIMD: one wave a SIMD gets half of what the LDS delivers
-
 // LDS behind the ring: mask words of WIN tiles, and a flag of each wave
 template <int NB> struct TreeLds { static constexpr int WIN = 4 / NB, bytes = WIN * 16 * NB * TREE_W * 4 + TREE_W * 4; };
 
@@ -682,7 +680,6 @@ static hipError_t launch_tree_k(const TreeParams& p, hipStream_t s, const PaTimi
 
 template <int HD, bool Q8>
 static hipError_t launch_tree_hd(const TreeParams& p, const TreePlan& pl, hipStream_t s, const PaTiming* t) {
-  if (pl.waves != TREE_W) return hipErrorInvalidValue;
   switch (pl.nb) {
     case 1: return (uint64_t)p.n_cols * p.group <= 8 ? launch_tree_k<HD, 1, Q8, true>(p, s, t) : launch_tree_k<HD, 1, Q8, false>(p, s, t);
     case 2: if constexpr (HD == 128 || !Q8) return launch_tree_k<HD, 2, Q8, false>(p, s, t); else return hipErrorInvalidValue;

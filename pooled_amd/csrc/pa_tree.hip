@@ -103,9 +103,8 @@ static TreePlan plan_tree(const pa_config& c, uint32_t n_cu, uint32_t base, uint
   for (uint32_t cap = narrow ? 128 : 256; cap >= 32; cap /= 2) {
     if (cap < 256 && cap / 2 >= rows && cap > 32) continue;                  // the same groups as the next cap's
     TreePlan pl{};
-    pl.waves = 8;
     pl.group_rows = (ceil_div(rows, ceil_div(rows, cap)) + 15) & ~15u;
-    pl.nb = ceil_div(pl.group_rows, 128);
+    pl.nb = ceil_div(pl.group_rows, 16 * TREE_W);
     pl.n_groups = ceil_div(rows, pl.group_rows);
     const uint32_t full = (uint32_t)std::max<uint64_t>(1, n_cu / ((uint64_t)pl.n_groups * c.n_kv_heads));
     for (uint32_t part : {1u, 2u, 4u, 8u, full}) {
@@ -123,7 +122,7 @@ static TreePlan plan_tree(const pa_config& c, uint32_t n_cu, uint32_t base, uint
 // the plan of a call, for the tests: {nb, waves, n_groups, group_rows, n_splits, split_tiles}
 extern "C" int pa_rule_tree(const pa_config* cfg, int n_cu, uint32_t base_pos, uint32_t n_cols, uint32_t splits, uint32_t most_splits, uint32_t* out) {
   const TreePlan pl = plan_tree(*cfg, (uint32_t)n_cu, base_pos, n_cols, splits, most_splits);
-  const uint32_t v[6] = {pl.nb, pl.waves, pl.n_groups, pl.group_rows, pl.n_splits, pl.split_tiles};
+  const uint32_t v[6] = {pl.nb, TREE_W, pl.n_groups, pl.group_rows, pl.n_splits, pl.split_tiles};
   memcpy(out, v, sizeof v);
   return 0;
 }

@@ -23,8 +23,9 @@ struct TreeParams {
   float scale;                                  // 1 / sqrt(hd)
   uint32_t ng_magic, ns_magic, g_magic, rows_magic; // div_magic of n_groups, n_splits, group and n_cols x group (set by the launchers)
 };
-// what a call runs as: rows a wave holds (16 nb), waves of a workgroup, groups of rows, splits
-struct TreePlan { uint32_t nb, waves, n_groups, group_rows, n_splits, split_tiles; };
+#define TREE_W 8              // waves of a workgroup, two a SIMD: one wave a SIMD gets half of what the LDS delivers
+// what a call runs as: rows a wave holds (16 nb), groups of rows, splits
+struct TreePlan { uint32_t nb, n_groups, group_rows, n_splits, split_tiles; };
 hipError_t pa_launch_tree(const TreeParams& p, const TreePlan& pl, uint32_t hd, hipStream_t s, const PaTiming* t);
 hipError_t pa_launch_tree_merge(const TreeParams& p, uint32_t hd, hipStream_t s, const PaTiming* t);
 
