@@ -42,7 +42,7 @@ def tree_bound(out, absolute, reach, v_max, rows, q8=False, out_f16=False):
         ds = reach (2^-11 + kv + 2^-16)  -- hd 2^-24 <= 2^-16 for the sums
       a weight is off by e^ds and by the rounding of P, numerator and denominator each; exp2 and the f32 sums add less than 2^-16; P below 2^-14 are off by 2^-25 each, of a sum of
         about 1 at the least (a row's reference is one of its own scores, whose weight is in the sum)
-      value rows of int8 caches are off by kv; the partials of splits are rounded to f16, and the output if it is f16."""
+      value rows of int8 caches are off by kv; the output is rounded if it is f16, and so may the partials of splits be."""
     half, kv = 2.0 ** -11, 2.0 ** -10 if q8 else 0.0
     ds = reach[..., None] * (half + kv + 2.0 ** -16)
     w = np.exp(2 * ds) * (1 + half) ** 2 * (1 + 2.0 ** -16) - 1

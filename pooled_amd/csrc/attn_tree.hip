@@ -16,8 +16,8 @@
 //   * The mask is looked at only in tiles that reach the drafted rows.  There a row's 32 bits are one word, cut out of its mask at the tile's offset with the rows in front
 //     of the draft as ones.  A drafted row that holds what is not finite must reach those columns alone that see it, and 0 x inf is not 0: such elements go into the product as
 //     zeros and are added to the outputs of the columns that see them.  Rows of the context, which all columns see, go into it as they are, also those of the draft's first tile.
-//   * Splits leave (m, l) and O / l in f16: a convex combination of f16 values loses 2^-12 of itself by that (mean of a rounding of at most 2^-11), below what the f16 P
-//     lose, and the partials are half the bytes; pa_tree_merge_kernel joins them.
+//   * Splits leave (m, l) and O / l in f32; pa_tree_merge_kernel joins them.  (In f16 they are half the bytes, which is 0 - 4 us of a call, and 2^-12 of an output: 63 splits of 17 columns at
+//     20003 int8 rows 25.7 us against 29.7, 16 of 24 at 2011 12.9 against 13.3.)
 //
 // Measured (24 query and 4 key heads of 256, 65536 rows of f16, 268 MB): 16 columns 52 us = 5.1 TB/s, which is what a large copy reaches; 48 columns 92 us = 840 TFLOP/s (a large matrix
 // product: 1330), and 3 % less with every tile read from the L2, so there the SIMDs' work bounds it: a tile of nine blocks, three of them on one SIMD, takes 1.3 us, of which the matrix
@@ -63,15 +63,15 @@ static __device__ inline Widen widen_of(float sc) {
   return w;
 }
 
-// What the drafted rows that column `col` sees hold that is not finite, added to eight dims of its output: rows of v head g, dims d ..
-static __device__ inline void add_not_finite(const TreeParams& p, uint32_t hd, uint32_t col, uint32_t g, uint32_t d, float (&o)[8]) {
+// What the drafted rows that column `col` sees hold that is not finite, added to E dims of its output (of one block of 32): rows of v head g, dims d ..
+template <int E> static __device__ inline void add_not_finite(const TreeParams& p, uint32_t hd, uint32_t col, uint32_t g, uint32_t d, float (&o)[E]) {
   const uint32_t* words = p.mask + (size_t)col * p.mask_stride;
 #pragma unroll 1
   for (uint32_t j = 0; j < p.n_cols; j++) {
     if (!(words[j / 32] >> (j % 32) & 1)) continue;
     const size_t row = (size_t)g * ((size_t)p.max_seq + 32) + p.base_pos + j;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
+    for (int e = 0; e < E; e++) {
       float v;
       if (p.v_scale) {                              // (as it was widened: what f16 does not hold is infinite)
         const Widen w = widen_of(p.v_scale[row * (hd / 32) + d / 32]);
@@ -102,16 +102,12 @@ template <int NB> struct TreeLds { static constexpr int WIN = 4 / NB, bytes = WI
 // sigmoid; the reciprocal is off by 2^-23 of itself, an exact division is a dozen instructions a value
 static __device__ inline float gate_of(float g) { return __builtin_amdgcn_rcpf(1.f + __expf(-g)); }
 
-// eight dims of an output column
-static __device__ inline void store8(const TreeParams& p, uint32_t col, uint32_t d, const float (&o)[8]) {
-  if (p.out_f16) {
-    _Float16* out = (_Float16*)p.out + (size_t)col * p.out_stride + d;
-    *(h4*)out = (h4){ (_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3] };        // (columns of f16 are 8 bytes aligned)
-    *(h4*)(out + 4) = (h4){ (_Float16)o[4], (_Float16)o[5], (_Float16)o[6], (_Float16)o[7] };
-  } else {
-    float* out = (float*)p.out + (size_t)col * p.out_stride + d;
-    *(f4*)out = (f4){ o[0], o[1], o[2], o[3] };
-    *(f4*)(out + 4) = (f4){ o[4], o[5], o[6], o[7] };
+// E dims of an output column, four or eight
+template <int E> static __device__ inline void store_dims(const TreeParams& p, uint32_t col, uint32_t d, const float (&o)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; e += 4) {
+    if (p.out_f16) *(h4*)((_Float16*)p.out + (size_t)col * p.out_stride + d + e) = (h4){ (_Float16)o[e], (_Float16)o[e + 1], (_Float16)o[e + 2], (_Float16)o[e + 3] };     // (columns of f16 are 8 bytes aligned)
+    else *(f4*)((float*)p.out + (size_t)col * p.out_stride + d + e) = (f4){ o[e], o[e + 1], o[e + 2], o[e + 3] };
   }
 }
 
@@ -497,6 +493,17 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   // partials: O [kv head][split][stacked row][HD], so that what a wave writes is one piece; (m, l) [kv head][stacked row][split]
   const uint32_t rows_all = p.n_cols * G, c = lane % (HD / 8);
   constexpr int RPI = 64 / (HD / 8);                // rows of the wave at once, eight dims a lane
+  constexpr int EROWS = RING / W / (HD * 4) < 16 ? 8 : 16;                  // f32 rows that a wave's part of the ring holds
+  static_assert(EROWS * HD * 4 * W <= RING, "the rows fit the ring");
+  float* os = (float*)(smem + wave * EROWS * HD * 4);
+  auto put = [&](int nb, int half, float inv) __attribute__((always_inline)) {
+    if (EROWS == 16 || (int)(ln / 8) == half) {
+      const uint32_t r = ln % EROWS;
+#pragma unroll
+      for (int db = 0; db < S::DB; db++) *(f4*)(os + r * HD + ((4 * db + kg) ^ r) * 4) = acc[db][nb] * inv;
+    }
+    wave_fence();
+  };
 #pragma unroll
   for (int nb = 0; nb < NL; nb++) {
     l_run[nb] += __shfl_xor(l_run[nb], 16, 64);
@@ -507,26 +514,19 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
       // (the sign of l says that a drafted row of the split holds what is not finite; a row of NaN scores may have found no reference)
       if (kg == 0 && r0 + ln < R)
         p.part_ml[((size_t)g * rows_all + x0 + r0 + ln) * p.n_splits + sp] = make_float2(l_run[nb] != l_run[nb] ? __builtin_inff() : m_ref[nb], bad ? -l_run[nb] : l_run[nb]);
-      unsigned char* os = smem + wave * 16 * S::ROWB;
-      static_assert(16 * W * S::ROWB <= RING, "sixteen rows of each wave fit the ring");
+      float* to = p.part_o + (((size_t)g * p.n_splits + sp) * rows_all + x0 + r0) * HD + lane * 4;
 #pragma unroll
-      for (int db = 0; db < S::DB; db++) {
-        const f4 o = acc[db][nb] * inv;
-        *(h4*)(os + ln * S::ROWB + ((2 * db + kg / 2) ^ ln) * 16 + kg % 2 * 8) = (h4){ (_Float16)o[0], (_Float16)o[1], (_Float16)o[2], (_Float16)o[3] };
-      }
-      wave_fence();
-      h8* to = (h8*)((_Float16*)p.part_o + (((size_t)g * p.n_splits + sp) * rows_all + x0 + r0) * HD) + lane;
+      for (int half = 0; half < 16 / EROWS; half++) {
+        put(nb, half, inv);
 #pragma unroll
-      for (int it = 0; it < 16 / RPI; it++) {
-        const uint32_t r = it * RPI + lane / (HD / 8);
-        const h8 v = *(const h8*)(os + r * S::ROWB + (c ^ r) * 16);
-        if (r0 + r < R) __builtin_nontemporal_store(v, to + it * 64);
+        for (int it = 0; it < EROWS * HD / 256; it++) {                       // (1 KB of rows at once)
+          const uint32_t r = it * 256 / HD + lane / (HD / 4), u = lane % (HD / 4);
+          const f4 v = *(const f4*)(os + r * HD + (u ^ r) * 4);
+          if (r0 + half * EROWS + r < R) __builtin_nontemporal_store(v, (f4*)(to + (half * EROWS * HD + it * 256)));
+        }
+        wave_fence();
       }
-      wave_fence();
     } else {
-      constexpr int EROWS = RING / W / (HD * 4) < 16 ? 8 : 16;              // f32 rows that a wave's part of the ring holds
-      static_assert(EROWS * HD * 4 * W <= RING, "the rows fit the ring");
-      float* os = (float*)(smem + wave * EROWS * HD * 4);
       // all of the block's gates ahead (one after the other they are a trip to memory each: 5 columns at 20 rows, 16 / 2 heads of 256, 9.5 us a call, so 8.8, and 7.7 with a reciprocal for the division)
       f4 gt[16 / RPI][2];
       if (p.gate) {
@@ -540,12 +540,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
       }
 #pragma unroll
       for (int half = 0; half < 16 / EROWS; half++) {
-        if (EROWS == 16 || (int)(ln / 8) == half) {
-          const uint32_t r = ln % EROWS;
-#pragma unroll
-          for (int db = 0; db < S::DB; db++) *(f4*)(os + r * HD + ((4 * db + kg) ^ r) * 4) = acc[db][nb] * inv;
-        }
-        wave_fence();
+        put(nb, half, inv);
 #pragma unroll
         for (int it = 0; it < EROWS / RPI; it++) {
           const uint32_t r = it * RPI + lane / (HD / 8), wr = r0 + half * EROWS + r;
@@ -559,7 +554,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
 #pragma unroll
             for (int i = 0; i < 4; i++) { o[i] *= gate_of(ga[i]); o[4 + i] *= gate_of(gb[i]); }
           }
-          store8(p, col, hq * HD + 8 * c, o);
+          store_dims(p, col, hq * HD + 8 * c, o);
         }
         wave_fence();
       }
@@ -572,21 +567,21 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   else if constexpr (NB == 2) run(std::integral_constant<int, 2>{});
 }
 
-// Joins the splits of a (column, head): w_s = l_s 2^(m_s - M), out = sum w_s o_s / sum w_s, times sigmoid(gate).  A wavefront takes LPG x 8 dims of a (column, head): LPG lanes of eight
+// Joins the splits of a (column, head): w_s = l_s 2^(m_s - M), out = sum w_s o_s / sum w_s, times sigmoid(gate).  A wavefront takes LPG x 4 dims of a (column, head): LPG lanes of four
 // dims, 64 / LPG groups of lanes over the splits in turn, eight splits of a group in one round trip.
 template <int HD, int LPG>
 __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
-  constexpr uint32_t NG = 64 / LPG, B = 8, SL = HD / 8 / LPG;
-  const uint32_t lane = threadIdx.x & 63, l8 = lane % LPG, grp = lane / LPG;
+  constexpr uint32_t NG = 64 / LPG, B = 8, SL = HD / 4 / LPG;
+  const uint32_t lane = threadIdx.x & 63, l4 = lane % LPG, grp = lane / LPG;
   const uint32_t wv = blockIdx.x * 4 + (threadIdx.x >> 6), row = wv / SL, rows_all = p.n_cols * p.group, ns = p.n_splits;
   if (row >= p.n_cols * p.n_heads) return;
   const uint32_t g = div_by(row, rows_all, p.rows_magic), x = row - g * rows_all;                 // kv head, stacked row
-  const uint32_t col = div_by(x, p.group, p.g_magic), h = g * p.group + x - col * p.group, d = (wv % SL * LPG + l8) * 8;
+  const uint32_t col = div_by(x, p.group, p.g_magic), h = g * p.group + x - col * p.group, d = (wv % SL * LPG + l4) * 4;
   const float2* ml = p.part_ml + (size_t)row * ns;
-  const _Float16* po = (const _Float16*)p.part_o + ((size_t)g * ns * rows_all + x) * HD + d;
+  const float* po = p.part_o + ((size_t)g * ns * rows_all + x) * HD + d;
   const size_t step = (size_t)rows_all * HD;
   float2 m[B];
-  h8 v[B];
+  f4 v[B];
   auto load = [&](uint32_t s0) __attribute__((always_inline)) {
 #pragma unroll
     for (uint32_t k = 0; k < B; k++) {
@@ -599,20 +594,15 @@ __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
     }
   };
   load(grp);
-  float gt[8];
-  if (p.gate) {
-    const float* gate = p.gate + (size_t)col * p.gate_stride + h * HD + d;
-    const f4 a = *(const f4*)gate, b = *(const f4*)(gate + 4);
-#pragma unroll
-    for (int i = 0; i < 4; i++) { gt[i] = a[i]; gt[4 + i] = b[i]; }
-  }
+  f4 gt = {0.f, 0.f, 0.f, 0.f};
+  if (p.gate) gt = *(const f4*)(p.gate + (size_t)col * p.gate_stride + h * HD + d);
   float M = NEG_INF;
 #pragma unroll
   for (uint32_t k = 0; k < B; k++) M = fmaxf(M, m[k].x);
   for (uint32_t s = grp + NG * B; s < ns; s += NG) M = fmaxf(M, ml[s].x);
 #pragma unroll
   for (uint32_t o = LPG; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o, 64));
-  float L = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float L = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
   uint32_t sign = 0;
   if (M != NEG_INF) {
     for (uint32_t s0 = grp;;) {
@@ -622,7 +612,7 @@ __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
         const float w = m[k].y == 0.f ? 0.f : __builtin_fabsf(m[k].y) * __builtin_amdgcn_exp2f(m[k].x - M);      // (a split that the row saw nothing of holds zeros)
         L += w;
 #pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = __builtin_fmaf(w, (float)v[k][i], o[i]);
+        for (int i = 0; i < 4; i++) o[i] = __builtin_fmaf(w, v[k][i], o[i]);
       }
       s0 += NG * B;
       if (s0 - grp >= ns) break;
@@ -633,19 +623,19 @@ __global__ __launch_bounds__(256) void pa_tree_merge_kernel(TreeParams p) {
   for (uint32_t k = LPG; k < 64; k <<= 1) {
     L += __shfl_xor(L, k, 64);
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] += __shfl_xor(o[i], k, 64);
+    for (int i = 0; i < 4; i++) o[i] += __shfl_xor(o[i], k, 64);
   }
   sign = __any(sign >> 31);
   if (grp) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
 #pragma unroll
-  for (int i = 0; i < 8; i++) o[i] *= inv;
+  for (int i = 0; i < 4; i++) o[i] *= inv;
   if (__builtin_expect(sign, 0)) add_not_finite(p, HD, col, g, d, o);
   if (p.gate) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) o[i] *= gate_of(gt[i]);
+    for (int i = 0; i < 4; i++) o[i] *= gate_of(gt[i]);
   }
-  store8(p, col, h * HD + d, o);
+  store_dims(p, col, h * HD + d, o);
 }
 
 // (the divisions at the head of the kernels, some thirty instructions each, cost 1 - 2 us a call)
@@ -693,15 +683,14 @@ hipError_t pa_launch_tree(const TreeParams& p, const TreePlan& pl, uint32_t hd, 
   return hipErrorInvalidValue;
 }
 
-// few splits: whole rows a wave, many: narrow slices, so that all of a row's splits are one round trip, with no more lanes than they need (1152 rows of 256, 32 splits: 7.0 us with 16 lanes a
-// slice, 8.8 with 8)
+// As many lanes a slice as leave groups for all of a row's splits in one round trip: whole rows a wave for few splits, narrow slices for many
 template <int HD>
 static void launch_merge(const TreeParams& p, hipStream_t s, const PaTiming* t) {
-  constexpr uint32_t LPR = HD / 8;
   const uint32_t rows = p.n_cols * p.n_heads;
-  auto grid = [&](uint32_t lpg) { return dim3((unsigned)(((uint64_t)rows * (LPR / lpg) + 3) / 4)); };
-  if (p.n_splits <= 64 / LPR * 8) PA_LAUNCH((pa_tree_merge_kernel<HD, LPR>), grid(LPR), dim3(256), 0, s, t, p);
-  else if (HD == 256 && p.n_splits <= 32) PA_LAUNCH((pa_tree_merge_kernel<256, 16>), grid(16), dim3(256), 0, s, t, p);
+  auto grid = [&](uint32_t lpg) { return dim3((unsigned)(((uint64_t)rows * (HD / 4 / lpg) + 3) / 4)); };
+  if (HD == 256 && p.n_splits <= 8) PA_LAUNCH((pa_tree_merge_kernel<256, 64>), grid(64), dim3(256), 0, s, t, p);
+  else if (p.n_splits <= 16) PA_LAUNCH((pa_tree_merge_kernel<HD, 32>), grid(32), dim3(256), 0, s, t, p);
+  else if (p.n_splits <= 32) PA_LAUNCH((pa_tree_merge_kernel<HD, 16>), grid(16), dim3(256), 0, s, t, p);
   else if (p.n_splits <= 64) PA_LAUNCH((pa_tree_merge_kernel<HD, 8>), grid(8), dim3(256), 0, s, t, p);
   else PA_LAUNCH((pa_tree_merge_kernel<HD, 4>), grid(4), dim3(256), 0, s, t, p);
 }

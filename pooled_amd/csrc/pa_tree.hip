@@ -72,13 +72,13 @@ extern "C" int pa_glue_kv_at(pa_ctx* ctx, uint32_t layer, const float* d_q_in, u
 
 // ---- attention -----------------------------------------------------------------------------------
 
-static size_t part_bytes(const pa_config& c, uint32_t n_cols, uint32_t splits) { return (size_t)n_cols * c.n_heads * splits * c.head_dim * 2; }
+static size_t part_bytes(const pa_config& c, uint32_t n_cols, uint32_t splits) { return (size_t)n_cols * c.n_heads * splits * c.head_dim * 4; }
 static size_t ml_bytes(const pa_config& c, uint32_t n_cols, uint32_t splits) { return (size_t)n_cols * c.n_heads * splits * 8; }
 
 // What a call takes, in us, fitted to 463 timed calls (16 / 2-, 24 / 4- and 16 / 8-head shapes, 2 - 64 columns at 64 - 65536 rows, f16 and int8 rows, 64 - 256 rows a workgroup, all CUs busy
 // down to an eighth of them; mean error 4 %, nine in ten within 8 %; what it chooses takes 100.8 % of the best plan tried, 109 % at worst).  The launches, the start of a workgroup and its
 // outputs; then its tiles, each so long for the barrier and the chain of one wave and so much for every block of 16 rows, or the stream of the cache if that is more; and the
-// partials, written and read again.
+// partials, written and read again (timed as f16; as f32 they take 0.0 - 0.3 us a MB more, and where twice the weight would choose another plan it takes as long: 26 cases, mean of the quotients 1.00).
 static double tree_us(const pa_config& c, uint32_t n_cu, uint32_t rows, uint32_t tiles, const TreePlan& pl) {
   const bool q8 = (c.flags & PA_FLAG_KV_Q8) != 0, wide = c.head_dim == 256;
   const double fixed = q8 ? (wide ? 10.1 : 7.6) : wide ? 8.6 : 7.2, out = q8 ? (wide ? 0.05 : 0.18) : wide ? 0.29 : 0.19;
@@ -89,8 +89,8 @@ static double tree_us(const pa_config& c, uint32_t n_cu, uint32_t rows, uint32_t
   // (a second launch and its trip to memory saved; 168 calls of 1 - 63 columns at 20 - 450 rows: one split is ahead up to some 200 rows of head_dim 128, 130 of 256, 30 - 150 of int8 rows;
   // 24 columns at 100 rows of 16 / 8 heads of 128 6.2 us against 8.5, at 300 9.2 against 8.7)
   const double merge = pl.n_splits > 1 ? 0.0 : q8 ? (wide ? 1.3 : 2.6) : wide ? 1.9 : 2.9;
-  const double partials = pl.n_splits > 1 ? 1e-6 * rows * c.n_kv_heads * pl.n_splits * c.head_dim * 2.0 : 0.0;
-  return fixed - merge + std::max(chain, stream) + out * blocks + 0.427 * partials;
+  const double partials = pl.n_splits > 1 ? 1e-6 * rows * c.n_kv_heads * pl.n_splits * c.head_dim * 4.0 : 0.0;
+  return fixed - merge + std::max(chain, stream) + out * blocks + 0.2135 * partials;
 }
 
 // Rows of a workgroup: up to 256, a wave two blocks of 16, or 128, 64 and 32, the groups then sharing the stream through their XCD's L2 (two blocks of int8 rows of head_dim 256 do not fit the
@@ -164,7 +164,7 @@ extern "C" int pa_attn_tree(pa_ctx* ctx, uint32_t layer, const float* d_q, uint3
   TreeParams p;
   memset(&p, 0, sizeof p);
   p.q = d_q; p.gate = d_gate; p.k_cache = L.k; p.v_cache = L.v; p.k_scale = L.ks; p.v_scale = L.vs; p.mask = d_mask;
-  p.part_o = (uint16_t*)ctx->part_o; p.part_ml = (float2*)ctx->part_ml; p.out = d_out;
+  p.part_o = ctx->part_o; p.part_ml = (float2*)ctx->part_ml; p.out = d_out;
   p.q_stride = q_stride; p.gate_stride = gate_stride; p.mask_stride = mask_stride; p.out_stride = out_stride;
   p.n_heads = c.n_heads; p.n_kv_heads = c.n_kv_heads; p.group = c.n_heads / c.n_kv_heads;
   p.base_pos = base_pos; p.n_cols = n_cols; p.max_seq = c.max_seq;

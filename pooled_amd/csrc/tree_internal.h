@@ -12,7 +12,7 @@ struct TreeParams {
   const void* k_cache; const void* v_cache;     // f16 or int8, [nKV][max_seq + 32][hd]
   const float* k_scale; const float* v_scale;   // int8 caches: one f32 scale per 32 values
   const uint32_t* mask;                         // [n_cols][mask_stride]: bit j: the column sees row base_pos + j
-  uint16_t* part_o; float2* part_ml;            // partials of the splits: O / l as f16 and (m, l), see attn_tree.hip
+  float* part_o; float2* part_ml;               // partials of the splits: O / l and (m, l), see attn_tree.hip
   void* out;                                    // [n_cols][out_stride]
   uint32_t q_stride, gate_stride, mask_stride, out_stride;
   uint32_t n_heads, n_kv_heads, group;          // group = nH / nKV

@@ -92,3 +92,29 @@ def test_queries_of_small_drafts(shape, base, splits):
         norm = np.sqrt(((got - ref) ** 2).sum() / (ref ** 2).sum())
         print("small draft %s base %d n %d: %.2e of the norm" % (shape, base, n, norm), flush=True)
         assert norm <= 2.0 ** -10
+
+
+@pytest.mark.parametrize("q8", [False, True])
+@pytest.mark.parametrize("shape", sorted(SHAPES))
+@pytest.mark.parametrize("base,n,splits", [(20, 9, 1), (40, 9, 2), (90, 17, 3), (300, 40, 7)])
+def test_parts_of_a_mean_are_kept_in_f32(shape, base, n, splits, q8):
+    """Queries of zeros weigh every seen row alike, exactly, over values in [1, 2) that f16 holds: an output is a mean, whose sums, and those of the splits' parts, are off by 2^-24 of themselves for every
+    row and every part at most, and by a few of that for reciprocal, product and gate (2^-22 for the hardware's reciprocal and exponential)."""
+    c = Case(dict(SHAPES[shape], kv_q8=q8), base, n, seed=base)
+    c.q[:] = 0
+    if q8:
+        c.parts[1] = (c.parts[1] & 63 | 64).astype(np.int8)
+        c.parts[3][:] = 2.0 ** -6
+        c.v = O.q8_dequantize(c.parts[1], c.parts[3])
+    else:
+        c.v = O.f16_round((1 + np.abs(c.v) % 1).astype(np.float32))
+        c.parts[1] = O.f16_bits(c.v)
+    assert c.v.min() >= 1 and c.v.max() <= 2
+    with c.context() as pa:
+        c.fill(pa)
+        pa.set_decode_splits(splits)
+        got = pa.run_attn_tree(0, c.q, c.seen, base, gate=c.gate)
+    ref = T.tree_attention(c.q, c.k, c.v, base, c.seen, c.gate)[0]
+    off = np.abs(got / ref - 1).max()
+    print("mean %s%s base %d n %d in %d: off by %.2e" % (shape, " q8" if q8 else "", base, n, splits, off), flush=True)
+    assert off <= (base + n + splits + 4) * 2.0 ** -24 + 2.0 ** -21
