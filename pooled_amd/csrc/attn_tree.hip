@@ -19,10 +19,10 @@
 //   * Splits leave (m, l) and O / l in f32; pa_tree_merge_kernel joins them.  (In f16 they are half the bytes, which is 0 - 4 us of a call, and 2^-12 of an output: 63 splits of 17 columns at
 //     20003 int8 rows 25.7 us against 29.7, 16 of 24 at 2011 12.9 against 13.3.)
 //
-// Measured (24 query and 4 key heads of 256, 65536 rows of f16, 268 MB): 16 columns 52 us = 5.1 TB/s, which is what a large copy reaches; 48 columns 92 us = 840 TFLOP/s (a large matrix
+// Measured (24 query and 4 key heads of 256, 65536 rows of f16, 268 MB): 16 columns 52 us = 5.1 TB/s, which is what a large copy reaches; 48 columns 94.6 us = 817 TFLOP/s (a large matrix
 // product: 1330), and 3 % less with every tile read from the L2, so there the SIMDs' work bounds it: a tile of nine blocks, three of them on one SIMD, takes 1.3 us, of which the matrix
-// instructions are 0.8 at the 1.9 GHz that the power limit leaves.  The merge adds 7 us there (19 MB of partials), 3 - 4 for small drafts, most of it the launch.  Int8: 17 columns at 20003 rows
-// 21.5 us and 6.5: the widening through registers, 1.1 us a tile of seven blocks.  5 columns at 190 rows, 16 and 8 heads of 128: 7.2 us a call in one launch, 7.8 with
+// instructions are 0.8 at the 1.9 GHz that the power limit leaves.  The merge adds 9.3 us there (38 MB of partials), 3 - 4 for small drafts, most of it the launch.  Int8: 17 columns at 20003 rows
+// 24.7 us and 7.5: the widening through registers, 1.1 us a tile of seven blocks, and 26 MB of partials.  5 columns at 190 rows, 16 and 8 heads of 128: 7.4 us a call in one launch, 7.8 with
 // seven splits and the merge; at 100 rows 5.9 and 8.3.
 #include "tree_internal.h"
 #include "pf_common.h"

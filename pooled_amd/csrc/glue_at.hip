@@ -6,7 +6,8 @@
 // A wavefront takes 512 values of query heads of one column (two heads of 256, four of 128), or as many of key heads with their value heads; every load of a wave goes out ahead of what
 // depends on one, the positions first.  Rows of a cache are packed through LDS, eight values a lane.
 // Bound: wide chunks by HBM: 5003 columns of 24 query and 4 key heads of 256 with gates (553 MB) take 100 us = 5.5 TB/s; with one head a wavefront 124.  1001 columns of 16 and 8 heads
-// of 128 (29 MB) 8.6 us, with one key head a wavefront 10.8.  A draft's columns by the chain position -> (cos, sin) -> rotation: 24 columns 2.6 us.
+// of 128 (29 MB) 8.6 us, with one key head a wavefront 10.8.  A draft's columns by the chain position -> (cos, sin) -> rotation: 24 columns 2.6 us.  Int8 rows, packed one by one:
+// 1001 columns of 16 and 8 heads of 128 13.1 us a call, f16 9.3; 24 of 16 and 2 heads of 256 4.3 and 4.0.
 #include "tree_internal.h"
 #include "glue_math.h"
 

@@ -7,7 +7,7 @@
 //             A segment reads without waiting for anybody and waits only for segments in front of it in its plane.  Workgroups take segments by ticket, in the order in which they
 //             start, so those in front are with workgroups that run already and every wait ends, whatever else the device runs and in whatever order workgroups start, as long as no other launch has the same flags meanwhile (each stream has its own).  Whole
 //             lines in and out, all CUs busy.  Flags and tickets are zero between calls: the plane's last workgroup through its wait clears them.
-// Bound by HBM (two transfers of each row that moves) or, for a few rows, by one launch.  8000 of 16003 rows of six layers of 8 heads of 128 (394 MB read and written): 77 us = 5.1 TB/s,
+// Bound by HBM (two transfers of each row that moves) or, for a few rows, by one launch.  8000 of 16003 rows of six layers of 8 heads of 128 (394 MB read and written): 78 us = 5.05 TB/s,
 // the rate of a large copy; 10001 of 30011 int8 rows of three layers of 4 heads of 256 (138 MB): 38 us, where the scales' 32 bytes a row cost whole lines of 128 (23 MB read for 8).  Five
 // rows in ten layers: 2.9 us.
 #include "tree_internal.h"
