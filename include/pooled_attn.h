@@ -225,8 +225,9 @@ int pa_attn_decode_gather(pa_ctx* ctx, uint32_t layer, const float* d_q, uint32_
  *   d_mask: u32 [n_cols][mask_stride]; bit j % 32 of word j / 32 of a column's words: it sees row base_pos + j (a node's own bit and its ancestors').  Any pattern; bits
  *           from n_cols on are not looked at; a column that sees nothing (base_pos 0, no bit) gives zeros.  A drafted row with infinities or NaN reaches those columns alone that see it.
  *   d_q, d_gate, d_out: as in pa_attn_decode, but the output shares no memory with the inputs (refused).
- * q, P and int8 rows' values go into the products as f16 (an int8 value that f16 does not hold is infinite); sums and softmax are f32.  With up to eight stacked rows, n_cols n_heads / n_kv_heads,
- * q counts to 2^-22 of itself, as in pa_attn_decode's blocks of so many.  Partials of a split context are kept in f32.  A column's results
+ * q, P and int8 rows' values go into the products as f16 (an int8 value that f16 does not hold is infinite); sums and softmax are f32.  q counts to 2^-22 of itself nonetheless, as in pa_attn_decode's
+ * blocks of up to eight stacked rows (n_cols n_heads / n_kv_heads), but for wide drafts over heads of 256 (more than 128 stacked rows, as the plan goes) and more than eight stacked rows over int8
+ * caches.  Partials of a split context are kept in f32.  A column's results
  * change in their rounding with the other columns, their masks and the splits; on a chain they agree with pa_attn_decode's to rounding; the same call gives the same bits, under stream capture too
  * if the scratch is that of an eager call before.  They are not those of one-column decodes: in a context with PA_FLAG_VERIFY_EXACT the call returns PA_ERR_UNSUPPORTED.
  * pa_set_decode_splits applies.  Partials share the context's scratch: a call that grows it allocates; under stream capture, where it cannot, the context is split into as many parts as there

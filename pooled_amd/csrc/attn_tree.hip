@@ -9,8 +9,9 @@
 //     directly, three of them in flight in a ring of four; one barrier a tile.  Int8 rows go through registers, two tiles ahead, and are widened on the way to a ring of two.
 //   * S^T = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_f16: Q fragments stay in registers, K fragments are 16-byte LDS reads, V^T fragments come from the
 //     LDS transpose read.  The accumulator of S^T is the operand of P V, so probabilities never leave registers.
-//   * q is rounded to f16, for its f16 products.  Up to eight stacked rows in all leave half of their one block free: its rows 8 .. 15 hold what that rounding drops of rows 0 .. 7, and the two
-//     halves' scores are added, so that a small draft's q counts to 2^-22 as it does in a verify block of so many rows.  More rows would need products of their own for it.
+//   * The products take f16, and q is rounded to it; what that drops of f16 rows' q goes into products of its own with the same K fragments, so that q counts to 2^-22 of itself.  Up to eight stacked
+//     rows in all leave half of their one block free, and its rows 8 .. 15 hold it, at no cost; else it is in fragments beside q's (24 columns at 2011 rows 13.3 -> 14.5 us a call, 63 at 7001 of heads of
+//     128 15.2 -> 16.5: half of the score products again).  Not where registers have no room, two blocks a wave of heads of 256, nor for more int8 rows, whose own rounding, K's to f16, is as large.
 //   * Online softmax in f32 in the exp2 domain: the reference of a row is raised, and O and l rescaled, only where a P comes out above 2^8 (exact enough in f16); l is
 //     the sum of the rounded P, so an output is a convex combination of value rows whatever that rounding did.
 //   * The mask is looked at only in tiles that reach the drafted rows.  There a row's 32 bits are one word, cut out of its mask at the tile's offset with the rows in front
@@ -111,10 +112,11 @@ template <int E> static __device__ inline void store_dims(const TreeParams& p, u
   }
 }
 
-// QP: rows 8 .. 15 of the one block are what f16 drops of rows 0 .. 7 (see the head of the file)
-template <int HD, int NB, bool Q8, int D, bool QP>
+// What f16 drops of q: left out, in rows 8 .. 15 of the one block, or in fragments of its own (see the head of the file)
+enum { Q_F16 = 0, Q_SPARE_ROWS = 1, Q_TWICE = 2 };
+template <int HD, int NB, bool Q8, int D, int QP>
 __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreeParams p) {
-  static_assert(!QP || NB == 1, "one block of rows");
+  static_assert(QP != Q_SPARE_ROWS || NB == 1, "one block of rows");
   constexpr int W = TREE_W, ROWS = 16 * NB * W;
   typedef TreeShape<HD, W> S;
   extern __shared__ __attribute__((aligned(1024))) unsigned char smem[];     // [D][K tile | V tile], mask words [WIN][ROWS], a flag of each wave
@@ -246,7 +248,8 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
   auto run = [&](auto BLOCKS) __attribute__((always_inline)) {
   constexpr int LIVE = decltype(BLOCKS)::value, NL = LIVE ? LIVE : 1, KD = NL == 1 ? 4 : 3, VD = NL == 1 ? 4 : 3;      // K and V^T fragments (NL products each) fetched ahead
   // Q: whole rows as they lie in memory, through a wave-private part of the ring's last buffer (taken by a tile only behind the first barrier), eight rows at a time, to the fragments: row ln of block nb, dims 32 ks + 8 kg .. + 7
-  h8 qf[NL][S::KS];
+  constexpr bool TWICE = QP == Q_TWICE;
+  h8 qf[NL][S::KS], ql[NL][TWICE ? S::KS : 1];
   if constexpr (LIVE == 0) { if (draft0 < n_tiles) fill_windows(0); } else {
     constexpr int LPQ = HD / 4, RPL = 64 / LPQ, QL = 8 / RPL;               // lanes of a row, rows of a load, loads of eight rows
     unsigned char* qs = smem + (D - 1) * 2 * S::TILE + wave * 8 * S::ROWB;
@@ -263,12 +266,15 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
 #pragma unroll
     for (int b = 0; b < 2 * NL; b++) {
 #pragma unroll
+      for (int part = 0; part < (TWICE ? 2 : 1); part++) {
+#pragma unroll
       for (int j = 0; j < QL; j++) {
         const uint32_t r = j * RPL + lane / LPQ, c = lane % LPQ;
-        f4 v = qv[b][j];
-        if (QP && b == 1) {
+        const bool low = part || (QP == Q_SPARE_ROWS && b == 1);
+        f4 v = qv[QP == Q_SPARE_ROWS ? 0 : b][j];
+        if (low) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) v[e] = qv[0][j][e] - (float)(_Float16)qv[0][j][e];
+          for (int e = 0; e < 4; e++) v[e] -= (float)(_Float16)v[e];
         }
         *(h4*)(qs + r * S::ROWB + ((c / 2) ^ r) * 16 + c % 2 * 8) = (h4){ (_Float16)v[0], (_Float16)v[1], (_Float16)v[2], (_Float16)v[3] };
       }
@@ -276,10 +282,11 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
 #pragma unroll
       for (int ks = 0; ks < S::KS; ks++) {
         const h8 f = *(const h8*)(qs + (ln & 7) * S::ROWB + ((ks * 4 + kg) ^ (ln & 7)) * 16);
-        if (b % 2 == 0) qf[b / 2][ks] = f;
-        else qf[b / 2][ks] = ln < 8 ? qf[b / 2][ks] : f;
+        h8& to = part ? ql[b / 2][TWICE ? ks : 0] : qf[b / 2][ks];
+        to = b % 2 == 0 || ln >= 8 ? f : to;
       }
       wave_fence();
+      }
     }
   }
   if constexpr (Q8) {
@@ -312,25 +319,34 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
     {
       constexpr int NF = 2 * S::KS;
       h8 ka[KD];
+      f4 sl[2][NL];
       auto at = [&](int f) __attribute__((always_inline)) { return kb + (k_rd ^ (f / 2 % 4 * 64)) + f / 8 * 256 + f % 2 * 16 * S::ROWB; };
 #pragma unroll
       for (int f = 0; f < KD; f++) ka[f] = *(const h8*)at(f);
 #pragma unroll
       for (int pb = 0; pb < 2; pb++)
 #pragma unroll
-        for (int nb = 0; nb < NL; nb++) s[pb][nb] = (f4){0.f, 0.f, 0.f, 0.f};
+        for (int nb = 0; nb < NL; nb++) s[pb][nb] = sl[pb][nb] = (f4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int f = 0; f < NF; f++) {
         const h8 a = ka[f % KD];
         if (f + KD < NF) ka[f % KD] = *(const h8*)at(f + KD);
 #pragma unroll
         for (int nb = 0; nb < NL; nb++) s[f % 2][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qf[nb][f / 2], s[f % 2][nb], 0, 0, 0);
+        if constexpr (TWICE) {
+#pragma unroll
+          for (int nb = 0; nb < NL; nb++) sl[f % 2][nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[nb][f / 2], sl[f % 2][nb], 0, 0, 0);
+        }
       }
       __builtin_amdgcn_sched_group_barrier(0x100, KD, 0);
 #pragma unroll
       for (int f = 0; f < NF; f++) {
-        __builtin_amdgcn_sched_group_barrier(0x008, NL, 0);
+        __builtin_amdgcn_sched_group_barrier(0x008, TWICE ? 2 * NL : NL, 0);
         if (f + KD < NF) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      if constexpr (TWICE) {
+#pragma unroll
+        for (int j = 0; j < 2 * NL; j++) s[j / NL][j % NL] += sl[j / NL][j % NL];
       }
     }
     // (the first fragments of V^T, with one block on their way during the softmax: with two the registers are full)
@@ -344,7 +360,7 @@ __global__ __launch_bounds__(TREE_W * 64, TREE_W / 4) void pa_tree_kernel(TreePa
 #pragma unroll
       for (int f = 0; f < VD; f++) fetch(f);
     }
-    if constexpr (QP) {
+    if constexpr (QP == Q_SPARE_ROWS) {
 #pragma unroll
       for (int j = 0; j < 8; j++) s[j / 4][0][j % 4] += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(s[j / 4][0][j % 4]), 0x128, 0xF, 0xF, false));     // row_ror:8
     }
@@ -647,7 +663,7 @@ static void set_magics(TreeParams& p) {
   p.rows_magic = div_magic((uint64_t)p.n_cols * p.n_heads, p.n_cols * p.group);
 }
 
-template <int HD, int NB, bool Q8, bool QP>
+template <int HD, int NB, bool Q8, int QP>
 static hipError_t launch_tree_k(const TreeParams& p, hipStream_t s, const PaTiming* t) {
   typedef TreeShape<HD, TREE_W> S;
   constexpr int D = Q8 ? 2 : 4;
@@ -656,7 +672,7 @@ static hipError_t launch_tree_k(const TreeParams& p, hipStream_t s, const PaTimi
   if (p.n_groups == 0 || p.group_rows == 0 || p.group_rows > 16u * NB * TREE_W || (uint64_t)(p.n_groups - 1) * p.group_rows >= (uint64_t)p.n_cols * p.group ||
       (uint64_t)p.n_groups * p.group_rows < (uint64_t)p.n_cols * p.group || p.n_splits == 0 ||
       (uint64_t)(p.n_splits - 1) * p.split_tiles * 32 >= (uint64_t)p.base_pos + p.n_cols || (uint64_t)p.n_splits * p.split_tiles * 32 < (uint64_t)p.base_pos + p.n_cols) return hipErrorInvalidValue;
-  if (QP && (uint64_t)p.n_cols * p.group > 8) return hipErrorInvalidValue;
+  if (QP == Q_SPARE_ROWS && (uint64_t)p.n_cols * p.group > 8) return hipErrorInvalidValue;
   const uint64_t total = (uint64_t)p.n_groups * p.n_kv_heads * p.n_splits;
   if (total > 0x7fffff00ull) return hipErrorInvalidValue;
   static PaPerDevice lds_set;
@@ -671,8 +687,8 @@ static hipError_t launch_tree_k(const TreeParams& p, hipStream_t s, const PaTimi
 template <int HD, bool Q8>
 static hipError_t launch_tree_hd(const TreeParams& p, const TreePlan& pl, hipStream_t s, const PaTiming* t) {
   switch (pl.nb) {
-    case 1: return (uint64_t)p.n_cols * p.group <= 8 ? launch_tree_k<HD, 1, Q8, true>(p, s, t) : launch_tree_k<HD, 1, Q8, false>(p, s, t);
-    case 2: if constexpr (HD == 128 || !Q8) return launch_tree_k<HD, 2, Q8, false>(p, s, t); else return hipErrorInvalidValue;
+    case 1: return (uint64_t)p.n_cols * p.group <= 8 ? launch_tree_k<HD, 1, Q8, Q_SPARE_ROWS>(p, s, t) : launch_tree_k<HD, 1, Q8, Q8 ? Q_F16 : Q_TWICE>(p, s, t);
+    case 2: if constexpr (HD == 128 || !Q8) return launch_tree_k<HD, 2, Q8, Q8 || HD == 256 ? Q_F16 : Q_TWICE>(p, s, t); else return hipErrorInvalidValue;
     default: return hipErrorInvalidValue;
   }
 }

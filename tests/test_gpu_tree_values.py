@@ -1,9 +1,10 @@
-"""Numbers that pa_attn_tree holds in f16, on the GPU against the oracle in 64 bits: int8 rows' values from the smallest to the largest scales, and the queries of small drafts."""
+"""Numbers that pa_attn_tree holds in f16, on the GPU against the oracle in 64 bits: int8 rows' values from the smallest to the largest scales, and queries."""
 import numpy as np
 import pytest
 from oracle import attn_oracle as O
 from oracle import tree_oracle as T
 from test_gpu_tree import Case
+from test_tree_rules import tree_rule
 from helpers import SHAPES
 
 pytestmark = pytest.mark.gpu
@@ -68,30 +69,63 @@ def test_an_infinite_int8_scale(base, n, at, splits, value):
     assert (got[sees][..., 64:96] == value).all() and np.isfinite(got[~sees]).all() and np.isfinite(np.delete(got, np.arange(64, 96), axis=2)).all()
 
 
+def long_queries(c):
+    """Long queries at right angles to the keys that their column sees, but for a small part: rounded to f16, their scores would be off by some hundredths."""
+    G, hd = c.cfg["n_heads"] // c.cfg["n_kv_heads"], c.cfg["head_dim"]
+    for g in range(c.cfg["n_kv_heads"]):
+        for col in range(c.n):
+            K = c.k[np.concatenate([np.ones(c.base, bool), c.seen[col]]), g].astype(np.float64)
+            assert 0 < K.shape[0] < hd
+            back, far = np.linalg.pinv(K), 20 * c.rng.standard_normal((hd, G))
+            c.q[col, g * G:g * G + G] = (far - back @ (K @ far) + back @ (np.sqrt(hd) * c.rng.standard_normal((K.shape[0], G)))).T
+
+
+def check_queries(c, splits, what):
+    """q counts to 2^-22 of itself (its f16 and what that leaves).  What is left are P and f32 sums, and an output of f16 or a part of the like: at most four roundings of half a step, 2^-11, that
+    add in squares (as in test_gpu_tree_run.check_some): 2^-10 of the norm."""
+    with c.context() as pa:
+        c.fill(pa)
+        pa.set_decode_splits(splits)
+        got = pa.run_attn_tree(0, c.q, c.seen, c.base, gate=c.gate)
+    ref = T.tree_attention(c.q, c.k, c.v, c.base, c.seen, c.gate)[0]
+    norm = np.sqrt(((got - ref) ** 2).sum() / (ref ** 2).sum())
+    print("%s base %d n %d: %.2e of the norm" % (what, c.base, c.n, norm), flush=True)
+    assert norm <= 2.0 ** -10
+
+
 @pytest.mark.parametrize("shape", sorted(SHAPES))
 @pytest.mark.parametrize("base,splits", [(0, 0), (3, 0), (40, 1), (59, 2)])
 def test_queries_of_small_drafts(shape, base, splits):
-    """Up to eight stacked rows: q counts to 2^-22 of itself (its f16 and what that leaves), as in a verify block of the same columns.  Long queries at right angles to the keys but for a small
-    part: rounded to f16, their scores would be off by some hundredths.  What is left are P, partials and f32 sums, at most four roundings of half a step, 2^-11, that add in squares (as in
-    test_gpu_tree_run.check_some): 2^-10 of the norm."""
+    """Up to eight stacked rows, as in a verify block of the same columns."""
     cfg = SHAPES[shape]
-    G, hd = cfg["n_heads"] // cfg["n_kv_heads"], cfg["head_dim"]
-    for n in sorted({1, 8 // G}):
+    for n in sorted({1, 8 // (cfg["n_heads"] // cfg["n_kv_heads"])}):
         c = Case(cfg, base, n, seed=base + n)
-        for h in range(cfg["n_heads"]):
-            K = c.k[:, h // G].astype(np.float64)
-            back = np.linalg.pinv(K)
-            for col in range(n):
-                far = 20 * c.rng.standard_normal(hd)
-                c.q[col, h] = far - back @ (K @ far) + back @ (np.sqrt(hd) * c.rng.standard_normal(K.shape[0]))
-        with c.context() as pa:
-            c.fill(pa)
-            pa.set_decode_splits(splits)
-            got = pa.run_attn_tree(0, c.q, c.seen, base, gate=c.gate)
-        ref = T.tree_attention(c.q, c.k, c.v, base, c.seen, c.gate)[0]
-        norm = np.sqrt(((got - ref) ** 2).sum() / (ref ** 2).sum())
-        print("small draft %s base %d n %d: %.2e of the norm" % (shape, base, n, norm), flush=True)
-        assert norm <= 2.0 ** -10
+        long_queries(c)
+        check_queries(c, splits, "small draft " + shape)
+
+
+@pytest.mark.parametrize("shape", sorted(SHAPES))
+@pytest.mark.parametrize("base,n,splits", [(0, 5, 0), (20, 9, 1), (20, 9, 2), (7, 24, 0), (40, 40, 3), (64, 60, 4)])
+def test_queries_of_more_rows(shape, base, n, splits):
+    """One block of rows a wave, and two of heads of 128."""
+    cfg = SHAPES[shape]
+    if cfg["head_dim"] == 256:
+        assert tree_rule(cfg, base, n, splits)[0] == 1
+    c = Case(cfg, base, n, seed=base + n)
+    long_queries(c)
+    check_queries(c, splits, "draft " + shape)
+
+
+@pytest.mark.parametrize("splits", [0, 3])
+def test_queries_of_two_blocks_a_wave(splits):
+    """Heads of 128 in a draft so wide that its plan has them, each column seeing a few rows."""
+    cfg, n = dict(n_heads=64, n_kv_heads=1, head_dim=128, n_rot=64, rope_theta=1e6, eps=1e-6, qk_norm=True, gate=False), 1000
+    assert tree_rule(cfg, 0, n, splits)[0] == 2
+    c = Case(cfg, 0, n, seed=n)
+    c.seen = c.rng.random((n, n)) < 0.006
+    c.seen[np.arange(n), np.arange(n)] = True
+    long_queries(c)
+    check_queries(c, splits, "two blocks a wave,")
 
 
 @pytest.mark.parametrize("q8", [False, True])
