@@ -11,7 +11,7 @@
 //     LDS transpose read.  The accumulator of S^T is the operand of P V, so probabilities never leave registers.
 //   * The products take f16, and q is rounded to it; what that drops of f16 rows' q goes into products of its own with the same K fragments, so that q counts to 2^-22 of itself.  Up to eight stacked
 //     rows in all leave half of their one block free, and its rows 8 .. 15 hold it, at no cost; else it is in fragments beside q's (24 columns at 2011 rows 13.3 -> 14.5 us a call, 63 at 7001 of heads of
-//     128 15.2 -> 16.5: half of the score products again).  Not where registers have no room, two blocks a wave of heads of 256, nor for more int8 rows, whose own rounding, K's to f16, is as large.
+//     128 15.2 -> 16.5: the score products once more).  Not where registers have no room, two blocks a wave of heads of 256, nor for more int8 rows, whose own rounding, K's to f16, is as large.
 //   * Online softmax in f32 in the exp2 domain: the reference of a row is raised, and O and l rescaled, only where a P comes out above 2^8 (exact enough in f16); l is
 //     the sum of the rounded P, so an output is a convex combination of value rows whatever that rounding did.
 //   * The mask is looked at only in tiles that reach the drafted rows.  There a row's 32 bits are one word, cut out of its mask at the tile's offset with the rows in front
@@ -20,11 +20,11 @@
 //   * Splits leave (m, l) and O / l in f32; pa_tree_merge_kernel joins them.  (In f16 they are half the bytes, which is 0 - 4 us of a call, and 2^-12 of an output: 63 splits of 17 columns at
 //     20003 int8 rows 25.7 us against 29.7, 16 of 24 at 2011 12.9 against 13.3.)
 //
-// Measured (24 query and 4 key heads of 256, 65536 rows of f16, 268 MB): 16 columns 52 us = 5.1 TB/s, which is what a large copy reaches; 48 columns 94.6 us = 817 TFLOP/s (a large matrix
+// Measured (24 query and 4 key heads of 256, 65536 rows of f16, 268 MB): 16 columns 52 us = 5.1 TB/s, which is what a large copy reaches; 48 columns 95 us = 813 TFLOP/s (a large matrix
 // product: 1330), and 3 % less with every tile read from the L2, so there the SIMDs' work bounds it: a tile of nine blocks, three of them on one SIMD, takes 1.3 us, of which the matrix
 // instructions are 0.8 at the 1.9 GHz that the power limit leaves.  The merge adds 9.3 us there (38 MB of partials), 3 - 4 for small drafts, most of it the launch.  Int8: 17 columns at 20003 rows
-// 24.7 us and 7.5: the widening through registers, 1.1 us a tile of seven blocks, and 26 MB of partials.  5 columns at 190 rows, 16 and 8 heads of 128: 7.4 us a call in one launch, 7.8 with
-// seven splits and the merge; at 100 rows 5.9 and 8.3.
+// 24.4 us and 7.5: the widening through registers, 1.1 us a tile of seven blocks, and 26 MB of partials.  5 columns at 190 rows, 16 and 8 heads of 128: 8.3 us a call in one launch; 7.2 before
+// q's second products, and then 7.8 with seven splits and the merge (at 100 rows 5.9 and 8.3).
 #include "tree_internal.h"
 #include "pf_common.h"
 #include "tree_mask.h"

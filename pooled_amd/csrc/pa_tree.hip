@@ -78,7 +78,8 @@ static size_t ml_bytes(const pa_config& c, uint32_t n_cols, uint32_t splits) { r
 // What a call takes, in us, fitted to 463 timed calls (16 / 2-, 24 / 4- and 16 / 8-head shapes, 2 - 64 columns at 64 - 65536 rows, f16 and int8 rows, 64 - 256 rows a workgroup, all CUs busy
 // down to an eighth of them; mean error 4 %, nine in ten within 8 %; what it chooses takes 100.8 % of the best plan tried, 109 % at worst).  The launches, the start of a workgroup and its
 // outputs; then its tiles, each so long for the barrier and the chain of one wave and so much for every block of 16 rows, or the stream of the cache if that is more; and the
-// partials, written and read again (timed as f16; as f32 they take 0.0 - 0.3 us a MB more, and where twice the weight would choose another plan it takes as long: 26 cases, mean of the quotients 1.00).
+// partials, written and read again (timed as f16; as f32 they take 0.0 - 0.3 us a MB more, and where twice the weight would choose another plan it takes as long: 26 cases, mean of the quotients 1.00).  q's second products came later too: over
+// 60 cases of 5 - 63 columns at 300 - 40000 rows the choice takes 102 % of the best cap's time, 125 % at worst, where the best is two blocks a wave of heads of 256, which are without them.
 static double tree_us(const pa_config& c, uint32_t n_cu, uint32_t rows, uint32_t tiles, const TreePlan& pl) {
   const bool q8 = (c.flags & PA_FLAG_KV_Q8) != 0, wide = c.head_dim == 256;
   const double fixed = q8 ? (wide ? 10.1 : 7.6) : wide ? 8.6 : 7.2, out = q8 ? (wide ? 0.05 : 0.18) : wide ? 0.29 : 0.19;
