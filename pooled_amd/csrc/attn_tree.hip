@@ -48,7 +48,7 @@ static __device__ inline bool not_finite2(uint32_t w) { return (w & 0x7c00u) == 
 
 // An int8 row's values v as f16: v 2^-k, exactly, times scale 2^k, which is given as the f16 nearest to it and the rest.  k brings the scale to [1, 2) where 2^-24 <= scale < 64 (-5 <= k <= 24), so that
 // the two parts hold it to 2^-24 of itself and the product is rounded once, to what f16 holds of it, subnormal numbers too (the part of the rest, rounded before, adds 2^-21 of a value, or 2^-25).
-// Smaller scales give zeros, larger ones what f16 holds; from 2^21 on they count as infinite.
+// Other scales give what f16 holds of their values too; from 2^21 on they count as infinite.
 // v 2^-k is the bit pattern of 2^(10 - k) + (v + 128) 2^-k, whose upper byte is (25 - k) << 2, less 1152 x 2^-k.
 struct Widen { _Float16 hi, lo, off; uint32_t top; };
 static __device__ inline Widen widen_of(float sc) {
